@@ -249,6 +249,106 @@ void tg_hip_attention_dev(int fmt_q, int fmt_k, int fmt_v, int fmt_o, const void
                           void *stream);
 size_t tg_hip_attention_scratch_bytes(int embed_dim, int n_heads, int n_kv_heads, int head_dim, int kv_max);
 
+/* ---- prompts and batches: packed rows of several sequences ----
+ * No counterpart in the reference, which runs attention row by row
+ * (tinygiant/engine.py:232-275).  The next three calls share these arguments:
+ *   rows      row cu_rows[s] + i of the packed rows is row i of sequence s
+ *             (cu_rows int32 [n_seqs + 1], not decreasing); rows in front of
+ *             cu_rows[0] and from cu_rows[n_seqs] on belong to no sequence.
+ *             A sequence may have no rows.
+ *   caches    kv_k, kv_v [n_slots][n_kv_heads][kv_max][head_dim], each slot
+ *             what tg_hip_attention_dev takes; kv_type 0 float32, 1 float16;
+ *             16-byte aligned.  Sequence s uses slot slots[s] (NULL: s), in
+ *             which kv_len[s] positions (NULL: 0) were cached before these
+ *             rows: row i is at position kv_len[s] + i.
+ *   shapes    head_dim a multiple of 8 and <= 128, n_heads <= 1024,
+ *             n_heads / n_kv_heads integral and <= 64, kv_max <= 2^20,
+ *             n_rows <= 2^22, n_seqs <= 2^16
+ *   strides   in floats from row to row, of at least a row's heads
+ * cu_rows, kv_len and slots are device arrays that the host does not see: a
+ * sequence whose slot is not below n_slots, or whose rows do not fit kv_max,
+ * is left out (its rows of the outputs and the caches stay as they were).
+ * n_rows = 0 or n_seqs = 0 does nothing.  A launch that HIP refuses is
+ * reported by tg_hip_last_error().  All of it can be captured and replayed;
+ * calls that overlap in time need scratch of their own.
+ *
+ * tg_hip_kv_append_dev prepares the rows for attention: the optional RMS
+ * norm of each query and K head (tg_rms_norm, csrc/libtinygiant.c:680-698;
+ * weights [head_dim], NULL: none), RoPE (apply_rope_inplace, :702-719) at
+ * position base_pos + kv_len[s] + i of the tables [rope_len][head_dim / 2]
+ * (both NULL: none; a row past the tables is left out), K and V stored into
+ * the cache (float16: rounded to nearest) and the query heads into q_out
+ * (NULL: only K and V; may be q with q's stride).  q, k and v may lie side
+ * by side in one array of rows.  base_pos is the length of a shared prefix.
+ * Two sequences of a call must not write the same positions of a slot. */
+void tg_hip_kv_append_dev(const float *q_dev, const float *k_dev, const float *v_dev, int q_stride, int kv_stride,
+                          const float *q_norm_w_dev, const float *k_norm_w_dev, float eps, const float *rope_cos_dev,
+                          const float *rope_sin_dev, int rope_len, const int32_t *cu_rows_dev,
+                          const int32_t *kv_len_dev, const int32_t *slots_dev, int n_seqs, int n_rows, int base_pos,
+                          int kv_type, void *kv_k_dev, void *kv_v_dev, int n_slots, int kv_max, int n_heads,
+                          int n_kv_heads, int head_dim, float *q_out_dev, int q_out_stride, void *stream);
+/* Causal attention of the rows over their sequences' slots, after
+ * tg_hip_kv_append_dev has stored their K and V (head_task, csrc/
+ * libtinygiant.c:862-904, for every row): row i of sequence s sees positions
+ * 0 .. kv_len[s] + i, with window > 0 the last `window` of them; scores
+ * scaled by 1 / sqrt(head_dim); sinks [n_heads] (NULL: none) are logits that
+ * take part in the softmax and carry no value.  Whole prompts (kv_len 0),
+ * chunks behind cached positions, verify passes and batches of one row a
+ * sequence are all this call.  out may be q with q's stride.  Values of
+ * positions that a row does not see never reach it, infinities and NaN
+ * included.  The arithmetic is f32 for both cache types (sums in f32; 16-bit
+ * operands of the matrix units only in exact or compensated form).
+ * scratch_dev holds tg_hip_attention_prompt_scratch_bytes(...) bytes
+ * (prefix_len 0), 16-byte aligned; it may be NULL where that is 0. */
+void tg_hip_attention_prompt_dev(const float *q_dev, int q_stride, int kv_type, const void *kv_k_dev,
+                                 const void *kv_v_dev, int n_slots, int kv_max, const int32_t *cu_rows_dev,
+                                 const int32_t *kv_len_dev, const int32_t *slots_dev, int n_seqs, int n_rows, int window,
+                                 const float *sinks_dev, int n_heads, int n_kv_heads, int head_dim, float *out_dev,
+                                 int out_stride, void *scratch_dev, void *stream);
+size_t tg_hip_attention_prompt_scratch_bytes(int n_rows, int n_seqs, int n_heads, int n_kv_heads, int head_dim,
+                                             int kv_max, int prefix_len);
+/* The same for a batch whose sequences share their first prefix_len
+ * positions: those are in prefix_k, prefix_v [n_kv_heads][prefix_max]
+ * [head_dim] (of kv_type, 16-byte aligned), held once and read once for the
+ * whole batch, and what follows in the sequences' own slots: row i is at
+ * position prefix_len + kv_len[s] + i.  prefix_len 0 is
+ * tg_hip_attention_prompt_dev. */
+void tg_hip_attention_prefix_dev(const float *q_dev, int q_stride, int kv_type, const void *kv_k_dev,
+                                 const void *kv_v_dev, int n_slots, int kv_max, const void *prefix_k_dev,
+                                 const void *prefix_v_dev, int prefix_len, int prefix_max, const int32_t *cu_rows_dev,
+                                 const int32_t *kv_len_dev, const int32_t *slots_dev, int n_seqs, int n_rows, int window,
+                                 const float *sinks_dev, int n_heads, int n_kv_heads, int head_dim, float *out_dev,
+                                 int out_stride, void *scratch_dev, void *stream);
+
+/* Adjusts k rows of logits [k][nrows] before a token is chosen from them, in
+ * this order, each step one f32 operation rounded to nearest:
+ *   l = l > 0 ? l / repetition : l * repetition   tokens in the row's history
+ *   l = l - frequency * c - presence              tokens generated c > 0 times
+ *   l = l + bias                                  tokens with a bias
+ *   l = -inf                                      tokens that are not allowed
+ * hist [k][hist_stride] (NULL: none) holds hist_len[j] tokens of row j, those
+ * from gen_start[j] on (NULL: 0) generated and the ones before the prompt's;
+ * penalties [k][3] = repetition, frequency, presence.  bias_tok, bias_val
+ * [k][bias_stride] (NULL: none) hold bias_len[j] entries (NULL: bias_stride);
+ * of a token listed more than once the last entry holds.  Tokens outside
+ * 0 .. nrows - 1 are skipped, lengths past their stride are cut to it.  allow
+ * (NULL: all) has a bit for each token, token t in bit t % 32 of word t / 32,
+ * allow_stride words a row or 0 for one row that all share.  A masked token
+ * is -inf whatever its logit was, NaN included.
+ * out (NULL: not written) may be logits.  argmax[j] is the first token with
+ * the largest adjusted logit (a NaN counts as the largest, as in
+ * numpy.argmax), -1 where all are -inf; maxval[j] that logit; either may be
+ * NULL.  They need tg_hip_logits_scratch_bytes(k, nrows) bytes of scratch,
+ * 8-byte aligned.  k <= 65535, nrows <= 2^24.  No counterpart in the
+ * reference, whose choice is numpy.argmax over the head's logits
+ * (tinygiant/specdec.py:77,90). */
+void tg_hip_logits_adjust_dev(const float *logits_dev, float *out_dev, int k, int nrows, const int32_t *hist_dev,
+                              int hist_stride, const int32_t *hist_len_dev, const int32_t *gen_start_dev,
+                              const float *penalties_dev, const int32_t *bias_tok_dev, const float *bias_val_dev,
+                              int bias_stride, const int32_t *bias_len_dev, const uint32_t *allow_dev, int allow_stride,
+                              int32_t *argmax_dev, float *maxval_dev, void *scratch_dev, void *stream);
+size_t tg_hip_logits_scratch_bytes(int k, int nrows);
+
 /* Output head over k (1..16) device-resident rows with the argmax fused in:
  * x_j = RMSNorm(inputs_j) * norm_w (skipped when norm_w_dev is NULL),
  * logits[j][r] = dot(mat row r, q8(x_j)) and argmax_dev[j] = the first r

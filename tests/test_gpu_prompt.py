@@ -1,0 +1,467 @@
+"""GPU checks of the prompt and batch path (tg_hip_kv_append_dev,
+tg_hip_attention_prompt_dev, tg_hip_attention_prefix_dev) against plain
+computations in 64 bits; tolerances: tests/_packed.py."""
+
+import ctypes
+import sys
+
+import numpy as np
+import pytest
+
+from tests._packed import EPS, Batch, Dev, Graph
+
+pytestmark = pytest.mark.gpu
+
+
+def say(*a):
+    print(*a, flush=True)
+    sys.stdout.flush()
+
+
+def _run(tg, b, **kw):
+    dev = Dev(tg)
+    tg.lib().tg_hip_clear_error()
+    out, was = b.call(dev, **kw)
+    tg.lib().tg_hip_synchronize()
+    assert tg.last_error() == "", tg.last_error()
+    got = dev.read(out, b.q)
+    dev.free()
+    return got, was
+
+
+LAYOUTS = [(8, 2, 128), (32, 4, 128), (8, 1, 64), (4, 4, 32), (15, 3, 80), (6, 1, 8), (14, 2, 112), (40, 1, 16)]
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("lens,past", [
+    ([1], [0]), ([1], [1]), ([5], [63]), ([0, 1, 3], [4, 0, 60]), ([33, 0, 64, 1], [0, 5, 1, 130]), ([130], [0]),
+    ([17, 31], [100, 257]), ([1] * 9, [0, 1, 15, 16, 63, 64, 65, 127, 300])])
+def test_prompt_matches_plain(tg, layout, lens, past, half):
+    nh, nkv, hd = layout
+    say(f"prompt {layout} lens={lens} past={past} half={half}")
+    b = Batch(hash((nh, hd, len(lens), sum(lens))) % 2 ** 31, nh, nkv, hd, lens, past, half, sinks=nh % 4 != 0, lead=len(lens) % 3,
+              tail=2, pad=4 * (nkv % 2))
+    got, was = _run(tg, b)
+    say(f"  worst error / tolerance {b.check(got, was):.3f}")
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("window", [1, 2, 31, 64, 128, 1000])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompt_windows(tg, window, hd, half):
+    say(f"prompt window={window} hd={hd} half={half}")
+    b = Batch(window + hd, 8, 1, hd, [1, 90, 200], [500, 0, 77], half, window=window, sinks=hd == 64)
+    got, was = _run(tg, b)
+    b.check(got, was)
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("nh,nkv,hd,lens,past", [
+    (32, 4, 128, [9], [4000]), (64, 8, 64, [3], [9000]), (8, 1, 128, [1], [20011]), (8, 2, 128, [600], [700]),
+    (8, 8, 64, [257, 300], [511, 0]), (16, 2, 128, [1] * 12, [37 * i * i % 2900 for i in range(12)])])
+def test_prompt_long(tg, nh, nkv, hd, lens, past, half):
+    """Long caches: the positions are split over workgroups where rows are few."""
+    say(f"prompt long {nh, nkv, hd} lens={lens} past={past[:3]} half={half}")
+    b = Batch(sum(lens), nh, nkv, hd, lens, past, half, sinks=hd == 64)
+    got, was = _run(tg, b)
+    say(f"  worst error / tolerance {b.check(got, was):.3f}")
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("layout", [(8, 2, 128), (64, 8, 64), (15, 3, 80), (40, 1, 16)])
+@pytest.mark.parametrize("prefix,lens,past,window", [
+    (1, [1], [0], 0), (64, [1, 1, 1], [0, 3, 64], 0), (65, [2, 0, 5], [0, 1, 9], 0), (700, [1] * 20, list(range(20)), 0),
+    (500, [1, 1, 4], [0, 100, 200], 150), (130, [1, 40], [300, 0], 128), (127, [3], [200], 16)])
+def test_prefix_matches_plain(tg, layout, prefix, lens, past, window, half):
+    nh, nkv, hd = layout
+    say(f"prefix {layout} prefix={prefix} lens={lens} window={window} half={half}")
+    b = Batch(prefix + nh, nh, nkv, hd, lens, past, half, window=window, sinks=nkv % 2 == 0, prefix=prefix, lead=1, tail=1)
+    got, was = _run(tg, b)
+    b.check(got, was)
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_out_over_q(tg, half):
+    for kw in (dict(lens=[70, 3], past=[0, 9]), dict(lens=[2], past=[3000]), dict(lens=[1, 2], past=[5, 0], prefix=400)):
+        say(f"out over q {kw} half={half}")
+        b = Batch(3, 16, 2, 64, half=half, lead=1, tail=1, **kw)
+        got, was = _run(tg, b, in_place=True)
+        b.check(got, was)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_values_a_row_does_not_see(tg, hd, half, bad):
+    """Infinities and NaN in K and V of positions behind a row, or in front of
+    its window, leave the row as it is; rows that see a NaN in V are NaN."""
+    say(f"unseen hd={hd} half={half} bad={bad}")
+    for window, at in ((0, 100), (40, 100), (0, 149)):
+        b = Batch(hd, 8, 2, hd, [140], [10], half, window=window)
+        ref = b.attend()
+        b.k[b.slots[0], :, at] = bad
+        b.v[b.slots[0], :, at] = bad
+        got, was = _run(tg, b)
+        hit = np.array([lo <= at <= hi for lo, hi in (b.seen(0, i) for i in range(140))])
+        err = np.abs(got[~hit] - ref[0][~hit])
+        assert np.all(err <= ref[1][~hit]), float(np.nanmax(err))
+        assert np.all(np.isnan(got[hit])) == bool(hit.any()) or not hit.any()
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_infinite_values(tg, half):
+    """An infinity in V alone is the output of the rows that see it, in its
+    dimension only, as the sum of weights times values gives it."""
+    say(f"infinite V half={half}")
+    for hd, lens, past in ((64, [70], [3]), (128, [2], [900])):
+        b = Batch(5, 8, 2, hd, lens, past, half, q_scale=0.5)
+        ref, tol = b.attend()
+        at = past[0] + 1
+        b.v[b.slots[0], :, at, 5] = np.inf
+        b.v[b.slots[0], :, at, 9] = -np.inf
+        got, was = _run(tg, b)
+        g, r = got.reshape(b.rows, 8, hd), ref.reshape(b.rows, 8, hd)
+        assert np.all(np.abs(g[:1] - r[:1]) <= tol.reshape(r.shape)[:1])
+        assert np.all(g[1:, :, 5] == np.inf) and np.all(g[1:, :, 9] == -np.inf)
+        rest = [d for d in range(hd) if d not in (5, 9)]
+        assert np.all(np.abs(g - r)[:, :, rest] <= tol.reshape(r.shape)[:, :, rest])
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("q_scale", [1e-30, 1e-3, 300.0])
+def test_score_ranges(tg, half, q_scale):
+    """Queries so small that all weights are equal, and so large that one is all."""
+    say(f"q_scale={q_scale} half={half}")
+    for hd in (64, 128):
+        b = Batch(11, 8, 2, hd, [50, 1], [20, 700], half, q_scale=q_scale, sinks=True)
+        got, was = _run(tg, b)
+        b.check(got, was)
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_cache_ranges(tg, half):
+    """Caches at the ends of their ranges: large values (f16's largest among
+    them) and tiny ones, next to each other in a row."""
+    say(f"cache ranges half={half}")
+    big = 65504.0 if half else 3e6
+    for hd in (64, 128):
+        b = Batch(12, 8, 2, hd, [40, 1], [9, 500], half, q_scale=1e-4)
+        for s in range(2):
+            m = b.lens[s] + b.past[s]
+            b.k[b.slots[s], :, :m, ::7] *= np.float32(big / 8)
+            b.k[b.slots[s], :, :m, 1::7] *= np.float32(1e-4)
+            np.clip(b.k, -big, big, out=b.k)
+            b.v[b.slots[s], :, :m] *= np.float32(big / 8)
+            np.clip(b.v, -big, big, out=b.v)
+        got, was = _run(tg, b)
+        b.check(got, was)
+
+
+def test_sequences_that_do_not_fit_are_left_out(tg):
+    """A slot out of range, a negative length, rows past kv_max: those
+    sequences' rows stay as they were, the others are computed."""
+    for key, vals in (("slots", (-1, 99, 2 ** 31 - 1)), ("kv_len", (-1, 10 ** 6, 2 ** 31 - 1))):
+        for v in vals:
+            for prefix in (0, 200):
+                say(f"left out: {key}={v} prefix={prefix}")
+                b = Batch(1, 8, 2, 64, [3, 4, 2], [50, 60, 70], False, prefix=prefix)
+                ref = b.attend()
+                getattr(b, key)[1] = v
+                got, was = _run(tg, b)
+                gone = slice(b.cu[1], b.cu[2])
+                assert np.array_equal(got[gone], was[gone])
+                keep = np.ones(b.rows, bool)
+                keep[gone] = False
+                assert np.all(np.abs(got[keep] - ref[0][keep]) <= ref[1][keep])
+
+
+def test_bad_row_offsets_stay_in_bounds(tg):
+    """Offsets past the rows and decreasing ones: what is computed of them is
+    not specified, the call ends and the rows outside stay."""
+    for cu in ([0, 5, 4000], [-7, 3, 6], [4, 2, 1]):
+        say(f"row offsets {cu}")
+        b = Batch(2, 8, 2, 64, [3, 4], [50, 60], False)
+        b.cu = np.array(cu, np.int32)
+        _run(tg, b)
+
+
+def test_null_lengths_and_slots(tg):
+    say("null kv_len and slots")
+    b = Batch(4, 8, 2, 128, [20, 7], [0, 0], False)
+    b.k, b.v = (np.concatenate([t[b.slots], t[:2]]) for t in (b.k, b.v))   # slot s is sequence s's
+    b.slots = np.arange(2, dtype=np.int32)
+    ref = b.attend()
+    dev = Dev(tg)
+    out, was = b.call(dev)
+    b.ptrs["len"] = b.ptrs["slots"] = None
+    b.queue(tg.lib())
+    tg.lib().tg_hip_synchronize()
+    b.check(dev.read(out, b.q), was, ref)
+    dev.free()
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_replayed_graph(tg, half):
+    """Captured once and replayed with other queries and lengths in the same
+    arrays, eager work in between; each replay gives the eager call's bits.
+    Two graphs with scratch of their own do not disturb each other."""
+    lib = tg.lib()
+    say(f"graph half={half}")
+    dev = Dev(tg)
+    bs = [Batch(20, 32, 4, 128, [5], [2500], half), Batch(21, 8, 2, 64, [1, 3], [40, 900], half, prefix=600)]
+    eager = []
+    for b in bs:
+        out, _ = b.call(dev)
+        lib.tg_hip_synchronize()
+        eager.append(dev.read(out, b.q))
+    graphs = [Graph(lambda s, b=b: b.queue(lib, s)) for b in bs]
+    for step in range(3):
+        for b, g, e in zip(bs, graphs, eager):
+            g.replay()
+            got = dev.read(b.ptrs["out"], b.q)
+            assert got.tobytes() == e.tobytes(), step
+            q2 = np.ascontiguousarray(b.q * np.float32(0.5))
+            lib.tg_hip_memcpy_h2d(b.ptrs["q"], q2.ctypes.data, q2.nbytes)
+            g.replay()
+            got = dev.read(b.ptrs["out"], b.q)
+            b.queue(lib)
+            lib.tg_hip_synchronize()
+            assert got.tobytes() == dev.read(b.ptrs["out"], b.q).tobytes()
+            lib.tg_hip_memcpy_h2d(b.ptrs["q"], np.ascontiguousarray(b.q).ctypes.data, b.q.nbytes)
+    # shorter caches through the graph that was captured with longer ones
+    b, g = bs[0], graphs[0]
+    b.past, b.kv_len = [7], np.array([7], np.int32)
+    lib.tg_hip_memcpy_h2d(b.ptrs["len"], b.kv_len.ctypes.data, 4)
+    b.k[b.slots[0], :, 12:], b.v[b.slots[0], :, 12:] = np.nan, np.nan
+    for key in "kv":
+        a = np.ascontiguousarray(getattr(b, key))
+        lib.tg_hip_memcpy_h2d(b.ptrs[key], a.ctypes.data, a.nbytes)
+    g.replay()
+    b.check(dev.read(b.ptrs["out"], b.q), np.full_like(b.q, 7.5))
+    for g in graphs:
+        g.free()
+    dev.free()
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_same_bits_every_time(tg, half):
+    say(f"same bits half={half}")
+    for b in (Batch(30, 32, 4, 128, [9], [3000], half), Batch(31, 64, 8, 64, [100, 1], [0, 800], half, sinks=True),
+              Batch(32, 8, 2, 128, [1] * 6, list(range(6)), half, prefix=900)):
+        dev = Dev(tg)
+        out, _ = b.call(dev)
+        tg.lib().tg_hip_synchronize()
+        first = dev.read(out, b.q)
+        for _ in range(3):
+            b.queue(tg.lib())
+            tg.lib().tg_hip_synchronize()
+            assert dev.read(out, b.q).tobytes() == first.tobytes()
+        dev.free()
+
+
+# ---- append ----
+
+def _rope_tables(n, hd):
+    half = hd // 2
+    ang = np.arange(n)[:, None] / (10000.0 ** (np.arange(half)[None, :] * 2.0 / hd))
+    return np.cos(ang).astype(np.float32), np.sin(ang).astype(np.float32)
+
+
+def _norm64(x, w, eps):
+    x = x.astype(np.float64)
+    return x if w is None else x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * w.astype(np.float64)
+
+
+def _rope64(x, c, s):
+    h = x.shape[-1] // 2
+    a, b = x[..., :h], x[..., h:]
+    c, s = c.astype(np.float64), s.astype(np.float64)
+    return np.concatenate([a * c - b * s, b * c + a * s], -1)
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("nh,nkv,hd", [(32, 4, 128), (64, 8, 64), (15, 3, 80), (6, 1, 8), (4, 4, 32), (14, 2, 112)])
+@pytest.mark.parametrize("norm,rope,in_place,base", [(True, True, False, 0), (False, True, True, 37), (True, False, True, 0)])
+def test_append_matches_plain(tg, nh, nkv, hd, half, norm, rope, in_place, base):
+    """Tolerance: f32 results are a norm (a sum of hd squares, a root, a
+    division, two products: hd / 2 + 6 roundings at most, of one sign only in
+    the worst case) and a rotation (two products and a sum of values up to
+    sqrt(2) of the head's largest); an f16 cache adds half a step of f16."""
+    say(f"append {nh, nkv, hd} half={half} norm={norm} rope={rope} in_place={in_place}")
+    lib, rng = tg.lib(), np.random.default_rng(nh + hd)
+    lens, past, lead, tail = [3, 0, 1, 20], [0, 4, 9, 2], 1, 2
+    rows, n, n_slots, kv_max = lead + sum(lens) + tail, 4, 6, 30
+    width = (nh + 2 * nkv) * hd + 12
+    qkv = rng.standard_normal((rows, width)).astype(np.float32)
+    qn, kn = (rng.uniform(0.5, 1.5, hd).astype(np.float32) if norm else None for _ in range(2))
+    cos, sin = _rope_tables(base + 22, hd) if rope else (None, None)
+    cu = (lead + np.concatenate([[0], np.cumsum(lens)])).astype(np.int32)
+    slots = np.array([5, 0, 2, 1], np.int32)
+    dtype = np.float16 if half else np.float32
+    k0 = rng.standard_normal((n_slots, nkv, kv_max, hd)).astype(dtype)
+    v0 = rng.standard_normal((n_slots, nkv, kv_max, hd)).astype(dtype)
+    dev = Dev(tg)
+    p, pk, pv = dev(qkv, 4), dev(k0), dev(v0)
+    q_at, k_at, v_at = p, p + 4 * nh * hd, p + 4 * (nh + nkv) * hd
+    q0 = qkv if in_place else np.full((rows, nh * hd + 4), 7.5, np.float32)
+    po = p if in_place else dev(q0)
+    lib.tg_hip_clear_error()
+    lib.tg_hip_kv_append_dev(q_at, k_at, v_at, width, width, dev(qn), dev(kn), 1e-6, dev(cos), dev(sin), base + 22,
+                             dev(cu), dev(np.array(past, np.int32)), dev(slots), n, rows, base, int(half), pk, pv, n_slots,
+                             kv_max, nh, nkv, hd, po, q0.shape[1], None)
+    lib.tg_hip_synchronize()
+    assert tg.last_error() == "", tg.last_error()
+    got_q, got_k, got_v = dev.read(po, q0), dev.read(pk, k0), dev.read(pv, v0)
+    dev.free()
+    want_q, want_k, want_v = q0.astype(np.float64), k0.astype(np.float64), v0.astype(np.float64)
+    for s in range(n):
+        for i in range(lens[s]):
+            r, at = cu[s] + i, past[s] + i
+            heads = qkv[r, :(nh + 2 * nkv) * hd].reshape(-1, hd)
+            q, k = _norm64(heads[:nh], qn, 1e-6), _norm64(heads[nh:nh + nkv], kn, 1e-6)
+            if rope:
+                q, k = (_rope64(x, cos[base + at], sin[base + at]) for x in (q, k))
+            want_q[r, :nh * hd] = q.reshape(-1)
+            want_k[slots[s], :, at], want_v[slots[s], :, at] = k, heads[nh + nkv:]
+    step = (hd / 2 + 6 + 4) * EPS * 1.5
+    cache = step + (2.0 ** -11 if half else 0)
+    assert np.all(np.abs(got_q - want_q) <= step * np.abs(want_q).max())
+    assert np.all(np.abs(got_k.astype(np.float64) - want_k) <= cache * np.maximum(np.abs(want_k), 0.1 * np.abs(want_k).max()) + step * np.abs(want_k).max())
+    assert np.array_equal(got_v, want_v.astype(dtype))     # V is stored, rounded once
+    stored = {(slots[s], past[s] + i) for s in range(n) for i in range(lens[s])}
+    for a, b in ((got_k, k0), (got_v, v0)):
+        for slot in range(n_slots):
+            for at in range(kv_max):
+                if (slot, at) not in stored:
+                    assert np.array_equal(a[slot, :, at], b[slot, :, at]), (slot, at)
+    live = np.zeros(rows, bool)
+    live[lead:lead + sum(lens)] = True
+    assert np.array_equal(got_q[~live], q0[~live]) and np.array_equal(got_q[:, nh * hd:], q0[:, nh * hd:])
+
+
+def test_append_leaves_out_what_does_not_fit(tg):
+    """Sequences with a bad slot or length, rows past the RoPE tables."""
+    lib, rng = tg.lib(), np.random.default_rng(0)
+    nh, nkv, hd, rows, kv_max = 4, 2, 64, 6, 10
+    qkv = rng.standard_normal((rows, (nh + 2 * nkv) * hd)).astype(np.float32)
+    cos, sin = _rope_tables(9, hd)
+    k0 = np.full((2, nkv, kv_max, hd), 3.0, np.float32)
+    for lens, slots, left in (([8, 0], [0, 1], [1, 2]), ([0, 0], [0, 7], [3, 4, 5]), ([0, -2], [1, 0], [3, 4, 5]),
+                              ([0, 7], [0, 1], [5])):
+        say(f"append left out: kv_len={lens} slots={slots}")
+        dev = Dev(tg)
+        p, pk, pv, q0 = dev(qkv), dev(k0), dev(k0), np.full((rows, nh * hd), 7.5, np.float32)
+        po, w = dev(q0), qkv.shape[1]
+        lib.tg_hip_kv_append_dev(p, p + 4 * nh * hd, p + 4 * (nh + nkv) * hd, w, w, None, None, 1e-6, dev(cos), dev(sin), 9,
+                                 dev(np.array([0, 3, 6], np.int32)), dev(np.array(lens, np.int32)),
+                                 dev(np.array(slots, np.int32)), 2, rows, 0, 0, pk, pv, 2, kv_max, nh, nkv, hd, po,
+                                 nh * hd, None)
+        lib.tg_hip_synchronize()
+        got, gk = dev.read(po, q0), dev.read(pk, k0)
+        dev.free()
+        same = np.all(got == 7.5, axis=1)
+        # kv_len 8 + 3 rows of 10 positions: the whole sequence is left out
+        want = np.zeros(rows, bool)
+        want[left if lens != [8, 0] else [0, 1, 2]] = True
+        assert np.array_equal(same, want), (same, want)
+        changed = int(np.any(gk != 3.0, axis=(1, 3)).sum())
+        assert changed == rows - int(want.sum())
+
+
+# ---- the calls together, as a program makes them ----
+
+@pytest.mark.parametrize("half", [False, True])
+def test_prompt_then_samples(tg, half):
+    """A prompt appended and attended in two chunks, then as the shared prefix
+    of five samples that append and attend one token each, twice; against the
+    same rows computed in one piece in 64 bits from the rows that were cached."""
+    say(f"prompt then samples half={half}")
+    lib, rng = tg.lib(), np.random.default_rng(77)
+    nh, nkv, hd, n_prompt, kv_max, n = 8, 2, 64, 150, 160, 5
+    width, dtype = (nh + 2 * nkv) * hd, np.float16 if half else np.float32
+    cos, sin = _rope_tables(200, hd)
+    dev = Dev(tg)
+    pc, ps = dev(cos), dev(sin)
+    pre_k, pre_v = (dev(np.zeros((1, nkv, kv_max, hd), dtype)) for _ in range(2))
+    own_k, own_v = (dev(np.zeros((n, nkv, 4, hd), dtype)) for _ in range(2))
+    scratch = dev.room(max(lib.tg_hip_attention_prompt_scratch_bytes(100, n, nh, nkv, hd, kv_max, n_prompt), 1 << 20))
+    scale = hd ** -0.5
+    lib.tg_hip_clear_error()
+
+    def attend(q, k, v, last):
+        z = k @ q * scale
+        p = np.exp(z[:last + 1] - z[:last + 1].max())
+        return (p @ v[:last + 1]) / p.sum()
+
+    def check(got, q, keys, vals, last):
+        for h in range(nh):
+            k, v = keys[h // 4].astype(np.float64), vals[h // 4].astype(np.float64)
+            ref = attend(q[h].astype(np.float64), k, v, last)
+            big = (np.abs(k[:last + 1]) @ np.abs(q[h])).max() * scale
+            off = (8 * np.sqrt(2 * hd) + 4) * EPS * big + (8 * np.sqrt(last + 1) + 24) * EPS
+            assert np.all(np.abs(got[h] - ref) <= 2 * off * np.abs(v).max())
+
+    def step(rows, cu, kv_len, n_seqs, base, caches, slots_max, call):
+        qkv = rng.standard_normal((rows, width)).astype(np.float32)
+        p = dev(qkv)
+        c, l = dev(np.array(cu, np.int32)), dev(np.array(kv_len, np.int32))
+        out = dev(np.zeros((rows, nh * hd), np.float32))
+        lib.tg_hip_kv_append_dev(p, p + 4 * nh * hd, p + 4 * (nh + nkv) * hd, width, width, None, None, 1e-6, pc, ps, 200,
+                                 c, l, None, n_seqs, rows, base, int(half), *caches, n_seqs, slots_max, nh, nkv, hd, p,
+                                 width, None)
+        front = (p, width, int(half), *caches, n_seqs, slots_max)
+        back = (c, l, None, n_seqs, rows, 0, None, nh, nkv, hd, out, nh * hd, scratch, None)
+        if call == "prefix":
+            lib.tg_hip_attention_prefix_dev(*front, pre_k, pre_v, n_prompt, kv_max, *back)
+        else:
+            lib.tg_hip_attention_prompt_dev(*front, *back)
+        lib.tg_hip_synchronize()
+        assert tg.last_error() == "", tg.last_error()
+        q = dev.read(p, qkv)[:, :nh * hd].reshape(rows, nh, hd)
+        return q, dev.read(out, np.empty((rows, nh, hd), np.float32))
+
+    for first, count in ((0, 90), (90, 60)):
+        q, got = step(count, [0, count], [first], 1, 0, (pre_k, pre_v), kv_max, "prompt")
+        keys, vals = (dev.read(x, np.empty((nkv, kv_max, hd), dtype)) for x in (pre_k, pre_v))
+        for i in range(0, count, 7):
+            check(got[i], q[i], keys, vals, first + i)
+    for t in range(2):
+        q, got = step(n, range(n + 1), [t] * n, n, n_prompt, (own_k, own_v), 4, "prefix")
+        ok, ov = (dev.read(x, np.empty((n, nkv, 4, hd), dtype)) for x in (own_k, own_v))
+        for s in range(n):
+            check(got[s], q[s], np.concatenate([keys[:, :n_prompt], ok[s]], 1), np.concatenate([vals[:, :n_prompt], ov[s]], 1),
+                  n_prompt + t)
+    dev.free()
+
+
+def test_one_row_agrees_with_decode_attention(tg):
+    """tg_hip_attention_dev's row (its own projections, norm and RoPE) and its
+    cache, read back through the packed calls."""
+    import oracle as O
+    from tests.test_gpu_attention import _case, _gpu
+    say("against tg_hip_attention_dev")
+    c = _case(5, 512, 8, 2, 64, (O.FMT_Q4K, O.FMT_Q4K, O.FMT_Q4K, O.FMT_Q4K), 64, 40, norms=True, sinks=True, x_scale=0.3)
+    _, att, kk, vv = _gpu(tg, c, 0)
+    lib, dev = tg.lib(), Dev(tg)
+    w, x = [dev(m) for m in c["w"]], dev(c["x"])
+    scr = dev.room(lib.tg_hip_matmul_scratch_bytes(1, 512))
+    qkv = dev.room(4 * 12 * 64)
+    for i, (at, rows) in enumerate(((0, 512), (512, 128), (640, 128))):
+        lib.tg_hip_matmul_dev(c["fmts"][i], w[i], None, x, qkv + 4 * at, rows, 512, 1, scr, None)
+    pk, pv, cu, past = dev(c["kv_k"]), dev(c["kv_v"]), dev(np.array([0, 1], np.int32)), dev(np.array([40], np.int32))
+    lib.tg_hip_kv_append_dev(qkv, qkv + 4 * 512, qkv + 4 * 640, 768, 768, dev(c["qn"]), dev(c["kn"]), ctypes.c_float(1e-6),
+                             dev(c["rc"]), dev(c["rs"]), 64, cu, past, None, 1, 1, 0, 0, pk, pv, 1, 64, 8, 2, 64, qkv, 768,
+                             None)
+    out = dev.room(4 * 512)
+    scratch = dev.room(lib.tg_hip_attention_prompt_scratch_bytes(1, 1, 8, 2, 64, 64, 0))
+    lib.tg_hip_attention_prompt_dev(qkv, 768, 0, pk, pv, 1, 64, cu, past, None, 1, 1, 0, dev(c["sinks"]), 8, 2, 64, out, 512,
+                                    scratch, None)
+    lib.tg_hip_synchronize()
+    assert tg.last_error() == "", tg.last_error()
+    got = dev.read(out, np.empty(512, np.float32))
+    # the same f32 formulas in another order: tests/test_gpu_attention.py's bars
+    assert np.abs(dev.read(pk, kk) - kk).max() <= 2e-5 * np.abs(kk).max()
+    assert np.abs(dev.read(pv, vv) - vv).max() <= 2e-5 * np.abs(vv).max()
+    assert np.abs(got - att).max() <= 1e-4 * np.abs(att).max()
+    dev.free()

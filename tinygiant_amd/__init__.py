@@ -17,6 +17,7 @@ from ._lib import find_library, load_tinygiant_lib  # noqa: F401
 FMT_Q4K, FMT_F16, FMT_Q6K, FMT_MXFP4, FMT_Q80 = 0, 1, 2, 3, 4
 FMT_NAMES = {"q4_k": 0, "float16": 1, "q6_k": 2, "mxfp4": 3, "q8_0": 4}   # tinygiant/engine.py:21
 ACT_SILU, ACT_GPTOSS = 0, 1
+KV_F32, KV_F16 = 0, 1   # element type of a KV cache (tg_hip_kv_append_dev, tg_hip_attention_prompt_dev)
 Q8_DTYPE = np.dtype([("scale", "<f4"), ("sum", "<i4"), ("bsums", "<i4", (8,)), ("qs", "i1", (256,))])
 
 _LIB = None

@@ -103,6 +103,15 @@ def register_extensions(lib):
     _reg(lib.tg_hip_attention_dev, [CI, CI, CI, CI, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, CI, CI, CI,
                                     VP, VP, VP, VP, CI, CI, CI, CI, CI, CF, VP, VP, VP])
     _reg(lib.tg_hip_attention_scratch_bytes, [CI, CI, CI, CI, CI], SZ)
+    _reg(lib.tg_hip_kv_append_dev, [VP, VP, VP, CI, CI, VP, VP, CF, VP, VP, CI, VP, VP, VP, CI, CI, CI, CI, VP, VP,
+                                    CI, CI, CI, CI, CI, VP, CI, VP])
+    _reg(lib.tg_hip_attention_prompt_scratch_bytes, [CI, CI, CI, CI, CI, CI, CI], SZ)
+    _reg(lib.tg_hip_attention_prompt_dev, [VP, CI, CI, VP, VP, CI, CI, VP, VP, VP, CI, CI, CI, VP, CI, CI, CI, VP, CI,
+                                           VP, VP])
+    _reg(lib.tg_hip_attention_prefix_dev, [VP, CI, CI, VP, VP, CI, CI, VP, VP, CI, CI, VP, VP, VP, CI, CI, CI, VP, CI,
+                                           CI, CI, VP, CI, VP, VP])
+    _reg(lib.tg_hip_logits_scratch_bytes, [CI, CI], SZ)
+    _reg(lib.tg_hip_logits_adjust_dev, [VP, VP, CI, CI, VP, CI, VP, VP, VP, VP, VP, CI, VP, VP, CI, VP, VP, VP, VP])
     _reg(lib.tg_hip_upload_file, [ctypes.c_char_p, ctypes.c_uint64, ctypes.c_uint64, VP, ctypes.c_uint64],
          ctypes.c_int64)
     _reg(lib.tg_hip_mark, [CI])

@@ -37,6 +37,8 @@
 #include "tg_attn.h"
 #include "tg_route.h"
 #include "tg_kernels.h"
+#include "tg_logits.h"
+#include "tg_prompt.h"
 #include "tg_synth.h"
 
 #define TG_API extern "C" __attribute__((visibility("default")))
@@ -1430,6 +1432,220 @@ TG_API void tg_attention_v2(int fmt_q, int fmt_k, int fmt_v, int fmt_o, const vo
     }
     HIPCHECK(hipMemcpyAsync(output, dev + io_out, (size_t)embed_dim * 4, hipMemcpyDeviceToHost, g.st));
     HIPCHECK(hipStreamSynchronize(g.st));
+}
+
+/* ---- packed rows of several sequences: cache append, attention ---- */
+static bool packed_validate(const char *who, const int32_t *cu_rows, int n_seqs, int n_rows, int kv_type,
+                            const void *kv_k, const void *kv_v, int n_slots, int kv_max, int n_heads, int n_kv,
+                            int head_dim) {
+    if (kv_type != TG_KV_F32 && kv_type != TG_KV_F16) {
+        set_err("%s: kv_type must be 0 (float32) or 1 (float16)", who);
+        return false;
+    }
+    if (n_seqs < 0 || n_seqs > PROMPT_MAX_SEQS || n_rows < 0 || n_rows > PROMPT_MAX_ROWS || n_slots <= 0 || kv_max <= 0 ||
+        kv_max > PROMPT_MAX_KV) {
+        set_err("%s: need 0 <= n_seqs <= %d, 0 <= n_rows <= %d, n_slots >= 1, 1 <= kv_max <= %d", who, PROMPT_MAX_SEQS,
+                PROMPT_MAX_ROWS, PROMPT_MAX_KV);
+        return false;
+    }
+    if (n_heads <= 0 || n_heads > 1024 || n_kv <= 0 || n_heads % n_kv || n_heads / n_kv > PROMPT_MAX_GQA || head_dim <= 0 ||
+        head_dim % 8 || head_dim > PROMPT_MAX_HEAD_DIM) {
+        set_err("%s: unsupported shape (head_dim %% 8 == 0 and <= %d, n_heads <= 1024, n_heads / n_kv_heads integral and "
+                "<= %d)", who, PROMPT_MAX_HEAD_DIM, PROMPT_MAX_GQA);
+        return false;
+    }
+    if (n_seqs && n_rows && (!cu_rows || !kv_k || !kv_v)) {
+        set_err("%s: null cu_rows or cache pointer", who);
+        return false;
+    }
+    if (((uintptr_t)kv_k | (uintptr_t)kv_v) & 15) {
+        set_err("%s: kv_k and kv_v must be 16-byte aligned", who);
+        return false;
+    }
+    return true;
+}
+
+/* a launch that HIP refuses is reported, the outputs are as they were */
+static void check_launch(const char *who) {
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) set_err("%s: launch failed (%s)", who, hipGetErrorString(e));
+}
+
+static PackedSeqs packed_seqs(const int32_t *cu_rows, const int32_t *kv_len, const int32_t *slots, int n_seqs, int n_rows,
+                              int n_slots, int kv_max) {
+    return PackedSeqs{cu_rows, kv_len, slots, n_seqs, n_rows, n_slots, kv_max};
+}
+
+TG_API void tg_hip_kv_append_dev(const float *q_dev, const float *k_dev, const float *v_dev, int q_stride, int kv_stride,
+                                 const float *q_norm_w_dev, const float *k_norm_w_dev, float eps,
+                                 const float *rope_cos_dev, const float *rope_sin_dev, int rope_len,
+                                 const int32_t *cu_rows_dev, const int32_t *kv_len_dev, const int32_t *slots_dev,
+                                 int n_seqs, int n_rows, int base_pos, int kv_type, void *kv_k_dev, void *kv_v_dev,
+                                 int n_slots, int kv_max, int n_heads, int n_kv_heads, int head_dim, float *q_out_dev,
+                                 int q_out_stride, void *stream) {
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    static const char who[] = "tg_hip_kv_append_dev";
+    if (!packed_validate(who, cu_rows_dev, n_seqs, n_rows, kv_type, kv_k_dev, kv_v_dev, n_slots, kv_max, n_heads,
+                         n_kv_heads, head_dim))
+        return;
+    if (q_out_dev ? !q_dev || q_stride < n_heads * head_dim || q_out_stride < n_heads * head_dim : false) {
+        set_err("%s: q_out without q, or a stride below n_heads * head_dim", who);
+        return;
+    }
+    if (q_out_dev && q_out_dev == q_dev && q_out_stride != q_stride) {
+        set_err("%s: q_out over q needs the same stride", who);
+        return;
+    }
+    if (kv_stride < n_kv_heads * head_dim || base_pos < 0 || (!rope_cos_dev) != (!rope_sin_dev) ||
+        (rope_cos_dev && rope_len <= 0) || base_pos > (1 << 30)) {
+        set_err("%s: need kv_stride >= n_kv_heads * head_dim, base_pos in 0..2^30, both RoPE tables with rope_len >= 1 or "
+                "neither", who);
+        return;
+    }
+    if (!n_seqs || !n_rows) return;
+    if (!k_dev || !v_dev) {
+        set_err("%s: null k or v", who);
+        return;
+    }
+    if (((uintptr_t)q_dev | (uintptr_t)k_dev | (uintptr_t)v_dev | (uintptr_t)q_out_dev) & 3) {
+        set_err("%s: rows must be 4-byte aligned", who);
+        return;
+    }
+    ensure_init();
+    AppendArgs a = {};
+    a.q = q_dev, a.k = k_dev, a.v = v_dev;
+    a.q_stride = q_stride, a.kv_stride = kv_stride;
+    a.q_norm = q_norm_w_dev, a.k_norm = k_norm_w_dev, a.eps = eps;
+    a.rope_cos = rope_cos_dev, a.rope_sin = rope_sin_dev, a.rope_len = rope_len, a.base_pos = base_pos;
+    a.s = packed_seqs(cu_rows_dev, kv_len_dev, slots_dev, n_seqs, n_rows, n_slots, kv_max);
+    a.kv_k = kv_k_dev, a.kv_v = kv_v_dev;
+    a.n_heads = n_heads, a.n_kv = n_kv_heads, a.head_dim = head_dim;
+    a.q_out = q_out_dev, a.q_out_stride = q_out_stride;
+    launch_kv_append(a, kv_type == TG_KV_F16, stream ? (hipStream_t)stream : g.st);
+    check_launch(who);
+}
+
+TG_API size_t tg_hip_attention_prompt_scratch_bytes(int n_rows, int n_seqs, int n_heads, int n_kv_heads, int head_dim,
+                                                    int kv_max, int prefix_len) {
+    if (n_rows <= 0 || n_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || head_dim <= 0 ||
+        head_dim > PROMPT_MAX_HEAD_DIM || kv_max <= 0 || prefix_len < 0)
+        return 0;
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    return attention_rows_scratch(n_rows, n_seqs, n_heads, n_kv_heads, head_dim, kv_max, prefix_len);
+}
+
+static void attention_rows(const char *who, const float *q_dev, int q_stride, int kv_type, const void *kv_k_dev,
+                           const void *kv_v_dev, int n_slots, int kv_max, const void *prefix_k_dev,
+                           const void *prefix_v_dev, int prefix_len, int prefix_max, const int32_t *cu_rows_dev,
+                           const int32_t *kv_len_dev, const int32_t *slots_dev, int n_seqs, int n_rows, int window,
+                           const float *sinks_dev, int n_heads, int n_kv_heads, int head_dim, float *out_dev,
+                           int out_stride, void *scratch_dev, void *stream) {
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    if (!packed_validate(who, cu_rows_dev, n_seqs, n_rows, kv_type, kv_k_dev, kv_v_dev, n_slots, kv_max, n_heads,
+                         n_kv_heads, head_dim))
+        return;
+    if (prefix_len < 0 || prefix_len > prefix_max || prefix_max > PROMPT_MAX_KV ||
+        (prefix_len && (!prefix_k_dev || !prefix_v_dev || (((uintptr_t)prefix_k_dev | (uintptr_t)prefix_v_dev) & 15)))) {
+        set_err("%s: need 0 <= prefix_len <= prefix_max <= %d and 16-byte aligned prefix_k and prefix_v", who,
+                PROMPT_MAX_KV);
+        return;
+    }
+    if (window < 0 || q_stride < n_heads * head_dim || out_stride < n_heads * head_dim) {
+        set_err("%s: need window >= 0 and strides of at least n_heads * head_dim", who);
+        return;
+    }
+    if (!n_seqs || !n_rows) return;
+    if (!q_dev || !out_dev || (((uintptr_t)q_dev | (uintptr_t)out_dev) & 3)) {
+        set_err("%s: null or not 4-byte aligned q or out", who);
+        return;
+    }
+    if (q_dev == out_dev && q_stride != out_stride) {
+        set_err("%s: out over q needs the same stride", who);
+        return;
+    }
+    ensure_init();
+    const size_t need = attention_rows_scratch(n_rows, n_seqs, n_heads, n_kv_heads, head_dim, kv_max, prefix_len);
+    if (need && (!scratch_dev || ((uintptr_t)scratch_dev & 15))) {
+        set_err("%s: needs %zu bytes of 16-byte aligned scratch", who, need);
+        return;
+    }
+    PromptArgs a = {};
+    a.q = q_dev, a.q_stride = q_stride;
+    a.kv_k = kv_k_dev, a.kv_v = kv_v_dev;
+    a.pre_k = prefix_k_dev, a.pre_v = prefix_v_dev, a.pre_len = prefix_len, a.pre_max = prefix_max;
+    a.s = packed_seqs(cu_rows_dev, kv_len_dev, slots_dev, n_seqs, n_rows, n_slots, kv_max);
+    a.window = window, a.sinks = sinks_dev;
+    a.n_heads = n_heads, a.n_kv = n_kv_heads, a.head_dim = head_dim;
+    a.out = out_dev, a.out_stride = out_stride;
+    launch_attention_rows(a, kv_type == TG_KV_F16, scratch_dev, stream ? (hipStream_t)stream : g.st);
+    check_launch(who);
+}
+
+TG_API void tg_hip_attention_prompt_dev(const float *q_dev, int q_stride, int kv_type, const void *kv_k_dev,
+                                        const void *kv_v_dev, int n_slots, int kv_max, const int32_t *cu_rows_dev,
+                                        const int32_t *kv_len_dev, const int32_t *slots_dev, int n_seqs, int n_rows,
+                                        int window, const float *sinks_dev, int n_heads, int n_kv_heads, int head_dim,
+                                        float *out_dev, int out_stride, void *scratch_dev, void *stream) {
+    attention_rows("tg_hip_attention_prompt_dev", q_dev, q_stride, kv_type, kv_k_dev, kv_v_dev, n_slots, kv_max, nullptr,
+                   nullptr, 0, 0, cu_rows_dev, kv_len_dev, slots_dev, n_seqs, n_rows, window, sinks_dev, n_heads,
+                   n_kv_heads, head_dim, out_dev, out_stride, scratch_dev, stream);
+}
+
+TG_API void tg_hip_attention_prefix_dev(const float *q_dev, int q_stride, int kv_type, const void *kv_k_dev,
+                                        const void *kv_v_dev, int n_slots, int kv_max, const void *prefix_k_dev,
+                                        const void *prefix_v_dev, int prefix_len, int prefix_max,
+                                        const int32_t *cu_rows_dev, const int32_t *kv_len_dev, const int32_t *slots_dev,
+                                        int n_seqs, int n_rows, int window, const float *sinks_dev, int n_heads,
+                                        int n_kv_heads, int head_dim, float *out_dev, int out_stride, void *scratch_dev,
+                                        void *stream) {
+    attention_rows("tg_hip_attention_prefix_dev", q_dev, q_stride, kv_type, kv_k_dev, kv_v_dev, n_slots, kv_max,
+                   prefix_k_dev, prefix_v_dev, prefix_len, prefix_max, cu_rows_dev, kv_len_dev, slots_dev, n_seqs, n_rows,
+                   window, sinks_dev, n_heads, n_kv_heads, head_dim, out_dev, out_stride, scratch_dev, stream);
+}
+
+/* ---- logits: penalties, biases, a grammar's mask ---- */
+TG_API size_t tg_hip_logits_scratch_bytes(int k, int nrows) {
+    if (k <= 0 || k > LOGITS_MAX_ROWS || nrows <= 0 || nrows > LOGITS_MAX_VOCAB) return 0;
+    return logits_scratch(k, nrows);
+}
+
+TG_API void tg_hip_logits_adjust_dev(const float *logits_dev, float *out_dev, int k, int nrows, const int32_t *hist_dev,
+                                     int hist_stride, const int32_t *hist_len_dev, const int32_t *gen_start_dev,
+                                     const float *penalties_dev, const int32_t *bias_tok_dev, const float *bias_val_dev,
+                                     int bias_stride, const int32_t *bias_len_dev, const uint32_t *allow_dev,
+                                     int allow_stride, int32_t *argmax_dev, float *maxval_dev, void *scratch_dev,
+                                     void *stream) {
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    static const char who[] = "tg_hip_logits_adjust_dev";
+    if (k < 0 || k > LOGITS_MAX_ROWS || nrows <= 0 || nrows > LOGITS_MAX_VOCAB || hist_stride < 0 ||
+        hist_stride >= (1 << 30) || bias_stride < 0) {
+        set_err("%s: need 0 <= k <= %d, 1 <= nrows <= %d, strides >= 0", who, LOGITS_MAX_ROWS, LOGITS_MAX_VOCAB);
+        return;
+    }
+    if (!k) return;
+    if (!logits_dev || (!out_dev && !argmax_dev && !maxval_dev) || ((argmax_dev || maxval_dev) && !scratch_dev) ||
+        ((uintptr_t)scratch_dev & 7)) {
+        set_err("%s: null logits, no output, or no 8-byte aligned scratch for the argmax", who);
+        return;
+    }
+    if (hist_dev && (!hist_len_dev || !penalties_dev)) {
+        set_err("%s: a history needs hist_len and penalties", who);
+        return;
+    }
+    if ((!bias_tok_dev) != (!bias_val_dev)) {
+        set_err("%s: bias_tok and bias_val belong together", who);
+        return;
+    }
+    if (allow_dev && allow_stride && allow_stride < (nrows + 31) / 32) {
+        set_err("%s: allow_stride holds %d words, a row needs %d (0: one row for all)", who, allow_stride, (nrows + 31) / 32);
+        return;
+    }
+    ensure_init();
+    const LogitsArgs a = {logits_dev, out_dev, k, nrows, hist_dev, hist_stride, hist_len_dev, gen_start_dev, penalties_dev,
+                          bias_tok_dev, bias_val_dev, bias_stride, bias_len_dev, allow_dev, allow_stride, argmax_dev,
+                          maxval_dev};
+    launch_logits_adjust(a, scratch_dev, stream ? (hipStream_t)stream : g.st);
+    check_launch(who);
 }
 
 /* ---- file -> HBM upload (the expert-cache loader's native part) ----

@@ -1,0 +1,165 @@
+/*
+ * tg_logits.hip -- penalties for repeated tokens, biases and a grammar's mask
+ * on rows of logits, with the argmax of the result.
+ *
+ *   l = l > 0 ? l / r : l r          tokens in the row's history
+ *   l = l - f c - p                  tokens generated c > 0 times
+ *   l = l + b                        tokens with a bias
+ *   l = -inf                         tokens whose bit is 0
+ *
+ * each step one correctly rounded f32 operation (products, differences and
+ * quotients are not contracted), so the results are the formulas' bits.
+ *
+ * A workgroup takes SLICE tokens of one row.  It scans the row's whole
+ * history and bias list and counts those that fall into its slice in LDS
+ * (integer atomics: the order does not matter), so no table of the
+ * vocabulary's size is cleared, written and read in memory; a history is at
+ * most some ten KB, which the slices of a row read from L2.  Then one pass
+ * over the slice's logits.  The largest value's key goes to the slice's word
+ * of the scratch; k_logits_pick takes the row's best.
+ */
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "tg_device.hpp"
+#include "tg_logits.h"
+
+namespace tg {
+
+namespace {
+
+constexpr int SLICE = 2048;
+constexpr int LT = 256;
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+
+/* Order of the values as unsigned words: -0 ties with +0, a NaN of either
+ * sign is the largest (numpy.argmax's rules), the lower index wins ties. */
+__device__ inline uint64_t pick_key(float v, uint32_t row) {
+    uint32_t u = v == 0.f ? 0u : __float_as_uint(v);
+    u = v != v ? 0x7FC00000u : u;
+    u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    return ((uint64_t)u << 32) | (uint64_t)(0xFFFFFFFFu - row);
+}
+constexpr uint32_t KEY_NEG_INF = ~0xFF800000u;
+
+__device__ inline uint64_t wave_max_key(uint64_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint32_t hi = (uint32_t)__shfl_xor((int)(uint32_t)(v >> 32), o, 64);
+        const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)v, o, 64);
+        const uint64_t w = ((uint64_t)hi << 32) | lo;
+        v = w > v ? w : v;
+    }
+    return v;
+}
+
+}  // namespace
+
+__global__ __launch_bounds__(LT) void k_logits_adjust(LogitsArgs a, int nslices, uint64_t *best) {
+#pragma clang fp contract(off)
+    __shared__ int cnt[SLICE];    /* times generated; bit 30: in the history's first part */
+    __shared__ int last[SLICE];   /* 1 + the place of the token's last bias entry */
+    __shared__ uint64_t red[LT / 64];
+    const int j = blockIdx.y, t0 = blockIdx.x * SLICE, tid = threadIdx.x;
+    const int n = min(SLICE, a.nrows - t0);
+    const int hl = a.hist ? min(max(a.hist_len[j], 0), a.hist_stride) : 0;
+    const int bl = a.bias_tok ? min(a.bias_len ? max(a.bias_len[j], 0) : a.bias_stride, a.bias_stride) : 0;
+    if (hl) {
+        for (int i = tid; i < SLICE; i += LT) cnt[i] = 0;
+    }
+    if (bl) {
+        for (int i = tid; i < SLICE; i += LT) last[i] = 0;
+    }
+    __syncthreads();
+    if (hl) {
+        const int gs = a.gen_start ? a.gen_start[j] : 0;
+        const int32_t *h = a.hist + (size_t)j * a.hist_stride;
+        for (int i = tid; i < hl; i += LT) {
+            const uint32_t t = (uint32_t)h[i] - (uint32_t)t0;
+            if (t < (uint32_t)n) {
+                if (i >= gs) atomicAdd(&cnt[t], 1);
+                else atomicOr(&cnt[t], 1 << 30);
+            }
+        }
+    }
+    if (bl) {
+        const int32_t *bt = a.bias_tok + (size_t)j * a.bias_stride;
+        for (int i = tid; i < bl; i += LT) {
+            const uint32_t t = (uint32_t)bt[i] - (uint32_t)t0;
+            if (t < (uint32_t)n) atomicMax(&last[t], i + 1);
+        }
+    }
+    __syncthreads();
+    const float rep = hl ? a.pen[3 * j] : 1.f, freq = hl ? a.pen[3 * j + 1] : 0.f, pres = hl ? a.pen[3 * j + 2] : 0.f;
+    const float *bv = a.bias_val + (size_t)j * a.bias_stride;
+    const uint32_t *al = a.allow ? a.allow + (size_t)j * a.allow_stride : nullptr;
+    const float *src = a.logits + (size_t)j * a.nrows + t0;
+    float *dst = a.out ? a.out + (size_t)j * a.nrows + t0 : nullptr;
+    uint64_t mine = 0;
+    for (int i = 4 * tid; i < n; i += 4 * LT) {
+        f4 v;
+        if (i + 4 <= n) v = *(const f4u *)(src + i);
+        else
+            for (int e = 0; e < 4; e++) v[e] = i + e < n ? src[i + e] : 0.f;
+        const uint32_t bits = al ? al[(uint32_t)(t0 + i) >> 5] >> ((t0 + i) & 31) : 15u;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            float x = v[e];
+            const int c = hl ? cnt[i + e] : 0;
+            if (c) {
+                x = x > 0.f ? x / rep : x * rep;
+                const int g = c & ((1 << 30) - 1);
+                if (g) x = x - freq * (float)g - pres;
+            }
+            const int b = bl ? last[i + e] : 0;
+            if (b) x = x + bv[b - 1];
+            if (!((bits >> e) & 1u)) x = -INFINITY;
+            v[e] = x;
+            const uint64_t key = pick_key(x, (uint32_t)(t0 + i + e));
+            if (i + e < n) mine = key > mine ? key : mine;
+        }
+        if (dst) {
+            if (i + 4 <= n) *(f4u *)(dst + i) = v;
+            else
+                for (int e = 0; e < 4; e++)
+                    if (i + e < n) dst[i + e] = v[e];
+        }
+    }
+    if (!best) return;
+    mine = wave_max_key(mine);
+    if ((tid & 63) == 0) red[tid >> 6] = mine;
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+        for (int w = 1; w < LT / 64; w++) mine = red[w] > mine ? red[w] : mine;
+        best[(size_t)j * nslices + blockIdx.x] = mine;
+    }
+}
+
+/* one wave a row: the best of its slices; -1 where nothing is above -inf */
+__global__ __launch_bounds__(64) void k_logits_pick(const uint64_t *best, int nslices, int32_t *argmax, float *maxval) {
+    const int j = blockIdx.x;
+    uint64_t m = 0;
+    for (int i = threadIdx.x; i < nslices; i += 64) {
+        const uint64_t k = best[(size_t)j * nslices + i];
+        m = k > m ? k : m;
+    }
+    m = wave_max_key(m);
+    if (threadIdx.x) return;
+    const uint32_t u = (uint32_t)(m >> 32);
+    if (argmax) argmax[j] = u <= KEY_NEG_INF ? -1 : (int32_t)(0xFFFFFFFFu - (uint32_t)m);
+    if (maxval) maxval[j] = __uint_as_float((u & 0x80000000u) ? (u & 0x7FFFFFFFu) : ~u);
+}
+
+size_t logits_scratch(int k, int nrows) { return (size_t)k * ((nrows + SLICE - 1) / SLICE) * 8; }
+
+void launch_logits_adjust(const LogitsArgs &a, void *scratch, hipStream_t st) {
+    const int nslices = (a.nrows + SLICE - 1) / SLICE;
+    uint64_t *best = a.argmax || a.maxval ? (uint64_t *)scratch : nullptr;
+    hipLaunchKernelGGL(k_logits_adjust, dim3(nslices, a.k), dim3(LT), 0, st, a, nslices, best);
+    if (best) hipLaunchKernelGGL(k_logits_pick, dim3(a.k), dim3(64), 0, st, best, nslices, a.argmax, a.maxval);
+}
+
+}  // namespace tg
