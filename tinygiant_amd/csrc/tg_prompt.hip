@@ -14,6 +14,7 @@
 
 #include "tg_device.hpp"
 #include "tg_prompt.h"
+#include "tg_xchg.hpp"
 
 namespace tg {
 
@@ -141,34 +142,169 @@ void launch_kv_append(const AppendArgs &a, bool half, hipStream_t st) {
 }
 
 /* ---- attention ----
- * One workgroup per (row, query head): 256 keys at a time, a thread a key's
- * score, then a thread an output value's sum; running maximum and sum. */
+ *
+ * Row i of a sequence and query head kh * ratio + j, of KV head kh, is "m-row"
+ * i * ratio + j: all query heads of a KV head read the same K and V, so they
+ * fill the matrix units' columns together, and any ratio and row count packs.
+ *
+ * A region is a run of cached positions with one base: a sequence's slot, or
+ * the shared prefix.  A workgroup takes MT m-rows of one KV head and a span of
+ * a region.  Where one workgroup covers all that its rows see, it writes the
+ * output; else it writes a record (reference exponent m, sum l, unnormalised
+ * o[head_dim]) a row and k_rows_combine merges the records.  Exponents are in
+ * base 2: weight 2^(z - m), z = score * log2 e. */
+struct RowsPlan {
+    int tiles, ns;          /* upper bound of the own-slot tiles, spans a tile */
+    int pre_tiles, pre_ns;  /* the same of the prefix */
+    int nrec;               /* records a row: pre_ns + ns; 0: written directly */
+    float *ml, *o;          /* [n_rows * n_heads][nrec][2], [..][nrec][head_dim] */
+};
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int MT = 128;   /* m-rows of a workgroup: 32 a wave */
+constexpr int KT = 64;    /* positions of a tile */
+
+/* what a workgroup works on, uniform over it */
+struct Work {
+    int kh, split, ns, rec;
+    bool prefix;
+    Seq sq;          /* own: the sequence; prefix: all rows of the call as one */
+    int m0;          /* the tile's first m-row */
+    int lo, hi;      /* positions of the region */
+};
+
+/* Tile t of all sequences' tiles of MTILE m-rows, late rows first (they see
+ * the most positions): a wave counts 64 sequences at a time. */
+template <int MTILE>
+__device__ inline bool find_tile(const PackedSeqs &p, int ratio, int t, Seq &sq, int &m0) {
+    const int lane = threadIdx.x & 63;
+    for (int s0 = 0; s0 < p.n; s0 += 64) {
+        const int s = s0 + lane;
+        Seq q = {0, 0, 0, 0};
+        if (s < p.n) q = seq_at(p, s);
+        const int n = (int)(((unsigned)q.n * (unsigned)ratio + MTILE - 1) / MTILE);
+        int end = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(end, o, 64);
+            if (lane >= o) end += v;
+        }
+        const uint64_t past = __ballot(end > t);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            sq.r0 = __builtin_amdgcn_readlane(q.r0, at);
+            sq.n = __builtin_amdgcn_readlane(q.n, at);
+            sq.past = __builtin_amdgcn_readlane(q.past, at);
+            sq.slot = __builtin_amdgcn_readlane(q.slot, at);
+            m0 = (__builtin_amdgcn_readlane(end, at) - 1 - t) * MTILE;
+            return true;
+        }
+        t -= __builtin_amdgcn_readlane(end, 63);
+    }
+    return false;
+}
+
+/* positions of the region that m-row m of the work sees: first .. last;
+ * false: no row there */
+__device__ inline bool row_sees(const PromptArgs &a, const Work &w, int m, int ratio, int &first, int &last) {
+    int i = m / ratio;
+    if (i >= w.sq.n) return false;
+    first = 0;
+    if (w.prefix) {
+        last = a.pre_len - 1;
+        if (a.window > 0) {
+            const int r = w.sq.r0 + i, s = seq_of(a.s, r);
+            if (s < 0) return false;
+            const Seq q = seq_at(a.s, s);
+            i = r - q.r0;
+            if (i < 0 || i >= q.n) return false;
+            first = max(0, a.pre_len + q.past + i + 1 - a.window);
+        }
+    } else {
+        last = w.sq.past + i;
+        if (a.window > 0) first = max(0, last + 1 - a.window);
+    }
+    return true;
+}
+
+/* This workgroup's work: block b of the prefix's, then of the sequences'
+ * items; KV heads fastest, so that (8 XCDs, workgroups dealt in turn) those
+ * of one head meet in as few L2 caches as possible.  False: none. */
+template <int MTILE>
+__device__ inline bool find_work(const PromptArgs &a, const RowsPlan &p, int ratio, Work &w) {
+    int b = blockIdx.x;
+    const int npre = p.pre_tiles * p.pre_ns * a.n_kv;
+    w.prefix = b < npre;
+    if (!w.prefix) b -= npre;
+    w.kh = b % a.n_kv;
+    b /= a.n_kv;
+    const int tiles = w.prefix ? p.pre_tiles : p.tiles;
+    const int t = b % tiles;
+    w.split = b / tiles;
+    w.ns = w.prefix ? p.pre_ns : p.ns;
+    w.rec = w.prefix ? w.split : p.pre_ns + w.split;
+    int lo, hi;
+    if (w.prefix) {
+        const int r0 = min(max(a.s.cu[0], 0), a.s.rows), r1 = min(max(a.s.cu[a.s.n], r0), a.s.rows);
+        w.sq = Seq{r0, r1 - r0, 0, 0};
+        w.m0 = t * MTILE;
+        if ((unsigned)w.m0 >= (unsigned)w.sq.n * (unsigned)ratio) return false;
+        lo = 0, hi = a.pre_len;
+        if (a.window > 0) {   /* the first position that any of the rows sees */
+            lo = hi;
+            for (int m = w.m0 + (int)(threadIdx.x & 63); m < w.m0 + MTILE; m += 64) {
+                int f, l;
+                if (row_sees(a, w, m, ratio, f, l)) lo = min(lo, f);
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) lo = min(lo, __shfl_xor(lo, o, 64));
+        }
+    } else {
+        if (!find_tile<MTILE>(a.s, ratio, t, w.sq, w.m0)) return false;
+        const int i0 = w.m0 / ratio, i1 = min(w.sq.n - 1, (w.m0 + MTILE - 1) / ratio);
+        lo = a.window > 0 ? max(0, w.sq.past + i0 + 1 - a.window) : 0;
+        hi = w.sq.past + i1 + 1;
+    }
+    /* this span, in whole tiles counted from the first one's */
+    lo = lo / KT * KT;
+    const int per = max(1, ((hi - lo + KT - 1) / KT + w.ns - 1) / w.ns) * KT;
+    w.lo = __builtin_amdgcn_readfirstlane(min(hi, lo + w.split * per));
+    w.hi = __builtin_amdgcn_readfirstlane(min(hi, w.lo + per));
+    return true;
+}
+
 template <typename T>
-__global__ __launch_bounds__(256) void k_attn_row(PromptArgs a) {
-    __shared__ float qs[PROMPT_MAX_HEAD_DIM];
-    __shared__ float sc[256];
-    __shared__ float red[4];
-    const int r = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, hd = a.head_dim;
-    const int s = seq_of(a.s, r);
-    if (s < 0) return;
-    const Seq sq = seq_at(a.s, s);
-    const int i = r - sq.r0;
-    if (i < 0 || i >= sq.n) return;
-    const int kh = h / (a.n_heads / a.n_kv);
-    const int pos = a.pre_len + sq.past + i;           /* the last position that the row sees */
-    const int first = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
-    if (tid < hd) qs[tid] = a.q[(size_t)r * a.q_stride + (size_t)h * hd + tid];
-    const T *pk = (const T *)a.pre_k + (size_t)kh * a.pre_max * hd, *pv = (const T *)a.pre_v + (size_t)kh * a.pre_max * hd;
-    const size_t own = ((size_t)sq.slot * a.n_kv + kh) * a.s.kv_max * hd;
-    const T *ok = (const T *)a.kv_k + own, *ov = (const T *)a.kv_v + own;
-    const float scale = 1.f / sqrtf((float)hd);
-    float m = -INFINITY, l = 0.f, o = 0.f;
+__device__ inline const T *region(const PromptArgs &a, const Work &w, const void *own, const void *pre) {
+    return w.prefix ? (const T *)pre + (size_t)w.kh * a.pre_max * a.head_dim
+                    : (const T *)own + ((size_t)w.sq.slot * a.n_kv + w.kh) * a.s.kv_max * a.head_dim;
+}
+
+/* One m-row over the work's span by the whole workgroup, from the formulas
+ * with plain loads: only positions that the row sees are read.  It is how
+ * rows are computed that came out of the matrix units not finite, which
+ * multiply every value of a tile: 0 * inf there is not a row's own result.
+ * lds: PROMPT_MAX_HEAD_DIM + 260 floats. */
+template <typename T>
+__device__ void slow_row(const PromptArgs &a, const RowsPlan &p, const Work &w, int m, int ratio, float *lds) {
+    float *qs = lds, *sc = lds + PROMPT_MAX_HEAD_DIM, *red = sc + 256;
+    const int tid = threadIdx.x, hd = a.head_dim;
+    const int i = m / ratio, h = w.kh * ratio + (m - i * ratio), r = w.sq.r0 + i;
+    int first = 0, last = -1;
+    (void)row_sees(a, w, m, ratio, first, last);
+    first = max(first, w.lo), last = min(last, w.hi - 1);
+    const T *k = region<T>(a, w, a.kv_k, a.pre_k), *v = region<T>(a, w, a.kv_v, a.pre_v);
+    const float scale = LOG2E / sqrtf((float)hd);
     __syncthreads();
-    for (int t0 = first; t0 <= pos; t0 += 256) {
-        const int p = t0 + tid;
+    if (tid < hd) qs[tid] = a.q[(size_t)r * a.q_stride + (size_t)h * hd + tid];
+    float mx = -INFINITY, l = 0.f, o = 0.f;
+    __syncthreads();
+    for (int t0 = first; t0 <= last; t0 += 256) {
+        const int pz = t0 + tid;
         float z = -INFINITY;
-        if (p <= pos) {
-            const T *row = p < a.pre_len ? pk + (size_t)p * hd : ok + (size_t)(p - a.pre_len) * hd;
+        if (pz <= last) {
+            const T *row = k + (size_t)pz * hd;
             float acc = 0.f;
             for (int d = 0; d < hd; d++) acc = fmaf(qs[d], (float)row[d], acc);
             z = acc * scale;
@@ -177,45 +313,630 @@ __global__ __launch_bounds__(256) void k_attn_row(PromptArgs a) {
         if ((tid & 63) == 0) red[tid >> 6] = t;
         __syncthreads();
         t = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const float mn = fmaxf(m, t), base = mn == -INFINITY ? 0.f : mn, alpha = expf(m - base);
-        const float e = p <= pos ? expf(z - base) : 0.f;
+        const float mn = fmaxf(mx, t), base = mn == -INFINITY ? 0.f : mn, alpha = exp2f(mx - base);
+        const float e = pz <= last ? exp2f(z - base) : 0.f;
         sc[tid] = e;
-        const float w = wave_sum(e);
+        const float s = wave_sum(e);
         __syncthreads();
-        if ((tid & 63) == 0) red[tid >> 6] = w;
+        if ((tid & 63) == 0) red[tid >> 6] = s;
         __syncthreads();
         l = l * alpha + ((red[0] + red[1]) + (red[2] + red[3]));
-        m = mn;
+        mx = mn;
         if (tid < hd) {
             o *= alpha;
-            const int n = min(256, pos + 1 - t0);
-            for (int j = 0; j < n; j++) {
-                const int p2 = t0 + j;
-                const T *row = p2 < a.pre_len ? pv + (size_t)p2 * hd : ov + (size_t)(p2 - a.pre_len) * hd;
-                o = fmaf(sc[j], (float)row[tid], o);
-            }
+            const int n = min(256, last + 1 - t0);
+            for (int j = 0; j < n; j++) o = fmaf(sc[j], (float)v[(size_t)(t0 + j) * hd + tid], o);
         }
         __syncthreads();
     }
-    if (tid >= hd) return;
-    if (a.sinks) {
-        const float sk = a.sinks[h], mn = fmaxf(m, sk), base = mn == -INFINITY ? 0.f : mn, f = expf(m - base);
-        l = l * f + expf(sk - base);
-        o *= f;
+    if (p.nrec) {
+        const size_t rec = ((size_t)r * a.n_heads + h) * p.nrec + w.rec;
+        if (tid == 0) p.ml[2 * rec] = mx, p.ml[2 * rec + 1] = l;
+        if (tid < hd) p.o[rec * hd + tid] = o;
+    } else if (tid < hd) {
+        if (a.sinks) {
+            const float sk = a.sinks[h] * LOG2E, mn = fmaxf(mx, sk), base = mn == -INFINITY ? 0.f : mn, f = exp2f(mx - base);
+            l = l * f + exp2f(sk - base);
+            o *= f;
+        }
+        a.out[(size_t)r * a.out_stride + (size_t)h * hd + tid] = o / l;
     }
-    a.out[(size_t)r * a.out_stride + (size_t)h * hd + tid] = o / l;
+}
+
+__device__ inline int div_up(int a, int b) { return (a + b - 1) / b; }
+
+}  // namespace
+
+/* ---- float16 caches on the matrix units ----
+ *
+ * S^T[position][m-row] = K Q^T and O^T[dim][m-row] += V^T P^T, both as
+ * v_mfma_f32_32x32x16_f16.  D of the first has m-row lane % 32, positions
+ * 8 (v / 4) + 4 (lane / 32) + v % 4 in register v: a lane holds one m-row's
+ * scores, so the softmax needs one exchange between the two halves of the
+ * wave, and its own registers are the B operand of the second product, whose
+ * k index is a permutation of the positions that V^T's fragments follow
+ * (ds_read_b64_tr_b16: four positions of one dim a lane).  O^T too has the
+ * m-row in the lane: rescaling needs no exchange.
+ *
+ * K and V are f16 as they are.  q and the weights are f32: each is the sum of
+ * two f16 (hi the nearest, lo the nearest to the rest: 22 bits), so each
+ * product is two MFMAs, and the result is as good as f32 sums.  What keeps
+ * lo out of f16's underflow: q is scaled by a power of two a row (its largest
+ * value to 2^13 .. 2^14), undone in the factor that takes scores to base 2;
+ * weights are taken times 2^13.
+ *
+ * K and V tiles of 64 positions go to LDS by direct copies, two buffers; the
+ * 16-byte pieces of a row are permuted by its position (swz) so that neither
+ * the K fragments (16 positions, one piece) nor the transposing reads (8
+ * positions, four pieces) meet in the same banks.  Rows past the region's end
+ * and dims past head_dim arrive as zeros. */
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+template <int HD>
+__device__ inline constexpr int swz(int key) {
+    return HD == 128 ? ((key & 3) << 2) | ((key >> 2) & 3) : (((key >> 1) & 1) << 2) | ((key >> 2) & 3);
+}
+
+__device__ inline h8 h8_of(h4 a, h4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+/* four values of one column of 16-bit values, rows in consecutive lanes' rows */
+__device__ inline h4 lds_column(uint32_t addr) {
+    typedef __fp16 g4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) g4 *P;
+    return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((P)(uintptr_t)addr));
+}
+__device__ inline h8 lds_row(uint32_t addr) {
+    typedef __attribute__((address_space(3))) h8 *P;
+    return *(P)(uintptr_t)addr;
+}
+__device__ inline float other_half_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float other_half_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+constexpr float W_SHIFT = 13.f;   /* weights are taken times 2^13 */
+
+/* A lane's m-row (both halves of a wave hold the same 32) and what its wave
+ * sees: positions any_lo .. any_hi by some row, all_lo .. all_hi by all. */
+struct Lane {
+    bool live;       /* false: no row there; its q is zero, nothing is masked, nothing written */
+    int first, last;
+    int r, h;        /* packed row, query head */
+    int any_lo, any_hi, all_lo, all_hi;
+};
+__device__ inline Lane lane_rows(const PromptArgs &a, const Work &w, int m, int ratio) {
+    Lane x;
+    x.first = 0, x.last = 0x7FFFFFFF;
+    x.live = row_sees(a, w, m, ratio, x.first, x.last);
+    const int i = x.live ? m / ratio : 0;
+    x.r = w.sq.r0 + i, x.h = w.kh * ratio + (x.live ? m - i * ratio : 0);
+    int lo = x.live ? x.first : 0x7FFFFFFF, hi = x.live ? x.last : -1, alo = x.live ? x.first : 0;
+    int ahi = x.live ? x.last : 0x7FFFFFFF;
+    if (!x.live) x.first = 0, x.last = 0x7FFFFFFF;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        lo = min(lo, __shfl_xor(lo, o, 64));
+        hi = max(hi, __shfl_xor(hi, o, 64));
+        alo = max(alo, __shfl_xor(alo, o, 64));
+        ahi = min(ahi, __shfl_xor(ahi, o, 64));
+    }
+    x.any_lo = __builtin_amdgcn_readfirstlane(lo), x.any_hi = __builtin_amdgcn_readfirstlane(hi);
+    x.all_lo = __builtin_amdgcn_readfirstlane(alo), x.all_hi = __builtin_amdgcn_readfirstlane(ahi);
+    return x;
+}
+
+/* the power of two that takes a largest magnitude to 2^13 .. 2^14, as its exponent */
+__device__ inline int scale_exp(float big) {
+    return big > 0.f && big < INFINITY ? min(14 - __builtin_amdgcn_frexp_expf(big), 100) : 0;
+}
+
+/* q of the lane's m-row as the B operands of the first product, two f16
+ * planes; returns the factor that takes scores of the planes to base 2 */
+template <int HD>
+__device__ inline float load_q(const PromptArgs &a, const Lane &x, int half, h8 (&qh)[HD / 16], h8 (&ql)[HD / 16]) {
+    float y[HD / 16][8], big = 0.f;
+    const float *src = a.q + (size_t)x.r * a.q_stride + (size_t)x.h * a.head_dim;
+#pragma unroll
+    for (int s = 0; s < HD / 16; s++) {
+        const int d = 16 * s + 8 * half;
+        const bool on = x.live && d < a.head_dim;
+        const f4 u = on ? (f4)*(const f4u *)(src + d) : f4{0.f, 0.f, 0.f, 0.f};
+        const f4 v = on ? (f4)*(const f4u *)(src + d + 4) : f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            y[s][e] = u[e], y[s][4 + e] = v[e];
+            big = fmaxf(big, fmaxf(fabsf(u[e]), fabsf(v[e])));
+        }
+    }
+    const int ex = scale_exp(other_half_max(big));
+#pragma unroll
+    for (int s = 0; s < HD / 16; s++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float z = __builtin_amdgcn_ldexpf(y[s][e], ex);
+            const _Float16 hi = (_Float16)z;
+            qh[s][e] = hi;
+            ql[s][e] = (_Float16)(z - (float)hi);
+        }
+    return __builtin_amdgcn_ldexpf(LOG2E / sqrtf((float)a.head_dim), -ex);
+}
+
+/* Byte offset in a tile of 16-bit rows of the lane's operand of the first
+ * product (step s: XOR s << 5, positions + 32: + 32 rows), and of the columns
+ * of the second (dims 32 d ..; e: the chunk's positions 8 e ..; 16 positions
+ * on: + 16 rows). */
+template <int HD>
+__device__ inline uint32_t k_operand(int lane) {
+    return (uint32_t)((lane & 31) * (HD * 2) + (((lane >> 5) ^ swz<HD>(lane & 31)) << 4));
+}
+template <int HD>
+__device__ inline uint32_t v_operand(int lane, int d, int e) {
+    const int key = 8 * e + 4 * (lane >> 5) + ((lane >> 2) & 3);
+    const int piece = 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+    return (uint32_t)(key * (HD * 2) + ((piece ^ swz<HD>(key)) << 4) + 8 * (lane & 1));
+}
+
+/* The wave's rows written: weights were summed in units of 2^(mx - W_SHIFT)
+ * relative to l, values besides in units of 2^-oexp.  Returns the m-rows that
+ * came out not finite, which are not written. */
+template <int HD>
+__device__ inline uint32_t write_rows(const PromptArgs &a, const RowsPlan &p, const Work &w, const Lane &x, int lane, float mx,
+                                      float l, int oexp, const f16v (&o)[HD / 32]) {
+    float nan = l * 0.f;
+#pragma unroll
+    for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) nan = fmaf(o[d][v], 0.f, nan);
+    const uint64_t mask = __ballot(x.live && !(nan == 0.f));
+    const uint32_t bad = (uint32_t)mask | (uint32_t)(mask >> 32);
+    if (!x.live || ((bad >> (lane & 31)) & 1u)) return bad;
+    const int half = lane >> 5, hd = a.head_dim;
+    float *dst, f;
+    if (p.nrec) {
+        const size_t rec = ((size_t)x.r * a.n_heads + x.h) * p.nrec + w.rec;
+        if (half == 0) *(float2 *)(p.ml + 2 * rec) = make_float2(mx, __builtin_amdgcn_ldexpf(l, -(int)W_SHIFT));
+        if (mx == -INFINITY) return bad;   /* a record of no position has no sums */
+        dst = p.o + rec * hd;
+        f = 1.f;
+        oexp += (int)W_SHIFT;
+    } else {
+        f = 1.f;
+        if (a.sinks) {
+            const float ref = mx - W_SHIFT, sk = a.sinks[x.h] * LOG2E, M = fmaxf(ref, sk), base = M == -INFINITY ? 0.f : M;
+            f = exp2f(ref - base);
+            l = l * f + exp2f(sk - base);
+        }
+        f /= l;
+        dst = a.out + (size_t)x.r * a.out_stride + (size_t)x.h * hd;
+    }
+#pragma unroll
+    for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            const int dim = 32 * d + 8 * v + 4 * half;
+            f4 y;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = __builtin_amdgcn_ldexpf(o[d][4 * v + e] * f, -oexp);
+            if (dim < hd) *(f4u *)(dst + dim) = y;
+        }
+    return bad;
+}
+
+#define MFMA_H(a, b, c) __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0)
+
+template <int HD>
+__global__ __launch_bounds__(256, 2) void k_rows_h(PromptArgs a, RowsPlan p) {
+    constexpr int RB = HD * 2, TILE = KT * RB;       /* bytes of a row in LDS, of a tile of K or V */
+    constexpr int NC = TILE / 1024 / 4;              /* copies of 1 KiB a wave, matrix and tile */
+    constexpr int DB = HD / 32, STEPS = HD / 16;
+    __shared__ __attribute__((aligned(1024))) uint8_t buf[2][2][TILE];
+    __shared__ uint32_t bad_rows[4];
+    const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
+    Work w;
+    if (!find_work<MT>(a, p, ratio, w)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int half = lane >> 5;
+    const Lane x = lane_rows(a, w, w.m0 + 32 * wave + (lane & 31), ratio);
+
+    /* copies: LDS byte 1024 n + 16 l of a tile is piece c' of row key; n = wave + 4 k */
+    const uint32_t rb = (uint32_t)hd * 2u;
+    const u32x4 kd = buf_desc(region<_Float16>(a, w, a.kv_k, a.pre_k), (uint32_t)w.hi * rb);
+    const u32x4 vd = buf_desc(region<_Float16>(a, w, a.kv_v, a.pre_v), (uint32_t)w.hi * rb);
+    const int ckey = (1024 * wave + 16 * lane) / RB, cpiece = (lane % (RB / 16)) ^ swz<HD>(ckey);
+    const uint32_t coff = 8 * cpiece < hd ? (uint32_t)ckey * rb + 16u * (uint32_t)cpiece : 0x7FFFFF00u;
+    auto copy_tile = [&](int t0, int b) __attribute__((always_inline)) {
+        const uint32_t at = coff + (uint32_t)t0 * rb;
+#pragma unroll
+        for (int k = 0; k < NC; k++) {
+            const uint32_t src = at + (uint32_t)k * (4096u / RB) * rb, dst = 1024u * (uint32_t)(wave + 4 * k);
+            copy_lanes(kd, src, lds_addr(buf[b][0]) + dst);
+            copy_lanes(vd, src, lds_addr(buf[b][1]) + dst);
+        }
+    };
+    if (w.lo < w.hi) copy_tile(w.lo, 0);
+
+    h8 qh[STEPS], ql[STEPS];
+    const float c = load_q<HD>(a, x, half, qh, ql);
+    f16v o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) o[d][v] = 0.f;
+    float mx = -INFINITY, l = 0.f;
+    const uint32_t kaddr = k_operand<HD>(lane);
+    uint32_t vaddr[DB][2];
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) vaddr[d][e] = v_operand<HD>(lane, d, e);
+
+    int b = 0;
+    for (int t = w.lo; t < w.hi; t += KT, b ^= 1) {
+        wait_copies();
+        bar_lds();   /* every wave's copies of this tile are there, and every wave is done with the other buffer */
+        if (t + KT < w.hi) copy_tile(t + KT, b ^ 1);
+        if (t > x.any_hi || t + KT <= x.any_lo) continue;   /* uniform in the wave */
+        const uint32_t kb = lds_addr(buf[b][0]), vb = lds_addr(buf[b][1]);
+        f16v s[2];
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) s[n][v] = 0.f;
+#pragma unroll
+        for (int st = 0; st < STEPS; st++) {
+            const uint32_t at = kb + (kaddr ^ (uint32_t)(st << 5));
+            const h8 k0 = lds_row(at), k1 = lds_row(at + 32 * RB);
+            s[0] = MFMA_H(k0, ql[st], s[0]);
+            s[1] = MFMA_H(k1, ql[st], s[1]);
+            s[0] = MFMA_H(k0, qh[st], s[0]);
+            s[1] = MFMA_H(k1, qh[st], s[1]);
+        }
+        if (t + KT - 1 > x.all_hi || t < x.all_lo) {   /* some row does not see all of the tile */
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    const int pos = t + 32 * n + 8 * (v >> 2) + 4 * half + (v & 3);
+                    s[n][v] = pos <= x.last && pos >= x.first ? s[n][v] : -INFINITY;
+                }
+        }
+        float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for (int v = 1; v < 16; v++) top = fmaxf(top, fmaxf(s[0][v], s[1][v]));
+        top = other_half_max(top) * c;
+        const float mn = fmaxf(mx, top), sh = mn == -INFINITY ? 0.f : W_SHIFT - mn;
+        if (__any(mn > mx)) {
+            const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DB; d++)
+#pragma unroll
+                for (int v = 0; v < 16; v++) o[d][v] *= alpha;
+        }
+        mx = mn;
+        h8 ph[4], pl[4];
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[n][v], c, sh));
+                sum[v & 3] += e;
+                const _Float16 hi = (_Float16)e;
+                ph[2 * n + (v >> 3)][v & 7] = hi;
+                pl[2 * n + (v >> 3)][v & 7] = (_Float16)(e - (float)hi);
+            }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+                const uint32_t at = vb + (uint32_t)(q * 16 * RB);
+                const h8 vt = h8_of(lds_column(at + vaddr[d][0]), lds_column(at + vaddr[d][1]));
+                o[d] = MFMA_H(vt, pl[q], o[d]);
+                o[d] = MFMA_H(vt, ph[q], o[d]);
+            }
+    }
+    const uint32_t bad = write_rows<HD>(a, p, w, x, lane, mx, other_half_sum(l), 0, o);
+    if (lane == 0) bad_rows[wave] = bad;
+    __syncthreads();
+    for (int wv = 0; wv < 4; wv++)
+        for (uint32_t y = bad_rows[wv]; y; y &= y - 1)
+            slow_row<_Float16>(a, p, w, w.m0 + 32 * wv + __builtin_ctz(y), ratio, (float *)buf);
+}
+
+/* ---- float32 caches on the f16 matrix units ----
+ *
+ * The same products with K and V split as q and the weights are: x 2^k = hi +
+ * lo, 22 bits, and three MFMAs a product (hi hi, hi lo, lo hi; lo lo is below
+ * 2^-22).  k is chosen for each group of 8 positions from its largest finite
+ * magnitude, so any f32 range fits: a value down to 2^-15 of its group's
+ * largest keeps 22 bits, a smaller one is off by 2^-38 of the largest.  (f32
+ * MFMAs run at a sixteenth of the f16 rate, three bf16 planes would take six
+ * products.)
+ *
+ * A group is one wave's share of a tile's loads, and positions 8 g .. 8 g + 7
+ * are registers 4 g .. 4 g + 3 of the scores in both halves of the wave: K's
+ * scale only changes the factor to base 2.  V's groups have scales of their
+ * own; o is in units of 2^-U, U the smallest k so far, and a group's weights
+ * take 2^(U - k).
+ *
+ * A tile of 32 positions is loaded into registers two tiles ahead, split and
+ * stored to one of two LDS buffers one tile ahead (plane [K hi, K lo, V hi,
+ * V lo][32][HD]). */
+constexpr int KF = 32;
+
+template <int HD, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void k_rows_f(PromptArgs a, RowsPlan p) {
+    constexpr int RB = HD * 2, PLANE = KF * RB;
+    constexpr int UNITS = 8 / NW;                    /* groups a wave loads: K 0 .. 3, V 4 .. 7 */
+    constexpr int LR = 256 / HD, NL = 8 / LR;        /* rows a load of the wave covers, loads a group */
+    constexpr int DB = HD / 32, STEPS = HD / 16;
+    __shared__ __attribute__((aligned(1024))) uint8_t buf[2][4][PLANE];
+    __shared__ int exps[2][8];
+    __shared__ uint32_t bad_rows[NW];
+    const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
+    Work w;
+    if (!find_work<32 * NW>(a, p, ratio, w)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int half = lane >> 5;
+    const Lane x = lane_rows(a, w, w.m0 + 32 * wave + (lane & 31), ratio);
+
+    /* loads: lane l of load j of group g holds dims 4 (l % (HD / 4)) .. of position 8 g + LR j + l / (HD / 4) */
+    const uint32_t rb = (uint32_t)hd * 4u;
+    const Buf kd = make_buf_uniform(region<float>(a, w, a.kv_k, a.pre_k), (uint32_t)w.hi * rb);
+    const Buf vd = make_buf_uniform(region<float>(a, w, a.kv_v, a.pre_v), (uint32_t)w.hi * rb);
+    const int lrow = lane / (HD / 4), ldim = 4 * (lane % (HD / 4));
+    const uint32_t loff = ldim < hd ? (uint32_t)lrow * rb + 4u * (uint32_t)ldim : 0x7FFFFF00u;
+    u32x4 raw[UNITS][NL];
+    auto load_tile = [&](int t0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) {
+            const int g = u * NW + wave;
+#pragma unroll
+            for (int j = 0; j < NL; j++) {
+                const uint32_t at = loff + (uint32_t)(t0 + 8 * (g & 3) + LR * j) * rb;
+                if (UNITS == 1) raw[u][j] = g < 4 ? ld16(kd, at) : ld16(vd, at);
+                else raw[u][j] = u == 0 ? ld16(kd, at) : ld16(vd, at);
+            }
+        }
+    };
+    auto split_tile = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) {
+            const int g = u * NW + wave;
+            float big = 0.f;
+#pragma unroll
+            for (int j = 0; j < NL; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) big = fmaxf(big, fabsf(__uint_as_float(raw[u][j][e])));
+            big = wave_max(big);
+            if (!(big < INFINITY)) {   /* uniform: the largest of the finite ones */
+                big = 0.f;
+#pragma unroll
+                for (int j = 0; j < NL; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float y = fabsf(__uint_as_float(raw[u][j][e]));
+                        big = fmaxf(big, y < INFINITY ? y : 0.f);
+                    }
+                big = wave_max(big);
+            }
+            const int ex = big > 0.f ? scale_exp(big) : 100;
+            const float f = __builtin_amdgcn_ldexpf(1.f, ex);
+            if (lane == 0) exps[b][g] = ex;
+#pragma unroll
+            for (int j = 0; j < NL; j++) {
+                const int key = 8 * (g & 3) + LR * j + lrow;
+                const uint32_t at = (uint32_t)(key * RB + (((ldim >> 3) ^ swz<HD>(key)) << 4) + 2 * (ldim & 4));
+                h4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float y = __uint_as_float(raw[u][j][e]) * f;
+                    hi[e] = (_Float16)y;
+                    lo[e] = (_Float16)(y - (float)hi[e]);
+                }
+                *(h4 *)(buf[b][2 * (g >> 2)] + at) = hi;
+                *(h4 *)(buf[b][2 * (g >> 2) + 1] + at) = lo;
+            }
+        }
+    };
+    if (w.lo < w.hi) load_tile(w.lo);
+
+    h8 qh[STEPS], ql[STEPS];
+    const float c = load_q<HD>(a, x, half, qh, ql);
+    f16v o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) o[d][v] = 0.f;
+    float mx = -INFINITY, l = 0.f;
+    int U = 100;
+    const uint32_t kaddr = k_operand<HD>(lane);
+    uint32_t vaddr[DB][2];
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) vaddr[d][e] = v_operand<HD>(lane, d, e);
+
+    if (w.lo < w.hi) {
+        split_tile(0);
+        load_tile(w.lo + KF);   /* past the region: zeros */
+    }
+    __syncthreads();
+    int b = 0;
+    for (int t = w.lo; t < w.hi; t += KF, b ^= 1) {
+        if (t <= x.any_hi && t + KF > x.any_lo) {   /* uniform in the wave */
+            const uint32_t kb = lds_addr(buf[b][0]), vb = lds_addr(buf[b][2]);
+            int ke[4], ve[4];
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                ke[g] = __builtin_amdgcn_readfirstlane(exps[b][g]);
+                ve[g] = __builtin_amdgcn_readfirstlane(exps[b][4 + g]);
+            }
+            f16v s;
+#pragma unroll
+            for (int v = 0; v < 16; v++) s[v] = 0.f;
+#pragma unroll
+            for (int st = 0; st < STEPS; st++) {
+                const uint32_t at = kb + (kaddr ^ (uint32_t)(st << 5));
+                const h8 kh = lds_row(at), kl = lds_row(at + PLANE);
+                s = MFMA_H(kl, qh[st], s);
+                s = MFMA_H(kh, ql[st], s);
+                s = MFMA_H(kh, qh[st], s);
+            }
+            if (t + KF - 1 > x.all_hi || t < x.all_lo) {   /* some row does not see all of the tile */
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    const int pos = t + 8 * (v >> 2) + 4 * half + (v & 3);
+                    s[v] = pos <= x.last && pos >= x.first ? s[v] : -INFINITY;
+                }
+            }
+            float cg[4], top = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                cg[g] = __builtin_amdgcn_ldexpf(c, -ke[g]);
+                top = fmaxf(top, fmaxf(fmaxf(s[4 * g], s[4 * g + 1]), fmaxf(s[4 * g + 2], s[4 * g + 3])) * cg[g]);
+            }
+            top = other_half_max(top);
+            const int un = min(min(U, min(ve[0], ve[1])), min(ve[2], ve[3]));
+            const float mn = fmaxf(mx, top), sh = mn == -INFINITY ? 0.f : W_SHIFT - mn;
+            if (__any(mn > mx) || un != U) {
+                const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
+                const float beta = __builtin_amdgcn_ldexpf(alpha, un - U);
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < DB; d++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) o[d][v] *= beta;
+            }
+            mx = mn, U = un;
+            h8 ph[2], pl[2];
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const float f = __builtin_amdgcn_ldexpf(1.f, un - ve[g]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float y = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], cg[g], sh));
+                    sum[e] += y;
+                    y *= f;
+                    const _Float16 hi = (_Float16)y;
+                    ph[g >> 1][4 * (g & 1) + e] = hi;
+                    pl[g >> 1][4 * (g & 1) + e] = (_Float16)(y - (float)hi);
+                }
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+            for (int q = 0; q < 2; q++)
+#pragma unroll
+                for (int d = 0; d < DB; d++) {
+                    const uint32_t at = vb + (uint32_t)(q * 16 * RB);
+                    const h8 vh = h8_of(lds_column(at + vaddr[d][0]), lds_column(at + vaddr[d][1]));
+                    const h8 vl = h8_of(lds_column(at + PLANE + vaddr[d][0]), lds_column(at + PLANE + vaddr[d][1]));
+                    o[d] = MFMA_H(vl, ph[q], o[d]);
+                    o[d] = MFMA_H(vh, pl[q], o[d]);
+                    o[d] = MFMA_H(vh, ph[q], o[d]);
+                }
+        }
+        if (t + KF < w.hi) {
+            split_tile(b ^ 1);
+            load_tile(t + 2 * KF);
+        }
+        bar_lds();
+    }
+    const uint32_t bad = write_rows<HD>(a, p, w, x, lane, mx, other_half_sum(l), U, o);
+    if (lane == 0) bad_rows[wave] = bad;
+    __syncthreads();
+    for (int wv = 0; wv < NW; wv++)
+        for (uint32_t y = bad_rows[wv]; y; y &= y - 1)
+            slow_row<float>(a, p, w, w.m0 + 32 * wv + __builtin_ctz(y), ratio, (float *)buf);
+}
+
+/* The records of a row and head, and its sink, as one: a wave each. */
+__global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) {
+    const int lane = threadIdx.x & 63, hd = a.head_dim;
+    const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= (long long)a.s.rows * a.n_heads) return;
+    const int r = (int)(at / a.n_heads), h = (int)(at - (long long)r * a.n_heads);
+    const int s = seq_of(a.s, r);
+    if (s < 0) return;
+    const Seq sq = seq_at(a.s, s);
+    if (r - sq.r0 < 0 || r - sq.r0 >= sq.n) return;
+    const float *ml = p.ml + 2 * (size_t)at * p.nrec, *po = p.o + (size_t)at * p.nrec * hd;
+    float M = a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
+    for (int c0 = 0; c0 < p.nrec; c0 += 64) M = fmaxf(M, wave_max(c0 + lane < p.nrec ? ml[2 * (c0 + lane)] : -INFINITY));
+    const float base = M == -INFINITY ? 0.f : M;
+    float l = 0.f, o0 = 0.f, o1 = 0.f;
+    const int d = 2 * lane;
+    for (int c0 = 0; c0 < p.nrec; c0 += 64) {
+        const int c = c0 + lane, n = min(64, p.nrec - c0);
+        const float m = c < p.nrec ? ml[2 * c] : -INFINITY;
+        const float e = m == -INFINITY ? 0.f : exp2f(m - base);
+        l += e == 0.f ? 0.f : ml[2 * c + 1] * e;
+        for (int j = 0; j < n; j++) {
+            const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(e), j));
+            if (f == 0.f || d >= hd) continue;   /* a record of no position has no sums */
+            const float2 v = *(const float2 *)(po + (size_t)(c0 + j) * hd + d);
+            o0 = fmaf(v.x, f, o0);
+            o1 = fmaf(v.y, f, o1);
+        }
+    }
+    l = wave_sum(l);
+    if (a.sinks) l += exp2f(a.sinks[h] * LOG2E - base);
+    if (d >= hd) return;
+    float *dst = a.out + (size_t)r * a.out_stride + (size_t)h * hd + d;
+    dst[0] = o0 / l;
+    dst[1] = o1 / l;
+}
+
+/* How a call is cut, from the host's arguments alone (the lengths are on the
+ * device): spans until about two workgroups a CU are there, of at least four
+ * tiles of the longest cache that the call can have. */
+static RowsPlan rows_plan(int n_rows, int n_seqs, int n_heads, int n_kv, int kv_max, int pre_len, int window) {
+    RowsPlan p = {};
+    const int ratio = n_heads / n_kv;
+    const long long m = (long long)n_rows * ratio;
+    auto spans = [&](long long wgs, int positions) {
+        const int want = (int)((512 + wgs - 1) / wgs), most = (positions + 4 * KT - 1) / (4 * KT);
+        return std::max(1, std::min(std::min(want, most), 128));
+    };
+    p.tiles = (int)std::min(m / MT + n_seqs, m);
+    p.ns = spans((long long)p.tiles * n_kv, kv_max);
+    if (pre_len) {
+        p.pre_tiles = (int)((m + MT - 1) / MT);
+        p.pre_ns = spans((long long)p.pre_tiles * n_kv, pre_len);
+    }
+    p.nrec = p.ns + p.pre_ns > 1 ? p.ns + p.pre_ns : 0;
+    (void)window;
+    return p;
+}
+
+static size_t ml_bytes(const RowsPlan &p, int n_rows, int n_heads) {
+    return ((size_t)n_rows * n_heads * p.nrec * 8 + 255) & ~(size_t)255;
 }
 
 size_t attention_rows_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len) {
-    (void)n_rows, (void)n_seqs, (void)n_heads, (void)n_kv, (void)head_dim, (void)kv_max, (void)pre_len;
-    return 0;
+    const RowsPlan p = rows_plan(n_rows, n_seqs, n_heads, n_kv, kv_max, pre_len, 0);
+    return p.nrec ? ml_bytes(p, n_rows, n_heads) + (size_t)n_rows * n_heads * p.nrec * head_dim * 4 : 0;
 }
 
 void launch_attention_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st) {
-    (void)scratch;
-    const dim3 grid(a.s.rows, a.n_heads);
-    if (half) hipLaunchKernelGGL(k_attn_row<_Float16>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(k_attn_row<float>, grid, dim3(256), 0, st, a);
+    RowsPlan p = rows_plan(a.s.rows, a.s.n, a.n_heads, a.n_kv, a.s.kv_max, a.pre_len, a.window);
+    p.ml = (float *)scratch;
+    p.o = (float *)((uint8_t *)scratch + ml_bytes(p, a.s.rows, a.n_heads));
+    const dim3 grid((unsigned)((p.tiles * p.ns + p.pre_tiles * p.pre_ns) * a.n_kv)), block(256);
+    if (!half && a.head_dim > 64) hipLaunchKernelGGL((k_rows_f<128, 4>), grid, block, 0, st, a, p);
+    else if (!half) hipLaunchKernelGGL((k_rows_f<64, 4>), grid, block, 0, st, a, p);
+    else if (a.head_dim > 64) hipLaunchKernelGGL(k_rows_h<128>, grid, block, 0, st, a, p);
+    else hipLaunchKernelGGL(k_rows_h<64>, grid, block, 0, st, a, p);
+    if (p.nrec)
+        hipLaunchKernelGGL(k_rows_combine, dim3((unsigned)(((long long)a.s.rows * a.n_heads + 3) / 4)), block, 0, st, a, p);
 }
 
 }  // namespace tg
