@@ -858,10 +858,251 @@ __global__ __launch_bounds__(64 * NW, 2) void k_rows_f(PromptArgs a, RowsPlan p)
             slow_row<float>(a, p, w, w.m0 + 32 * wv + __builtin_ctz(y), ratio, (float *)buf);
 }
 
-/* The records of a row and head, and its sink, as one: a wave each. */
+/* ---- few rows: positions over the waves ----
+ *
+ * A workgroup of four waves takes 16 m-rows; a wave walks tiles of 16
+ * positions (every fourth) with K and V straight from the cache into the
+ * operands, no LDS and no barrier until the end, where the four waves' sums
+ * meet.  S^T[position][m-row] on 16x16 MFMAs: D lane l holds m-row l % 16,
+ * positions 4 (l / 16) + v, which is B of the second product over positions
+ * 4 (l / 16) + i as it lies.  The second product is f32 (16x16x4) for both
+ * cache types: V converts exactly, the weights are not rounded, and the rate
+ * is above what the cache's bytes allow.  The first is f32 for an f32 cache
+ * and two f16 products (q in two planes) for an f16 one. */
+typedef float v4f __attribute__((ext_vector_type(4)));
+constexpr int MN = 16;
+
+template <typename T, int HD>
+struct NarrowK {   /* float: K pieces of 4 dims, dims 16 j + 4 kq + e in MFMA (j, e) */
+    static constexpr int J = HD / 16;
+    v4f q[J];
+    u32x4 k[J];
+    __device__ inline float load_q(const PromptArgs &a, const Lane &x, int kq) {
+        const float *src = a.q + (size_t)x.r * a.q_stride + (size_t)x.h * a.head_dim;
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const int d = 16 * j + 4 * kq;
+            q[j] = x.live && d < a.head_dim ? (v4f)*(const f4u *)(src + d) : v4f{0.f, 0.f, 0.f, 0.f};
+        }
+        return LOG2E / sqrtf((float)a.head_dim);
+    }
+    __device__ inline void load_k(Buf kd, uint32_t row, int kq, int hd) {
+#pragma unroll
+        for (int j = 0; j < J; j++) k[j] = ld16(kd, 16 * j + 4 * kq < hd ? row + 64u * j + 16u * (uint32_t)kq : 0x7FFFFF00u);
+    }
+    __device__ inline v4f scores() const {
+        v4f s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;   /* two chains */
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float y = __uint_as_float(k[j][e]);
+                if (e & 1) s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(y, q[j][e], s1, 0, 0, 0);
+                else s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(y, q[j][e], s0, 0, 0, 0);
+            }
+        return s0 + s1;
+    }
+};
+template <int HD>
+struct NarrowK<_Float16, HD> {   /* K pieces of 8 dims, dims 32 j + 8 kq + e in MFMA j */
+    static constexpr int J = HD / 32;
+    h8 qh[J], ql[J];
+    u32x4 k[J];
+    __device__ inline float load_q(const PromptArgs &a, const Lane &x, int kq) {
+        const float *src = a.q + (size_t)x.r * a.q_stride + (size_t)x.h * a.head_dim;
+        f4 u[J], v[J];
+        float big = 0.f;
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const int d = 32 * j + 8 * kq;
+            const bool on = x.live && d < a.head_dim;
+            u[j] = on ? (f4)*(const f4u *)(src + d) : f4{0.f, 0.f, 0.f, 0.f};
+            v[j] = on ? (f4)*(const f4u *)(src + d + 4) : f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 4; e++) big = fmaxf(big, fmaxf(fabsf(u[j][e]), fabsf(v[j][e])));
+        }
+        big = fmaxf(big, __shfl_xor(big, 16, 64));
+        const int ex = scale_exp(fmaxf(big, __shfl_xor(big, 32, 64)));
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float z = __builtin_amdgcn_ldexpf(e < 4 ? u[j][e & 3] : v[j][e & 3], ex);
+                const _Float16 hi = (_Float16)z;
+                qh[j][e] = hi;
+                ql[j][e] = (_Float16)(z - (float)hi);
+            }
+        return __builtin_amdgcn_ldexpf(LOG2E / sqrtf((float)a.head_dim), -ex);
+    }
+    __device__ inline void load_k(Buf kd, uint32_t row, int kq, int hd) {
+#pragma unroll
+        for (int j = 0; j < J; j++) k[j] = ld16(kd, 32 * j + 8 * kq < hd ? row + 64u * j + 16u * (uint32_t)kq : 0x7FFFFF00u);
+    }
+    __device__ inline v4f scores() const {
+        v4f s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const h8 y = __builtin_bit_cast(h8, k[j]);
+            s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, qh[j], s0, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, ql[j], s1, 0, 0, 0);
+        }
+        return s0 + s1;
+    }
+};
+
+/* V of a lane's position: HD / 16 dims; dim(i, t) is the t-th of lane i % 16 */
+template <typename T, int HD>
+struct NarrowV {
+    static constexpr int N = HD / 16;
+    u32x4 v[N / 4];
+    static __device__ inline int dim(int i, int t) { return 64 * (t >> 2) + 4 * i + (t & 3); }
+    __device__ inline void load(Buf vd, uint32_t row, int i, int hd) {
+#pragma unroll
+        for (int n = 0; n < N / 4; n++) v[n] = ld16(vd, 64 * n + 4 * i < hd ? row + 256u * n + 16u * (uint32_t)i : 0x7FFFFF00u);
+    }
+    __device__ inline float at(int t) const { return __uint_as_float(v[t >> 2][t & 3]); }
+};
+template <int HD>
+struct NarrowV<_Float16, HD> {
+    static constexpr int N = HD / 16;
+    typedef _Float16 H __attribute__((ext_vector_type(N)));
+    H v;
+    static __device__ inline int dim(int i, int t) { return N * i + t; }
+    __device__ inline void load(Buf vd, uint32_t row, int i, int hd) {
+        const uint32_t at = N * i < hd ? row + 2u * N * (uint32_t)i : 0x7FFFFF00u;
+        if constexpr (N == 8) v = __builtin_bit_cast(H, ld16(vd, at));
+        else v = __builtin_bit_cast(H, ld8(vd, at));
+    }
+    __device__ inline float at(int t) const { return (float)v[t]; }
+};
+
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
+    constexpr int N = HD / 16;
+    __shared__ __attribute__((aligned(16))) float mo[4][MN][HD];
+    __shared__ float mm[4][MN], ml[4][MN];
+    __shared__ uint32_t bad_rows;
+    const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
+    Work w;
+    if (!find_work<MN>(a, p, ratio, w)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c16 = lane & 15, kq = lane >> 4;
+    const Lane x = lane_rows(a, w, w.m0 + c16, ratio);
+    if (tid == 0) bad_rows = 0;
+
+    const uint32_t rb = (uint32_t)hd * (uint32_t)sizeof(T);
+    const Buf kd = make_buf_uniform(region<T>(a, w, a.kv_k, a.pre_k), (uint32_t)w.hi * rb);
+    const Buf vd = make_buf_uniform(region<T>(a, w, a.kv_v, a.pre_v), (uint32_t)w.hi * rb);
+    NarrowK<T, HD> K;
+    NarrowV<T, HD> V[4];
+    auto load_v = [&](int t0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) V[i].load(vd, (uint32_t)(t0 + 4 * kq + i) * rb, c16, hd);
+    };
+    int t = w.lo + 16 * wave;
+    K.load_k(kd, (uint32_t)(t + c16) * rb, kq, hd);   /* past the span: zeros, no memory access */
+    load_v(t);
+    const float c = K.load_q(a, x, kq);
+    float mx = -INFINITY, l = 0.f;
+    v4f o[N];
+#pragma unroll
+    for (int n = 0; n < N; n++) o[n] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (; t < w.hi; t += 64) {
+        v4f s = K.scores();
+        K.load_k(kd, (uint32_t)(t + 64 + c16) * rb, kq, hd);
+        const bool masked = t + 15 > x.all_hi || t < x.all_lo;   /* uniform */
+        float top = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            const int pos = t + 4 * kq + v;
+            if (masked) s[v] = pos <= x.last && pos >= x.first ? s[v] : -INFINITY;
+            top = fmaxf(top, s[v]);
+        }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64)) * c;
+        const float mn = fmaxf(mx, top), base = mn == -INFINITY ? 0.f : mn;
+        if (__any(mn > mx)) {
+            const float alpha = __builtin_amdgcn_exp2f(mx - base);
+            l *= alpha;
+#pragma unroll
+            for (int n = 0; n < N; n++) o[n] *= alpha;
+        }
+        mx = mn;
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], c, -base));
+            l += s[v];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int n = 0; n < N; n++) o[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(V[i].at(n), s[i], o[n], 0, 0, 0);
+        load_v(t + 64);
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+#pragma unroll
+    for (int v = 0; v < 4; v++)
+#pragma unroll
+        for (int n = 0; n < N; n += 4) {
+            const int d = NarrowV<T, HD>::dim(4 * kq + v, n);   /* the next three follow */
+            *(f4 *)&mo[wave][c16][d] = f4{o[n][v], o[n + 1][v], o[n + 2][v], o[n + 3][v]};
+        }
+    if (kq == 0) mm[wave][c16] = mx, ml[wave][c16] = l;
+    __syncthreads();
+    /* the four waves' sums as one, in wave order: 16 threads a row, HD / 16 dims each */
+    const int row = tid >> 4, d0 = (tid & 15) * N;
+    const Lane y = lane_rows(a, w, w.m0 + row, ratio);
+    float M = fmaxf(fmaxf(mm[0][row], mm[1][row]), fmaxf(mm[2][row], mm[3][row]));
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f, r[N];
+#pragma unroll
+    for (int n = 0; n < N; n++) r[n] = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const float e = __builtin_amdgcn_exp2f(mm[q][row] - base);
+        L = fmaf(ml[q][row], e, L);
+#pragma unroll
+        for (int n = 0; n < N; n++) r[n] = fmaf(mo[q][row][d0 + n], e, r[n]);
+    }
+    float nan = L * 0.f;
+#pragma unroll
+    for (int n = 0; n < N; n++) nan = fmaf(r[n], 0.f, nan);
+    if (y.live && !(nan == 0.f)) atomicOr(&bad_rows, 1u << row);
+    __syncthreads();
+    const uint32_t bad = bad_rows;
+    if (y.live && !((bad >> row) & 1u) && d0 < hd) {
+        float *dst, f = 1.f;
+        if (p.nrec) {
+            const size_t rec = ((size_t)y.r * a.n_heads + y.h) * p.nrec + w.rec;
+            if (d0 == 0) *(float2 *)(p.ml + 2 * rec) = make_float2(M, L);
+            dst = p.o + rec * hd + d0;
+        } else {
+            if (a.sinks) {
+                const float sk = a.sinks[y.h] * LOG2E, mn = fmaxf(M, sk), b2 = mn == -INFINITY ? 0.f : mn;
+                f = exp2f(M - b2);
+                L = L * f + exp2f(sk - b2);
+            }
+            f /= L;
+            dst = a.out + (size_t)y.r * a.out_stride + (size_t)y.h * hd + d0;
+        }
+        if (!p.nrec || M > -INFINITY) {
+#pragma unroll
+            for (int n = 0; n < N; n += 4) *(f4u *)(dst + n) = f4{r[n] * f, r[n + 1] * f, r[n + 2] * f, r[n + 3] * f};
+        }
+    }
+    for (uint32_t z = bad; z; z &= z - 1) slow_row<T>(a, p, w, w.m0 + __builtin_ctz(z), ratio, &mo[0][0][0]);
+}
+
+/* The records of a row and head, and its sink, as one: W waves each, wave g
+ * the records g (mod W), G lanes a record (four dims a lane). */
+template <int W, int G>
 __global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) {
-    const int lane = threadIdx.x & 63, hd = a.head_dim;
-    const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    __shared__ __attribute__((aligned(16))) float so[W > 1 ? W : 1][4 * G];
+    __shared__ float sl[W];
+    constexpr int PER = 64 / G;   /* records a wave reads at a time */
+    const int tid = threadIdx.x, lane = tid & 63, wave = W > 1 ? tid >> 6 : 0, hd = a.head_dim;
+    const long long at = W > 1 ? (long long)blockIdx.x : (long long)blockIdx.x * 4 + (tid >> 6);
     if (at >= (long long)a.s.rows * a.n_heads) return;
     const int r = (int)(at / a.n_heads), h = (int)(at - (long long)r * a.n_heads);
     const int s = seq_of(a.s, r);
@@ -869,52 +1110,80 @@ __global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) 
     const Seq sq = seq_at(a.s, s);
     if (r - sq.r0 < 0 || r - sq.r0 >= sq.n) return;
     const float *ml = p.ml + 2 * (size_t)at * p.nrec, *po = p.o + (size_t)at * p.nrec * hd;
-    float M = a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
-    for (int c0 = 0; c0 < p.nrec; c0 += 64) M = fmaxf(M, wave_max(c0 + lane < p.nrec ? ml[2 * (c0 + lane)] : -INFINITY));
+    const float sink = a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
+    /* lane i: record W i + wave of each 64 W */
+    float M = -INFINITY;
+    for (int c = lane; c < p.nrec; c += 64) M = fmaxf(M, ml[2 * c]);
+    M = fmaxf(wave_max(M), sink);
     const float base = M == -INFINITY ? 0.f : M;
-    float l = 0.f, o0 = 0.f, o1 = 0.f;
-    const int d = 2 * lane;
-    for (int c0 = 0; c0 < p.nrec; c0 += 64) {
-        const int c = c0 + lane, n = min(64, p.nrec - c0);
-        const float m = c < p.nrec ? ml[2 * c] : -INFINITY;
-        const float e = m == -INFINITY ? 0.f : exp2f(m - base);
-        l += e == 0.f ? 0.f : ml[2 * c + 1] * e;
-        for (int j = 0; j < n; j++) {
-            const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(e), j));
+    float l = 0.f;
+    f4 o = {0.f, 0.f, 0.f, 0.f};
+    const int g = lane / G, d = 4 * (lane % G);
+    for (int c0 = 0; c0 < p.nrec; c0 += 64 * W) {
+        const int c = c0 + W * lane + wave;
+        const float2 x = c < p.nrec ? *(const float2 *)(ml + 2 * c) : make_float2(-INFINITY, 0.f);
+        const float e = x.x == -INFINITY ? 0.f : exp2f(x.x - base);
+        l += e == 0.f ? 0.f : x.y * e;
+        const int n = min(64, (p.nrec - c0 - wave + W - 1) / W);
+#pragma unroll 4
+        for (int j = g; j < n; j += PER) {
+            const float f = __shfl(e, j, 64);
             if (f == 0.f || d >= hd) continue;   /* a record of no position has no sums */
-            const float2 v = *(const float2 *)(po + (size_t)(c0 + j) * hd + d);
-            o0 = fmaf(v.x, f, o0);
-            o1 = fmaf(v.y, f, o1);
+            o += *(const f4 *)(po + (size_t)(c0 + W * j + wave) * hd + d) * f;
         }
     }
     l = wave_sum(l);
-    if (a.sinks) l += exp2f(a.sinks[h] * LOG2E - base);
-    if (d >= hd) return;
-    float *dst = a.out + (size_t)r * a.out_stride + (size_t)h * hd + d;
-    dst[0] = o0 / l;
-    dst[1] = o1 / l;
+#pragma unroll
+    for (int q = 32; q >= G; q >>= 1)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] += __shfl_xor(o[e], q, 64);
+    if constexpr (W > 1) {
+        if (lane < G) *(f4 *)&so[wave][4 * lane] = o;
+        if (lane == 0) sl[wave] = l;
+        __syncthreads();
+        if (wave) return;
+        if (lane < G) {
+#pragma unroll
+            for (int q = 1; q < W; q++) {
+                o += *(const f4 *)&so[q][4 * lane];
+                l += sl[q];
+            }
+        }
+    }
+    if (lane >= G || d >= hd) return;
+    if (a.sinks) l += exp2f(sink - base);
+    const f4 y = o / l;
+    *(f4u *)(a.out + (size_t)r * a.out_stride + (size_t)h * hd + d) = y;
 }
 
 /* How a call is cut, from the host's arguments alone (the lengths are on the
- * device): spans until about two workgroups a CU are there, of at least four
- * tiles of the longest cache that the call can have. */
-static RowsPlan rows_plan(int n_rows, int n_seqs, int n_heads, int n_kv, int kv_max, int pre_len, int window) {
-    RowsPlan p = {};
+ * device).  A part (the sequences' slots; the prefix) runs on the narrow
+ * kernel where its tiles would have few m-rows. */
+struct Cut {
+    RowsPlan p;
+    bool narrow, pre_narrow;
+};
+static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int kv_max, int pre_len) {
+    Cut k = {};
+    RowsPlan &p = k.p;
     const int ratio = n_heads / n_kv;
     const long long m = (long long)n_rows * ratio;
-    auto spans = [&](long long wgs, int positions) {
-        const int want = (int)((512 + wgs - 1) / wgs), most = (positions + 4 * KT - 1) / (4 * KT);
+    auto spans = [&](long long wgs, int positions, bool narrow) {
+        const int least = narrow ? 128 : 4 * KT;
+        const int want = (int)((512 + wgs - 1) / wgs), most = (positions + least - 1) / least;
         return std::max(1, std::min(std::min(want, most), 128));
     };
-    p.tiles = (int)std::min(m / MT + n_seqs, m);
-    p.ns = spans((long long)p.tiles * n_kv, kv_max);
+    k.narrow = m <= 64ll * n_seqs;
+    k.pre_narrow = m <= 64;
+    p.tiles = (int)std::min(m / (k.narrow ? MN : MT) + n_seqs, m);
+    p.ns = spans((long long)p.tiles * n_kv, kv_max, k.narrow);
     if (pre_len) {
-        p.pre_tiles = (int)((m + MT - 1) / MT);
-        p.pre_ns = spans((long long)p.pre_tiles * n_kv, pre_len);
+        const int mt = k.pre_narrow ? MN : MT;
+        p.pre_tiles = (int)((m + mt - 1) / mt);
+        p.pre_ns = spans((long long)p.pre_tiles * n_kv, pre_len, k.pre_narrow);
     }
     p.nrec = p.ns + p.pre_ns > 1 ? p.ns + p.pre_ns : 0;
-    (void)window;
-    return p;
+    return k;
 }
 
 static size_t ml_bytes(const RowsPlan &p, int n_rows, int n_heads) {
@@ -922,21 +1191,55 @@ static size_t ml_bytes(const RowsPlan &p, int n_rows, int n_heads) {
 }
 
 size_t attention_rows_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len) {
-    const RowsPlan p = rows_plan(n_rows, n_seqs, n_heads, n_kv, kv_max, pre_len, 0);
+    const RowsPlan p = rows_cut(n_rows, n_seqs, n_heads, n_kv, kv_max, pre_len).p;
     return p.nrec ? ml_bytes(p, n_rows, n_heads) + (size_t)n_rows * n_heads * p.nrec * head_dim * 4 : 0;
 }
 
+/* the workgroups of one part, or of both */
+static void launch_part(const PromptArgs &a, const RowsPlan &p, bool half, bool narrow, hipStream_t st) {
+    const dim3 grid((unsigned)((p.tiles * p.ns + p.pre_tiles * p.pre_ns) * a.n_kv)), block(256);
+    const bool big = a.head_dim > 64;
+    if (!grid.x) return;
+#define ROWS(K) hipLaunchKernelGGL((K), grid, block, 0, st, a, p)
+    if (narrow) {
+        if (half && big) ROWS((k_rows_n<_Float16, 128>));
+        else if (half) ROWS((k_rows_n<_Float16, 64>));
+        else if (big) ROWS((k_rows_n<float, 128>));
+        else ROWS((k_rows_n<float, 64>));
+    } else {
+        if (half && big) ROWS(k_rows_h<128>);
+        else if (half) ROWS(k_rows_h<64>);
+        else if (big) ROWS((k_rows_f<128, 4>));
+        else ROWS((k_rows_f<64, 4>));
+    }
+#undef ROWS
+}
+
 void launch_attention_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st) {
-    RowsPlan p = rows_plan(a.s.rows, a.s.n, a.n_heads, a.n_kv, a.s.kv_max, a.pre_len, a.window);
+    Cut k = rows_cut(a.s.rows, a.s.n, a.n_heads, a.n_kv, a.s.kv_max, a.pre_len);
+    RowsPlan &p = k.p;
     p.ml = (float *)scratch;
     p.o = (float *)((uint8_t *)scratch + ml_bytes(p, a.s.rows, a.n_heads));
-    const dim3 grid((unsigned)((p.tiles * p.ns + p.pre_tiles * p.pre_ns) * a.n_kv)), block(256);
-    if (!half && a.head_dim > 64) hipLaunchKernelGGL((k_rows_f<128, 4>), grid, block, 0, st, a, p);
-    else if (!half) hipLaunchKernelGGL((k_rows_f<64, 4>), grid, block, 0, st, a, p);
-    else if (a.head_dim > 64) hipLaunchKernelGGL(k_rows_h<128>, grid, block, 0, st, a, p);
-    else hipLaunchKernelGGL(k_rows_h<64>, grid, block, 0, st, a, p);
-    if (p.nrec)
-        hipLaunchKernelGGL(k_rows_combine, dim3((unsigned)(((long long)a.s.rows * a.n_heads + 3) / 4)), block, 0, st, a, p);
+    if (p.pre_tiles && k.narrow != k.pre_narrow) {
+        RowsPlan one = p;
+        one.tiles = 0;
+        launch_part(a, one, half, k.pre_narrow, st);
+        one = p;
+        one.pre_tiles = 0;
+        launch_part(a, one, half, k.narrow, st);
+    } else {
+        launch_part(a, p, half, k.narrow, st);
+    }
+    if (!p.nrec) return;
+    const long long rows = (long long)a.s.rows * a.n_heads;
+    const dim3 one((unsigned)((rows + 3) / 4)), each((unsigned)rows), block(256);
+    if (a.head_dim > 64) {
+        if (p.nrec > 16) hipLaunchKernelGGL((k_rows_combine<4, 32>), each, block, 0, st, a, p);
+        else hipLaunchKernelGGL((k_rows_combine<1, 32>), one, block, 0, st, a, p);
+    } else {
+        if (p.nrec > 16) hipLaunchKernelGGL((k_rows_combine<4, 16>), each, block, 0, st, a, p);
+        else hipLaunchKernelGGL((k_rows_combine<1, 16>), one, block, 0, st, a, p);
+    }
 }
 
 }  // namespace tg
