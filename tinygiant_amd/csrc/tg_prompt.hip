@@ -163,7 +163,6 @@ struct RowsPlan {
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int MT = 128;   /* m-rows of a workgroup: 32 a wave */
 constexpr int KT = 64;    /* positions of a tile */
 
 /* what a workgroup works on, uniform over it */
@@ -281,7 +280,7 @@ __device__ inline const T *region(const PromptArgs &a, const Work &w, const void
                     : (const T *)own + ((size_t)w.sq.slot * a.n_kv + w.kh) * a.s.kv_max * a.head_dim;
 }
 
-/* One m-row over the work's span by the whole workgroup, from the formulas
+/* One m-row over the work's span by 256 threads of the workgroup, from the formulas
  * with plain loads: only positions that the row sees are read.  It is how
  * rows are computed that came out of the matrix units not finite, which
  * multiply every value of a tile: 0 * inf there is not a row's own result.
@@ -290,6 +289,7 @@ template <typename T>
 __device__ void slow_row(const PromptArgs &a, const RowsPlan &p, const Work &w, int m, int ratio, float *lds) {
     float *qs = lds, *sc = lds + PROMPT_MAX_HEAD_DIM, *red = sc + 256;
     const int tid = threadIdx.x, hd = a.head_dim;
+    const bool on = tid < 256;   /* further threads only keep the barriers */
     const int i = m / ratio, h = w.kh * ratio + (m - i * ratio), r = w.sq.r0 + i;
     int first = 0, last = -1;
     (void)row_sees(a, w, m, ratio, first, last);
@@ -303,22 +303,22 @@ __device__ void slow_row(const PromptArgs &a, const RowsPlan &p, const Work &w, 
     for (int t0 = first; t0 <= last; t0 += 256) {
         const int pz = t0 + tid;
         float z = -INFINITY;
-        if (pz <= last) {
+        if (on && pz <= last) {
             const T *row = k + (size_t)pz * hd;
             float acc = 0.f;
             for (int d = 0; d < hd; d++) acc = fmaf(qs[d], (float)row[d], acc);
             z = acc * scale;
         }
         float t = wave_max(z);
-        if ((tid & 63) == 0) red[tid >> 6] = t;
+        if (on && (tid & 63) == 0) red[tid >> 6] = t;
         __syncthreads();
         t = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
         const float mn = fmaxf(mx, t), base = mn == -INFINITY ? 0.f : mn, alpha = exp2f(mx - base);
-        const float e = pz <= last ? exp2f(z - base) : 0.f;
-        sc[tid] = e;
+        const float e = on && pz <= last ? exp2f(z - base) : 0.f;
+        if (on) sc[tid] = e;
         const float s = wave_sum(e);
         __syncthreads();
-        if ((tid & 63) == 0) red[tid >> 6] = s;
+        if (on && (tid & 63) == 0) red[tid >> 6] = s;
         __syncthreads();
         l = l * alpha + ((red[0] + red[1]) + (red[2] + red[3]));
         mx = mn;
@@ -380,19 +380,38 @@ __device__ inline constexpr int swz(int key) {
 
 __device__ inline h8 h8_of(h4 a, h4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
+/* LDS by pointer, so that constant offsets go into the instructions */
+typedef const __attribute__((address_space(3))) uint8_t *Lds;
 /* four values of one column of 16-bit values, rows in consecutive lanes' rows */
-__device__ inline h4 lds_column(uint32_t addr) {
+__device__ inline h4 lds_column(Lds at) {
     typedef __fp16 g4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) g4 *P;
-    return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((P)(uintptr_t)addr));
+    return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((P)at));
 }
-__device__ inline h8 lds_row(uint32_t addr) {
-    typedef __attribute__((address_space(3))) h8 *P;
-    return *(P)(uintptr_t)addr;
+__device__ inline h8 lds_row(Lds at) { return *(const __attribute__((address_space(3))) h8 *)at; }
+/* The larger of two, NaN if either is: one instruction, where fmaxf quiets
+ * operands that may be signalling first (50 instead of 16 in a tile's
+ * softmax).  A NaN makes its row not finite, and such rows are done again. */
+__device__ inline float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+/* y = x f = hi + lo in two f16, each to nearest, for two values: one packed
+ * conversion and a mixed-precision fma each.  The empty asm keeps the packed
+ * pair as it is (the compiler would convert each value once more for lo); a
+ * factor that it knows to be 1 would make the fma three instructions. */
+__device__ inline void split2(float y0, float y1, float x0, float x1, float f, h2 &hi, h2 &lo) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    hi = __builtin_convertvector((f2{y0, y1}), h2);
+    asm("" : "+v"(hi));
+    lo = h2{(_Float16)fmaf(x0, f, -(float)hi[0]), (_Float16)fmaf(x1, f, -(float)hi[1])};
+}
+__device__ inline float opaque_one() {
+    float f = 1.f;
+    asm("" : "+s"(f));
+    return f;
 }
 __device__ inline float other_half_max(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    return max_nan(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ inline float other_half_sum(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -409,25 +428,50 @@ struct Lane {
     int r, h;        /* packed row, query head */
     int any_lo, any_hi, all_lo, all_hi;
 };
-__device__ inline Lane lane_rows(const PromptArgs &a, const Work &w, int m, int ratio) {
+/* ms: the wave's m-rows from m0 on, of which the lane takes m0 + at */
+__device__ inline Lane lane_rows(const PromptArgs &a, const Work &w, int m0, int at, int ms, int ratio) {
     Lane x;
-    x.first = 0, x.last = 0x7FFFFFFF;
-    x.live = row_sees(a, w, m, ratio, x.first, x.last);
+    int first = 0, last = 0;
+    const int m = m0 + at;
+    x.live = row_sees(a, w, m, ratio, first, last);
     const int i = x.live ? m / ratio : 0;
     x.r = w.sq.r0 + i, x.h = w.kh * ratio + (x.live ? m - i * ratio : 0);
-    int lo = x.live ? x.first : 0x7FFFFFFF, hi = x.live ? x.last : -1, alo = x.live ? x.first : 0;
-    int ahi = x.live ? x.last : 0x7FFFFFFF;
-    if (!x.live) x.first = 0, x.last = 0x7FFFFFFF;
+    x.first = x.live ? first : 0, x.last = x.live ? last : 0x7FFFFFFF;
+    const int i0 = m0 / ratio, i1 = min(w.sq.n - 1, (m0 + ms - 1) / ratio);   /* uniform */
+    if (i0 > i1) {
+        x.any_lo = 0x7FFFFFFF, x.any_hi = -1, x.all_lo = 0, x.all_hi = 0x7FFFFFFF;
+    } else if (!w.prefix) {   /* later rows see later positions */
+        const int l0 = w.sq.past + i0, l1 = w.sq.past + i1;
+        x.any_hi = l1, x.all_hi = l0;
+        x.any_lo = a.window > 0 ? max(0, l0 + 1 - a.window) : 0;
+        x.all_lo = a.window > 0 ? max(0, l1 + 1 - a.window) : 0;
+    } else if (a.window <= 0) {
+        x.any_lo = x.all_lo = 0, x.any_hi = x.all_hi = a.pre_len - 1;
+    } else {   /* rows of sequences of any length */
+        int lo = x.live ? first : 0x7FFFFFFF, hi = x.live ? last : -1, alo = x.first, ahi = x.last;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        lo = min(lo, __shfl_xor(lo, o, 64));
-        hi = max(hi, __shfl_xor(hi, o, 64));
-        alo = max(alo, __shfl_xor(alo, o, 64));
-        ahi = min(ahi, __shfl_xor(ahi, o, 64));
+        for (int o = 32; o > 0; o >>= 1) {
+            lo = min(lo, __shfl_xor(lo, o, 64));
+            hi = max(hi, __shfl_xor(hi, o, 64));
+            alo = max(alo, __shfl_xor(alo, o, 64));
+            ahi = min(ahi, __shfl_xor(ahi, o, 64));
+        }
+        x.any_lo = lo, x.any_hi = hi, x.all_lo = alo, x.all_hi = ahi;
     }
-    x.any_lo = __builtin_amdgcn_readfirstlane(lo), x.any_hi = __builtin_amdgcn_readfirstlane(hi);
-    x.all_lo = __builtin_amdgcn_readfirstlane(alo), x.all_hi = __builtin_amdgcn_readfirstlane(ahi);
+    x.any_lo = __builtin_amdgcn_readfirstlane(x.any_lo), x.any_hi = __builtin_amdgcn_readfirstlane(x.any_hi);
+    x.all_lo = __builtin_amdgcn_readfirstlane(x.all_lo), x.all_hi = __builtin_amdgcn_readfirstlane(x.all_hi);
     return x;
+}
+
+/* the largest of the wave's words, uniform */
+__device__ inline uint32_t wave_umax(uint32_t v) {
+    v = max(v, (uint32_t)dpp_i<0xB1>((int)v));
+    v = max(v, (uint32_t)dpp_i<0x4E>((int)v));
+    v = max(v, (uint32_t)dpp_i<0x141>((int)v));
+    v = max(v, (uint32_t)dpp_i<0x140>((int)v));
+    const uint32_t a = (uint32_t)__builtin_amdgcn_readlane((int)v, 15), b = (uint32_t)__builtin_amdgcn_readlane((int)v, 31);
+    const uint32_t c = (uint32_t)__builtin_amdgcn_readlane((int)v, 47), d = (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+    return max(max(a, b), max(c, d));
 }
 
 /* the power of two that takes a largest magnitude to 2^13 .. 2^14, as its exponent */
@@ -527,38 +571,76 @@ __device__ inline uint32_t write_rows(const PromptArgs &a, const RowsPlan &p, co
     return bad;
 }
 
+/* Group 1's sums of a workgroup whose two groups of MW waves took the tiles
+ * in turn, through LDS (room: MW * 64 * (HD / 2 + 3) floats), into group 0's.
+ * oexp as in write_rows. */
+template <int HD, int MW>
+__device__ inline void merge_groups(float *lds, int wave, int lane, float &mx, float &l, int &oexp, f16v (&o)[HD / 32]) {
+    constexpr int N = HD / 2;   /* o values a lane */
+    float *at = lds + (wave % MW) * 64 * (N + 3);
+    __syncthreads();
+    if (wave >= MW) {
+#pragma unroll
+        for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+            for (int v = 0; v < 16; v += 4)
+                *(f4 *)&at[((16 * d + v) / 4 * 64 + lane) * 4] = f4{o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]};
+        at[64 * N + lane] = mx, at[64 * (N + 1) + lane] = l, at[64 * (N + 2) + lane] = __int_as_float(oexp);
+    }
+    __syncthreads();
+    if (wave >= MW) return;
+    const float m1 = at[64 * N + lane], M = max_nan(mx, m1), base = M == -INFINITY ? 0.f : M;
+    const int e1 = __float_as_int(at[64 * (N + 2) + lane]), e = min(oexp, e1);
+    const float a0 = __builtin_amdgcn_exp2f(mx - base), a1 = __builtin_amdgcn_exp2f(m1 - base);
+    const float f0 = __builtin_amdgcn_ldexpf(a0, e - oexp), f1 = __builtin_amdgcn_ldexpf(a1, e - e1);
+    l = fmaf(l, a0, at[64 * (N + 1) + lane] * a1);
+    mx = M, oexp = e;
+#pragma unroll
+    for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+        for (int v = 0; v < 16; v += 4) {
+            const f4 y = *(const f4 *)&at[((16 * d + v) / 4 * 64 + lane) * 4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) o[d][v + q] = fmaf(o[d][v + q], f0, y[q] * f1);
+        }
+}
+
 #define MFMA_H(a, b, c) __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0)
 
-template <int HD>
-__global__ __launch_bounds__(256, 2) void k_rows_h(PromptArgs a, RowsPlan p) {
+/* MW waves of 32 m-rows; with KG = 2, two groups of them take the tiles in turn */
+template <int HD, int MW, int KG>
+__global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_h(PromptArgs a, RowsPlan p) {
     constexpr int RB = HD * 2, TILE = KT * RB;       /* bytes of a row in LDS, of a tile of K or V */
-    constexpr int NC = TILE / 1024 / 4;              /* copies of 1 KiB a wave, matrix and tile */
+    constexpr int NC = TILE / 1024 / MW;             /* copies of 1 KiB a wave, matrix and tile */
     constexpr int DB = HD / 32, STEPS = HD / 16;
-    __shared__ __attribute__((aligned(1024))) uint8_t buf[2][2][TILE];
-    __shared__ uint32_t bad_rows[4];
+    __shared__ __attribute__((aligned(1024))) uint8_t bufs[KG][2][2][TILE];
+    __shared__ uint32_t bad_rows[MW];
     const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
     Work w;
-    if (!find_work<MT>(a, p, ratio, w)) return;
+    if (!find_work<32 * MW>(a, p, ratio, w)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int half = lane >> 5;
-    const Lane x = lane_rows(a, w, w.m0 + 32 * wave + (lane & 31), ratio);
+    const int half = lane >> 5, group = wave / MW, mwave = wave % MW;
+    static_assert(KG == 1 || sizeof bufs >= MW * 256 * (HD / 2 + 3), "merge_groups");
+    uint8_t(*buf)[2][TILE] = bufs[group];
 
-    /* copies: LDS byte 1024 n + 16 l of a tile is piece c' of row key; n = wave + 4 k */
+    /* copies: LDS byte 1024 n + 16 l of a tile is piece c' of row key; n = mwave + MW k */
     const uint32_t rb = (uint32_t)hd * 2u;
     const u32x4 kd = buf_desc(region<_Float16>(a, w, a.kv_k, a.pre_k), (uint32_t)w.hi * rb);
     const u32x4 vd = buf_desc(region<_Float16>(a, w, a.kv_v, a.pre_v), (uint32_t)w.hi * rb);
-    const int ckey = (1024 * wave + 16 * lane) / RB, cpiece = (lane % (RB / 16)) ^ swz<HD>(ckey);
+    const int ckey = (1024 * mwave + 16 * lane) / RB, cpiece = (lane % (RB / 16)) ^ swz<HD>(ckey);
     const uint32_t coff = 8 * cpiece < hd ? (uint32_t)ckey * rb + 16u * (uint32_t)cpiece : 0x7FFFFF00u;
     auto copy_tile = [&](int t0, int b) __attribute__((always_inline)) {
         const uint32_t at = coff + (uint32_t)t0 * rb;
 #pragma unroll
         for (int k = 0; k < NC; k++) {
-            const uint32_t src = at + (uint32_t)k * (4096u / RB) * rb, dst = 1024u * (uint32_t)(wave + 4 * k);
+            const uint32_t src = at + (uint32_t)k * (MW * 1024u / RB) * rb, dst = 1024u * (uint32_t)(mwave + MW * k);
             copy_lanes(kd, src, lds_addr(buf[b][0]) + dst);
             copy_lanes(vd, src, lds_addr(buf[b][1]) + dst);
         }
     };
-    if (w.lo < w.hi) copy_tile(w.lo, 0);
+    static_assert(MW * 1024 / RB % 16 == 0, "swz of a copy's rows is that of the first");
+    if (w.lo + group * KT < w.hi) copy_tile(w.lo + group * KT, 0);
+    const Lane x = lane_rows(a, w, w.m0 + 32 * mwave, lane & 31, 32, ratio);
 
     h8 qh[STEPS], ql[STEPS];
     const float c = load_q<HD>(a, x, half, qh, ql);
@@ -573,29 +655,38 @@ __global__ __launch_bounds__(256, 2) void k_rows_h(PromptArgs a, RowsPlan p) {
 #pragma unroll
     for (int d = 0; d < DB; d++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) vaddr[d][e] = v_operand<HD>(lane, d, e);
+        for (int e = 0; e < 2; e++) vaddr[d][e] = TILE + v_operand<HD>(lane, d, e);
 
+    const float one = opaque_one();
     int b = 0;
-    for (int t = w.lo; t < w.hi; t += KT, b ^= 1) {
+    for (int t0 = w.lo; t0 < w.hi; t0 += KG * KT, b ^= 1) {
+        const int t = t0 + group * KT;
         wait_copies();
         bar_lds();   /* every wave's copies of this tile are there, and every wave is done with the other buffer */
-        if (t + KT < w.hi) copy_tile(t + KT, b ^ 1);
-        if (t > x.any_hi || t + KT <= x.any_lo) continue;   /* uniform in the wave */
-        const uint32_t kb = lds_addr(buf[b][0]), vb = lds_addr(buf[b][1]);
+        if (t + KG * KT < w.hi) copy_tile(t + KG * KT, b ^ 1);
+        if (t > x.any_hi || t + KT <= x.any_lo || t >= w.hi) continue;   /* uniform in the wave */
+        const Lds tile = (Lds)buf[b][0];
         f16v s[2];
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
             for (int v = 0; v < 16; v++) s[n][v] = 0.f;
+        h8 k0 = lds_row(tile + kaddr), k1 = lds_row(tile + kaddr + 32 * RB);
 #pragma unroll
-        for (int st = 0; st < STEPS; st++) {
-            const uint32_t at = kb + (kaddr ^ (uint32_t)(st << 5));
-            const h8 k0 = lds_row(at), k1 = lds_row(at + 32 * RB);
+        for (int st = 0; st < STEPS; st++) {   /* the next step's operands are read a step ahead */
+            const Lds at = tile + (kaddr ^ (uint32_t)((st + 1) << 5));
+            const h8 n0 = st + 1 < STEPS ? lds_row(at) : k0, n1 = st + 1 < STEPS ? lds_row(at + 32 * RB) : k1;
             s[0] = MFMA_H(k0, ql[st], s[0]);
             s[1] = MFMA_H(k1, ql[st], s[1]);
             s[0] = MFMA_H(k0, qh[st], s[0]);
             s[1] = MFMA_H(k1, qh[st], s[1]);
+            k0 = n0, k1 = n1;
         }
+        auto column = [&](int i) __attribute__((always_inline)) {
+            const int q = i / DB, d = i % DB;
+            return h8_of(lds_column(tile + vaddr[d][0] + q * 16 * RB), lds_column(tile + vaddr[d][1] + q * 16 * RB));
+        };
+        h8 v0 = column(0), v1 = column(1);
         if (t + KT - 1 > x.all_hi || t < x.all_lo) {   /* some row does not see all of the tile */
 #pragma unroll
             for (int n = 0; n < 2; n++)
@@ -605,11 +696,11 @@ __global__ __launch_bounds__(256, 2) void k_rows_h(PromptArgs a, RowsPlan p) {
                     s[n][v] = pos <= x.last && pos >= x.first ? s[n][v] : -INFINITY;
                 }
         }
-        float top = fmaxf(s[0][0], s[1][0]);
+        float top = max_nan(s[0][0], s[1][0]);
 #pragma unroll
-        for (int v = 1; v < 16; v++) top = fmaxf(top, fmaxf(s[0][v], s[1][v]));
+        for (int v = 1; v < 16; v++) top = max_nan(max_nan(top, s[0][v]), s[1][v]);
         top = other_half_max(top) * c;
-        const float mn = fmaxf(mx, top), sh = mn == -INFINITY ? 0.f : W_SHIFT - mn;
+        const float mn = max_nan(mx, top), sh = mn == -INFINITY ? 0.f : W_SHIFT - mn;
         if (__any(mn > mx)) {
             const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
             l *= alpha;
@@ -624,30 +715,39 @@ __global__ __launch_bounds__(256, 2) void k_rows_h(PromptArgs a, RowsPlan p) {
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
-            for (int v = 0; v < 16; v++) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(s[n][v], c, sh));
-                sum[v & 3] += e;
-                const _Float16 hi = (_Float16)e;
-                ph[2 * n + (v >> 3)][v & 7] = hi;
-                pl[2 * n + (v >> 3)][v & 7] = (_Float16)(e - (float)hi);
+            for (int v = 0; v < 16; v += 2) {
+                const float e0 = __builtin_amdgcn_exp2f(fmaf(s[n][v], c, sh));
+                const float e1 = __builtin_amdgcn_exp2f(fmaf(s[n][v + 1], c, sh));
+                sum[v & 3] += e0, sum[(v & 3) + 1] += e1;
+                h2 hi, lo;
+                split2(e0, e1, e0, e1, one, hi, lo);
+                const int q = 2 * n + (v >> 3), at = v & 7;
+                ph[q][at] = hi[0], ph[q][at + 1] = hi[1];
+                pl[q][at] = lo[0], pl[q][at + 1] = lo[1];
             }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-        for (int q = 0; q < 4; q++)
-#pragma unroll
-            for (int d = 0; d < DB; d++) {
-                const uint32_t at = vb + (uint32_t)(q * 16 * RB);
-                const h8 vt = h8_of(lds_column(at + vaddr[d][0]), lds_column(at + vaddr[d][1]));
-                o[d] = MFMA_H(vt, pl[q], o[d]);
-                o[d] = MFMA_H(vt, ph[q], o[d]);
-            }
+        for (int i = 0; i < 4 * DB; i += 2) {
+            const h8 n0 = i + 2 < 4 * DB ? column(i + 2) : v0, n1 = i + 2 < 4 * DB ? column(i + 3) : v1;
+            const int q = i / DB, d = i % DB;
+            o[d] = MFMA_H(v0, pl[q], o[d]);
+            o[d + 1] = MFMA_H(v1, pl[q], o[d + 1]);
+            o[d] = MFMA_H(v0, ph[q], o[d]);
+            o[d + 1] = MFMA_H(v1, ph[q], o[d + 1]);
+            v0 = n0, v1 = n1;
+        }
     }
-    const uint32_t bad = write_rows<HD>(a, p, w, x, lane, mx, other_half_sum(l), 0, o);
-    if (lane == 0) bad_rows[wave] = bad;
+    l = other_half_sum(l);
+    int oexp = 0;
+    if constexpr (KG == 2) merge_groups<HD, MW>((float *)bufs, wave, lane, mx, l, oexp, o);
+    if (group == 0) {
+        const uint32_t bad = write_rows<HD>(a, p, w, x, lane, mx, l, oexp, o);
+        if (lane == 0) bad_rows[wave] = bad;
+    }
     __syncthreads();
-    for (int wv = 0; wv < 4; wv++)
+    for (int wv = 0; wv < MW; wv++)
         for (uint32_t y = bad_rows[wv]; y; y &= y - 1)
-            slow_row<_Float16>(a, p, w, w.m0 + 32 * wv + __builtin_ctz(y), ratio, (float *)buf);
+            slow_row<_Float16>(a, p, w, w.m0 + 32 * wv + __builtin_ctz(y), ratio, (float *)bufs);
 }
 
 /* ---- float32 caches on the f16 matrix units ----
@@ -671,64 +771,67 @@ __global__ __launch_bounds__(256, 2) void k_rows_h(PromptArgs a, RowsPlan p) {
  * V lo][32][HD]). */
 constexpr int KF = 32;
 
-template <int HD, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void k_rows_f(PromptArgs a, RowsPlan p) {
+template <int HD, int MW, int KG>
+__global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPlan p) {
     constexpr int RB = HD * 2, PLANE = KF * RB;
-    constexpr int UNITS = 8 / NW;                    /* groups a wave loads: K 0 .. 3, V 4 .. 7 */
+    constexpr int UNITS = 8 / MW;                    /* groups a wave loads: K 0 .. 3, V 4 .. 7 */
     constexpr int LR = 256 / HD, NL = 8 / LR;        /* rows a load of the wave covers, loads a group */
     constexpr int DB = HD / 32, STEPS = HD / 16;
-    __shared__ __attribute__((aligned(1024))) uint8_t buf[2][4][PLANE];
-    __shared__ int exps[2][8];
-    __shared__ uint32_t bad_rows[NW];
+    __shared__ __attribute__((aligned(1024))) uint8_t bufs[KG][2][4][PLANE];
+    __shared__ int all_exps[KG][2][8];
+    __shared__ uint32_t bad_rows[MW];
     const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
     Work w;
-    if (!find_work<32 * NW>(a, p, ratio, w)) return;
+    if (!find_work<32 * MW>(a, p, ratio, w)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int half = lane >> 5;
-    const Lane x = lane_rows(a, w, w.m0 + 32 * wave + (lane & 31), ratio);
+    const int half = lane >> 5, group = wave / MW, mwave = wave % MW;
+    static_assert(KG == 1 || sizeof bufs >= MW * 256 * (HD / 2 + 3), "merge_groups");
+    uint8_t(*buf)[4][PLANE] = bufs[group];
+    int(*exps)[8] = all_exps[group];
 
     /* loads: lane l of load j of group g holds dims 4 (l % (HD / 4)) .. of position 8 g + LR j + l / (HD / 4) */
     const uint32_t rb = (uint32_t)hd * 4u;
-    const Buf kd = make_buf_uniform(region<float>(a, w, a.kv_k, a.pre_k), (uint32_t)w.hi * rb);
-    const Buf vd = make_buf_uniform(region<float>(a, w, a.kv_v, a.pre_v), (uint32_t)w.hi * rb);
+    const float *kp = region<float>(a, w, a.kv_k, a.pre_k), *vp = region<float>(a, w, a.kv_v, a.pre_v);
+    const Buf kd = make_buf_uniform(UNITS == 2 || mwave < 4 ? kp : vp, (uint32_t)w.hi * rb);   /* of the first unit */
+    const Buf vd = make_buf_uniform(vp, (uint32_t)w.hi * rb);
     const int lrow = lane / (HD / 4), ldim = 4 * (lane % (HD / 4));
     const uint32_t loff = ldim < hd ? (uint32_t)lrow * rb + 4u * (uint32_t)ldim : 0x7FFFFF00u;
     u32x4 raw[UNITS][NL];
     auto load_tile = [&](int t0) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < UNITS; u++) {
-            const int g = u * NW + wave;
+            const int g = u * MW + mwave;
 #pragma unroll
             for (int j = 0; j < NL; j++) {
                 const uint32_t at = loff + (uint32_t)(t0 + 8 * (g & 3) + LR * j) * rb;
-                if (UNITS == 1) raw[u][j] = g < 4 ? ld16(kd, at) : ld16(vd, at);
-                else raw[u][j] = u == 0 ? ld16(kd, at) : ld16(vd, at);
+                raw[u][j] = ld16(u == 0 ? kd : vd, at);
             }
         }
     };
     auto split_tile = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < UNITS; u++) {
-            const int g = u * NW + wave;
+            const int g = u * MW + mwave;
             float big = 0.f;
 #pragma unroll
             for (int j = 0; j < NL; j++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) big = fmaxf(big, fabsf(__uint_as_float(raw[u][j][e])));
-            big = wave_max(big);
-            if (!(big < INFINITY)) {   /* uniform: the largest of the finite ones */
-                big = 0.f;
+                for (int e = 0; e < 4; e += 2)
+                    big = max_nan(max_nan(big, fabsf(__uint_as_float(raw[u][j][e]))), fabsf(__uint_as_float(raw[u][j][e + 1])));
+            uint32_t bits = wave_umax(__float_as_uint(big));
+            if (bits >= 0x7F800000u) {   /* uniform: the largest of the finite ones */
+                uint32_t fin = 0;
 #pragma unroll
                 for (int j = 0; j < NL; j++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float y = fabsf(__uint_as_float(raw[u][j][e]));
-                        big = fmaxf(big, y < INFINITY ? y : 0.f);
+                        const uint32_t y = raw[u][j][e] & 0x7FFFFFFFu;
+                        fin = max(fin, y < 0x7F800000u ? y : 0u);
                     }
-                big = wave_max(big);
+                bits = wave_umax(fin);
             }
-            const int ex = big > 0.f ? scale_exp(big) : 100;
-            const float f = __builtin_amdgcn_ldexpf(1.f, ex);
+            const int ex = min(140 - (int)(bits >> 23), 100);   /* scale_exp, and 100 where all are zero */
+            const float f = __uint_as_float((uint32_t)(ex + 127) << 23);
             if (lane == 0) exps[b][g] = ex;
 #pragma unroll
             for (int j = 0; j < NL; j++) {
@@ -736,17 +839,20 @@ __global__ __launch_bounds__(64 * NW, 2) void k_rows_f(PromptArgs a, RowsPlan p)
                 const uint32_t at = (uint32_t)(key * RB + (((ldim >> 3) ^ swz<HD>(key)) << 4) + 2 * (ldim & 4));
                 h4 hi, lo;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float y = __uint_as_float(raw[u][j][e]) * f;
-                    hi[e] = (_Float16)y;
-                    lo[e] = (_Float16)(y - (float)hi[e]);
+                for (int e = 0; e < 4; e += 2) {
+                    h2 y, z;
+                    const float x0 = __uint_as_float(raw[u][j][e]), x1 = __uint_as_float(raw[u][j][e + 1]);
+                    split2(x0 * f, x1 * f, x0, x1, f, y, z);
+                    hi[e] = y[0], hi[e + 1] = y[1], lo[e] = z[0], lo[e + 1] = z[1];
                 }
                 *(h4 *)(buf[b][2 * (g >> 2)] + at) = hi;
                 *(h4 *)(buf[b][2 * (g >> 2) + 1] + at) = lo;
             }
         }
     };
-    if (w.lo < w.hi) load_tile(w.lo);
+    const int t1 = w.lo + group * KF;   /* the group's first tile; past the span: zeros */
+    load_tile(t1);
+    const Lane x = lane_rows(a, w, w.m0 + 32 * mwave, lane & 31, 32, ratio);
 
     h8 qh[STEPS], ql[STEPS];
     const float c = load_q<HD>(a, x, half, qh, ql);
@@ -762,34 +868,44 @@ __global__ __launch_bounds__(64 * NW, 2) void k_rows_f(PromptArgs a, RowsPlan p)
 #pragma unroll
     for (int d = 0; d < DB; d++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) vaddr[d][e] = v_operand<HD>(lane, d, e);
+        for (int e = 0; e < 2; e++) vaddr[d][e] = 2 * PLANE + v_operand<HD>(lane, d, e);
 
-    if (w.lo < w.hi) {
-        split_tile(0);
-        load_tile(w.lo + KF);   /* past the region: zeros */
-    }
+    split_tile(0);
+    load_tile(t1 + KG * KF);
     __syncthreads();
     int b = 0;
-    for (int t = w.lo; t < w.hi; t += KF, b ^= 1) {
-        if (t <= x.any_hi && t + KF > x.any_lo) {   /* uniform in the wave */
-            const uint32_t kb = lds_addr(buf[b][0]), vb = lds_addr(buf[b][2]);
+    for (int t0 = w.lo; t0 < w.hi; t0 += KG * KF, b ^= 1) {
+        const int t = t0 + group * KF;
+        if (t <= x.any_hi && t + KF > x.any_lo && t < w.hi) {   /* uniform in the wave */
+            const Lds tile = (Lds)buf[b][0];
+            const int ex = exps[b][lane & 7];
             int ke[4], ve[4];
 #pragma unroll
             for (int g = 0; g < 4; g++) {
-                ke[g] = __builtin_amdgcn_readfirstlane(exps[b][g]);
-                ve[g] = __builtin_amdgcn_readfirstlane(exps[b][4 + g]);
+                ke[g] = __builtin_amdgcn_readlane(ex, g);
+                ve[g] = __builtin_amdgcn_readlane(ex, 4 + g);
             }
             f16v s;
 #pragma unroll
             for (int v = 0; v < 16; v++) s[v] = 0.f;
+            h8 kh = lds_row(tile + kaddr), kl = lds_row(tile + kaddr + PLANE);
+            f16v z = s;   /* two chains */
 #pragma unroll
-            for (int st = 0; st < STEPS; st++) {
-                const uint32_t at = kb + (kaddr ^ (uint32_t)(st << 5));
-                const h8 kh = lds_row(at), kl = lds_row(at + PLANE);
-                s = MFMA_H(kl, qh[st], s);
-                s = MFMA_H(kh, ql[st], s);
+            for (int st = 0; st < STEPS; st++) {   /* the next step's operands are read a step ahead */
+                const Lds at = tile + (kaddr ^ (uint32_t)((st + 1) << 5));
+                const h8 nh = st + 1 < STEPS ? lds_row(at) : kh, nl = st + 1 < STEPS ? lds_row(at + PLANE) : kl;
+                z = MFMA_H(kl, qh[st], z);
                 s = MFMA_H(kh, qh[st], s);
+                z = MFMA_H(kh, ql[st], z);
+                kh = nh, kl = nl;
             }
+#pragma unroll
+            for (int v = 0; v < 16; v++) s[v] += z[v];
+            auto column = [&](int i, int lo) __attribute__((always_inline)) {
+                const int q = i / DB, d = i % DB, at = q * 16 * RB + lo * PLANE;
+                return h8_of(lds_column(tile + vaddr[d][0] + at), lds_column(tile + vaddr[d][1] + at));
+            };
+            h8 vh = column(0, 0), vl = column(0, 1);
             if (t + KF - 1 > x.all_hi || t < x.all_lo) {   /* some row does not see all of the tile */
 #pragma unroll
                 for (int v = 0; v < 16; v++) {
@@ -801,11 +917,11 @@ __global__ __launch_bounds__(64 * NW, 2) void k_rows_f(PromptArgs a, RowsPlan p)
 #pragma unroll
             for (int g = 0; g < 4; g++) {
                 cg[g] = __builtin_amdgcn_ldexpf(c, -ke[g]);
-                top = fmaxf(top, fmaxf(fmaxf(s[4 * g], s[4 * g + 1]), fmaxf(s[4 * g + 2], s[4 * g + 3])) * cg[g]);
+                top = max_nan(top, max_nan(max_nan(max_nan(s[4 * g], s[4 * g + 1]), s[4 * g + 2]), s[4 * g + 3]) * cg[g]);
             }
             top = other_half_max(top);
             const int un = min(min(U, min(ve[0], ve[1])), min(ve[2], ve[3]));
-            const float mn = fmaxf(mx, top), sh = mn == -INFINITY ? 0.f : W_SHIFT - mn;
+            const float mn = max_nan(mx, top), sh = mn == -INFINITY ? 0.f : W_SHIFT - mn;
             if (__any(mn > mx) || un != U) {
                 const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
                 const float beta = __builtin_amdgcn_ldexpf(alpha, un - U);
@@ -822,40 +938,44 @@ __global__ __launch_bounds__(64 * NW, 2) void k_rows_f(PromptArgs a, RowsPlan p)
             for (int g = 0; g < 4; g++) {
                 const float f = __builtin_amdgcn_ldexpf(1.f, un - ve[g]);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float y = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], cg[g], sh));
-                    sum[e] += y;
-                    y *= f;
-                    const _Float16 hi = (_Float16)y;
-                    ph[g >> 1][4 * (g & 1) + e] = hi;
-                    pl[g >> 1][4 * (g & 1) + e] = (_Float16)(y - (float)hi);
+                for (int e = 0; e < 4; e += 2) {
+                    const float y0 = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], cg[g], sh));
+                    const float y1 = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e + 1], cg[g], sh));
+                    sum[e] += y0, sum[e + 1] += y1;
+                    h2 hi, lo;
+                    split2(y0 * f, y1 * f, y0, y1, f, hi, lo);
+                    const int at = 4 * (g & 1) + e;
+                    ph[g >> 1][at] = hi[0], ph[g >> 1][at + 1] = hi[1];
+                    pl[g >> 1][at] = lo[0], pl[g >> 1][at + 1] = lo[1];
                 }
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-            for (int q = 0; q < 2; q++)
-#pragma unroll
-                for (int d = 0; d < DB; d++) {
-                    const uint32_t at = vb + (uint32_t)(q * 16 * RB);
-                    const h8 vh = h8_of(lds_column(at + vaddr[d][0]), lds_column(at + vaddr[d][1]));
-                    const h8 vl = h8_of(lds_column(at + PLANE + vaddr[d][0]), lds_column(at + PLANE + vaddr[d][1]));
-                    o[d] = MFMA_H(vl, ph[q], o[d]);
-                    o[d] = MFMA_H(vh, pl[q], o[d]);
-                    o[d] = MFMA_H(vh, ph[q], o[d]);
-                }
+            for (int i = 0; i < 2 * DB; i++) {
+                const h8 nh = i + 1 < 2 * DB ? column(i + 1, 0) : vh, nl = i + 1 < 2 * DB ? column(i + 1, 1) : vl;
+                const int q = i / DB, d = i % DB;
+                o[d] = MFMA_H(vl, ph[q], o[d]);
+                o[d] = MFMA_H(vh, pl[q], o[d]);
+                o[d] = MFMA_H(vh, ph[q], o[d]);
+                vh = nh, vl = nl;
+            }
         }
-        if (t + KF < w.hi) {
+        if (t + KG * KF < w.hi) {
             split_tile(b ^ 1);
-            load_tile(t + 2 * KF);
+            load_tile(t + 2 * KG * KF);
         }
         bar_lds();
     }
-    const uint32_t bad = write_rows<HD>(a, p, w, x, lane, mx, other_half_sum(l), U, o);
-    if (lane == 0) bad_rows[wave] = bad;
+    l = other_half_sum(l);
+    if constexpr (KG == 2) merge_groups<HD, MW>((float *)bufs, wave, lane, mx, l, U, o);
+    if (group == 0) {
+        const uint32_t bad = write_rows<HD>(a, p, w, x, lane, mx, l, U, o);
+        if (lane == 0) bad_rows[wave] = bad;
+    }
     __syncthreads();
-    for (int wv = 0; wv < NW; wv++)
+    for (int wv = 0; wv < MW; wv++)
         for (uint32_t y = bad_rows[wv]; y; y &= y - 1)
-            slow_row<float>(a, p, w, w.m0 + 32 * wv + __builtin_ctz(y), ratio, (float *)buf);
+            slow_row<float>(a, p, w, w.m0 + 32 * wv + __builtin_ctz(y), ratio, (float *)bufs);
 }
 
 /* ---- few rows: positions over the waves ----
@@ -987,7 +1107,7 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
     if (!find_work<MN>(a, p, ratio, w)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c16 = lane & 15, kq = lane >> 4;
-    const Lane x = lane_rows(a, w, w.m0 + c16, ratio);
+    const Lane x = lane_rows(a, w, w.m0, c16, 16, ratio);
     if (tid == 0) bad_rows = 0;
 
     const uint32_t rb = (uint32_t)hd * (uint32_t)sizeof(T);
@@ -1052,7 +1172,7 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
     __syncthreads();
     /* the four waves' sums as one, in wave order: 16 threads a row, HD / 16 dims each */
     const int row = tid >> 4, d0 = (tid & 15) * N;
-    const Lane y = lane_rows(a, w, w.m0 + row, ratio);
+    const Lane y = lane_rows(a, w, w.m0, row, 16, ratio);
     float M = fmaxf(fmaxf(mm[0][row], mm[1][row]), fmaxf(mm[2][row], mm[3][row]));
     const float base = M == -INFINITY ? 0.f : M;
     float L = 0.f, r[N];
@@ -1125,11 +1245,19 @@ __global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) 
         const float e = x.x == -INFINITY ? 0.f : exp2f(x.x - base);
         l += e == 0.f ? 0.f : x.y * e;
         const int n = min(64, (p.nrec - c0 - wave + W - 1) / W);
-#pragma unroll 4
-        for (int j = g; j < n; j += PER) {
-            const float f = __shfl(e, j, 64);
-            if (f == 0.f || d >= hd) continue;   /* a record of no position has no sums */
-            o += *(const f4 *)(po + (size_t)(c0 + W * j + wave) * hd + d) * f;
+        for (int j0 = 0; j0 < n; j0 += 4 * PER) {   /* four records' loads at a time */
+            f4 y[4];
+            float f[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int j = j0 + q * PER + g;
+                f[q] = __shfl(e, j & 63, 64);
+                y[q] = f4{0.f, 0.f, 0.f, 0.f};
+                if (j < n && f[q] != 0.f && d < hd)   /* a record of no position has no sums */
+                    y[q] = *(const f4 *)(po + (size_t)(c0 + W * j + wave) * hd + d);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; q++) o += y[q] * f[q];
         }
     }
     l = wave_sum(l);
@@ -1157,30 +1285,41 @@ __global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) 
 }
 
 /* How a call is cut, from the host's arguments alone (the lengths are on the
- * device).  A part (the sequences' slots; the prefix) runs on the narrow
- * kernel where its tiles would have few m-rows. */
+ * device).  Each part, the sequences' slots and the prefix, has a shape:
+ *   narrow  16 m-rows a workgroup, positions over its waves
+ *   wide    128 m-rows, two groups of four waves on tiles in turn: two waves
+ *           a SIMD where there are no more workgroups than CUs
+ *   full    128 m-rows, four waves; several workgroups a CU
+ *   tall    256 m-rows, eight waves (f32 caches): half the splitting of K and
+ *           V a row */
+enum Shape { NARROW, WIDE, FULL, TALL };
+constexpr int SHAPE_ROWS[] = {16, 128, 128, 256}, SHAPE_THREADS[] = {256, 512, 256, 512};
 struct Cut {
     RowsPlan p;
-    bool narrow, pre_narrow;
+    Shape own, pre;
 };
-static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int kv_max, int pre_len) {
+static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int kv_max, int pre_len, bool half) {
     Cut k = {};
     RowsPlan &p = k.p;
     const int ratio = n_heads / n_kv;
     const long long m = (long long)n_rows * ratio;
-    auto spans = [&](long long wgs, int positions, bool narrow) {
-        const int least = narrow ? 128 : 4 * KT;
-        const int want = (int)((512 + wgs - 1) / wgs), most = (positions + least - 1) / least;
+    auto shape = [&](long long seqs, int positions) {
+        if (m <= 64 * seqs) return NARROW;
+        if (!half && m / 256 * n_kv * positions >= 512ll * 2048) return TALL;
+        return m / 128 * n_kv >= 512 ? FULL : WIDE;
+    };
+    auto spans = [&](Shape s, long long wgs, int positions) {
+        const int least = s == NARROW ? 128 : 4 * KT, most = (positions + least - 1) / least;
+        const int want = (int)((s == WIDE || s == TALL ? 256 : 512) / wgs);
         return std::max(1, std::min(std::min(want, most), 128));
     };
-    k.narrow = m <= 64ll * n_seqs;
-    k.pre_narrow = m <= 64;
-    p.tiles = (int)std::min(m / (k.narrow ? MN : MT) + n_seqs, m);
-    p.ns = spans((long long)p.tiles * n_kv, kv_max, k.narrow);
+    k.own = shape(n_seqs, kv_max);
+    p.tiles = (int)std::min(m / SHAPE_ROWS[k.own] + n_seqs, m);
+    p.ns = spans(k.own, (long long)p.tiles * n_kv, kv_max);
     if (pre_len) {
-        const int mt = k.pre_narrow ? MN : MT;
-        p.pre_tiles = (int)((m + mt - 1) / mt);
-        p.pre_ns = spans((long long)p.pre_tiles * n_kv, pre_len, k.pre_narrow);
+        k.pre = shape(1, pre_len);
+        p.pre_tiles = (int)((m + SHAPE_ROWS[k.pre] - 1) / SHAPE_ROWS[k.pre]);
+        p.pre_ns = spans(k.pre, (long long)p.pre_tiles * n_kv, pre_len);
     }
     p.nrec = p.ns + p.pre_ns > 1 ? p.ns + p.pre_ns : 0;
     return k;
@@ -1191,55 +1330,58 @@ static size_t ml_bytes(const RowsPlan &p, int n_rows, int n_heads) {
 }
 
 size_t attention_rows_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len) {
-    const RowsPlan p = rows_cut(n_rows, n_seqs, n_heads, n_kv, kv_max, pre_len).p;
-    return p.nrec ? ml_bytes(p, n_rows, n_heads) + (size_t)n_rows * n_heads * p.nrec * head_dim * 4 : 0;
+    size_t most = 0;
+    for (int half = 0; half < 2; half++) {
+        const RowsPlan p = rows_cut(n_rows, n_seqs, n_heads, n_kv, kv_max, pre_len, half).p;
+        if (p.nrec) most = std::max(most, ml_bytes(p, n_rows, n_heads) + (size_t)n_rows * n_heads * p.nrec * head_dim * 4);
+    }
+    return most;
 }
 
 /* the workgroups of one part, or of both */
-static void launch_part(const PromptArgs &a, const RowsPlan &p, bool half, bool narrow, hipStream_t st) {
-    const dim3 grid((unsigned)((p.tiles * p.ns + p.pre_tiles * p.pre_ns) * a.n_kv)), block(256);
-    const bool big = a.head_dim > 64;
+template <int HD>
+static void launch_part(const PromptArgs &a, const RowsPlan &p, bool half, Shape s, hipStream_t st) {
+    const dim3 grid((unsigned)((p.tiles * p.ns + p.pre_tiles * p.pre_ns) * a.n_kv)), block(SHAPE_THREADS[s]);
     if (!grid.x) return;
-#define ROWS(K) hipLaunchKernelGGL((K), grid, block, 0, st, a, p)
-    if (narrow) {
-        if (half && big) ROWS((k_rows_n<_Float16, 128>));
-        else if (half) ROWS((k_rows_n<_Float16, 64>));
-        else if (big) ROWS((k_rows_n<float, 128>));
-        else ROWS((k_rows_n<float, 64>));
+#define ROWS(...) hipLaunchKernelGGL((__VA_ARGS__), grid, block, 0, st, a, p)
+    if (half) {
+        if (s == NARROW) ROWS(k_rows_n<_Float16, HD>);
+        else if (s == WIDE) ROWS(k_rows_h<HD, 4, 2>);
+        else ROWS(k_rows_h<HD, 4, 1>);
     } else {
-        if (half && big) ROWS(k_rows_h<128>);
-        else if (half) ROWS(k_rows_h<64>);
-        else if (big) ROWS((k_rows_f<128, 4>));
-        else ROWS((k_rows_f<64, 4>));
+        if (s == NARROW) ROWS(k_rows_n<float, HD>);
+        else if (s == WIDE) ROWS(k_rows_f<HD, 4, 2>);
+        else if (s == FULL) ROWS(k_rows_f<HD, 4, 1>);
+        else ROWS(k_rows_f<HD, 8, 1>);
     }
 #undef ROWS
 }
 
-void launch_attention_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st) {
-    Cut k = rows_cut(a.s.rows, a.s.n, a.n_heads, a.n_kv, a.s.kv_max, a.pre_len);
+template <int HD>
+static void launch_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st) {
+    Cut k = rows_cut(a.s.rows, a.s.n, a.n_heads, a.n_kv, a.s.kv_max, a.pre_len, half);
     RowsPlan &p = k.p;
     p.ml = (float *)scratch;
     p.o = (float *)((uint8_t *)scratch + ml_bytes(p, a.s.rows, a.n_heads));
-    if (p.pre_tiles && k.narrow != k.pre_narrow) {
+    if (p.pre_tiles && k.own != k.pre) {
         RowsPlan one = p;
         one.tiles = 0;
-        launch_part(a, one, half, k.pre_narrow, st);
+        launch_part<HD>(a, one, half, k.pre, st);
         one = p;
         one.pre_tiles = 0;
-        launch_part(a, one, half, k.narrow, st);
+        launch_part<HD>(a, one, half, k.own, st);
     } else {
-        launch_part(a, p, half, k.narrow, st);
+        launch_part<HD>(a, p, half, k.own, st);
     }
     if (!p.nrec) return;
     const long long rows = (long long)a.s.rows * a.n_heads;
-    const dim3 one((unsigned)((rows + 3) / 4)), each((unsigned)rows), block(256);
-    if (a.head_dim > 64) {
-        if (p.nrec > 16) hipLaunchKernelGGL((k_rows_combine<4, 32>), each, block, 0, st, a, p);
-        else hipLaunchKernelGGL((k_rows_combine<1, 32>), one, block, 0, st, a, p);
-    } else {
-        if (p.nrec > 16) hipLaunchKernelGGL((k_rows_combine<4, 16>), each, block, 0, st, a, p);
-        else hipLaunchKernelGGL((k_rows_combine<1, 16>), one, block, 0, st, a, p);
-    }
+    if (p.nrec > 16) hipLaunchKernelGGL((k_rows_combine<4, HD / 4>), dim3((unsigned)rows), dim3(256), 0, st, a, p);
+    else hipLaunchKernelGGL((k_rows_combine<1, HD / 4>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, p);
+}
+
+void launch_attention_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st) {
+    if (a.head_dim > 64) launch_rows<128>(a, half, scratch, st);
+    else launch_rows<64>(a, half, scratch, st);
 }
 
 }  // namespace tg
