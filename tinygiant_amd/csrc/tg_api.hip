@@ -1531,7 +1531,11 @@ TG_API size_t tg_hip_attention_prompt_scratch_bytes(int n_rows, int n_seqs, int 
         head_dim > PROMPT_MAX_HEAD_DIM || kv_max <= 0 || prefix_len < 0)
         return 0;
     std::lock_guard<std::recursive_mutex> lk(g_mu);
-    return attention_rows_scratch(n_rows, n_seqs, n_heads, n_kv_heads, head_dim, kv_max, prefix_len);
+    /* enough for either cache type and any window (a window only takes spans away) */
+    size_t most = 0;
+    for (int half = 0; half < 2; half++)
+        most = std::max(most, attention_rows_scratch(n_rows, n_seqs, n_heads, n_kv_heads, head_dim, kv_max, prefix_len, 0, half));
+    return most;
 }
 
 static void attention_rows(const char *who, const float *q_dev, int q_stride, int kv_type, const void *kv_k_dev,
@@ -1564,7 +1568,8 @@ static void attention_rows(const char *who, const float *q_dev, int q_stride, in
         return;
     }
     ensure_init();
-    const size_t need = attention_rows_scratch(n_rows, n_seqs, n_heads, n_kv_heads, head_dim, kv_max, prefix_len);
+    const size_t need = attention_rows_scratch(n_rows, n_seqs, n_heads, n_kv_heads, head_dim, kv_max, prefix_len, window,
+                                               kv_type == TG_KV_F16);
     if (need && (!scratch_dev || ((uintptr_t)scratch_dev & 15))) {
         set_err("%s: needs %zu bytes of 16-byte aligned scratch", who, need);
         return;

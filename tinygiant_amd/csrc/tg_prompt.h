@@ -55,7 +55,8 @@ struct PromptArgs {
     int out_stride;
 };
 void launch_attention_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st);
-size_t attention_rows_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len);
+size_t attention_rows_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len,
+                              int window, bool half);
 
 }  // namespace tg
 #endif

@@ -154,10 +154,14 @@ void launch_kv_append(const AppendArgs &a, bool half, hipStream_t st) {
  * o[head_dim]) a row and k_rows_combine merges the records.  Exponents are in
  * base 2: weight 2^(z - m), z = score * log2 e. */
 struct RowsPlan {
-    int tiles, ns;          /* upper bound of the own-slot tiles, spans a tile */
-    int pre_tiles, pre_ns;  /* the same of the prefix */
-    int nrec;               /* records a row: pre_ns + ns; 0: written directly */
-    float *ml, *o;          /* [n_rows * n_heads][nrec][2], [..][nrec][head_dim] */
+    int items;              /* upper bound of the own-slot tiles' spans, per KV head */
+    int cap;                /* spans a tile has at most */
+    int target;             /* spans that the positions of all tiles are cut into, about */
+    int unit;               /* a span is a multiple of this */
+    int pre_tiles, pre_ns;  /* tiles of the prefix, spans of each */
+    int nrec;               /* room for a row's records: pre_ns + cap; 0: written directly */
+    float *ml, *o;          /* [n_rows * n_heads][nrec][4]: m, l, and in the first own span's the count of those;
+                               [..][nrec][head_dim] */
 };
 
 namespace {
@@ -167,40 +171,86 @@ constexpr int KT = 64;    /* positions of a tile */
 
 /* what a workgroup works on, uniform over it */
 struct Work {
-    int kh, split, ns, rec;
+    int kh, rec;
+    int count;       /* own slots' first span: how many spans the tile has; else 0 */
     bool prefix;
     Seq sq;          /* own: the sequence; prefix: all rows of the call as one */
     int m0;          /* the tile's first m-row */
     int lo, hi;      /* positions of the region */
 };
 
-/* Tile t of all sequences' tiles of MTILE m-rows, late rows first (they see
- * the most positions): a wave counts 64 sequences at a time. */
+__device__ inline int div_up(int a, int b) { return (int)(((unsigned)a + (unsigned)b - 1u) / (unsigned)b); }
+
+/* inclusive sum over the wave's lanes */
+__device__ inline int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   /* row_shr:1, 2, 4, 8 */
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   /* row_bcast:15, :31 */
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+
+/* Item b of the sequences' spans: tiles of MTILE m-rows, late rows first
+ * (they see the most positions), cut into spans of one length for all
+ * sequences, so that long and short ones finish together: that length is what
+ * cuts the positions of all tiles into about p.target spans (a sequence's
+ * tiles count as its longest).  A wave counts 64 sequences at a time; sums of
+ * positions are floats, the same in every workgroup. */
 template <int MTILE>
-__device__ inline bool find_tile(const PackedSeqs &p, int ratio, int t, Seq &sq, int &m0) {
+__device__ inline bool find_item(const PromptArgs &a, const RowsPlan &p, int ratio, int b, Work &w) {
+    const PackedSeqs &c = a.s;
     const int lane = threadIdx.x & 63;
-    for (int s0 = 0; s0 < p.n; s0 += 64) {
-        const int s = s0 + lane;
-        Seq q = {0, 0, 0, 0};
-        if (s < p.n) q = seq_at(p, s);
-        const int n = (int)(((unsigned)q.n * (unsigned)ratio + MTILE - 1) / MTILE);
-        int end = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(end, o, 64);
-            if (lane >= o) end += v;
+    Seq q = {0, 0, 0, 0};
+    auto load = [&](int s0) {
+        q.n = 0;
+        if (s0 + lane < c.n) q = seq_at(c, s0 + lane);
+    };
+    auto tiles = [&]() { return div_up(q.n * ratio, MTILE); };
+    auto sees = [&]() {   /* positions of the sequence's tiles, at most */
+        const int n = q.past + q.n;
+        return a.window > 0 ? min(n, a.window + (MTILE - 1) / ratio + 1) : n;
+    };
+    int per = 0x40000000;
+    load(0);
+    if (p.cap > 1) {
+        float sum = 0.f;
+        for (int s0 = 0; s0 < c.n; s0 += 64) {
+            if (s0) load(s0);
+            sum += wave_sum((float)tiles() * (float)sees());
         }
-        const uint64_t past = __ballot(end > t);
+        per = div_up(max(1, (int)fminf(sum / (float)p.target, 1e9f)), p.unit) * p.unit;
+        if (c.n > 64) load(0);
+    }
+    for (int s0 = 0; s0 < c.n; s0 += 64) {
+        if (s0) load(s0);
+        const int nt = tiles(), end = wave_scan(nt * min(div_up(sees(), per), p.cap));
+        const uint64_t past = __ballot(end > b);
         if (past) {
-            const int at = __builtin_ctzll(past);
-            sq.r0 = __builtin_amdgcn_readlane(q.r0, at);
-            sq.n = __builtin_amdgcn_readlane(q.n, at);
-            sq.past = __builtin_amdgcn_readlane(q.past, at);
-            sq.slot = __builtin_amdgcn_readlane(q.slot, at);
-            m0 = (__builtin_amdgcn_readlane(end, at) - 1 - t) * MTILE;
+            const int at = __builtin_ctzll(past), n = __builtin_amdgcn_readlane(nt, at);
+            w.sq.r0 = __builtin_amdgcn_readlane(q.r0, at);
+            w.sq.n = __builtin_amdgcn_readlane(q.n, at);
+            w.sq.past = __builtin_amdgcn_readlane(q.past, at);
+            w.sq.slot = __builtin_amdgcn_readlane(q.slot, at);
+            if (at) b -= __builtin_amdgcn_readlane(end, at - 1);
+            const int split = b / n;
+            w.m0 = (n - 1 - (b - split * n)) * MTILE;
+            const int i0 = w.m0 / ratio, i1 = min(w.sq.n - 1, (w.m0 + MTILE - 1) / ratio);
+            const int lo = a.window > 0 ? max(0, w.sq.past + i0 + 1 - a.window) : 0, hi = w.sq.past + i1 + 1;
+            int count = div_up(hi - lo, per);
+            if (count > p.cap) {
+                per = div_up(div_up(hi - lo, p.cap), p.unit) * p.unit;
+                count = div_up(hi - lo, per);
+            }
+            if (split >= count) return false;
+            w.rec = p.pre_ns + split;
+            w.count = split ? 0 : count;
+            w.lo = lo + split * per;
+            w.hi = min(hi, w.lo + per);
             return true;
         }
-        t -= __builtin_amdgcn_readlane(end, 63);
+        b -= __builtin_amdgcn_readlane(end, 63);
     }
     return false;
 }
@@ -228,50 +278,45 @@ __device__ inline bool row_sees(const PromptArgs &a, const Work &w, int m, int r
     return true;
 }
 
-/* This workgroup's work: block b of the prefix's, then of the sequences'
- * items; KV heads fastest, so that (8 XCDs, workgroups dealt in turn) those
- * of one head meet in as few L2 caches as possible.  False: none. */
+/* This workgroup's work: the prefix's items, then the sequences'; KV heads
+ * fastest, so that (8 XCDs, workgroups dealt in turn) those of one head meet
+ * in as few L2 caches as possible.  False: none. */
 template <int MTILE>
 __device__ inline bool find_work(const PromptArgs &a, const RowsPlan &p, int ratio, Work &w) {
     int b = blockIdx.x;
     const int npre = p.pre_tiles * p.pre_ns * a.n_kv;
     w.prefix = b < npre;
     if (!w.prefix) b -= npre;
-    w.kh = b % a.n_kv;
-    b /= a.n_kv;
-    const int tiles = w.prefix ? p.pre_tiles : p.tiles;
-    const int t = b % tiles;
-    w.split = b / tiles;
-    w.ns = w.prefix ? p.pre_ns : p.ns;
-    w.rec = w.prefix ? w.split : p.pre_ns + w.split;
-    int lo, hi;
-    if (w.prefix) {
-        const int r0 = min(max(a.s.cu[0], 0), a.s.rows), r1 = min(max(a.s.cu[a.s.n], r0), a.s.rows);
-        w.sq = Seq{r0, r1 - r0, 0, 0};
-        w.m0 = t * MTILE;
-        if ((unsigned)w.m0 >= (unsigned)w.sq.n * (unsigned)ratio) return false;
-        lo = 0, hi = a.pre_len;
-        if (a.window > 0) {   /* the first position that any of the rows sees */
-            lo = hi;
-            for (int m = w.m0 + (int)(threadIdx.x & 63); m < w.m0 + MTILE; m += 64) {
-                int f, l;
-                if (row_sees(a, w, m, ratio, f, l)) lo = min(lo, f);
-            }
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) lo = min(lo, __shfl_xor(lo, o, 64));
+    const int item = b / a.n_kv;
+    w.kh = b - item * a.n_kv;
+    if (!w.prefix) return find_item<MTILE>(a, p, ratio, item, w);
+    const int split = item / p.pre_tiles;
+    const int r0 = min(max(a.s.cu[0], 0), a.s.rows), r1 = min(max(a.s.cu[a.s.n], r0), a.s.rows);
+    w.rec = split, w.count = 0;
+    w.sq = Seq{r0, r1 - r0, 0, 0};
+    w.m0 = (item - split * p.pre_tiles) * MTILE;
+    if ((unsigned)w.m0 >= (unsigned)w.sq.n * (unsigned)ratio) return false;
+    int lo = 0;
+    const int hi = a.pre_len;
+    if (a.window > 0) {   /* the first position that any of the rows sees */
+        lo = hi;
+        for (int m = w.m0 + (int)(threadIdx.x & 63); m < w.m0 + MTILE; m += 64) {
+            int f, l;
+            if (row_sees(a, w, m, ratio, f, l)) lo = min(lo, f);
         }
-    } else {
-        if (!find_tile<MTILE>(a.s, ratio, t, w.sq, w.m0)) return false;
-        const int i0 = w.m0 / ratio, i1 = min(w.sq.n - 1, (w.m0 + MTILE - 1) / ratio);
-        lo = a.window > 0 ? max(0, w.sq.past + i0 + 1 - a.window) : 0;
-        hi = w.sq.past + i1 + 1;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) lo = min(lo, __shfl_xor(lo, o, 64));
+        lo = min(__builtin_amdgcn_readfirstlane(lo), hi);
     }
-    /* this span, in whole tiles counted from the first one's */
-    lo = lo / KT * KT;
-    const int per = max(1, ((hi - lo + KT - 1) / KT + w.ns - 1) / w.ns) * KT;
-    w.lo = __builtin_amdgcn_readfirstlane(min(hi, lo + w.split * per));
-    w.hi = __builtin_amdgcn_readfirstlane(min(hi, w.lo + per));
+    const int per = max(1, div_up(div_up(hi - lo, p.pre_ns), p.unit)) * p.unit;
+    w.lo = min(hi, lo + split * per);
+    w.hi = min(hi, w.lo + per);
     return true;
+}
+
+/* a record's statistics */
+__device__ inline void write_ml(const RowsPlan &p, const Work &w, size_t rec, float m, float l) {
+    *(f4 *)(p.ml + 4 * rec) = f4{m, l, __int_as_float(w.count), 0.f};
 }
 
 template <typename T>
@@ -331,7 +376,7 @@ __device__ void slow_row(const PromptArgs &a, const RowsPlan &p, const Work &w, 
     }
     if (p.nrec) {
         const size_t rec = ((size_t)r * a.n_heads + h) * p.nrec + w.rec;
-        if (tid == 0) p.ml[2 * rec] = mx, p.ml[2 * rec + 1] = l;
+        if (tid == 0) write_ml(p, w, rec, mx, l);
         if (tid < hd) p.o[rec * hd + tid] = o;
     } else if (tid < hd) {
         if (a.sinks) {
@@ -342,8 +387,6 @@ __device__ void slow_row(const PromptArgs &a, const RowsPlan &p, const Work &w, 
         a.out[(size_t)r * a.out_stride + (size_t)h * hd + tid] = o / l;
     }
 }
-
-__device__ inline int div_up(int a, int b) { return (a + b - 1) / b; }
 
 }  // namespace
 
@@ -498,14 +541,14 @@ __device__ inline float load_q(const PromptArgs &a, const Lane &x, int half, h8 
         }
     }
     const int ex = scale_exp(other_half_max(big));
+    const float f = __builtin_amdgcn_ldexpf(1.f, ex);
 #pragma unroll
     for (int s = 0; s < HD / 16; s++)
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float z = __builtin_amdgcn_ldexpf(y[s][e], ex);
-            const _Float16 hi = (_Float16)z;
-            qh[s][e] = hi;
-            ql[s][e] = (_Float16)(z - (float)hi);
+        for (int e = 0; e < 8; e += 2) {
+            h2 hi, lo;
+            split2(y[s][e] * f, y[s][e + 1] * f, y[s][e], y[s][e + 1], f, hi, lo);
+            qh[s][e] = hi[0], qh[s][e + 1] = hi[1], ql[s][e] = lo[0], ql[s][e + 1] = lo[1];
         }
     return __builtin_amdgcn_ldexpf(LOG2E / sqrtf((float)a.head_dim), -ex);
 }
@@ -526,28 +569,28 @@ __device__ inline uint32_t v_operand(int lane, int d, int e) {
 }
 
 /* The wave's rows written: weights were summed in units of 2^(mx - W_SHIFT)
- * relative to l, values besides in units of 2^-oexp.  Returns the m-rows that
+ * relative to l, values (SCALED) besides in units of 2^-oexp.  Returns the m-rows that
  * came out not finite, which are not written. */
-template <int HD>
+template <int HD, bool SCALED>
 __device__ inline uint32_t write_rows(const PromptArgs &a, const RowsPlan &p, const Work &w, const Lane &x, int lane, float mx,
                                       float l, int oexp, const f16v (&o)[HD / 32]) {
-    float nan = l * 0.f;
+    float big = fabsf(l);   /* NaN where anything is */
 #pragma unroll
     for (int d = 0; d < HD / 32; d++)
 #pragma unroll
-        for (int v = 0; v < 16; v++) nan = fmaf(o[d][v], 0.f, nan);
-    const uint64_t mask = __ballot(x.live && !(nan == 0.f));
+        for (int v = 0; v < 16; v++) big = max_nan(big, fabsf(o[d][v]));
+    const uint64_t mask = __ballot(x.live && !(big < INFINITY));
     const uint32_t bad = (uint32_t)mask | (uint32_t)(mask >> 32);
     if (!x.live || ((bad >> (lane & 31)) & 1u)) return bad;
     const int half = lane >> 5, hd = a.head_dim;
     float *dst, f;
     if (p.nrec) {
         const size_t rec = ((size_t)x.r * a.n_heads + x.h) * p.nrec + w.rec;
-        if (half == 0) *(float2 *)(p.ml + 2 * rec) = make_float2(mx, __builtin_amdgcn_ldexpf(l, -(int)W_SHIFT));
+        constexpr float one = 1.f / 8192.f;   /* 2^-W_SHIFT */
+        if (half == 0) write_ml(p, w, rec, mx, l * one);
         if (mx == -INFINITY) return bad;   /* a record of no position has no sums */
         dst = p.o + rec * hd;
-        f = 1.f;
-        oexp += (int)W_SHIFT;
+        f = one;
     } else {
         f = 1.f;
         if (a.sinks) {
@@ -565,7 +608,7 @@ __device__ inline uint32_t write_rows(const PromptArgs &a, const RowsPlan &p, co
             const int dim = 32 * d + 8 * v + 4 * half;
             f4 y;
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = __builtin_amdgcn_ldexpf(o[d][4 * v + e] * f, -oexp);
+            for (int e = 0; e < 4; e++) y[e] = SCALED ? __builtin_amdgcn_ldexpf(o[d][4 * v + e] * f, -oexp) : o[d][4 * v + e] * f;
             if (dim < hd) *(f4u *)(dst + dim) = y;
         }
     return bad;
@@ -739,9 +782,10 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_h(PromptArgs a, RowsPl
     }
     l = other_half_sum(l);
     int oexp = 0;
-    if constexpr (KG == 2) merge_groups<HD, MW>((float *)bufs, wave, lane, mx, l, oexp, o);
+    if constexpr (KG == 2)
+        if (w.hi - w.lo > KT) merge_groups<HD, MW>((float *)bufs, wave, lane, mx, l, oexp, o);   /* else group 1 had no tile */
     if (group == 0) {
-        const uint32_t bad = write_rows<HD>(a, p, w, x, lane, mx, l, oexp, o);
+        const uint32_t bad = write_rows<HD, false>(a, p, w, x, lane, mx, l, oexp, o);
         if (lane == 0) bad_rows[wave] = bad;
     }
     __syncthreads();
@@ -967,9 +1011,10 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPl
         bar_lds();
     }
     l = other_half_sum(l);
-    if constexpr (KG == 2) merge_groups<HD, MW>((float *)bufs, wave, lane, mx, l, U, o);
+    if constexpr (KG == 2)
+        if (w.hi - w.lo > KF) merge_groups<HD, MW>((float *)bufs, wave, lane, mx, l, U, o);   /* else group 1 had no tile */
     if (group == 0) {
-        const uint32_t bad = write_rows<HD>(a, p, w, x, lane, mx, l, U, o);
+        const uint32_t bad = write_rows<HD, true>(a, p, w, x, lane, mx, l, U, o);
         if (lane == 0) bad_rows[wave] = bad;
     }
     __syncthreads();
@@ -1195,7 +1240,7 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
         float *dst, f = 1.f;
         if (p.nrec) {
             const size_t rec = ((size_t)y.r * a.n_heads + y.h) * p.nrec + w.rec;
-            if (d0 == 0) *(float2 *)(p.ml + 2 * rec) = make_float2(M, L);
+            if (d0 == 0) write_ml(p, w, rec, M, L);
             dst = p.o + rec * hd + d0;
         } else {
             if (a.sinks) {
@@ -1229,22 +1274,26 @@ __global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) 
     if (s < 0) return;
     const Seq sq = seq_at(a.s, s);
     if (r - sq.r0 < 0 || r - sq.r0 >= sq.n) return;
-    const float *ml = p.ml + 2 * (size_t)at * p.nrec, *po = p.o + (size_t)at * p.nrec * hd;
+    const float *ml = p.ml + 4 * (size_t)at * p.nrec, *po = p.o + (size_t)at * p.nrec * hd;
     const float sink = a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
-    /* lane i: record W i + wave of each 64 W */
+    /* the prefix's records and the tile's own; lane i: record W i + wave of each 64 W */
+    const int own = __float_as_int(ml[4 * p.pre_ns + 2]), nrec = min(p.pre_ns + max(own, 0), p.nrec);
     float M = -INFINITY;
-    for (int c = lane; c < p.nrec; c += 64) M = fmaxf(M, ml[2 * c]);
+    for (int c = lane; c < p.nrec; c += 64) {   /* read past the count too, which arrives with them */
+        const float m = ml[4 * c];
+        M = c < nrec ? fmaxf(M, m) : M;
+    }
     M = fmaxf(wave_max(M), sink);
     const float base = M == -INFINITY ? 0.f : M;
     float l = 0.f;
     f4 o = {0.f, 0.f, 0.f, 0.f};
     const int g = lane / G, d = 4 * (lane % G);
-    for (int c0 = 0; c0 < p.nrec; c0 += 64 * W) {
+    for (int c0 = 0; c0 < nrec; c0 += 64 * W) {
         const int c = c0 + W * lane + wave;
-        const float2 x = c < p.nrec ? *(const float2 *)(ml + 2 * c) : make_float2(-INFINITY, 0.f);
+        const float2 x = c < nrec ? *(const float2 *)(ml + 4 * c) : make_float2(-INFINITY, 0.f);
         const float e = x.x == -INFINITY ? 0.f : exp2f(x.x - base);
         l += e == 0.f ? 0.f : x.y * e;
-        const int n = min(64, (p.nrec - c0 - wave + W - 1) / W);
+        const int n = min(64, (nrec - c0 - wave + W - 1) / W);
         for (int j0 = 0; j0 < n; j0 += 4 * PER) {   /* four records' loads at a time */
             f4 y[4];
             float f[4];
@@ -1298,7 +1347,8 @@ struct Cut {
     RowsPlan p;
     Shape own, pre;
 };
-static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int kv_max, int pre_len, bool half) {
+static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len, int window,
+                    bool half) {
     Cut k = {};
     RowsPlan &p = k.p;
     const int ratio = n_heads / n_kv;
@@ -1308,40 +1358,56 @@ static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int kv_max, i
         if (!half && m / 256 * n_kv * positions >= 512ll * 2048) return TALL;
         return m / 128 * n_kv >= 512 ? FULL : WIDE;
     };
-    auto spans = [&](Shape s, long long wgs, int positions) {
-        const int least = s == NARROW ? 128 : 4 * KT, most = (positions + least - 1) / least;
-        const int want = (int)((s == WIDE || s == TALL ? 256 : 512) / wgs);
-        return std::max(1, std::min(std::min(want, most), 128));
+    /* Spans of a tile at `positions`: us(n) = time of a span + what the
+     * records of n spans take to write and read (+ the combine's launch,
+     * where it is not there anyway).  A workgroup takes 3.4 us for 128
+     * positions of 128-value heads (WIDE; half of that for 64), 1.2 us for 64
+     * on the narrow kernel, the copies stream at 4.5 TB/s. */
+    auto spans = [&](Shape s, long long wgs, int positions, bool joined) {
+        const double t = positions * (s == NARROW ? 1.2 / 64 : 3.4 / 128) * (head_dim > 64 ? 1 : 0.5);
+        const double r = (double)m * n_kv * head_dim * 8 / 4.5e6;
+        const int most = (int)std::min<long long>({64, (positions + 127) / 128, std::max(1ll, (s == NARROW ? 512 : 256) / wgs)});
+        int best = 1;
+        double least = t + (joined ? r : 0);
+        for (int n = 2; n <= most; n++) {
+            const double us = t / n + r * n + (joined ? 0 : 4);
+            if (us < least) least = us, best = n;
+        }
+        return best;
     };
+    auto tiles = [&](Shape s, long long seqs) { return std::max((m + SHAPE_ROWS[s] - 1) / SHAPE_ROWS[s], seqs); };
     k.own = shape(n_seqs, kv_max);
-    p.tiles = (int)std::min(m / SHAPE_ROWS[k.own] + n_seqs, m);
-    p.ns = spans(k.own, (long long)p.tiles * n_kv, kv_max);
+    const int sees = window > 0 ? (int)std::min<long long>(kv_max, window + SHAPE_ROWS[k.own] / ratio + 1) : kv_max;
+    const long long own_tiles = tiles(k.own, n_seqs);
+    p.cap = spans(k.own, own_tiles * n_kv, sees, pre_len > 0);
+    p.target = std::max(1, (k.own == NARROW ? 512 : 256) / n_kv);
+    if (n_seqs > 1 && p.cap > 1)   /* room for a sequence much longer than the others */
+        p.cap = (int)std::min<long long>({64, (sees + 127) / 128, std::max<long long>(4ll * p.cap, 4ll * p.target / own_tiles)});
+    p.items = (int)std::min(m / SHAPE_ROWS[k.own] + n_seqs, m) + (p.cap > 1 ? p.target : 0);
+    p.unit = 128;
     if (pre_len) {
         k.pre = shape(1, pre_len);
-        p.pre_tiles = (int)((m + SHAPE_ROWS[k.pre] - 1) / SHAPE_ROWS[k.pre]);
-        p.pre_ns = spans(k.pre, (long long)p.pre_tiles * n_kv, pre_len);
+        p.pre_tiles = (int)tiles(k.pre, 1);
+        p.pre_ns = spans(k.pre, (long long)p.pre_tiles * n_kv, pre_len, true);
     }
-    p.nrec = p.ns + p.pre_ns > 1 ? p.ns + p.pre_ns : 0;
+    p.nrec = p.cap + p.pre_ns > 1 ? p.cap + p.pre_ns : 0;
     return k;
 }
 
 static size_t ml_bytes(const RowsPlan &p, int n_rows, int n_heads) {
-    return ((size_t)n_rows * n_heads * p.nrec * 8 + 255) & ~(size_t)255;
+    return ((size_t)n_rows * n_heads * p.nrec * 16 + 255) & ~(size_t)255;
 }
 
-size_t attention_rows_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len) {
-    size_t most = 0;
-    for (int half = 0; half < 2; half++) {
-        const RowsPlan p = rows_cut(n_rows, n_seqs, n_heads, n_kv, kv_max, pre_len, half).p;
-        if (p.nrec) most = std::max(most, ml_bytes(p, n_rows, n_heads) + (size_t)n_rows * n_heads * p.nrec * head_dim * 4);
-    }
-    return most;
+size_t attention_rows_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len,
+                              int window, bool half) {
+    const RowsPlan p = rows_cut(n_rows, n_seqs, n_heads, n_kv, head_dim, kv_max, pre_len, window, half).p;
+    return p.nrec ? ml_bytes(p, n_rows, n_heads) + (size_t)n_rows * n_heads * p.nrec * head_dim * 4 : 0;
 }
 
 /* the workgroups of one part, or of both */
 template <int HD>
 static void launch_part(const PromptArgs &a, const RowsPlan &p, bool half, Shape s, hipStream_t st) {
-    const dim3 grid((unsigned)((p.tiles * p.ns + p.pre_tiles * p.pre_ns) * a.n_kv)), block(SHAPE_THREADS[s]);
+    const dim3 grid((unsigned)((p.items + p.pre_tiles * p.pre_ns) * a.n_kv)), block(SHAPE_THREADS[s]);
     if (!grid.x) return;
 #define ROWS(...) hipLaunchKernelGGL((__VA_ARGS__), grid, block, 0, st, a, p)
     if (half) {
@@ -1359,13 +1425,13 @@ static void launch_part(const PromptArgs &a, const RowsPlan &p, bool half, Shape
 
 template <int HD>
 static void launch_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st) {
-    Cut k = rows_cut(a.s.rows, a.s.n, a.n_heads, a.n_kv, a.s.kv_max, a.pre_len, half);
+    Cut k = rows_cut(a.s.rows, a.s.n, a.n_heads, a.n_kv, a.head_dim, a.s.kv_max, a.pre_len, a.window, half);
     RowsPlan &p = k.p;
     p.ml = (float *)scratch;
     p.o = (float *)((uint8_t *)scratch + ml_bytes(p, a.s.rows, a.n_heads));
     if (p.pre_tiles && k.own != k.pre) {
         RowsPlan one = p;
-        one.tiles = 0;
+        one.items = 0;
         launch_part<HD>(a, one, half, k.pre, st);
         one = p;
         one.pre_tiles = 0;
