@@ -568,6 +568,22 @@ __device__ inline uint32_t v_operand(int lane, int d, int e) {
     return (uint32_t)(key * (HD * 2) + ((piece ^ swz<HD>(key)) << 4) + 8 * (lane & 1));
 }
 
+/* scores of 32 positions, register v at position at + 8 (v / 4) + v % 4: -inf
+ * for those that the row does not see (most tiles: none, by uniform tests) */
+__device__ inline void mask_scores(f16v &s, int at, const Lane &x) {
+    const int t = __builtin_amdgcn_readfirstlane(at);   /* lane 0: the first position */
+    if (t + 31 > x.all_hi) {
+        const int n = x.last - at;
+#pragma unroll
+        for (int v = 0; v < 16; v++) s[v] = 8 * (v >> 2) + (v & 3) <= n ? s[v] : -INFINITY;
+    }
+    if (t < x.all_lo) {
+        const int n = x.first - at;
+#pragma unroll
+        for (int v = 0; v < 16; v++) s[v] = 8 * (v >> 2) + (v & 3) >= n ? s[v] : -INFINITY;
+    }
+}
+
 /* The wave's rows written: weights were summed in units of 2^(mx - W_SHIFT)
  * relative to l, values (SCALED) besides in units of 2^-oexp.  Returns the m-rows that
  * came out not finite, which are not written. */
@@ -650,8 +666,11 @@ __device__ inline void merge_groups(float *lds, int wave, int lane, float &mx, f
 
 #define MFMA_H(a, b, c) __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0)
 
-/* MW waves of 32 m-rows; with KG = 2, two groups of them take the tiles in turn */
-template <int HD, int MW, int KG>
+/* MW waves of 32 m-rows; with KG = 2, two groups of them take the tiles in
+ * turn.  J blocks of 32 positions are computed together: two overlap their
+ * latencies (8192 tokens: 928 us, one at a time 965), one is half the code
+ * and skips what a window hides (4,096 tokens, window 128: 46.2, 48.6). */
+template <int HD, int MW, int KG, int J>
 __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_h(PromptArgs a, RowsPlan p) {
     constexpr int RB = HD * 2, TILE = KT * RB;       /* bytes of a row in LDS, of a tile of K or V */
     constexpr int NC = TILE / 1024 / MW;             /* copies of 1 KiB a wave, matrix and tile */
@@ -708,76 +727,80 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_h(PromptArgs a, RowsPl
         bar_lds();   /* every wave's copies of this tile are there, and every wave is done with the other buffer */
         if (t + KG * KT < w.hi) copy_tile(t + KG * KT, b ^ 1);
         if (t > x.any_hi || t + KT <= x.any_lo || t >= w.hi) continue;   /* uniform in the wave */
-        const Lds tile = (Lds)buf[b][0];
-        f16v s[2];
+#pragma unroll 1
+        for (int n = 0; n < KT; n += 32 * J) {
+            const int at = t + n;
+            if (J == 1 && (at > x.any_hi || at + 32 <= x.any_lo)) continue;
+            const Lds tile = (Lds)buf[b][0] + n * RB;
+            f16v s[J];
+            h8 k0[J], k1[J];
 #pragma unroll
-        for (int n = 0; n < 2; n++)
+            for (int j = 0; j < J; j++) {
 #pragma unroll
-            for (int v = 0; v < 16; v++) s[n][v] = 0.f;
-        h8 k0 = lds_row(tile + kaddr), k1 = lds_row(tile + kaddr + 32 * RB);
-#pragma unroll
-        for (int st = 0; st < STEPS; st++) {   /* the next step's operands are read a step ahead */
-            const Lds at = tile + (kaddr ^ (uint32_t)((st + 1) << 5));
-            const h8 n0 = st + 1 < STEPS ? lds_row(at) : k0, n1 = st + 1 < STEPS ? lds_row(at + 32 * RB) : k1;
-            s[0] = MFMA_H(k0, ql[st], s[0]);
-            s[1] = MFMA_H(k1, ql[st], s[1]);
-            s[0] = MFMA_H(k0, qh[st], s[0]);
-            s[1] = MFMA_H(k1, qh[st], s[1]);
-            k0 = n0, k1 = n1;
-        }
-        auto column = [&](int i) __attribute__((always_inline)) {
-            const int q = i / DB, d = i % DB;
-            return h8_of(lds_column(tile + vaddr[d][0] + q * 16 * RB), lds_column(tile + vaddr[d][1] + q * 16 * RB));
-        };
-        h8 v0 = column(0), v1 = column(1);
-        if (t + KT - 1 > x.all_hi || t < x.all_lo) {   /* some row does not see all of the tile */
-#pragma unroll
-            for (int n = 0; n < 2; n++)
-#pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    const int pos = t + 32 * n + 8 * (v >> 2) + 4 * half + (v & 3);
-                    s[n][v] = pos <= x.last && pos >= x.first ? s[n][v] : -INFINITY;
-                }
-        }
-        float top = max_nan(s[0][0], s[1][0]);
-#pragma unroll
-        for (int v = 1; v < 16; v++) top = max_nan(max_nan(top, s[0][v]), s[1][v]);
-        top = other_half_max(top) * c;
-        const float mn = max_nan(mx, top), sh = mn == -INFINITY ? 0.f : W_SHIFT - mn;
-        if (__any(mn > mx)) {
-            const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
-            l *= alpha;
-#pragma unroll
-            for (int d = 0; d < DB; d++)
-#pragma unroll
-                for (int v = 0; v < 16; v++) o[d][v] *= alpha;
-        }
-        mx = mn;
-        h8 ph[4], pl[4];
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int n = 0; n < 2; n++)
-#pragma unroll
-            for (int v = 0; v < 16; v += 2) {
-                const float e0 = __builtin_amdgcn_exp2f(fmaf(s[n][v], c, sh));
-                const float e1 = __builtin_amdgcn_exp2f(fmaf(s[n][v + 1], c, sh));
-                sum[v & 3] += e0, sum[(v & 3) + 1] += e1;
-                h2 hi, lo;
-                split2(e0, e1, e0, e1, one, hi, lo);
-                const int q = 2 * n + (v >> 3), at = v & 7;
-                ph[q][at] = hi[0], ph[q][at + 1] = hi[1];
-                pl[q][at] = lo[0], pl[q][at + 1] = lo[1];
+                for (int v = 0; v < 16; v++) s[j][v] = 0.f;
+                k0[j] = lds_row(tile + kaddr + j * 32 * RB);
             }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-        for (int i = 0; i < 4 * DB; i += 2) {
-            const h8 n0 = i + 2 < 4 * DB ? column(i + 2) : v0, n1 = i + 2 < 4 * DB ? column(i + 3) : v1;
-            const int q = i / DB, d = i % DB;
-            o[d] = MFMA_H(v0, pl[q], o[d]);
-            o[d + 1] = MFMA_H(v1, pl[q], o[d + 1]);
-            o[d] = MFMA_H(v0, ph[q], o[d]);
-            o[d + 1] = MFMA_H(v1, ph[q], o[d + 1]);
-            v0 = n0, v1 = n1;
+            for (int st = 0; st < STEPS; st++) {   /* the next step's operands are read a step ahead */
+                const Lds next = tile + (kaddr ^ (uint32_t)((st + 1) << 5));
+#pragma unroll
+                for (int j = 0; j < J; j++) k1[j] = st + 1 < STEPS ? lds_row(next + j * 32 * RB) : k0[j];
+#pragma unroll
+                for (int j = 0; j < J; j++) s[j] = MFMA_H(k0[j], ql[st], s[j]);
+#pragma unroll
+                for (int j = 0; j < J; j++) s[j] = MFMA_H(k0[j], qh[st], s[j]);
+#pragma unroll
+                for (int j = 0; j < J; j++) k0[j] = k1[j];
+            }
+            auto column = [&](int i) __attribute__((always_inline)) {
+                const int q = i / DB, d = i % DB;
+                return h8_of(lds_column(tile + vaddr[d][0] + q * 16 * RB), lds_column(tile + vaddr[d][1] + q * 16 * RB));
+            };
+            h8 v0 = column(0), v1 = column(1);
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                mask_scores(s[j], at + 32 * j + 4 * half, x);
+#pragma unroll
+                for (int v = 0; v < 16; v++) top = max_nan(top, s[j][v]);
+            }
+            top = other_half_max(top) * c;
+            const float mn = max_nan(mx, top), sh = mn == -INFINITY ? 0.f : W_SHIFT - mn;
+            if (__any(mn > mx)) {
+                const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < DB; d++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) o[d][v] *= alpha;
+            }
+            mx = mn;
+            h8 ph[2 * J], pl[2 * J];
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < J; j++)
+#pragma unroll
+                for (int v = 0; v < 16; v += 2) {
+                    const float e0 = __builtin_amdgcn_exp2f(fmaf(s[j][v], c, sh));
+                    const float e1 = __builtin_amdgcn_exp2f(fmaf(s[j][v + 1], c, sh));
+                    sum[v & 3] += e0, sum[(v & 3) + 1] += e1;
+                    h2 hi, lo;
+                    split2(e0, e1, e0, e1, one, hi, lo);
+                    const int q = 2 * j + (v >> 3), e = v & 7;
+                    ph[q][e] = hi[0], ph[q][e + 1] = hi[1], pl[q][e] = lo[0], pl[q][e + 1] = lo[1];
+                }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+            for (int i = 0; i < 2 * J * DB; i += 2) {
+                const bool more = i + 2 < 2 * J * DB;
+                const h8 n0 = more ? column(i + 2) : v0, n1 = more ? column(i + 3) : v1;
+                const int q = i / DB, d = i % DB;
+                o[d] = MFMA_H(v0, pl[q], o[d]);
+                o[d + 1] = MFMA_H(v1, pl[q], o[d + 1]);
+                o[d] = MFMA_H(v0, ph[q], o[d]);
+                o[d + 1] = MFMA_H(v1, ph[q], o[d + 1]);
+                v0 = n0, v1 = n1;
+            }
         }
     }
     l = other_half_sum(l);
@@ -950,13 +973,7 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPl
                 return h8_of(lds_column(tile + vaddr[d][0] + at), lds_column(tile + vaddr[d][1] + at));
             };
             h8 vh = column(0, 0), vl = column(0, 1);
-            if (t + KF - 1 > x.all_hi || t < x.all_lo) {   /* some row does not see all of the tile */
-#pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    const int pos = t + 8 * (v >> 2) + 4 * half + (v & 3);
-                    s[v] = pos <= x.last && pos >= x.first ? s[v] : -INFINITY;
-                }
-            }
+            mask_scores(s, t + 4 * half, x);
             float cg[4], top = -INFINITY;
 #pragma unroll
             for (int g = 0; g < 4; g++) {
@@ -1338,11 +1355,12 @@ __global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) 
  *   narrow  16 m-rows a workgroup, positions over its waves
  *   wide    128 m-rows, two groups of four waves on tiles in turn: two waves
  *           a SIMD where there are no more workgroups than CUs
- *   full    128 m-rows, four waves; several workgroups a CU
+ *   short   128 m-rows, four waves, for few positions a row
+ *   full    the same, several workgroups a CU on long spans
  *   tall    256 m-rows, eight waves (f32 caches): half the splitting of K and
  *           V a row */
-enum Shape { NARROW, WIDE, FULL, TALL };
-constexpr int SHAPE_ROWS[] = {16, 128, 128, 256}, SHAPE_THREADS[] = {256, 512, 256, 512};
+enum Shape { NARROW, SHORT, WIDE, FULL, TALL };
+constexpr int SHAPE_ROWS[] = {16, 128, 128, 128, 256}, SHAPE_THREADS[] = {256, 256, 512, 256, 512};
 struct Cut {
     RowsPlan p;
     Shape own, pre;
@@ -1355,8 +1373,9 @@ static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim,
     const long long m = (long long)n_rows * ratio;
     auto shape = [&](long long seqs, int positions) {
         if (m <= 64 * seqs) return NARROW;
-        if (!half && m / 256 * n_kv * positions >= 512ll * 2048) return TALL;
-        return m / 128 * n_kv >= 512 ? FULL : WIDE;
+        if (positions < 512) return SHORT;
+        if (!half && m / 256 * n_kv * positions >= 512ll * 4096) return TALL;
+        return m / 128 * n_kv > 512 ? FULL : WIDE;
     };
     /* Spans of a tile at `positions`: us(n) = time of a span + what the
      * records of n spans take to write and read (+ the combine's launch,
@@ -1376,13 +1395,14 @@ static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim,
         return best;
     };
     auto tiles = [&](Shape s, long long seqs) { return std::max((m + SHAPE_ROWS[s] - 1) / SHAPE_ROWS[s], seqs); };
-    k.own = shape(n_seqs, kv_max);
-    const int sees = window > 0 ? (int)std::min<long long>(kv_max, window + SHAPE_ROWS[k.own] / ratio + 1) : kv_max;
+    auto sees = [&](int rows) { return window > 0 ? (int)std::min<long long>(kv_max, (long long)window + rows / ratio + 1) : kv_max; };
+    k.own = shape(n_seqs, sees(128));
+    const int own_sees = sees(SHAPE_ROWS[k.own]);
     const long long own_tiles = tiles(k.own, n_seqs);
-    p.cap = spans(k.own, own_tiles * n_kv, sees, pre_len > 0);
+    p.cap = spans(k.own, own_tiles * n_kv, own_sees, pre_len > 0);
     p.target = std::max(1, (k.own == NARROW ? 512 : 256) / n_kv);
     if (n_seqs > 1 && p.cap > 1)   /* room for a sequence much longer than the others */
-        p.cap = (int)std::min<long long>({64, (sees + 127) / 128, std::max<long long>(4ll * p.cap, 4ll * p.target / own_tiles)});
+        p.cap = (int)std::min<long long>({64, (own_sees + 127) / 128, std::max<long long>(4ll * p.cap, 4ll * p.target / own_tiles)});
     p.items = (int)std::min(m / SHAPE_ROWS[k.own] + n_seqs, m) + (p.cap > 1 ? p.target : 0);
     p.unit = 128;
     if (pre_len) {
@@ -1412,13 +1432,14 @@ static void launch_part(const PromptArgs &a, const RowsPlan &p, bool half, Shape
 #define ROWS(...) hipLaunchKernelGGL((__VA_ARGS__), grid, block, 0, st, a, p)
     if (half) {
         if (s == NARROW) ROWS(k_rows_n<_Float16, HD>);
-        else if (s == WIDE) ROWS(k_rows_h<HD, 4, 2>);
-        else ROWS(k_rows_h<HD, 4, 1>);
+        else if (s == SHORT) ROWS(k_rows_h<HD, 4, 1, 1>);
+        else if (s == WIDE) ROWS(k_rows_h<HD, 4, 2, 2>);
+        else ROWS(k_rows_h<HD, 4, 1, 2>);
     } else {
         if (s == NARROW) ROWS(k_rows_n<float, HD>);
         else if (s == WIDE) ROWS(k_rows_f<HD, 4, 2>);
-        else if (s == FULL) ROWS(k_rows_f<HD, 4, 1>);
-        else ROWS(k_rows_f<HD, 8, 1>);
+        else if (s == TALL) ROWS(k_rows_f<HD, 8, 1>);
+        else ROWS(k_rows_f<HD, 4, 1>);
     }
 #undef ROWS
 }
