@@ -264,7 +264,8 @@ size_t tg_hip_attention_scratch_bytes(int embed_dim, int n_heads, int n_kv_heads
  *   shapes    head_dim a multiple of 8 and <= 128, n_heads <= 1024,
  *             n_heads / n_kv_heads integral and <= 64, kv_max <= 2^20,
  *             n_rows <= 2^22, n_seqs <= 2^16
- *   strides   in floats from row to row, of at least a row's heads
+ *   strides   in floats from row to row, of at least a row's heads and at most
+ *             2^21
  * cu_rows, kv_len and slots are device arrays that the host does not see: a
  * sequence whose slot is not below n_slots, or whose rows do not fit kv_max,
  * is left out (its rows of the outputs and the caches stay as they were).

@@ -38,7 +38,7 @@ def _logits(**kw):
     (dict(n_rows=1 << 23), "n_rows"), (dict(n_slots=0), "n_slots"), (dict(kv_max=0), "kv_max"), (dict(kv_max=(1 << 20) + 1), "kv_max"),
     (dict(hd=60), "shape"), (dict(hd=0), "shape"), (dict(hd=136), "shape"), (dict(nh=9), "shape"), (dict(nkv=0), "shape"),
     (dict(nh=130, nkv=1), "shape"), (dict(nh=2048, nkv=1024), "shape"), (dict(cu=None), "cu_rows"), (dict(k=None), "cache"),
-    (dict(v=P + 4), "16-byte"), (dict(window=-1), "window"), (dict(q_stride=511), "stride"), (dict(out_stride=100), "stride"),
+    (dict(v=P + 4), "16-byte"), (dict(window=-1), "window"), (dict(q_stride=511), "stride"), (dict(out_stride=100), "stride"), (dict(q_stride=(1 << 21) + 1), "stride"),
     (dict(q=None), "q or out"), (dict(out=None), "q or out"), (dict(q=P + 2), "q or out"),
     (dict(out=P, out_stride=600), "same stride"), (dict(plen=21), "prefix_len"), (dict(plen=-1), "prefix_len"),
     (dict(pk=None), "prefix_k"), (dict(pv=P + 8), "prefix_k"), (dict(pmax=1 << 21), "prefix_len")])

@@ -1554,8 +1554,9 @@ static void attention_rows(const char *who, const float *q_dev, int q_stride, in
                 PROMPT_MAX_KV);
         return;
     }
-    if (window < 0 || q_stride < n_heads * head_dim || out_stride < n_heads * head_dim) {
-        set_err("%s: need window >= 0 and strides of at least n_heads * head_dim", who);
+    if (window < 0 || q_stride < n_heads * head_dim || out_stride < n_heads * head_dim || q_stride > PROMPT_MAX_STRIDE ||
+        out_stride > PROMPT_MAX_STRIDE) {
+        set_err("%s: need window >= 0 and strides of at least n_heads * head_dim and at most %d", who, PROMPT_MAX_STRIDE);
         return;
     }
     if (!n_seqs || !n_rows) return;

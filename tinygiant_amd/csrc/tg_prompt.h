@@ -12,6 +12,7 @@
 #define PROMPT_MAX_GQA 64         /* query heads per KV head, at most this */
 #define PROMPT_MAX_KV (1 << 20)   /* kv_max, prefix_max: offsets in one head's rows stay below 2^30 bytes */
 #define PROMPT_MAX_ROWS (1 << 22)
+#define PROMPT_MAX_STRIDE (1 << 21)   /* floats from row to row: a tile's rows within 2^31 bytes */
 #define PROMPT_MAX_SEQS (1 << 16)
 
 namespace tg {

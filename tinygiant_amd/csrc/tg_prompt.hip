@@ -176,8 +176,20 @@ struct Work {
     bool prefix;
     Seq sq;          /* own: the sequence; prefix: all rows of the call as one */
     int m0;          /* the tile's first m-row */
+    int i0, j0;      /* its row of the sequence and its query head of the group */
+    uint32_t inv;    /* x / ratio = x inv >> 16 for x < 1024 */
     int lo, hi;      /* positions of the region */
+    /* row of the sequence and query head of the group of m-row m0 + at */
+    __device__ inline void row(int at, int ratio, int &i, int &j) const {
+        const int x = j0 + at, d = (int)(((uint32_t)x * inv) >> 16);
+        i = i0 + d, j = x - d * ratio;
+    }
 };
+
+__device__ inline void set_rows(Work &w, int ratio) {
+    w.i0 = w.m0 / ratio, w.j0 = w.m0 - w.i0 * ratio;
+    w.inv = (65536u + (uint32_t)ratio - 1u) / (uint32_t)ratio;   /* off by less than ratio <= 64: exact below 1024 */
+}
 
 __device__ inline int div_up(int a, int b) { return (int)(((unsigned)a + (unsigned)b - 1u) / (unsigned)b); }
 
@@ -236,8 +248,11 @@ __device__ inline bool find_item(const PromptArgs &a, const RowsPlan &p, int rat
             if (at) b -= __builtin_amdgcn_readlane(end, at - 1);
             const int split = b / n;
             w.m0 = (n - 1 - (b - split * n)) * MTILE;
-            const int i0 = w.m0 / ratio, i1 = min(w.sq.n - 1, (w.m0 + MTILE - 1) / ratio);
-            const int lo = a.window > 0 ? max(0, w.sq.past + i0 + 1 - a.window) : 0, hi = w.sq.past + i1 + 1;
+            set_rows(w, ratio);
+            int i1, j1;
+            w.row(MTILE - 1, ratio, i1, j1);
+            const int lo = a.window > 0 ? max(0, w.sq.past + w.i0 + 1 - a.window) : 0;
+            const int hi = w.sq.past + min(w.sq.n - 1, i1) + 1;
             int count = div_up(hi - lo, per);
             if (count > p.cap) {
                 per = div_up(div_up(hi - lo, p.cap), p.unit) * p.unit;
@@ -255,10 +270,9 @@ __device__ inline bool find_item(const PromptArgs &a, const RowsPlan &p, int rat
     return false;
 }
 
-/* positions of the region that m-row m of the work sees: first .. last;
- * false: no row there */
-__device__ inline bool row_sees(const PromptArgs &a, const Work &w, int m, int ratio, int &first, int &last) {
-    int i = m / ratio;
+/* positions of the region that row i of the work's sequence sees: first ..
+ * last; false: no row there */
+__device__ inline bool row_sees(const PromptArgs &a, const Work &w, int i, int &first, int &last) {
     if (i >= w.sq.n) return false;
     first = 0;
     if (w.prefix) {
@@ -296,13 +310,15 @@ __device__ inline bool find_work(const PromptArgs &a, const RowsPlan &p, int rat
     w.sq = Seq{r0, r1 - r0, 0, 0};
     w.m0 = (item - split * p.pre_tiles) * MTILE;
     if ((unsigned)w.m0 >= (unsigned)w.sq.n * (unsigned)ratio) return false;
+    set_rows(w, ratio);
     int lo = 0;
     const int hi = a.pre_len;
     if (a.window > 0) {   /* the first position that any of the rows sees */
         lo = hi;
-        for (int m = w.m0 + (int)(threadIdx.x & 63); m < w.m0 + MTILE; m += 64) {
-            int f, l;
-            if (row_sees(a, w, m, ratio, f, l)) lo = min(lo, f);
+        for (int at = (int)(threadIdx.x & 63); at < MTILE; at += 64) {
+            int f, l, i, j;
+            w.row(at, ratio, i, j);
+            if (row_sees(a, w, i, f, l)) lo = min(lo, f);
         }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) lo = min(lo, __shfl_xor(lo, o, 64));
@@ -331,13 +347,14 @@ __device__ inline const T *region(const PromptArgs &a, const Work &w, const void
  * multiply every value of a tile: 0 * inf there is not a row's own result.
  * lds: PROMPT_MAX_HEAD_DIM + 260 floats. */
 template <typename T>
-__device__ void slow_row(const PromptArgs &a, const RowsPlan &p, const Work &w, int m, int ratio, float *lds) {
+__device__ void slow_row(const PromptArgs &a, const RowsPlan &p, const Work &w, int at, int ratio, float *lds) {
     float *qs = lds, *sc = lds + PROMPT_MAX_HEAD_DIM, *red = sc + 256;
     const int tid = threadIdx.x, hd = a.head_dim;
     const bool on = tid < 256;   /* further threads only keep the barriers */
-    const int i = m / ratio, h = w.kh * ratio + (m - i * ratio), r = w.sq.r0 + i;
-    int first = 0, last = -1;
-    (void)row_sees(a, w, m, ratio, first, last);
+    int i, j, first = 0, last = -1;
+    w.row(at, ratio, i, j);
+    const int h = w.kh * ratio + j, r = w.sq.r0 + i;
+    (void)row_sees(a, w, i, first, last);
     first = max(first, w.lo), last = min(last, w.hi - 1);
     const T *k = region<T>(a, w, a.kv_k, a.pre_k), *v = region<T>(a, w, a.kv_v, a.pre_v);
     const float scale = LOG2E / sqrtf((float)hd);
@@ -370,7 +387,7 @@ __device__ void slow_row(const PromptArgs &a, const RowsPlan &p, const Work &w, 
         if (tid < hd) {
             o *= alpha;
             const int n = min(256, last + 1 - t0);
-            for (int j = 0; j < n; j++) o = fmaf(sc[j], (float)v[(size_t)(t0 + j) * hd + tid], o);
+            for (int n1 = 0; n1 < n; n1++) o = fmaf(sc[n1], (float)v[(size_t)(t0 + n1) * hd + tid], o);
         }
         __syncthreads();
     }
@@ -471,16 +488,16 @@ struct Lane {
     int r, h;        /* packed row, query head */
     int any_lo, any_hi, all_lo, all_hi;
 };
-/* ms: the wave's m-rows from m0 on, of which the lane takes m0 + at */
-__device__ inline Lane lane_rows(const PromptArgs &a, const Work &w, int m0, int at, int ms, int ratio) {
+/* ms: the wave's m-rows, from the tile's from on, of which the lane takes at */
+__device__ inline Lane lane_rows(const PromptArgs &a, const Work &w, int from, int at, int ms, int ratio) {
     Lane x;
-    int first = 0, last = 0;
-    const int m = m0 + at;
-    x.live = row_sees(a, w, m, ratio, first, last);
-    const int i = x.live ? m / ratio : 0;
-    x.r = w.sq.r0 + i, x.h = w.kh * ratio + (x.live ? m - i * ratio : 0);
+    int first = 0, last = 0, i, j, i0, i1, u;
+    w.row(from + at, ratio, i, j);
+    x.live = row_sees(a, w, i, first, last);
+    x.r = w.sq.r0 + (x.live ? i : 0), x.h = w.kh * ratio + (x.live ? j : 0);
     x.first = x.live ? first : 0, x.last = x.live ? last : 0x7FFFFFFF;
-    const int i0 = m0 / ratio, i1 = min(w.sq.n - 1, (m0 + ms - 1) / ratio);   /* uniform */
+    w.row(from, ratio, i0, u), w.row(from + ms - 1, ratio, i1, u);   /* uniform */
+    i1 = min(w.sq.n - 1, i1);
     if (i0 > i1) {
         x.any_lo = 0x7FFFFFFF, x.any_hi = -1, x.all_lo = 0, x.all_hi = 0x7FFFFFFF;
     } else if (!w.prefix) {   /* later rows see later positions */
@@ -523,34 +540,80 @@ __device__ inline int scale_exp(float big) {
 }
 
 /* q of the lane's m-row as the B operands of the first product, two f16
- * planes; returns the factor that takes scores of the planes to base 2 */
-template <int HD>
-__device__ inline float load_q(const PromptArgs &a, const Lane &x, int half, h8 (&qh)[HD / 16], h8 (&ql)[HD / 16]) {
-    float y[HD / 16][8], big = 0.f;
-    const float *src = a.q + (size_t)x.r * a.q_stride + (size_t)x.h * a.head_dim;
+ * planes, from its 16-byte pieces (of which fetch(i) is the i-th, zeros past
+ * the row); returns the factor that takes scores of the planes to base 2 */
+template <int HD, typename F>
+__device__ inline float load_q(int head_dim, int half, const F &fetch, h8 (&qh)[HD / 16], h8 (&ql)[HD / 16]) {
+    f4 y[HD / 8];
+    float big = 0.f;
 #pragma unroll
-    for (int s = 0; s < HD / 16; s++) {
-        const int d = 16 * s + 8 * half;
-        const bool on = x.live && d < a.head_dim;
-        const f4 u = on ? (f4)*(const f4u *)(src + d) : f4{0.f, 0.f, 0.f, 0.f};
-        const f4 v = on ? (f4)*(const f4u *)(src + d + 4) : f4{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < HD / 16; s++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            y[s][e] = u[e], y[s][4 + e] = v[e];
-            big = fmaxf(big, fmaxf(fabsf(u[e]), fabsf(v[e])));
+        for (int e = 0; e < 2; e++) {
+            const f4 u = y[2 * s + e] = fetch(4 * s + 2 * half + e);
+            big = max_nan(big, max_nan(max_nan(fabsf(u[0]), fabsf(u[1])), max_nan(fabsf(u[2]), fabsf(u[3]))));
         }
-    }
     const int ex = scale_exp(other_half_max(big));
     const float f = __builtin_amdgcn_ldexpf(1.f, ex);
 #pragma unroll
     for (int s = 0; s < HD / 16; s++)
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
+            const float y0 = y[2 * s + (e >> 2)][e & 3], y1 = y[2 * s + (e >> 2)][(e & 3) + 1];
             h2 hi, lo;
-            split2(y[s][e] * f, y[s][e + 1] * f, y[s][e], y[s][e + 1], f, hi, lo);
+            split2(y0 * f, y1 * f, y0, y1, f, hi, lo);
             qh[s][e] = hi[0], qh[s][e + 1] = hi[1], ql[s][e] = lo[0], ql[s][e + 1] = lo[1];
         }
-    return __builtin_amdgcn_ldexpf(LOG2E / sqrtf((float)a.head_dim), -ex);
+    return __builtin_amdgcn_ldexpf(LOG2E / sqrtf((float)head_dim), -ex);
+}
+
+/* ... straight from memory */
+__device__ inline auto memory_q(const PromptArgs &a, const Lane &x) {
+    const float *src = a.q + (size_t)x.r * a.q_stride + (size_t)x.h * a.head_dim;
+    const int n = x.live ? a.head_dim / 4 : 0;
+    return [=](int i) { return i < n ? (f4)*(const f4u *)(src + 4 * i) : f4{0.f, 0.f, 0.f, 0.f}; };
+}
+
+/* With two groups, the m-rows' q and outputs go through LDS, row by row: a lane
+ * holds one m-row's values, and 64 rows in an access of 16 bytes a lane are
+ * many lines for the address unit (loading q took 2.2 - 3.6 us of a
+ * workgroup's prologue that way, writing o 2.4).  512 tokens 22.5 -> 21.0 us;
+ * with one group, whose q would have to come before its first tile, 16 tokens
+ * took 10.0 instead of 8.8.  Rows of HD floats, 16-byte piece i of row r at
+ * place i ^ (r mod HD / 4), where neither order of access meets itself in a
+ * bank. */
+template <int HD>
+__device__ inline uint32_t row_piece(int row, int piece) {
+    return (uint32_t)((piece ^ (row & (HD / 4 - 1))) << 4);
+}
+/* q of the tile's ROWS m-rows by direct copies, `waves` of them from `wave`
+ * on: the first half of the rows to lo, the second to hi */
+template <int HD, int ROWS>
+__device__ inline void copy_q(const PromptArgs &a, const Work &w, int ratio, int wave, int waves, uint8_t *lo, uint8_t *hi) {
+    constexpr int R = 256 / HD, N = ROWS / R;   /* rows of a copy, copies */
+    const int lane = threadIdx.x & 63, place = lane % (HD / 4);
+    const u32x4 d = buf_desc(a.q + (size_t)(w.sq.r0 + w.i0) * a.q_stride + (size_t)w.kh * ratio * a.head_dim, 0x7FFFFF00u);
+    for (int n = wave; n < N; n += waves) {
+        const int row = R * n + lane / (HD / 4), piece = place ^ (row & (HD / 4 - 1));
+        int i, j;
+        w.row(row, ratio, i, j);
+        const uint32_t off = ((uint32_t)(i - w.i0) * (uint32_t)a.q_stride + (uint32_t)(j * a.head_dim + 4 * piece)) * 4u;
+        copy_lanes(d, i < w.sq.n && 4 * piece < a.head_dim ? off : 0x7FFFFF00u,
+                   lds_addr(n < N / 2 ? lo : hi) + 1024u * (uint32_t)(n % (N / 2)));
+    }
+}
+/* the staged outputs, rows of wave v at lds + v * stride, to where they go */
+template <int HD, int ROWS>
+__device__ inline void store_rows(int head_dim, const uint8_t *lds, int stride, const long long *where, float *base, int wave,
+                                  int waves) {
+    constexpr int R = 256 / HD;
+    const int lane = threadIdx.x & 63, piece = lane % (HD / 4);
+    for (int n = wave; n < ROWS / R; n += waves) {
+        const int row = R * n + lane / (HD / 4);
+        const long long at = where[row];
+        const f4 y = *(const f4 *)(lds + (row >> 5) * stride + (row & 31) * (HD * 4) + row_piece<HD>(row, piece));
+        if (at >= 0 && 4 * piece < head_dim) *(f4u *)(base + at + 4 * piece) = y;
+    }
 }
 
 /* Byte offset in a tile of 16-bit rows of the lane's operand of the first
@@ -584,12 +647,14 @@ __device__ inline void mask_scores(f16v &s, int at, const Lane &x) {
     }
 }
 
-/* The wave's rows written: weights were summed in units of 2^(mx - W_SHIFT)
- * relative to l, values (SCALED) besides in units of 2^-oexp.  Returns the m-rows that
+/* The wave's rows finished: weights were summed in units of 2^(mx - W_SHIFT)
+ * relative to l, values (SCALED) besides in units of 2^-oexp.  They go to
+ * `stage` (LDS, the wave's 32 rows), where[] saying where in p.o or a.out each
+ * belongs (-1: nowhere), or without stage to memory.  Returns the m-rows that
  * came out not finite, which are not written. */
 template <int HD, bool SCALED>
 __device__ inline uint32_t write_rows(const PromptArgs &a, const RowsPlan &p, const Work &w, const Lane &x, int lane, float mx,
-                                      float l, int oexp, const f16v (&o)[HD / 32]) {
+                                      float l, int oexp, const f16v (&o)[HD / 32], uint8_t *stage, long long *where) {
     float big = fabsf(l);   /* NaN where anything is */
 #pragma unroll
     for (int d = 0; d < HD / 32; d++)
@@ -597,26 +662,28 @@ __device__ inline uint32_t write_rows(const PromptArgs &a, const RowsPlan &p, co
         for (int v = 0; v < 16; v++) big = max_nan(big, fabsf(o[d][v]));
     const uint64_t mask = __ballot(x.live && !(big < INFINITY));
     const uint32_t bad = (uint32_t)mask | (uint32_t)(mask >> 32);
-    if (!x.live || ((bad >> (lane & 31)) & 1u)) return bad;
-    const int half = lane >> 5, hd = a.head_dim;
-    float *dst, f;
+    const int half = lane >> 5, row = lane & 31, hd = a.head_dim;
+    bool write = x.live && !((bad >> row) & 1u);
+    long long at;
+    float f = 1.f;
     if (p.nrec) {
         const size_t rec = ((size_t)x.r * a.n_heads + x.h) * p.nrec + w.rec;
         constexpr float one = 1.f / 8192.f;   /* 2^-W_SHIFT */
-        if (half == 0) write_ml(p, w, rec, mx, l * one);
-        if (mx == -INFINITY) return bad;   /* a record of no position has no sums */
-        dst = p.o + rec * hd;
+        if (write && half == 0) write_ml(p, w, rec, mx, l * one);
+        write = write && mx > -INFINITY;      /* a record of no position has no sums */
+        at = (long long)(rec * hd);
         f = one;
     } else {
-        f = 1.f;
-        if (a.sinks) {
+        if (a.sinks && write) {
             const float ref = mx - W_SHIFT, sk = a.sinks[x.h] * LOG2E, M = fmaxf(ref, sk), base = M == -INFINITY ? 0.f : M;
             f = exp2f(ref - base);
             l = l * f + exp2f(sk - base);
         }
         f /= l;
-        dst = a.out + (size_t)x.r * a.out_stride + (size_t)x.h * hd;
+        at = (long long)x.r * a.out_stride + (long long)x.h * hd;
     }
+    if (stage && half == 0) where[row] = write ? at : -1;
+    float *dst = (p.nrec ? p.o : a.out) + at;
 #pragma unroll
     for (int d = 0; d < HD / 32; d++)
 #pragma unroll
@@ -625,7 +692,8 @@ __device__ inline uint32_t write_rows(const PromptArgs &a, const RowsPlan &p, co
             f4 y;
 #pragma unroll
             for (int e = 0; e < 4; e++) y[e] = SCALED ? __builtin_amdgcn_ldexpf(o[d][4 * v + e] * f, -oexp) : o[d][4 * v + e] * f;
-            if (dim < hd) *(f4u *)(dst + dim) = y;
+            if (stage) *(f4 *)(stage + row * (HD * 4) + row_piece<HD>(row, 8 * d + 2 * v + half)) = y;
+            else if (write && dim < hd) *(f4u *)(dst + dim) = y;
         }
     return bad;
 }
@@ -671,12 +739,13 @@ __device__ inline void merge_groups(float *lds, int wave, int lane, float &mx, f
  * latencies (8192 tokens: 928 us, one at a time 965), one is half the code
  * and skips what a window hides (4,096 tokens, window 128: 46.2, 48.6). */
 template <int HD, int MW, int KG, int J>
-__global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_h(PromptArgs a, RowsPlan p) {
+__global__ __launch_bounds__(64 * MW * KG, HD == 64 && J == 1 ? 4 : 2) void k_rows_h(PromptArgs a, RowsPlan p) {
     constexpr int RB = HD * 2, TILE = KT * RB;       /* bytes of a row in LDS, of a tile of K or V */
     constexpr int NC = TILE / 1024 / MW;             /* copies of 1 KiB a wave, matrix and tile */
     constexpr int DB = HD / 32, STEPS = HD / 16;
     __shared__ __attribute__((aligned(1024))) uint8_t bufs[KG][2][2][TILE];
     __shared__ uint32_t bad_rows[MW];
+    __shared__ long long where[KG == 2 ? 32 * MW : 1];
     const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
     Work w;
     if (!find_work<32 * MW>(a, p, ratio, w)) return;
@@ -702,10 +771,22 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_h(PromptArgs a, RowsPl
     };
     static_assert(MW * 1024 / RB % 16 == 0, "swz of a copy's rows is that of the first");
     if (w.lo + group * KT < w.hi) copy_tile(w.lo + group * KT, 0);
-    const Lane x = lane_rows(a, w, w.m0 + 32 * mwave, lane & 31, 32, ratio);
+    /* two groups: q comes by way of their second buffers, with the first tiles
+     * (one group would have to fetch one after the other) */
+    static_assert(KG == 1 || 32 * MW * HD * 4 == sizeof bufs / 2, "q fits");
+    if constexpr (KG == 2) copy_q<HD, 32 * MW>(a, w, ratio, wave, MW * KG, bufs[0][1][0], bufs[1][1][0]);
+    const Lane x = lane_rows(a, w, 32 * mwave, lane & 31, 32, ratio);
 
     h8 qh[STEPS], ql[STEPS];
-    const float c = load_q<HD>(a, x, half, qh, ql);
+    float c;
+    if constexpr (KG == 2) {
+        wait_copies();
+        bar_lds();
+        const uint8_t *mine = bufs[mwave / (MW / 2)][1][0] + (mwave % (MW / 2) * 32 + (lane & 31)) * (HD * 4);
+        c = load_q<HD>(hd, half, [&](int i) { return *(const f4 *)(mine + row_piece<HD>(lane & 31, i)); }, qh, ql);
+    } else {
+        c = load_q<HD>(hd, half, memory_q(a, x), qh, ql);
+    }
     f16v o[DB];
 #pragma unroll
     for (int d = 0; d < DB; d++)
@@ -805,16 +886,22 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_h(PromptArgs a, RowsPl
     }
     l = other_half_sum(l);
     int oexp = 0;
-    if constexpr (KG == 2)
-        if (w.hi - w.lo > KT) merge_groups<HD, MW>((float *)bufs, wave, lane, mx, l, oexp, o);   /* else group 1 had no tile */
+    if (KG == 2 && w.hi - w.lo > KT) merge_groups<HD, MW>((float *)bufs, wave, lane, mx, l, oexp, o);
+    else __syncthreads();   /* one group, or the second had no tile: all are done with the tiles */
+    constexpr int STRIDE = 64 * (HD / 2 + 3) * 4;   /* a wave's share of merge_groups' room */
     if (group == 0) {
-        const uint32_t bad = write_rows<HD, false>(a, p, w, x, lane, mx, l, oexp, o);
+        const uint32_t bad = write_rows<HD, false>(a, p, w, x, lane, mx, l, oexp, o, KG == 2 ? (uint8_t *)bufs + wave * STRIDE : nullptr,
+                                                   where + (KG == 2 ? 32 * wave : 0));
         if (lane == 0) bad_rows[wave] = bad;
     }
     __syncthreads();
+    if constexpr (KG == 2) {
+        store_rows<HD, 32 * MW>(hd, (const uint8_t *)bufs, STRIDE, where, p.nrec ? p.o : a.out, wave, MW * KG);
+        __syncthreads();
+    }
     for (int wv = 0; wv < MW; wv++)
         for (uint32_t y = bad_rows[wv]; y; y &= y - 1)
-            slow_row<_Float16>(a, p, w, w.m0 + 32 * wv + __builtin_ctz(y), ratio, (float *)bufs);
+            slow_row<_Float16>(a, p, w, 32 * wv + __builtin_ctz(y), ratio, (float *)bufs);
 }
 
 /* ---- float32 caches on the f16 matrix units ----
@@ -847,6 +934,7 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPl
     __shared__ __attribute__((aligned(1024))) uint8_t bufs[KG][2][4][PLANE];
     __shared__ int all_exps[KG][2][8];
     __shared__ uint32_t bad_rows[MW];
+    __shared__ long long where[KG == 2 ? 32 * MW : 1];
     const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
     Work w;
     if (!find_work<32 * MW>(a, p, ratio, w)) return;
@@ -919,10 +1007,19 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPl
     };
     const int t1 = w.lo + group * KF;   /* the group's first tile; past the span: zeros */
     load_tile(t1);
-    const Lane x = lane_rows(a, w, w.m0 + 32 * mwave, lane & 31, 32, ratio);
+    if constexpr (KG == 2) copy_q<HD, 32 * MW>(a, w, ratio, wave, MW * KG, bufs[0][1][0], bufs[1][1][0]);
+    const Lane x = lane_rows(a, w, 32 * mwave, lane & 31, 32, ratio);
 
     h8 qh[STEPS], ql[STEPS];
-    const float c = load_q<HD>(a, x, half, qh, ql);
+    float c;
+    if constexpr (KG == 2) {
+        wait_copies();
+        bar_lds();
+        const uint8_t *mine = bufs[mwave / (MW / 2)][1][0] + (mwave % (MW / 2) * 32 + (lane & 31)) * (HD * 4);
+        c = load_q<HD>(hd, half, [&](int i) { return *(const f4 *)(mine + row_piece<HD>(lane & 31, i)); }, qh, ql);
+    } else {
+        c = load_q<HD>(hd, half, memory_q(a, x), qh, ql);
+    }
     f16v o[DB];
 #pragma unroll
     for (int d = 0; d < DB; d++)
@@ -1028,16 +1125,22 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPl
         bar_lds();
     }
     l = other_half_sum(l);
-    if constexpr (KG == 2)
-        if (w.hi - w.lo > KF) merge_groups<HD, MW>((float *)bufs, wave, lane, mx, l, U, o);   /* else group 1 had no tile */
+    if (KG == 2 && w.hi - w.lo > KF) merge_groups<HD, MW>((float *)bufs, wave, lane, mx, l, U, o);
+    else __syncthreads();   /* one group, or the second had no tile: all are done with the tiles */
+    constexpr int STRIDE = 64 * (HD / 2 + 3) * 4;   /* a wave's share of merge_groups' room */
     if (group == 0) {
-        const uint32_t bad = write_rows<HD, true>(a, p, w, x, lane, mx, l, U, o);
+        const uint32_t bad = write_rows<HD, true>(a, p, w, x, lane, mx, l, U, o, KG == 2 ? (uint8_t *)bufs + wave * STRIDE : nullptr,
+                                                  where + (KG == 2 ? 32 * wave : 0));
         if (lane == 0) bad_rows[wave] = bad;
     }
     __syncthreads();
+    if constexpr (KG == 2) {
+        store_rows<HD, 32 * MW>(hd, (const uint8_t *)bufs, STRIDE, where, p.nrec ? p.o : a.out, wave, MW * KG);
+        __syncthreads();
+    }
     for (int wv = 0; wv < MW; wv++)
         for (uint32_t y = bad_rows[wv]; y; y &= y - 1)
-            slow_row<float>(a, p, w, w.m0 + 32 * wv + __builtin_ctz(y), ratio, (float *)bufs);
+            slow_row<float>(a, p, w, 32 * wv + __builtin_ctz(y), ratio, (float *)bufs);
 }
 
 /* ---- few rows: positions over the waves ----
@@ -1169,7 +1272,7 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
     if (!find_work<MN>(a, p, ratio, w)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c16 = lane & 15, kq = lane >> 4;
-    const Lane x = lane_rows(a, w, w.m0, c16, 16, ratio);
+    const Lane x = lane_rows(a, w, 0, c16, 16, ratio);
     if (tid == 0) bad_rows = 0;
 
     const uint32_t rb = (uint32_t)hd * (uint32_t)sizeof(T);
@@ -1234,7 +1337,7 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
     __syncthreads();
     /* the four waves' sums as one, in wave order: 16 threads a row, HD / 16 dims each */
     const int row = tid >> 4, d0 = (tid & 15) * N;
-    const Lane y = lane_rows(a, w, w.m0, row, 16, ratio);
+    const Lane y = lane_rows(a, w, 0, row, 16, ratio);
     float M = fmaxf(fmaxf(mm[0][row], mm[1][row]), fmaxf(mm[2][row], mm[3][row]));
     const float base = M == -INFINITY ? 0.f : M;
     float L = 0.f, r[N];
@@ -1273,7 +1376,7 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
             for (int n = 0; n < N; n += 4) *(f4u *)(dst + n) = f4{r[n] * f, r[n + 1] * f, r[n + 2] * f, r[n + 3] * f};
         }
     }
-    for (uint32_t z = bad; z; z &= z - 1) slow_row<T>(a, p, w, w.m0 + __builtin_ctz(z), ratio, &mo[0][0][0]);
+    for (uint32_t z = bad; z; z &= z - 1) slow_row<T>(a, p, w, __builtin_ctz(z), ratio, &mo[0][0][0]);
 }
 
 /* The records of a row and head, and its sink, as one: W waves each, wave g
