@@ -158,6 +158,50 @@ def test_cache_ranges(tg, half):
         b.check(got, was)
 
 
+@pytest.mark.parametrize("what", ["k", "v", "both"])
+@pytest.mark.parametrize("big", [3e38, 1e12, 7e4])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_large_neighbours(tg, hd, big, what):
+    """A position's huge but finite K or V (f32 caches) leaves the rows that do
+    not see it as they are to their own precision: in front of it in one group
+    of positions, in the next, and where a window has passed it."""
+    say(f"large neighbours hd={hd} big={big} {what}")
+    for lens, past, window, at in (([5], [0], 0, 4), ([40], [3], 0, 12), ([200], [0], 0, 150), ([60, 9], [100, 700], 30, 107)):
+        b = Batch(hd, 8, 2, hd, lens, past, False, window=window, q_scale=0.5)
+        ref, tol = b.attend()
+        for name in "kv" if what == "both" else what:
+            getattr(b, name)[b.slots[0], :, at] *= np.float32(big / 4)
+        np.clip(b.k, -3e38, 3e38, out=b.k)
+        np.clip(b.v, -3e38, 3e38, out=b.v)
+        got, was = _run(tg, b)
+        blind = np.zeros(b.rows, bool)
+        for s in range(b.n):
+            for i in range(b.lens[s]):
+                lo, hi = b.seen(s, i)
+                blind[b.cu[s] + i] = s != 0 or not lo <= at <= hi
+        assert blind.any()
+        err = np.abs(got - ref)[blind]
+        assert np.all(err <= tol[blind]), float((err / tol[blind]).max())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_values_of_many_sizes(tg, hd):
+    """f32 caches whose positions differ by powers of two up to 2^14 keep the
+    matrix units' path, beyond that the plain one; zeros count as neither."""
+    for top, zero in ((10, False), (14, True), (40, True)):
+        say(f"values of many sizes hd={hd} top={top}")
+        b = Batch(hd + top, 8, 2, hd, [33, 4], [90, 300], False, q_scale=0.5)
+        rng = np.random.default_rng(top)
+        for s in range(2):
+            m = b.lens[s] + b.past[s]
+            for t in (b.k, b.v):
+                t[b.slots[s], :, :m] *= np.exp2(-rng.integers(0, top, m)).astype(np.float32)[None, :, None]
+                if zero:
+                    t[b.slots[s], :, 5:17] = 0
+        got, was = _run(tg, b)
+        b.check(got, was)
+
+
 def test_sequences_that_do_not_fit_are_left_out(tg):
     """A slot out of range, a negative length, rows past kv_max: those
     sequences' rows stay as they were, the others are computed."""

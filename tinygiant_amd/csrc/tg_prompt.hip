@@ -422,8 +422,8 @@ __device__ void slow_row(const PromptArgs &a, const RowsPlan &p, const Work &w, 
  * two f16 (hi the nearest, lo the nearest to the rest: 22 bits), so each
  * product is two MFMAs, and the result is as good as f32 sums.  What keeps
  * lo out of f16's underflow: q is scaled by a power of two a row (its largest
- * value to 2^13 .. 2^14), undone in the factor that takes scores to base 2;
- * weights are taken times 2^13.
+ * value to 2^14 .. 2^15), undone in the factor that takes scores to base 2;
+ * weights are taken times 2^15.
  *
  * K and V tiles of 64 positions go to LDS by direct copies, two buffers; the
  * 16-byte pieces of a row are permuted by its position (swz) so that neither
@@ -478,7 +478,7 @@ __device__ inline float other_half_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-constexpr float W_SHIFT = 13.f;   /* weights are taken times 2^13 */
+constexpr float W_SHIFT = 15.f;   /* weights are taken times 2^15, below f16's largest */
 
 /* A lane's m-row (both halves of a wave hold the same 32) and what its wave
  * sees: positions any_lo .. any_hi by some row, all_lo .. all_hi by all. */
@@ -534,9 +534,9 @@ __device__ inline uint32_t wave_umax(uint32_t v) {
     return max(max(a, b), max(c, d));
 }
 
-/* the power of two that takes a largest magnitude to 2^13 .. 2^14, as its exponent */
+/* the power of two that takes a largest magnitude to 2^14 .. 2^15, as its exponent */
 __device__ inline int scale_exp(float big) {
-    return big > 0.f && big < INFINITY ? min(14 - __builtin_amdgcn_frexp_expf(big), 100) : 0;
+    return big > 0.f && big < INFINITY ? min(15 - __builtin_amdgcn_frexp_expf(big), 100) : 0;
 }
 
 /* q of the lane's m-row as the B operands of the first product, two f16
@@ -668,7 +668,7 @@ __device__ inline uint32_t write_rows(const PromptArgs &a, const RowsPlan &p, co
     float f = 1.f;
     if (p.nrec) {
         const size_t rec = ((size_t)x.r * a.n_heads + x.h) * p.nrec + w.rec;
-        constexpr float one = 1.f / 8192.f;   /* 2^-W_SHIFT */
+        constexpr float one = 1.f / 32768.f;   /* 2^-W_SHIFT */
         if (write && half == 0) write_ml(p, w, rec, mx, l * one);
         write = write && mx > -INFINITY;      /* a record of no position has no sums */
         at = (long long)(rec * hd);
@@ -909,21 +909,35 @@ __global__ __launch_bounds__(64 * MW * KG, HD == 64 && J == 1 ? 4 : 2) void k_ro
  * The same products with K and V split as q and the weights are: x 2^k = hi +
  * lo, 22 bits, and three MFMAs a product (hi hi, hi lo, lo hi; lo lo is below
  * 2^-22).  k is chosen for each group of 8 positions from its largest finite
- * magnitude, so any f32 range fits: a value down to 2^-15 of its group's
- * largest keeps 22 bits, a smaller one is off by 2^-38 of the largest.  (f32
- * MFMAs run at a sixteenth of the f16 rate, three bf16 planes would take six
- * products.)
+ * magnitude: a value down to 2^-17 of that keeps 22 bits, a smaller one is off
+ * by 2^-39 of it.  (f32 MFMAs run at a sixteenth of the f16 rate, three bf16
+ * planes would take six products.)
  *
  * A group is one wave's share of a tile's loads, and positions 8 g .. 8 g + 7
  * are registers 4 g .. 4 g + 3 of the scores in both halves of the wave: K's
  * scale only changes the factor to base 2.  V's groups have scales of their
  * own; o is in units of 2^-U, U the smallest k so far, and a group's weights
- * take 2^(U - k).
+ * take 2^(U - k), which is part of their exponent and taken back in their sum.
+ *
+ * What a position holds must not cost the others their precision, the less so
+ * where a row does not see it.  So the positions of a group may differ by
+ * 2^SPREAD in their largest magnitudes (zeros aside), and so may the groups
+ * of V; where they differ by more, the workgroup's rows are computed value by
+ * value, as those are that are not finite.
  *
  * A tile of 32 positions is loaded into registers two tiles ahead, split and
  * stored to one of two LDS buffers one tile ahead (plane [K hi, K lo, V hi,
  * V lo][32][HD]). */
-constexpr int KF = 32;
+constexpr int KF = 32, SPREAD = 15;
+constexpr int ALL_ZERO = 100;   /* exponent of a group of zeros; no other is larger */
+
+/* HD / 4 lanes hold a position: whether each has a bit in m, or none in any */
+template <int HD>
+__device__ inline bool every_row(uint64_t m, uint64_t any) {
+    if (HD == 128) return ((uint32_t)m || !(uint32_t)any) && ((uint32_t)(m >> 32) || !(uint32_t)(any >> 32));
+    constexpr uint64_t L = 0x7FFF7FFF7FFF7FFFull;   /* 16-bit fields: the top bit of those that are not 0 */
+    return ((((m & L) + L) | m | ~(((any & L) + L) | any)) | L) == ~0ull;
+}
 
 template <int HD, int MW, int KG>
 __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPlan p) {
@@ -933,6 +947,7 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPl
     constexpr int DB = HD / 32, STEPS = HD / 16;
     __shared__ __attribute__((aligned(1024))) uint8_t bufs[KG][2][4][PLANE];
     __shared__ int all_exps[KG][2][8];
+    __shared__ int range[MW * KG][2];   /* each wave's least and most */
     __shared__ uint32_t bad_rows[MW];
     __shared__ long long where[KG == 2 ? 32 * MW : 1];
     const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
@@ -963,29 +978,49 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPl
             }
         }
     };
+    const uint64_t padding = __ballot(ldim >= hd);
+    int least = ALL_ZERO, most = -2 * ALL_ZERO;   /* exponents of the wave's groups of V; 1000: a group is too wide */
     auto split_tile = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < UNITS; u++) {
             const int g = u * MW + mwave;
-            float big = 0.f;
+            float top[NL], big = 0.f;
 #pragma unroll
-            for (int j = 0; j < NL; j++)
-#pragma unroll
-                for (int e = 0; e < 4; e += 2)
-                    big = max_nan(max_nan(big, fabsf(__uint_as_float(raw[u][j][e]))), fabsf(__uint_as_float(raw[u][j][e + 1])));
+            for (int j = 0; j < NL; j++) {
+                const f4 y = __builtin_bit_cast(f4, raw[u][j]);
+                top[j] = max_nan(max_nan(max_nan(fabsf(y[0]), fabsf(y[1])), fabsf(y[2])), fabsf(y[3]));
+                big = max_nan(big, top[j]);
+            }
             uint32_t bits = wave_umax(__float_as_uint(big));
             if (bits >= 0x7F800000u) {   /* uniform: the largest of the finite ones */
                 uint32_t fin = 0;
 #pragma unroll
-                for (int j = 0; j < NL; j++)
+                for (int j = 0; j < NL; j++) {
+                    uint32_t of_row = 0;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const uint32_t y = raw[u][j][e] & 0x7FFFFFFFu;
-                        fin = max(fin, y < 0x7F800000u ? y : 0u);
+                        of_row = max(of_row, y < 0x7F800000u ? y : 0u);
                     }
+                    top[j] = __uint_as_float(of_row);
+                    fin = max(fin, of_row);
+                }
                 bits = wave_umax(fin);
             }
-            const int ex = min(140 - (int)(bits >> 23), 100);   /* scale_exp, and 100 where all are zero */
+            const int ex = min(141 - (int)(bits >> 23), ALL_ZERO);   /* scale_exp's */
+            /* every position comes near the largest: mostly in each lane's
+             * share of each, else it takes one lane of a position, or zeros */
+            const float near = __uint_as_float(bits > ((uint32_t)SPREAD << 23) ? bits - ((uint32_t)SPREAD << 23) : 0u);
+            float low = top[0];
+#pragma unroll
+            for (int j = 1; j < NL; j++) low = fminf(low, top[j]);
+            if ((__ballot(low >= near) | padding) != ~0ull) {
+                bool narrow = true;
+#pragma unroll
+                for (int j = 0; j < NL; j++) narrow = narrow && every_row<HD>(__ballot(top[j] >= near), __ballot(top[j] > 0.f));
+                if (!narrow) most = 1000;
+            }
+            if (g >= 4 && ex < ALL_ZERO) least = min(least, ex), most = max(most, ex);
             const float f = __uint_as_float((uint32_t)(ex + 127) << 23);
             if (lane == 0) exps[b][g] = ex;
 #pragma unroll
@@ -1026,7 +1061,8 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPl
 #pragma unroll
         for (int v = 0; v < 16; v++) o[d][v] = 0.f;
     float mx = -INFINITY, l = 0.f;
-    int U = 100;
+    int U = ALL_ZERO;
+    const float one = opaque_one();
     const uint32_t kaddr = k_operand<HD>(lane);
     uint32_t vaddr[DB][2];
 #pragma unroll
@@ -1091,23 +1127,24 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPl
             }
             mx = mn, U = un;
             h8 ph[2], pl[2];
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int g = 0; g < 4; g++) {
-                const float f = __builtin_amdgcn_ldexpf(1.f, un - ve[g]);
+                const int d = min(ve[g] - un, SPREAD);   /* more: zeros, or the rows are done again */
+                const float shg = sh - (float)d;
+                float sum[2] = {0.f, 0.f};
 #pragma unroll
                 for (int e = 0; e < 4; e += 2) {
-                    const float y0 = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], cg[g], sh));
-                    const float y1 = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e + 1], cg[g], sh));
-                    sum[e] += y0, sum[e + 1] += y1;
+                    const float y0 = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], cg[g], shg));
+                    const float y1 = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e + 1], cg[g], shg));
+                    sum[0] += y0, sum[1] += y1;
                     h2 hi, lo;
-                    split2(y0 * f, y1 * f, y0, y1, f, hi, lo);
+                    split2(y0, y1, y0, y1, one, hi, lo);
                     const int at = 4 * (g & 1) + e;
                     ph[g >> 1][at] = hi[0], ph[g >> 1][at + 1] = hi[1];
                     pl[g >> 1][at] = lo[0], pl[g >> 1][at + 1] = lo[1];
                 }
+                l = fmaf(sum[0] + sum[1], __uint_as_float((uint32_t)(d + 127) << 23), l);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
             for (int i = 0; i < 2 * DB; i++) {
                 const h8 nh = i + 1 < 2 * DB ? column(i + 1, 0) : vh, nl = i + 1 < 2 * DB ? column(i + 1, 1) : vl;
@@ -1124,11 +1161,14 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPl
         }
         bar_lds();
     }
+    if (lane == 0) range[wave][0] = least, range[wave][1] = most;
     l = other_half_sum(l);
     if (KG == 2 && w.hi - w.lo > KF) merge_groups<HD, MW>((float *)bufs, wave, lane, mx, l, U, o);
     else __syncthreads();   /* one group, or the second had no tile: all are done with the tiles */
     constexpr int STRIDE = 64 * (HD / 2 + 3) * 4;   /* a wave's share of merge_groups' room */
     if (group == 0) {
+        for (int v = 0; v < MW * KG; v++) least = min(least, range[v][0]), most = max(most, range[v][1]);
+        if (most - least > SPREAD) l = NAN;
         const uint32_t bad = write_rows<HD, true>(a, p, w, x, lane, mx, l, U, o, KG == 2 ? (uint8_t *)bufs + wave * STRIDE : nullptr,
                                                   where + (KG == 2 ? 32 * wave : 0));
         if (lane == 0) bad_rows[wave] = bad;
