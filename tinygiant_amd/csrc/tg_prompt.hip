@@ -52,6 +52,30 @@ __device__ inline int seq_of(const PackedSeqs &p, int r) {
     return lo;
 }
 
+/* The sequence of row r, the same r in the whole wave: 64 sequences at a time,
+ * all that is read of them in one batch.  False: none. */
+__device__ inline bool wave_seq_of(const PackedSeqs &p, int r, Seq &q, int &i) {
+    const int lane = threadIdx.x & 63;
+    Seq mine = {0, 0, 0, 0};
+    uint64_t m = 0;
+    for (int s0 = 0; s0 < p.n; s0 += 64) {
+        const bool on = s0 + lane < p.n;
+        Seq next = {0, 0, 0, 0};
+        if (on) next = seq_at(p, s0 + lane);
+        const uint64_t from = __ballot(on && next.r0 <= r);
+        if (!from) break;
+        m = from, mine = next;
+    }
+    if (!m) return false;
+    const int at = 63 - __builtin_clzll(m);   /* the last that starts at or before r */
+    q.r0 = __builtin_amdgcn_readlane(mine.r0, at);
+    q.n = __builtin_amdgcn_readlane(mine.n, at);
+    q.past = __builtin_amdgcn_readlane(mine.past, at);
+    q.slot = __builtin_amdgcn_readlane(mine.slot, at);
+    i = r - q.r0;
+    return i >= 0 && i < q.n;
+}
+
 }  // namespace
 
 /* ---- append ----
@@ -63,11 +87,10 @@ __device__ inline int seq_of(const PackedSeqs &p, int r) {
  * nearest. */
 template <bool HALF, int G>
 __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
-    const int r = blockIdx.x, s = seq_of(a.s, r);
-    if (s < 0) return;
-    const Seq sq = seq_at(a.s, s);
-    const int i = r - sq.r0;
-    if (i < 0 || i >= sq.n) return;
+    const int r = blockIdx.x;
+    Seq sq;
+    int i;
+    if (!wave_seq_of(a.s, r, sq, i)) return;
     const int at = sq.past + i, pos = a.base_pos + at;
     const bool turn = a.rope_cos != nullptr;
     if (turn && pos >= a.rope_len) return;
@@ -1430,43 +1453,50 @@ __global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) 
     const long long at = W > 1 ? (long long)blockIdx.x : (long long)blockIdx.x * 4 + (tid >> 6);
     if (at >= (long long)a.s.rows * a.n_heads) return;
     const int r = (int)(at / a.n_heads), h = (int)(at - (long long)r * a.n_heads);
-    const int s = seq_of(a.s, r);
-    if (s < 0) return;
-    const Seq sq = seq_at(a.s, s);
-    if (r - sq.r0 < 0 || r - sq.r0 >= sq.n) return;
     const float *ml = p.ml + 4 * (size_t)at * p.nrec, *po = p.o + (size_t)at * p.nrec * hd;
+    const int g = lane / G, d = 4 * (lane % G);
+    /* lane i holds record W i + wave of each 64 W.  The first ones' statistics
+     * and sums are read before it is known that they are there (there is room
+     * for them), so that nothing waits for the row's sequence. */
+    constexpr int N = 4;   /* records of a lane's loads at a time */
+    f4 stat = {-INFINITY, 0.f, 0.f, 0.f}, y[N];
+    if (W * lane + wave < p.nrec) stat = *(const f4 *)(ml + 4 * (W * lane + wave));
+    float m0 = -INFINITY, m1 = -INFINITY;   /* at most 128 records (rows_cut) */
+    if (lane < p.nrec) m0 = ml[4 * lane];
+    if (lane + 64 < p.nrec) m1 = ml[4 * (lane + 64)];
+    const int count = __float_as_int(ml[4 * p.pre_ns + 2]);
+    auto load = [&](int c0, int j0) {
+#pragma unroll
+        for (int q = 0; q < N; q++) {
+            const int c = c0 + W * (j0 + q * PER + g) + wave;
+            y[q] = f4{0.f, 0.f, 0.f, 0.f};
+            if (c < p.nrec && d < hd) y[q] = *(const f4 *)(po + (size_t)c * hd + d);
+        }
+    };
+    load(0, 0);
+    Seq sq;
+    int i;
+    if (!wave_seq_of(a.s, r, sq, i)) return;
     const float sink = a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
-    /* the prefix's records and the tile's own; lane i: record W i + wave of each 64 W */
-    const int own = __float_as_int(ml[4 * p.pre_ns + 2]), nrec = min(p.pre_ns + max(own, 0), p.nrec);
-    float M = -INFINITY;
-    for (int c = lane; c < p.nrec; c += 64) {   /* read past the count too, which arrives with them */
-        const float m = ml[4 * c];
-        M = c < nrec ? fmaxf(M, m) : M;
-    }
-    M = fmaxf(wave_max(M), sink);
+    const int nrec = min(p.pre_ns + max(count, 0), p.nrec);   /* the prefix's records and the tile's own */
+    const float M = fmaxf(wave_max(fmaxf(lane < nrec ? m0 : -INFINITY, lane + 64 < nrec ? m1 : -INFINITY)), sink);
     const float base = M == -INFINITY ? 0.f : M;
     float l = 0.f;
     f4 o = {0.f, 0.f, 0.f, 0.f};
-    const int g = lane / G, d = 4 * (lane % G);
     for (int c0 = 0; c0 < nrec; c0 += 64 * W) {
         const int c = c0 + W * lane + wave;
-        const float2 x = c < nrec ? *(const float2 *)(ml + 4 * c) : make_float2(-INFINITY, 0.f);
-        const float e = x.x == -INFINITY ? 0.f : exp2f(x.x - base);
-        l += e == 0.f ? 0.f : x.y * e;
+        if (c0 && c < p.nrec) stat = *(const f4 *)(ml + 4 * c);
+        const float e = c < nrec && stat[0] != -INFINITY ? exp2f(stat[0] - base) : 0.f;
+        l += e == 0.f ? 0.f : stat[1] * e;
         const int n = min(64, (nrec - c0 - wave + W - 1) / W);
-        for (int j0 = 0; j0 < n; j0 += 4 * PER) {   /* four records' loads at a time */
-            f4 y[4];
-            float f[4];
+        for (int j0 = 0; j0 < n; j0 += N * PER) {
+            if (c0 + j0) load(c0, j0);
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
+            for (int q = 0; q < N; q++) {
                 const int j = j0 + q * PER + g;
-                f[q] = __shfl(e, j & 63, 64);
-                y[q] = f4{0.f, 0.f, 0.f, 0.f};
-                if (j < n && f[q] != 0.f && d < hd)   /* a record of no position has no sums */
-                    y[q] = *(const f4 *)(po + (size_t)(c0 + W * j + wave) * hd + d);
+                const float f = __shfl(e, j & 63, 64);
+                if (j < n && f != 0.f) o += y[q] * f;   /* a record of no position has no sums */
             }
-#pragma unroll
-            for (int q = 0; q < 4; q++) o += y[q] * f[q];
         }
     }
     l = wave_sum(l);
@@ -1489,8 +1519,7 @@ __global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) 
     }
     if (lane >= G || d >= hd) return;
     if (a.sinks) l += exp2f(sink - base);
-    const f4 y = o / l;
-    *(f4u *)(a.out + (size_t)r * a.out_stride + (size_t)h * hd + d) = y;
+    *(f4u *)(a.out + (size_t)r * a.out_stride + (size_t)h * hd + d) = o / l;
 }
 
 /* How a call is cut, from the host's arguments alone (the lengths are on the
