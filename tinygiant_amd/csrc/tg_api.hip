@@ -1531,11 +1531,7 @@ TG_API size_t tg_hip_attention_prompt_scratch_bytes(int n_rows, int n_seqs, int 
         head_dim > PROMPT_MAX_HEAD_DIM || kv_max <= 0 || prefix_len < 0)
         return 0;
     std::lock_guard<std::recursive_mutex> lk(g_mu);
-    /* enough for either cache type and any window (a window only takes spans away) */
-    size_t most = 0;
-    for (int half = 0; half < 2; half++)
-        most = std::max(most, attention_rows_scratch(n_rows, n_seqs, n_heads, n_kv_heads, head_dim, kv_max, prefix_len, 0, half));
-    return most;
+    return attention_rows_scratch(n_rows, n_seqs, n_heads, n_kv_heads, head_dim, kv_max, prefix_len);
 }
 
 static void attention_rows(const char *who, const float *q_dev, int q_stride, int kv_type, const void *kv_k_dev,
@@ -1569,12 +1565,6 @@ static void attention_rows(const char *who, const float *q_dev, int q_stride, in
         return;
     }
     ensure_init();
-    const size_t need = attention_rows_scratch(n_rows, n_seqs, n_heads, n_kv_heads, head_dim, kv_max, prefix_len, window,
-                                               kv_type == TG_KV_F16);
-    if (need && (!scratch_dev || ((uintptr_t)scratch_dev & 15))) {
-        set_err("%s: needs %zu bytes of 16-byte aligned scratch", who, need);
-        return;
-    }
     PromptArgs a = {};
     a.q = q_dev, a.q_stride = q_stride;
     a.kv_k = kv_k_dev, a.kv_v = kv_v_dev;
@@ -1583,7 +1573,11 @@ static void attention_rows(const char *who, const float *q_dev, int q_stride, in
     a.window = window, a.sinks = sinks_dev;
     a.n_heads = n_heads, a.n_kv = n_kv_heads, a.head_dim = head_dim;
     a.out = out_dev, a.out_stride = out_stride;
-    launch_attention_rows(a, kv_type == TG_KV_F16, scratch_dev, stream ? (hipStream_t)stream : g.st);
+    const size_t need = launch_attention_rows(a, kv_type == TG_KV_F16, scratch_dev, stream ? (hipStream_t)stream : g.st);
+    if (need) {
+        set_err("%s: needs %zu bytes of 16-byte aligned scratch", who, need);
+        return;
+    }
     check_launch(who);
 }
 

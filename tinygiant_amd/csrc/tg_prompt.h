@@ -55,9 +55,10 @@ struct PromptArgs {
     float *out;
     int out_stride;
 };
-void launch_attention_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st);
-size_t attention_rows_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len,
-                              int window, bool half);
+/* 0, or the scratch bytes that are needed where `scratch` is null or not
+ * 16-byte aligned (nothing is launched then) */
+size_t launch_attention_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st);
+size_t attention_rows_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len);
 
 }  // namespace tg
 #endif

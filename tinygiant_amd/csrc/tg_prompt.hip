@@ -11,6 +11,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "tg_device.hpp"
 #include "tg_prompt.h"
@@ -761,14 +762,20 @@ __device__ inline void merge_groups(float *lds, int wave, int lane, float &mx, f
  * turn.  J blocks of 32 positions are computed together: two overlap their
  * latencies (8192 tokens: 928 us, one at a time 965), one is half the code
  * and skips what a window hides (4,096 tokens, window 128: 46.2, 48.6). */
+template <int HD, int MW, int KG>
+struct SharedH {
+    __attribute__((aligned(1024))) uint8_t bufs[KG][2][2][KT * HD * 2];
+    uint32_t bad_rows[MW];
+    long long where[KG == 2 ? 32 * MW : 1];
+};
 template <int HD, int MW, int KG, int J>
-__global__ __launch_bounds__(64 * MW * KG, HD == 64 && J == 1 ? 4 : 2) void k_rows_h(PromptArgs a, RowsPlan p) {
+__device__ inline __attribute__((always_inline)) void rows_h(const PromptArgs &a, const RowsPlan &p, SharedH<HD, MW, KG> &sh) {
     constexpr int RB = HD * 2, TILE = KT * RB;       /* bytes of a row in LDS, of a tile of K or V */
     constexpr int NC = TILE / 1024 / MW;             /* copies of 1 KiB a wave, matrix and tile */
     constexpr int DB = HD / 32, STEPS = HD / 16;
-    __shared__ __attribute__((aligned(1024))) uint8_t bufs[KG][2][2][TILE];
-    __shared__ uint32_t bad_rows[MW];
-    __shared__ long long where[KG == 2 ? 32 * MW : 1];
+    auto &bufs = sh.bufs;
+    auto &bad_rows = sh.bad_rows;
+    auto &where = sh.where;
     const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
     Work w;
     if (!find_work<32 * MW>(a, p, ratio, w)) return;
@@ -927,6 +934,12 @@ __global__ __launch_bounds__(64 * MW * KG, HD == 64 && J == 1 ? 4 : 2) void k_ro
             slow_row<_Float16>(a, p, w, 32 * wv + __builtin_ctz(y), ratio, (float *)bufs);
 }
 
+template <int HD, int MW, int KG, int J>
+__global__ __launch_bounds__(64 * MW * KG, HD == 64 && J == 1 ? 4 : 2) void k_rows_h(PromptArgs a, RowsPlan p) {
+    __shared__ SharedH<HD, MW, KG> sh;
+    rows_h<HD, MW, KG, J>(a, p, sh);
+}
+
 /* ---- float32 caches on the f16 matrix units ----
  *
  * The same products with K and V split as q and the weights are: x 2^k = hi +
@@ -963,16 +976,23 @@ __device__ inline bool every_row(uint64_t m, uint64_t any) {
 }
 
 template <int HD, int MW, int KG>
-__global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPlan p) {
+struct SharedF {
+    __attribute__((aligned(1024))) uint8_t bufs[KG][2][4][KF * HD * 2];
+    int exps[KG][2][8];
+    int range[MW * KG][2];   /* each wave's least and most */
+    uint32_t bad_rows[MW];
+    long long where[KG == 2 ? 32 * MW : 1];
+};
+template <int HD, int MW, int KG>
+__device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a, const RowsPlan &p, SharedF<HD, MW, KG> &sh) {
     constexpr int RB = HD * 2, PLANE = KF * RB;
     constexpr int UNITS = 8 / MW;                    /* groups a wave loads: K 0 .. 3, V 4 .. 7 */
     constexpr int LR = 256 / HD, NL = 8 / LR;        /* rows a load of the wave covers, loads a group */
     constexpr int DB = HD / 32, STEPS = HD / 16;
-    __shared__ __attribute__((aligned(1024))) uint8_t bufs[KG][2][4][PLANE];
-    __shared__ int all_exps[KG][2][8];
-    __shared__ int range[MW * KG][2];   /* each wave's least and most */
-    __shared__ uint32_t bad_rows[MW];
-    __shared__ long long where[KG == 2 ? 32 * MW : 1];
+    auto &bufs = sh.bufs;
+    auto &range = sh.range;
+    auto &bad_rows = sh.bad_rows;
+    auto &where = sh.where;
     const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
     Work w;
     if (!find_work<32 * MW>(a, p, ratio, w)) return;
@@ -980,7 +1000,7 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPl
     const int half = lane >> 5, group = wave / MW, mwave = wave % MW;
     static_assert(KG == 1 || sizeof bufs >= MW * 256 * (HD / 2 + 3), "merge_groups");
     uint8_t(*buf)[4][PLANE] = bufs[group];
-    int(*exps)[8] = all_exps[group];
+    int(*exps)[8] = sh.exps[group];
 
     /* loads: lane l of load j of group g holds dims 4 (l % (HD / 4)) .. of position 8 g + LR j + l / (HD / 4) */
     const uint32_t rb = (uint32_t)hd * 4u;
@@ -1112,18 +1132,15 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPl
 #pragma unroll
             for (int v = 0; v < 16; v++) s[v] = 0.f;
             h8 kh = lds_row(tile + kaddr), kl = lds_row(tile + kaddr + PLANE);
-            f16v z = s;   /* two chains */
 #pragma unroll
             for (int st = 0; st < STEPS; st++) {   /* the next step's operands are read a step ahead */
                 const Lds at = tile + (kaddr ^ (uint32_t)((st + 1) << 5));
                 const h8 nh = st + 1 < STEPS ? lds_row(at) : kh, nl = st + 1 < STEPS ? lds_row(at + PLANE) : kl;
-                z = MFMA_H(kl, qh[st], z);
+                s = MFMA_H(kl, qh[st], s);
+                s = MFMA_H(kh, ql[st], s);
                 s = MFMA_H(kh, qh[st], s);
-                z = MFMA_H(kh, ql[st], z);
                 kh = nh, kl = nl;
             }
-#pragma unroll
-            for (int v = 0; v < 16; v++) s[v] += z[v];
             auto column = [&](int i, int lo) __attribute__((always_inline)) {
                 const int q = i / DB, d = i % DB, at = q * 16 * RB + lo * PLANE;
                 return h8_of(lds_column(tile + vaddr[d][0] + at), lds_column(tile + vaddr[d][1] + at));
@@ -1204,6 +1221,12 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPl
     for (int wv = 0; wv < MW; wv++)
         for (uint32_t y = bad_rows[wv]; y; y &= y - 1)
             slow_row<float>(a, p, w, 32 * wv + __builtin_ctz(y), ratio, (float *)bufs);
+}
+
+template <int HD, int MW, int KG>
+__global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPlan p) {
+    __shared__ SharedF<HD, MW, KG> sh;
+    rows_f<HD, MW, KG>(a, p, sh);
 }
 
 /* ---- few rows: positions over the waves ----
@@ -1324,12 +1347,19 @@ struct NarrowV<_Float16, HD> {
     __device__ inline float at(int t) const { return (float)v[t]; }
 };
 
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
+template <int HD, int NW>
+struct SharedN {
+    __attribute__((aligned(16))) float mo[NW][MN][HD];
+    float mm[NW][MN], ml[NW][MN];
+    uint32_t bad_rows;
+};
+template <typename T, int HD, int NW>
+__device__ inline __attribute__((always_inline)) void rows_n(const PromptArgs &a, const RowsPlan &p, SharedN<HD, NW> &sh) {
     constexpr int N = HD / 16;
-    __shared__ __attribute__((aligned(16))) float mo[4][MN][HD];
-    __shared__ float mm[4][MN], ml[4][MN];
-    __shared__ uint32_t bad_rows;
+    auto &mo = sh.mo;
+    auto &mm = sh.mm;
+    auto &ml = sh.ml;
+    auto &bad_rows = sh.bad_rows;
     const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
     Work w;
     if (!find_work<MN>(a, p, ratio, w)) return;
@@ -1355,9 +1385,9 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
     v4f o[N];
 #pragma unroll
     for (int n = 0; n < N; n++) o[n] = v4f{0.f, 0.f, 0.f, 0.f};
-    for (; t < w.hi; t += 64) {
+    for (; t < w.hi; t += 16 * NW) {
         v4f s = K.scores();
-        K.load_k(kd, (uint32_t)(t + 64 + c16) * rb, kq, hd);
+        K.load_k(kd, (uint32_t)(t + 16 * NW + c16) * rb, kq, hd);
         const bool masked = t + 15 > x.all_hi || t < x.all_lo;   /* uniform */
         float top = -INFINITY;
 #pragma unroll
@@ -1385,7 +1415,7 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int n = 0; n < N; n++) o[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(V[i].at(n), s[i], o[n], 0, 0, 0);
-        load_v(t + 64);
+        load_v(t + 16 * NW);
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -1398,16 +1428,19 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
         }
     if (kq == 0) mm[wave][c16] = mx, ml[wave][c16] = l;
     __syncthreads();
-    /* the four waves' sums as one, in wave order: 16 threads a row, HD / 16 dims each */
-    const int row = tid >> 4, d0 = (tid & 15) * N;
+    /* the waves' sums as one, in wave order: 16 threads a row, HD / 16 dims each */
+    const bool on = tid < 16 * MN;
+    const int row = (tid >> 4) & (MN - 1), d0 = (tid & 15) * N;
     const Lane y = lane_rows(a, w, 0, row, 16, ratio);
-    float M = fmaxf(fmaxf(mm[0][row], mm[1][row]), fmaxf(mm[2][row], mm[3][row]));
+    float M = mm[0][row];
+#pragma unroll
+    for (int q = 1; q < NW; q++) M = fmaxf(M, mm[q][row]);
     const float base = M == -INFINITY ? 0.f : M;
     float L = 0.f, r[N];
 #pragma unroll
     for (int n = 0; n < N; n++) r[n] = 0.f;
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
+    for (int q = 0; q < NW; q++) {
         const float e = __builtin_amdgcn_exp2f(mm[q][row] - base);
         L = fmaf(ml[q][row], e, L);
 #pragma unroll
@@ -1416,10 +1449,10 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
     float nan = L * 0.f;
 #pragma unroll
     for (int n = 0; n < N; n++) nan = fmaf(r[n], 0.f, nan);
-    if (y.live && !(nan == 0.f)) atomicOr(&bad_rows, 1u << row);
+    if (on && y.live && !(nan == 0.f)) atomicOr(&bad_rows, 1u << row);
     __syncthreads();
     const uint32_t bad = bad_rows;
-    if (y.live && !((bad >> row) & 1u) && d0 < hd) {
+    if (on && y.live && !((bad >> row) & 1u) && d0 < hd) {
         float *dst, f = 1.f;
         if (p.nrec) {
             const size_t rec = ((size_t)y.r * a.n_heads + y.h) * p.nrec + w.rec;
@@ -1440,6 +1473,12 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
         }
     }
     for (uint32_t z = bad; z; z &= z - 1) slow_row<T>(a, p, w, __builtin_ctz(z), ratio, &mo[0][0][0]);
+}
+
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
+    __shared__ SharedN<HD, 4> sh;
+    rows_n<T, HD, 4>(a, p, sh);
 }
 
 /* The records of a row and head, and its sink, as one: W waves each, wave g
@@ -1554,17 +1593,15 @@ static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim,
      * where it is not there anyway).  A workgroup takes 3.4 us for 128
      * positions of 128-value heads (WIDE; half of that for 64), 1.2 us for 64
      * on the narrow kernel, the copies stream at 4.5 TB/s. */
+    auto slots = [](Shape s) { return s == NARROW ? 512 : 256; };   /* workgroups at once */
     auto spans = [&](Shape s, long long wgs, int positions, bool joined) {
         const double t = positions * (s == NARROW ? 1.2 / 64 : 3.4 / 128) * (head_dim > 64 ? 1 : 0.5);
         const double r = (double)m * n_kv * head_dim * 8 / 4.5e6;
-        const int most = (int)std::min<long long>({64, (positions + 127) / 128, std::max(1ll, (s == NARROW ? 512 : 256) / wgs)});
-        int best = 1;
-        double least = t + (joined ? r : 0);
-        for (int n = 2; n <= most; n++) {
-            const double us = t / n + r * n + (joined ? 0 : 4);
-            if (us < least) least = us, best = n;
-        }
-        return best;
+        const int most = (int)std::min<long long>({64, (positions + 127) / 128, std::max(1ll, slots(s) / wgs)});
+        auto us = [&](int n) { return t / n + r * n + (joined || n == 1 ? 0 : 4) - (joined || n > 1 ? 0 : r); };
+        const int n = std::max(1, std::min(most, (int)std::sqrt(t / r)));   /* the best, or the next */
+        const int best = n < most && us(n + 1) < us(n) ? n + 1 : n;
+        return us(best) < us(1) ? best : 1;
     };
     auto tiles = [&](Shape s, long long seqs) { return std::max((m + SHAPE_ROWS[s] - 1) / SHAPE_ROWS[s], seqs); };
     auto sees = [&](int rows) { return window > 0 ? (int)std::min<long long>(kv_max, (long long)window + rows / ratio + 1) : kv_max; };
@@ -1572,7 +1609,7 @@ static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim,
     const int own_sees = sees(SHAPE_ROWS[k.own]);
     const long long own_tiles = tiles(k.own, n_seqs);
     p.cap = spans(k.own, own_tiles * n_kv, own_sees, pre_len > 0);
-    p.target = std::max(1, (k.own == NARROW ? 512 : 256) / n_kv);
+    p.target = std::max(1, slots(k.own) / n_kv);
     if (n_seqs > 1 && p.cap > 1)   /* room for a sequence much longer than the others */
         p.cap = (int)std::min<long long>({64, (own_sees + 127) / 128, std::max<long long>(4ll * p.cap, 4ll * p.target / own_tiles)});
     p.items = (int)std::min(m / SHAPE_ROWS[k.own] + n_seqs, m) + (p.cap > 1 ? p.target : 0);
@@ -1590,10 +1627,18 @@ static size_t ml_bytes(const RowsPlan &p, int n_rows, int n_heads) {
     return ((size_t)n_rows * n_heads * p.nrec * 16 + 255) & ~(size_t)255;
 }
 
-size_t attention_rows_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len,
-                              int window, bool half) {
-    const RowsPlan p = rows_cut(n_rows, n_seqs, n_heads, n_kv, head_dim, kv_max, pre_len, window, half).p;
+static size_t scratch_bytes(const RowsPlan &p, int n_rows, int n_heads, int head_dim) {
     return p.nrec ? ml_bytes(p, n_rows, n_heads) + (size_t)n_rows * n_heads * p.nrec * head_dim * 4 : 0;
+}
+
+/* For either cache type and any window: a window only takes spans away (the
+ * best count rises with the positions, and so do its bounds). */
+size_t attention_rows_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len) {
+    size_t most = 0;
+    for (int half = 0; half < 2; half++)
+        most = std::max(most, scratch_bytes(rows_cut(n_rows, n_seqs, n_heads, n_kv, head_dim, kv_max, pre_len, 0, half).p, n_rows,
+                                            n_heads, head_dim));
+    return most;
 }
 
 /* the workgroups of one part, or of both */
@@ -1617,9 +1662,8 @@ static void launch_part(const PromptArgs &a, const RowsPlan &p, bool half, Shape
 }
 
 template <int HD>
-static void launch_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st) {
-    Cut k = rows_cut(a.s.rows, a.s.n, a.n_heads, a.n_kv, a.head_dim, a.s.kv_max, a.pre_len, a.window, half);
-    RowsPlan &p = k.p;
+static void launch_rows(const PromptArgs &a, const Cut &k, bool half, void *scratch, hipStream_t st) {
+    RowsPlan p = k.p;
     p.ml = (float *)scratch;
     p.o = (float *)((uint8_t *)scratch + ml_bytes(p, a.s.rows, a.n_heads));
     if (p.pre_tiles && k.own != k.pre) {
@@ -1638,9 +1682,13 @@ static void launch_rows(const PromptArgs &a, bool half, void *scratch, hipStream
     else hipLaunchKernelGGL((k_rows_combine<1, HD / 4>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, p);
 }
 
-void launch_attention_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st) {
-    if (a.head_dim > 64) launch_rows<128>(a, half, scratch, st);
-    else launch_rows<64>(a, half, scratch, st);
+size_t launch_attention_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st) {
+    const Cut k = rows_cut(a.s.rows, a.s.n, a.n_heads, a.n_kv, a.head_dim, a.s.kv_max, a.pre_len, a.window, half);
+    const size_t need = scratch_bytes(k.p, a.s.rows, a.n_heads, a.head_dim);
+    if (need && (!scratch || ((uintptr_t)scratch & 15))) return need;
+    if (a.head_dim > 64) launch_rows<128>(a, k, half, scratch, st);
+    else launch_rows<64>(a, k, half, scratch, st);
+    return 0;
 }
 
 }  // namespace tg
