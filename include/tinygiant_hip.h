@@ -263,7 +263,8 @@ size_t tg_hip_attention_scratch_bytes(int embed_dim, int n_heads, int n_kv_heads
  *             rows: row i is at position kv_len[s] + i.
  *   shapes    head_dim a multiple of 8 and <= 128, n_heads <= 1024,
  *             n_heads / n_kv_heads integral and <= 64, kv_max <= 2^20,
- *             n_rows <= 2^22, n_seqs <= 2^16
+ *             n_rows <= 2^22, n_seqs <= 2^16, n_rows * n_heads <= 2^25,
+ *             n_seqs * n_kv_heads <= 2^20
  *   strides   in floats from row to row, of at least a row's heads and at most
  *             2^21
  * cu_rows, kv_len and slots are device arrays that the host does not see: a

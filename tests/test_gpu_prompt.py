@@ -304,6 +304,85 @@ def test_same_bits_every_time(tg, half):
         dev.free()
 
 
+@pytest.mark.parametrize("half", [False, True])
+def test_spans_that_end_behind_a_multiple(tg, half):
+    """Sequences that see one position more than a whole number of spans, of
+    one KV head, so that the call has its most spans; the records are NaN
+    before it."""
+    for spans in ([58, 58] + [57] * 7, [33] * 16, [64, 2] * 8):
+        say(f"spans {spans[:3]} half={half}")
+        b = Batch(50, 1, 1, 64, [1] * len(spans), [128 * x for x in spans], half)
+        dev = Dev(tg)
+        need = tg.lib().tg_hip_attention_prompt_scratch_bytes(b.rows, b.n, 1, 1, 64, b.kv_max, 0)
+        out, was = b.call(dev, scratch=dev(np.full(need // 4, np.nan, np.float32)))
+        tg.lib().tg_hip_synchronize()
+        got = dev.read(out, b.q)
+        dev.free()
+        b.check(got, was)
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_nan_queries(tg, half):
+    """A NaN in q makes its own row and head NaN, whether or not its positions
+    are split and with sinks too; the others stay."""
+    for lens, past, prefix in (([3], [2000], 0), ([2, 1], [5, 0], 900), ([300], [0], 0)):
+        say(f"nan in q half={half} past={past} prefix={prefix}")
+        b = Batch(60, 8, 2, 64, lens, past, half, prefix=prefix, sinks=True)
+        ref, tol = b.attend()
+        b.q[1, 3 * 64 + 5] = np.nan
+        got, _ = _run(tg, b)
+        hit = np.zeros(got.shape, bool)
+        hit[1, 3 * 64:4 * 64] = True
+        assert np.all(np.isnan(got[hit]))
+        assert np.all(np.abs(got - ref)[~hit] <= tol[~hit])
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_infinite_value_of_a_vanishing_weight(tg, half):
+    """An infinity in V stays one, or becomes NaN where its weight underflows,
+    however the positions are split."""
+    say(f"infinite V of a vanishing weight half={half}")
+    b = Batch(61, 8, 2, 64, [2], [3000], half, q_scale=300.0)
+    b.v[b.slots[0], :, ::256, 7] = np.inf
+    got, _ = _run(tg, b)
+    assert not np.isfinite(got.reshape(2, 8, 64)[:, :, 7]).any()
+    assert np.isfinite(got.reshape(2, 8, 64)[:, :, 8]).all()
+
+
+def test_scratch_is_enough_for_every_call(tg):
+    """What a call says it needs, with any window and cache type, is at most
+    what the size function answers.  The calls have no rows on the device."""
+    say("scratch sizes")
+    lib, dev, rng = tg.lib(), Dev(tg), np.random.default_rng(5)
+    p, cu, seen = dev(np.zeros(1 << 16, np.float32)), dev(np.zeros(1 << 14, np.int32)), 0
+    for _ in range(4000):
+        nkv = int(rng.choice([1, 2, 3, 4, 8, 16]))
+        nh = nkv * int(rng.choice([1, 2, 4, 5, 8, 16]))
+        hd = int(rng.choice([8, 64, 80, 128]))
+        kv_max = int(2 ** rng.uniform(0, 18))
+        n_rows = int(2 ** rng.uniform(0, 12))
+        n_seqs = min(int(2 ** rng.uniform(0, 9)), 2 * n_rows)
+        prefix = int(rng.choice([0, 0, 1])) * int(2 ** rng.uniform(0, 15))
+        window = int(rng.choice([0, 1, 1])) * int(2 ** rng.uniform(0, 18))
+        half = int(rng.integers(2))
+        size = lib.tg_hip_attention_prompt_scratch_bytes(n_rows, n_seqs, nh, nkv, hd, kv_max, prefix)
+        lib.tg_hip_clear_error()
+        front = (p, nh * hd, half, p, p, 1, kv_max)
+        back = (cu, cu, None, n_seqs, n_rows, window, None, nh, nkv, hd, p, nh * hd, None, None)
+        if prefix:
+            lib.tg_hip_attention_prefix_dev(*front, p, p, prefix, prefix, *back)
+        else:
+            lib.tg_hip_attention_prompt_dev(*front, *back)
+        e = tg.last_error()
+        need = int(e.split("needs ")[1].split()[0]) if e else 0
+        assert need <= size, (need, size, n_rows, n_seqs, nh, nkv, hd, kv_max, prefix, window, half)
+        seen += need > 0
+    lib.tg_hip_synchronize()
+    lib.tg_hip_clear_error()
+    dev.free()
+    assert seen > 1000
+
+
 # ---- append ----
 
 def _rope_tables(n, hd):

@@ -41,6 +41,7 @@ def _logits(**kw):
     (dict(v=P + 4), "16-byte"), (dict(window=-1), "window"), (dict(q_stride=511), "stride"), (dict(out_stride=100), "stride"), (dict(q_stride=(1 << 21) + 1), "stride"),
     (dict(q=None), "q or out"), (dict(out=None), "q or out"), (dict(q=P + 2), "q or out"),
     (dict(out=P, out_stride=600), "same stride"), (dict(plen=21), "prefix_len"), (dict(plen=-1), "prefix_len"),
+    (dict(n_rows=1 << 22, nh=64, nkv=8, q_stride=4096, out_stride=4096), "too many"), (dict(n_seqs=1 << 16, nkv=32, nh=32), "too many"),
     (dict(pk=None), "prefix_k"), (dict(pv=P + 8), "prefix_k"), (dict(pmax=1 << 21), "prefix_len")])
 def test_attention_refuses(tg, kw, word):
     lib = tg.lib()
@@ -69,7 +70,8 @@ def test_append_refuses(tg, kw, word):
     (dict(hist_stride=-1), "strides"), (dict(bstride=-1), "strides"), (dict(logits=None), "null logits"),
     (dict(out=None, arg=None, top=None), "no output"), (dict(scratch=None), "scratch"), (dict(scratch=P + 4), "scratch"),
     (dict(hist_len=None), "history"), (dict(pen=None), "history"), (dict(bval=None), "bias"), (dict(btok=None), "bias"),
-    (dict(allow_stride=3), "allow_stride"), (dict(allow_stride=-4), "allow_stride")])
+    (dict(allow_stride=3), "allow_stride"), (dict(allow_stride=-4), "allow_stride"),
+    (dict(logits=P + 2), "4-byte"), (dict(out=P + 1), "4-byte"), (dict(hist=P + 2), "4-byte")])
 def test_logits_refuses(tg, kw, word):
     lib = tg.lib()
     lib.tg_hip_clear_error()
@@ -95,7 +97,8 @@ def test_scratch_sizes(tg):
     assert lib.tg_hip_logits_scratch_bytes(0, 5) == 0 and lib.tg_hip_logits_scratch_bytes(5, 0) == 0
     assert lib.tg_hip_logits_scratch_bytes(1, 1) >= 8
     for bad in ((0, 1, 8, 2, 64, 64, 0), (1, 0, 8, 2, 64, 64, 0), (1, 1, 9, 2, 64, 64, 0), (1, 1, 8, 2, 64, 0, 0),
-                (1, 1, 8, 2, 200, 64, 0), (1, 1, 8, 2, 64, 64, -1)):
+                (1, 1, 8, 2, 200, 64, 0), (1, 1, 8, 2, 64, 64, -1), (1 << 23, 1, 8, 2, 64, 64, 0),
+                (1, 1 << 17, 8, 2, 64, 64, 0), (1, 1, 2048, 1024, 64, 64, 0), (1, 1, 8, 2, 64, 1 << 21, 0)):
         assert lib.tg_hip_attention_prompt_scratch_bytes(*bad) == 0
 
 

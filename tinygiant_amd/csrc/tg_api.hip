@@ -1454,6 +1454,11 @@ static bool packed_validate(const char *who, const int32_t *cu_rows, int n_seqs,
                 "<= %d)", who, PROMPT_MAX_HEAD_DIM, PROMPT_MAX_GQA);
         return false;
     }
+    if ((long long)n_rows * n_heads > PROMPT_MAX_ROW_HEADS || (long long)n_seqs * n_kv > PROMPT_MAX_SEQ_HEADS) {
+        set_err("%s: too many rows or sequences for one call (n_rows * n_heads <= %d, n_seqs * n_kv_heads <= %d)", who,
+                PROMPT_MAX_ROW_HEADS, PROMPT_MAX_SEQ_HEADS);
+        return false;
+    }
     if (n_seqs && n_rows && (!cu_rows || !kv_k || !kv_v)) {
         set_err("%s: null cu_rows or cache pointer", who);
         return false;
@@ -1465,10 +1470,11 @@ static bool packed_validate(const char *who, const int32_t *cu_rows, int n_seqs,
     return true;
 }
 
-/* a launch that HIP refuses is reported, the outputs are as they were */
-static void check_launch(const char *who) {
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) set_err("%s: launch failed (%s)", who, hipGetErrorString(e));
+/* A launch that HIP refuses is reported; an error that was there before
+ * (`before`, hipPeekAtLastError's) is its caller's and stays. */
+static void check_launch(const char *who, hipError_t before) {
+    if (before != hipSuccess || hipPeekAtLastError() == hipSuccess) return;
+    set_err("%s: launch failed (%s)", who, hipGetErrorString(hipGetLastError()));
 }
 
 static PackedSeqs packed_seqs(const int32_t *cu_rows, const int32_t *kv_len, const int32_t *slots, int n_seqs, int n_rows,
@@ -1521,14 +1527,16 @@ TG_API void tg_hip_kv_append_dev(const float *q_dev, const float *k_dev, const f
     a.kv_k = kv_k_dev, a.kv_v = kv_v_dev;
     a.n_heads = n_heads, a.n_kv = n_kv_heads, a.head_dim = head_dim;
     a.q_out = q_out_dev, a.q_out_stride = q_out_stride;
+    const hipError_t before = hipPeekAtLastError();
     launch_kv_append(a, kv_type == TG_KV_F16, stream ? (hipStream_t)stream : g.st);
-    check_launch(who);
+    check_launch(who, before);
 }
 
 TG_API size_t tg_hip_attention_prompt_scratch_bytes(int n_rows, int n_seqs, int n_heads, int n_kv_heads, int head_dim,
                                                     int kv_max, int prefix_len) {
     if (n_rows <= 0 || n_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || head_dim <= 0 ||
-        head_dim > PROMPT_MAX_HEAD_DIM || kv_max <= 0 || prefix_len < 0)
+        head_dim > PROMPT_MAX_HEAD_DIM || kv_max <= 0 || prefix_len < 0 || n_rows > PROMPT_MAX_ROWS ||
+        n_seqs > PROMPT_MAX_SEQS || n_heads > 1024 || kv_max > PROMPT_MAX_KV || prefix_len > PROMPT_MAX_KV)
         return 0;
     std::lock_guard<std::recursive_mutex> lk(g_mu);
     return attention_rows_scratch(n_rows, n_seqs, n_heads, n_kv_heads, head_dim, kv_max, prefix_len);
@@ -1573,12 +1581,13 @@ static void attention_rows(const char *who, const float *q_dev, int q_stride, in
     a.window = window, a.sinks = sinks_dev;
     a.n_heads = n_heads, a.n_kv = n_kv_heads, a.head_dim = head_dim;
     a.out = out_dev, a.out_stride = out_stride;
+    const hipError_t before = hipPeekAtLastError();
     const size_t need = launch_attention_rows(a, kv_type == TG_KV_F16, scratch_dev, stream ? (hipStream_t)stream : g.st);
     if (need) {
         set_err("%s: needs %zu bytes of 16-byte aligned scratch", who, need);
         return;
     }
-    check_launch(who);
+    check_launch(who, before);
 }
 
 TG_API void tg_hip_attention_prompt_dev(const float *q_dev, int q_stride, int kv_type, const void *kv_k_dev,
@@ -1628,6 +1637,10 @@ TG_API void tg_hip_logits_adjust_dev(const float *logits_dev, float *out_dev, in
         set_err("%s: null logits, no output, or no 8-byte aligned scratch for the argmax", who);
         return;
     }
+    if (((uintptr_t)logits_dev | (uintptr_t)out_dev | (uintptr_t)hist_dev) & 3) {
+        set_err("%s: rows must be 4-byte aligned", who);
+        return;
+    }
     if (hist_dev && (!hist_len_dev || !penalties_dev)) {
         set_err("%s: a history needs hist_len and penalties", who);
         return;
@@ -1644,8 +1657,9 @@ TG_API void tg_hip_logits_adjust_dev(const float *logits_dev, float *out_dev, in
     const LogitsArgs a = {logits_dev, out_dev, k, nrows, hist_dev, hist_stride, hist_len_dev, gen_start_dev, penalties_dev,
                           bias_tok_dev, bias_val_dev, bias_stride, bias_len_dev, allow_dev, allow_stride, argmax_dev,
                           maxval_dev};
+    const hipError_t before = hipPeekAtLastError();
     launch_logits_adjust(a, scratch_dev, stream ? (hipStream_t)stream : g.st);
-    check_launch(who);
+    check_launch(who, before);
 }
 
 /* ---- file -> HBM upload (the expert-cache loader's native part) ----

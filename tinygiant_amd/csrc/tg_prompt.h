@@ -14,6 +14,10 @@
 #define PROMPT_MAX_ROWS (1 << 22)
 #define PROMPT_MAX_STRIDE (1 << 21)   /* floats from row to row: a tile's rows within 2^31 bytes */
 #define PROMPT_MAX_SEQS (1 << 16)
+/* What a grid holds: 2^32 work-items, of which a row and head take 64 in the
+ * combine, a sequence and KV head 256 (one tile of its own). */
+#define PROMPT_MAX_ROW_HEADS (1 << 25)
+#define PROMPT_MAX_SEQ_HEADS (1 << 20)
 
 namespace tg {
 

@@ -256,7 +256,8 @@ __device__ inline bool find_item(const PromptArgs &a, const RowsPlan &p, int rat
             if (s0) load(s0);
             sum += wave_sum((float)tiles() * (float)sees());
         }
-        per = div_up(max(1, (int)fminf(sum / (float)p.target, 1e9f)), p.unit) * p.unit;
+        /* rounded up: a shorter span would make more of them than p.items has room for */
+        per = div_up(max(1, (int)fminf(ceilf(sum / (float)p.target), 1e9f)), p.unit) * p.unit;
         if (c.n > 64) load(0);
     }
     for (int s0 = 0; s0 < c.n; s0 += 64) {
@@ -417,7 +418,8 @@ __device__ void slow_row(const PromptArgs &a, const RowsPlan &p, const Work &w, 
     }
     if (p.nrec) {
         const size_t rec = ((size_t)r * a.n_heads + h) * p.nrec + w.rec;
-        if (tid == 0) write_ml(p, w, rec, mx, l);
+        /* scores that are all NaN leave mx at -inf, which is the record of no position */
+        if (tid == 0) write_ml(p, w, rec, l != l ? l : mx, l);
         if (tid < hd) p.o[rec * hd + tid] = o;
     } else if (tid < hd) {
         if (a.sinks) {
@@ -1525,8 +1527,9 @@ __global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) 
     for (int c0 = 0; c0 < nrec; c0 += 64 * W) {
         const int c = c0 + W * lane + wave;
         if (c0 && c < p.nrec) stat = *(const f4 *)(ml + 4 * c);
-        const float e = c < nrec && stat[0] != -INFINITY ? exp2f(stat[0] - base) : 0.f;
-        l += e == 0.f ? 0.f : stat[1] * e;
+        /* -1: a record of no position, whose sums are not written */
+        const float e = c < nrec && stat[0] != -INFINITY ? exp2f(stat[0] - base) : -1.f;
+        l += e < 0.f ? 0.f : stat[1] * e;
         const int n = min(64, (nrec - c0 - wave + W - 1) / W);
         for (int j0 = 0; j0 < n; j0 += N * PER) {
             if (c0 + j0) load(c0, j0);
@@ -1534,7 +1537,7 @@ __global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) 
             for (int q = 0; q < N; q++) {
                 const int j = j0 + q * PER + g;
                 const float f = __shfl(e, j & 63, 64);
-                if (j < n && f != 0.f) o += y[q] * f;   /* a record of no position has no sums */
+                if (j < n && !(f < 0.f)) o += y[q] * f;
             }
         }
     }
@@ -1576,20 +1579,23 @@ struct Cut {
     RowsPlan p;
     Shape own, pre;
 };
+/* The shape for m m-rows (a KV head) in `seqs` sequences that see `positions`.
+ * 9 rows of 8 heads on narrow and wide: 13.6 and 19.6 us behind 1,000
+ * positions (f32; f16 13.2 and 16.1), 29.0 and 26.6 behind 8,000. */
+constexpr long long NARROW_WORK = 1 << 18, TALL_WORK = 512 * 4096;
+constexpr int SHORT_BELOW = 512;
+static Shape shape_of(long long m, long long seqs, int n_kv, int positions, bool half) {
+    if (m <= 16 * seqs || (m <= 128 * seqs && m * positions <= NARROW_WORK)) return NARROW;
+    if (positions < SHORT_BELOW) return SHORT;
+    if (!half && m / 256 * n_kv * positions >= TALL_WORK) return TALL;
+    return m / 128 * n_kv > 512 ? FULL : WIDE;
+}
 static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len, int window,
-                    bool half) {
+                    bool half, const Shape *own) {
     Cut k = {};
     RowsPlan &p = k.p;
     const int ratio = n_heads / n_kv;
     const long long m = (long long)n_rows * ratio;
-    auto shape = [&](long long seqs, int positions) {
-        /* 9 rows of 8 heads on narrow and wide: 13.6 and 19.6 us behind 1,000
-         * positions (f32; f16 13.2 and 16.1), 29.0 and 26.6 behind 8,000 */
-        if (m <= 16 * seqs || (m <= 128 * seqs && m * positions <= 1 << 18)) return NARROW;
-        if (positions < 512) return SHORT;
-        if (!half && m / 256 * n_kv * positions >= 512ll * 4096) return TALL;
-        return m / 128 * n_kv > 512 ? FULL : WIDE;
-    };
     /* Spans of a tile at `positions`: us(n) = time of a span + what the
      * records of n spans take to write and read (+ the combine's launch,
      * where it is not there anyway).  A workgroup takes 3.4 us for 128
@@ -1607,7 +1613,7 @@ static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim,
     };
     auto tiles = [&](Shape s, long long seqs) { return std::max((m + SHAPE_ROWS[s] - 1) / SHAPE_ROWS[s], seqs); };
     auto sees = [&](int rows) { return window > 0 ? (int)std::min<long long>(kv_max, (long long)window + rows / ratio + 1) : kv_max; };
-    k.own = shape(n_seqs, sees(128));
+    k.own = own ? *own : shape_of(m, n_seqs, n_kv, sees(128), half);
     const int own_sees = sees(SHAPE_ROWS[k.own]);
     const long long own_tiles = tiles(k.own, n_seqs);
     p.cap = spans(k.own, own_tiles * n_kv, own_sees, pre_len > 0);
@@ -1617,7 +1623,7 @@ static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim,
     p.items = (int)std::min(m / SHAPE_ROWS[k.own] + n_seqs, m) + (p.cap > 1 ? p.target : 0);
     p.unit = 128;
     if (pre_len) {
-        k.pre = shape(1, pre_len);
+        k.pre = shape_of(m, 1, n_kv, pre_len, half);
         p.pre_tiles = (int)tiles(k.pre, 1);
         p.pre_ns = spans(k.pre, (long long)p.pre_tiles * n_kv, pre_len, true);
     }
@@ -1633,13 +1639,20 @@ static size_t scratch_bytes(const RowsPlan &p, int n_rows, int n_heads, int head
     return p.nrec ? ml_bytes(p, n_rows, n_heads) + (size_t)n_rows * n_heads * p.nrec * head_dim * 4 : 0;
 }
 
-/* For either cache type and any window: a window only takes spans away (the
- * best count rises with the positions, and so do its bounds). */
+/* For either cache type and any window: with one shape, a window only takes
+ * spans away (the best count rises with the positions, and so do its bounds);
+ * so the most over the shapes that some window leads to. */
 size_t attention_rows_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len) {
+    const long long m = (long long)n_rows * (n_heads / n_kv), tall = m / 256 * n_kv;
+    /* the largest number of positions for each */
+    const long long ends[] = {kv_max, NARROW_WORK / m, SHORT_BELOW - 1, tall ? (TALL_WORK - 1) / tall : kv_max};
     size_t most = 0;
     for (int half = 0; half < 2; half++)
-        most = std::max(most, scratch_bytes(rows_cut(n_rows, n_seqs, n_heads, n_kv, head_dim, kv_max, pre_len, 0, half).p, n_rows,
-                                            n_heads, head_dim));
+        for (const long long e : ends) {
+            const Shape s = shape_of(m, n_seqs, n_kv, (int)std::min<long long>(e, kv_max), half);
+            const Cut k = rows_cut(n_rows, n_seqs, n_heads, n_kv, head_dim, kv_max, pre_len, 0, half, &s);
+            most = std::max(most, scratch_bytes(k.p, n_rows, n_heads, head_dim));
+        }
     return most;
 }
 
@@ -1685,7 +1698,8 @@ static void launch_rows(const PromptArgs &a, const Cut &k, bool half, void *scra
 }
 
 size_t launch_attention_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st) {
-    const Cut k = rows_cut(a.s.rows, a.s.n, a.n_heads, a.n_kv, a.head_dim, a.s.kv_max, a.pre_len, a.window, half);
+    const Cut k = rows_cut(a.s.rows, a.s.n, a.n_heads, a.n_kv, a.head_dim, a.s.kv_max, a.pre_len, a.window, half,
+                           nullptr);
     const size_t need = scratch_bytes(k.p, a.s.rows, a.n_heads, a.head_dim);
     if (need && (!scratch || ((uintptr_t)scratch & 15))) return need;
     if (a.head_dim > 64) launch_rows<128>(a, k, half, scratch, st);
