@@ -383,6 +383,83 @@ def test_scratch_is_enough_for_every_call(tg):
     assert seen > 1000
 
 
+def test_calls_on_two_streams(tg):
+    """Calls queued on two streams at once, each with scratch of its own, give
+    the bits that they give alone."""
+    from tests.test_gpu_decode import _hip_runtime
+    say("two streams")
+    lib, hip, dev = tg.lib(), _hip_runtime(), Dev(tg)
+    bs = [Batch(70, 32, 4, 128, [9, 1], [3000, 40], False), Batch(71, 8, 2, 64, [1] * 5, [40] * 5, True, prefix=1500)]
+    alone, streams = [], []
+    for b in bs:
+        out, _ = b.call(dev)
+        lib.tg_hip_synchronize()
+        alone.append(dev.read(out, b.q))
+        streams.append(ctypes.c_void_p())
+        assert hip.hipStreamCreate(ctypes.byref(streams[-1])) == 0
+    for _ in range(20):
+        for b, s in zip(bs, streams):
+            b.queue(lib, s)
+    for b, s, want in zip(bs, streams, alone):
+        assert hip.hipStreamSynchronize(s) == 0
+        assert dev.read(b.ptrs["out"], b.q).tobytes() == want.tobytes()
+    for s in streams:
+        hip.hipStreamDestroy(s)
+    dev.free()
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_offsets_past_32_bits(tg, half):
+    """Slots, rows of q and rows of the output whose byte offsets pass 2^32:
+    the last slot of a cache of 2^20 positions, rows 2^21 floats apart."""
+    say(f"offsets half={half}")
+    lib, dev, rng = tg.lib(), Dev(tg), np.random.default_rng(9)
+    nh, nkv, hd, kv_max, slots, stride, rows, past = 8, 4, 128, 1 << 20, 4, 1 << 21, 600, (1 << 20) - 700
+    dtype = np.float16 if half else np.float32
+    size = np.dtype(dtype).itemsize
+    k = rng.standard_normal((nkv, 700, hd)).astype(dtype)
+    v = rng.standard_normal((nkv, 700, hd)).astype(dtype)
+    q = rng.standard_normal((rows, nh * hd)).astype(np.float32)
+    pk, pv = (dev.room(slots * nkv * kv_max * hd * size) for _ in range(2))
+    pq, po = (dev.room(rows * stride * 4) for _ in range(2))
+    for h in range(nkv):
+        at = (((slots - 1) * nkv + h) * kv_max + past) * hd * size
+        lib.tg_hip_memcpy_h2d(pk + at, k[h].ctypes.data, k[h].nbytes)
+        lib.tg_hip_memcpy_h2d(pv + at, v[h].ctypes.data, v[h].nbytes)
+    for r in range(rows):
+        lib.tg_hip_memcpy_h2d(pq + 4 * r * stride, q[r].ctypes.data, q[r].nbytes)
+    cu, n, slot = (dev(np.array(x, np.int32)) for x in ([0, rows], [past + 50], [slots - 1]))
+    scratch = dev.room(lib.tg_hip_attention_prompt_scratch_bytes(rows, 1, nh, nkv, hd, kv_max, 0))
+    lib.tg_hip_clear_error()
+    for window in (1, 40):   # the slot in front of the last 650 positions holds anything
+        lib.tg_hip_attention_prompt_dev(pq, stride, int(half), pk, pv, slots, kv_max, cu, n, slot, 1, rows, window, None, nh, nkv,
+                                        hd, po, stride, scratch, None)
+        lib.tg_hip_synchronize()
+        assert tg.last_error() == "", tg.last_error()
+        for r in (0, 1, 300, 599):
+            got = dev.read(po + 4 * r * stride, np.empty((nh, hd), np.float32))
+            lo, hi = max(0, 50 + r + 1 - window), 50 + r + 1
+            for h in range(nh):
+                kk, vv = (x[h // 2, lo:hi].astype(np.float64) for x in (k, v))
+                qq = q[r, h * hd:(h + 1) * hd].astype(np.float64)
+                z = kk @ qq * hd ** -0.5
+                p = np.exp(z - z.max())
+                off = (8 * np.sqrt(2 * hd) + 4) * EPS * (np.abs(kk) @ np.abs(qq)).max() * hd ** -0.5 + (8 * np.sqrt(hi - lo) + 24) * EPS
+                assert np.all(np.abs(got[h] - (p @ vv) / p.sum()) <= 2 * off * np.abs(vv).max()), (window, r, h)
+    # and the append's: three rows at the end of the last slot, from rows 2^21 floats apart
+    n2 = dev(np.array([kv_max - 3], np.int32))
+    cu2 = dev(np.array([rows - 3, rows], np.int32))
+    lib.tg_hip_kv_append_dev(None, pq, pq + 4 * nkv * hd, stride, stride, None, None, 1e-6, None, None, 0, cu2, n2, slot, 1, rows,
+                             0, int(half), pk, pv, slots, kv_max, nh, nkv, hd, None, 0, None)
+    lib.tg_hip_synchronize()
+    assert tg.last_error() == "", tg.last_error()
+    for h in range(nkv):
+        at = (((slots - 1) * nkv + h) * kv_max + kv_max - 3) * hd * size
+        for ptr, first in ((pk, h * hd), (pv, (nkv + h) * hd)):
+            assert np.array_equal(dev.read(ptr + at, np.empty((3, hd), dtype)), q[rows - 3:, first:first + hd].astype(dtype))
+    dev.free()
+
+
 # ---- append ----
 
 def _rope_tables(n, hd):
