@@ -181,7 +181,7 @@ struct RowsPlan {
     int items;              /* upper bound of the own-slot tiles' spans, per KV head */
     int cap;                /* spans a tile has at most */
     int target;             /* spans that the positions of all tiles are cut into, about */
-    int unit;               /* a span is a multiple of this */
+    int unit, pre_unit;     /* a span is a multiple of this; the prefix's */
     int pre_tiles, pre_ns;  /* tiles of the prefix, spans of each */
     int nrec;               /* room for a row's records: pre_ns + cap; 0: written directly */
     float *ml, *o;          /* [n_rows * n_heads][nrec][4]: m, l, and in the first own span's the count of those;
@@ -349,7 +349,7 @@ __device__ inline bool find_work(const PromptArgs &a, const RowsPlan &p, int rat
         for (int o = 32; o > 0; o >>= 1) lo = min(lo, __shfl_xor(lo, o, 64));
         lo = min(__builtin_amdgcn_readfirstlane(lo), hi);
     }
-    const int per = max(1, div_up(div_up(hi - lo, p.pre_ns), p.unit)) * p.unit;
+    const int per = max(1, div_up(div_up(hi - lo, p.pre_ns), p.pre_unit)) * p.pre_unit;
     w.lo = min(hi, lo + split * per);
     w.hi = min(hi, w.lo + per);
     return true;
@@ -1599,13 +1599,17 @@ static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim,
     /* Spans of a tile at `positions`: us(n) = time of a span + what the
      * records of n spans take to write and read (+ the combine's launch,
      * where it is not there anyway).  A workgroup takes 3.4 us for 128
-     * positions of 128-value heads (WIDE; half of that for 64), 1.2 us for 64
-     * on the narrow kernel, the copies stream at 4.5 TB/s. */
+     * positions of 128-value heads of f16 caches, 5.9 of f32 (half of that
+     * for 64 values), 1.2 us for 64 on the narrow kernel; the records stream
+     * at 4.5 TB/s. */
     auto slots = [](Shape s) { return s == NARROW ? 512 : 256; };   /* workgroups at once */
+    /* two tiles, one of each group: 32 positions each of f32 caches (64 rows
+     * behind 2,000 positions, in multiples of 128: 26.2 and 28.3 us) */
+    auto unit = [&](Shape s) { return !half && s != NARROW ? 64 : 128; };
     auto spans = [&](Shape s, long long wgs, int positions, bool joined) {
-        const double t = positions * (s == NARROW ? 1.2 / 64 : 3.4 / 128) * (head_dim > 64 ? 1 : 0.5);
+        const double t = positions * (s == NARROW ? 1.2 / 64 : (half ? 3.4 : 5.9) / 128) * (head_dim > 64 ? 1 : 0.5);
         const double r = (double)m * n_kv * head_dim * 8 / 4.5e6;
-        const int most = (int)std::min<long long>({64, (positions + 127) / 128, std::max(1ll, slots(s) / wgs)});
+        const int most = (int)std::min<long long>({64, (positions + unit(s) - 1) / unit(s), std::max(1ll, slots(s) / wgs)});
         auto us = [&](int n) { return t / n + r * n + (joined || n == 1 ? 0 : 4) - (joined || n > 1 ? 0 : r); };
         const int n = std::max(1, std::min(most, (int)std::sqrt(t / r)));   /* the best, or the next */
         const int best = n < most && us(n + 1) < us(n) ? n + 1 : n;
@@ -1618,13 +1622,14 @@ static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim,
     const long long own_tiles = tiles(k.own, n_seqs);
     p.cap = spans(k.own, own_tiles * n_kv, own_sees, pre_len > 0);
     p.target = std::max(1, slots(k.own) / n_kv);
+    p.unit = unit(k.own);
     if (n_seqs > 1 && p.cap > 1)   /* room for a sequence much longer than the others */
-        p.cap = (int)std::min<long long>({64, (own_sees + 127) / 128, std::max<long long>(4ll * p.cap, 4ll * p.target / own_tiles)});
+        p.cap = (int)std::min<long long>({64, (own_sees + p.unit - 1) / p.unit, std::max<long long>(4ll * p.cap, 4ll * p.target / own_tiles)});
     p.items = (int)std::min(m / SHAPE_ROWS[k.own] + n_seqs, m) + (p.cap > 1 ? p.target : 0);
-    p.unit = 128;
     if (pre_len) {
         k.pre = shape_of(m, 1, n_kv, pre_len, half);
         p.pre_tiles = (int)tiles(k.pre, 1);
+        p.pre_unit = unit(k.pre);
         p.pre_ns = spans(k.pre, (long long)p.pre_tiles * n_kv, pre_len, true);
     }
     p.nrec = p.cap + p.pre_ns > 1 ? p.cap + p.pre_ns : 0;
