@@ -186,8 +186,8 @@ def test_large_neighbours(tg, hd, big, what):
 
 @pytest.mark.parametrize("hd", [64, 128])
 def test_values_of_many_sizes(tg, hd):
-    """f32 caches whose positions differ by powers of two up to 2^14 keep the
-    matrix units' path, beyond that the plain one; zeros count as neither."""
+    """f32 caches whose positions differ by powers of two: a little (the matrix
+    units' path), a lot (value by value); zeros count as neither."""
     for top, zero in ((10, False), (14, True), (40, True)):
         say(f"values of many sizes hd={hd} top={top}")
         b = Batch(hd + top, 8, 2, hd, [33, 4], [90, 300], False, q_scale=0.5)

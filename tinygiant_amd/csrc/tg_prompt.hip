@@ -449,7 +449,11 @@ __device__ void slow_row(const PromptArgs &a, const RowsPlan &p, const Work &w, 
  * product is two MFMAs, and the result is as good as f32 sums.  What keeps
  * lo out of f16's underflow: q is scaled by a power of two a row (its largest
  * value to 2^14 .. 2^15), undone in the factor that takes scores to base 2;
- * weights are taken times 2^15.
+ * weights are taken times 2^SHIFT.
+ *
+ * The reference exponent m follows a row's largest score only when that is
+ * more than LAG above it, so most tiles rescale nothing (8192 tokens: 917 us,
+ * with m the largest score 939).  SHIFT + LAG stays below f16's largest, 2^16.
  *
  * K and V tiles of 64 positions go to LDS by direct copies, two buffers; the
  * 16-byte pieces of a row are permuted by its position (swz) so that neither
@@ -504,7 +508,11 @@ __device__ inline float other_half_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-constexpr float W_SHIFT = 15.f;   /* weights are taken times 2^15, below f16's largest */
+/* f16 caches: a weight is off by 2^-25 2^-SHIFT beside its own 2^-22.  f32
+ * caches, whose groups of positions shift weights by up to SPREAD more, keep
+ * 2^-25 with SHIFT = SPREAD. */
+constexpr float SHIFT_H = 8.f, LAG_H = 7.f;
+constexpr float SHIFT_F = 12.f, LAG_F = 3.f;
 
 /* A lane's m-row (both halves of a wave hold the same 32) and what its wave
  * sees: positions any_lo .. any_hi by some row, all_lo .. all_hi by all. */
@@ -673,14 +681,15 @@ __device__ inline void mask_scores(f16v &s, int at, const Lane &x) {
     }
 }
 
-/* The wave's rows finished: weights were summed in units of 2^(mx - W_SHIFT)
- * relative to l, values (SCALED) besides in units of 2^-oexp.  They go to
+/* The wave's rows finished: weights were summed times 2^SHIFT
+ * relative to 2^mx, values (SCALED) besides in units of 2^-oexp.  They go to
  * `stage` (LDS, the wave's 32 rows), where[] saying where in p.o or a.out each
  * belongs (-1: nowhere), or without stage to memory.  Returns the m-rows that
  * came out not finite, which are not written. */
 template <int HD, bool SCALED>
 __device__ inline uint32_t write_rows(const PromptArgs &a, const RowsPlan &p, const Work &w, const Lane &x, int lane, float mx,
                                       float l, int oexp, const f16v (&o)[HD / 32], uint8_t *stage, long long *where) {
+    constexpr float SHIFT = SCALED ? SHIFT_F : SHIFT_H;
     float big = fabsf(l);   /* NaN where anything is */
 #pragma unroll
     for (int d = 0; d < HD / 32; d++)
@@ -694,14 +703,14 @@ __device__ inline uint32_t write_rows(const PromptArgs &a, const RowsPlan &p, co
     float f = 1.f;
     if (p.nrec) {
         const size_t rec = ((size_t)x.r * a.n_heads + x.h) * p.nrec + w.rec;
-        constexpr float one = 1.f / 32768.f;   /* 2^-W_SHIFT */
+        constexpr float one = 1.f / (float)(1 << (int)SHIFT);
         if (write && half == 0) write_ml(p, w, rec, mx, l * one);
         write = write && mx > -INFINITY;      /* a record of no position has no sums */
         at = (long long)(rec * hd);
         f = one;
     } else {
         if (a.sinks && write) {
-            const float ref = mx - W_SHIFT, sk = a.sinks[x.h] * LOG2E, M = fmaxf(ref, sk), base = M == -INFINITY ? 0.f : M;
+            const float ref = mx - SHIFT, sk = a.sinks[x.h] * LOG2E, M = fmaxf(ref, sk), base = M == -INFINITY ? 0.f : M;
             f = exp2f(ref - base);
             l = l * f + exp2f(sk - base);
         }
@@ -878,16 +887,17 @@ __device__ inline __attribute__((always_inline)) void rows_h(const PromptArgs &a
                 for (int v = 0; v < 16; v++) top = max_nan(top, s[j][v]);
             }
             top = other_half_max(top) * c;
-            const float mn = max_nan(mx, top), sh = mn == -INFINITY ? 0.f : W_SHIFT - mn;
-            if (__any(mn > mx)) {
+            if (__any(top > mx + LAG_H)) {
+                const float mn = max_nan(mx, top);
                 const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
+                mx = mn;
                 l *= alpha;
 #pragma unroll
                 for (int d = 0; d < DB; d++)
 #pragma unroll
                     for (int v = 0; v < 16; v++) o[d][v] *= alpha;
             }
-            mx = mn;
+            const float sh = mx == -INFINITY ? 0.f : SHIFT_H - mx;
             h8 ph[2 * J], pl[2 * J];
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -966,7 +976,7 @@ __global__ __launch_bounds__(64 * MW * KG, HD == 64 && J == 1 ? 4 : 2) void k_ro
  * A tile of 32 positions is loaded into registers two tiles ahead, split and
  * stored to one of two LDS buffers one tile ahead (plane [K hi, K lo, V hi,
  * V lo][32][HD]). */
-constexpr int KF = 32, SPREAD = 15;
+constexpr int KF = 32, SPREAD = 12;
 constexpr int ALL_ZERO = 100;   /* exponent of a group of zeros; no other is larger */
 
 /* HD / 4 lanes hold a position: whether each has a bit in m, or none in any */
@@ -1157,9 +1167,10 @@ __device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a
             }
             top = other_half_max(top);
             const int un = min(min(U, min(ve[0], ve[1])), min(ve[2], ve[3]));
-            const float mn = max_nan(mx, top), sh = mn == -INFINITY ? 0.f : W_SHIFT - mn;
-            if (__any(mn > mx) || un != U) {
+            if (__any(top > mx + LAG_F) || un != U) {
+                const float mn = max_nan(mx, top);
                 const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
+                mx = mn;
                 const float beta = __builtin_amdgcn_ldexpf(alpha, un - U);
                 l *= alpha;
 #pragma unroll
@@ -1167,7 +1178,8 @@ __device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a
 #pragma unroll
                     for (int v = 0; v < 16; v++) o[d][v] *= beta;
             }
-            mx = mn, U = un;
+            U = un;
+            const float sh = mx == -INFINITY ? 0.f : SHIFT_F - mx;
             h8 ph[2], pl[2];
 #pragma unroll
             for (int g = 0; g < 4; g++) {
