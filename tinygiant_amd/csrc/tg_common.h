@@ -7,7 +7,6 @@
 #define TG_COMMON_H
 
 enum { TG_FMT_Q4K = 0, TG_FMT_F16 = 1, TG_FMT_Q6K = 2, TG_FMT_MXFP4 = 3, TG_FMT_Q80 = 4 };
-enum { TG_KV_F32 = 0, TG_KV_F16 = 1 };   /* element type of a KV cache */
 enum { TG_ACT_SILU = 0, TG_ACT_GPTOSS = 1 };
 
 #define TG_QK 256            /* values per q8 activation block */

@@ -8,6 +8,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+enum { TG_KV_F32 = 0, TG_KV_F16 = 1 };   /* element type of a KV cache */
+
 #define PROMPT_MAX_HEAD_DIM 128   /* head_dim: a multiple of 8, at most this */
 #define PROMPT_MAX_GQA 64         /* query heads per KV head, at most this */
 #define PROMPT_MAX_KV (1 << 20)   /* kv_max, prefix_max: offsets in one head's rows stay below 2^30 bytes */
