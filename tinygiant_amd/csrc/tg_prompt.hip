@@ -4,7 +4,21 @@
  *
  * The reference runs attention one row at a time (tg_attention_v2,
  * csrc/libtinygiant.c:939-983, called row by row at tinygiant/engine.py:
- * 232-275); these are the same formulas for many rows a call.
+ * 232-275); these are the same formulas for many rows a call:
+ *
+ *   append     K and V of each row, normed and rotated, into its slot; q normed
+ *              and rotated (k_kv_append)
+ *   attention  o = sum_j p_j v_j / (sum_j p_j + p_sink),
+ *              p_j = exp(q k_j / sqrt(head_dim) - m), over the positions that
+ *              the row sees, in one pass with running m and sums
+ *
+ * Kernels of the attention, chosen by sizes alone (rows_cut):
+ *   k_rows_h        f16 caches, 128 query rows of a KV head a workgroup
+ *   k_rows_f        f32 caches, 128 or 256
+ *   k_rows_n        either, 16: few rows
+ *   k_rows_combine  joins what several workgroups made of a row's positions
+ * A row that does not come out finite is computed again from the formulas
+ * with plain loads (slow_row).
  */
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -85,7 +99,9 @@ __device__ inline bool wave_seq_of(const PackedSeqs &p, int r, Seq &q, int &i) {
  * so the loads are 16 bytes and RoPE needs no exchange.  The norm is
  * tg_rms_norm's (csrc/libtinygiant.c:680-698), the rotation
  * apply_rope_inplace's (:702-719); an f16 cache gets K and V rounded once, to
- * nearest. */
+ * nearest.  Bound: the bytes.  4,001 rows of 64 + 2 x 8 heads of 64 into an f32
+ * cache: 165 MB in 32.9 us, 5.0 TB/s, a large copy's rate; 8 rows 5.6 us, the
+ * launch and two dependent reads. */
 template <bool HALF, int G>
 __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
     const int r = blockIdx.x;
@@ -771,8 +787,15 @@ __device__ inline void merge_groups(float *lds, int wave, int lane, float &mx, f
 
 /* MW waves of 32 m-rows; with KG = 2, two groups of them take the tiles in
  * turn.  J blocks of 32 positions are computed together: two overlap their
- * latencies (8192 tokens: 928 us, one at a time 965), one is half the code
- * and skips what a window hides (4,096 tokens, window 128: 46.2, 48.6). */
+ * latencies (8192 tokens: 918 us, one at a time 928), one is half the code
+ * and skips what a window hides (4,096 tokens, window 128: 43.5, 46.0).
+ *
+ * Bound for long prompts: the matrix units at the power limit.  8192 tokens of
+ * 32 heads of 128: 903 us, 1.22 PFLOP/s counting both products (a large f16
+ * product runs at 1.23), the clock at 1.45 GHz.  4,096 tokens of 64 heads of
+ * 64 with a window of 128: 43.3 us, 142 MB; two rounds of workgroups that load
+ * (5 us), compute (8: a block's softmax takes more issue slots than its
+ * products) and store (2) with little overlap between those of a CU. */
 template <int HD, int MW, int KG>
 struct SharedH {
     __attribute__((aligned(1024))) uint8_t bufs[KG][2][2][KT * HD * 2];
@@ -977,7 +1000,12 @@ __global__ __launch_bounds__(64 * MW * KG, HD == 64 && J == 1 ? 4 : 2) void k_ro
  *
  * A tile of 32 positions is loaded into registers two tiles ahead, split and
  * stored to one of two LDS buffers one tile ahead (plane [K hi, K lo, V hi,
- * V lo][32][HD]). */
+ * V lo][32][HD]).
+ *
+ * Bound: the matrix units and the splitting beside them.  500 rows of 64 heads
+ * of 64 behind 30,001 positions: 803 us, 0.93 PFLOP/s counting the three
+ * products, 75% of a large f16 product's rate; 2,020 packed rows of 32 heads
+ * of 128: 59 us, where the longest sequence's last tiles are most of it. */
 constexpr int KF = 32, SPREAD = 12;
 constexpr int ALL_ZERO = 100;   /* exponent of a group of zeros; no other is larger */
 
@@ -1266,7 +1294,12 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPl
  * 4 (l / 16) + i as it lies.  The second product is f32 (16x16x4) for both
  * cache types: V converts exactly, the weights are not rounded, and the rate
  * is above what the cache's bytes allow.  The first is f32 for an f32 cache
- * and two f16 products (q in two planes) for an f16 one. */
+ * and two f16 products (q in two planes) for an f16 one.
+ *
+ * Bound: the cache's bytes.  One row of each of 32 sequences of 2,091 positions
+ * on average, 4 KV heads of 128, f16: 137 MB in 32 us, 4.3 TB/s; at 1,500
+ * positions and less the chain of a workgroup (find its work 1 us, q and the
+ * first tile 3, merge and write 3). */
 typedef float v4f __attribute__((ext_vector_type(4)));
 constexpr int MN = 16;
 
@@ -1509,7 +1542,9 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
 }
 
 /* The records of a row and head, and its sink, as one: W waves each, wave g
- * the records g (mod W), G lanes a record (four dims a lane). */
+ * the records g (mod W), G lanes a record (four dims a lane).  1,536 rows of 25
+ * records of 128 values, 20 MB: 7.4 us with four waves; few rows 3 - 4 us, the
+ * launch and two memory round trips. */
 template <int W, int G>
 __global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) {
     __shared__ __attribute__((aligned(16))) float so[W > 1 ? W : 1][4 * G];
@@ -1593,11 +1628,14 @@ __global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) 
  * device).  Each part, the sequences' slots and the prefix, has a shape:
  *   narrow  16 m-rows a workgroup, positions over its waves
  *   wide    128 m-rows, two groups of four waves on tiles in turn: two waves
- *           a SIMD where there are no more workgroups than CUs
- *   short   128 m-rows, four waves, for few positions a row
- *   full    the same, several workgroups a CU on long spans
- *   tall    256 m-rows, eight waves (f32 caches): half the splitting of K and
- *           V a row */
+ *           a SIMD where there are few workgroups (1,024 tokens of 32 heads of
+ *           128, f16 and f32: 33.1 and 52.2 us, full 36.7 and 70.6)
+ *   short   128 m-rows, four waves, for few positions a row (128 tokens, f16:
+ *           11.6 us, wide 12.3)
+ *   full    the same, two workgroups a CU on long spans (8,192 tokens, f16:
+ *           907 us, wide 963; 3,000 146 and 153; 2,048 78 and 74)
+ *   tall    256 m-rows, eight waves, long f32 caches: half the splitting of K
+ *           and V a row (4,096 tokens: 403 us, full 468; 3,000 250 and 248) */
 enum Shape { NARROW, SHORT, WIDE, FULL, TALL };
 constexpr int SHAPE_ROWS[] = {16, 128, 128, 128, 256}, SHAPE_THREADS[] = {256, 256, 512, 256, 512};
 struct Cut {
