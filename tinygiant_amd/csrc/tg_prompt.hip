@@ -1542,10 +1542,11 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
 }
 
 /* The records of a row and head, and its sink, as one: W waves each, wave g
- * the records g (mod W), G lanes a record (four dims a lane).  1,536 rows of 25
+ * the records g (mod W), G lanes a record (four dims a lane), N records of a
+ * lane's loads at a time.  1,536 rows of 25
  * records of 128 values, 20 MB: 7.4 us with four waves; few rows 3 - 4 us, the
  * launch and two memory round trips. */
-template <int W, int G>
+template <int W, int G, int N>
 __global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) {
     __shared__ __attribute__((aligned(16))) float so[W > 1 ? W : 1][4 * G];
     __shared__ float sl[W];
@@ -1559,7 +1560,6 @@ __global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) 
     /* lane i holds record W i + wave of each 64 W.  The first ones' statistics
      * and sums are read before it is known that they are there (there is room
      * for them), so that nothing waits for the row's sequence. */
-    constexpr int N = 4;   /* records of a lane's loads at a time */
     f4 stat = {-INFINITY, 0.f, 0.f, 0.f}, y[N];
     if (W * lane + wave < p.nrec) stat = *(const f4 *)(ml + 4 * (W * lane + wave));
     float m0 = -INFINITY, m1 = -INFINITY;   /* at most 128 records (rows_cut) */
@@ -1621,7 +1621,7 @@ __global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) 
     }
     if (lane >= G || d >= hd) return;
     if (a.sinks) l += exp2f(sink - base);
-    *(f4u *)(a.out + (size_t)r * a.out_stride + (size_t)h * hd + d) = o / l;
+    *(f4u *)(a.out + (size_t)r * a.out_stride + (size_t)h * hd + d) = o * (1.f / l);
 }
 
 /* How a call is cut, from the host's arguments alone (the lengths are on the
@@ -1761,8 +1761,10 @@ static void launch_rows(const PromptArgs &a, const Cut &k, bool half, void *scra
     }
     if (!p.nrec) return;
     const long long rows = (long long)a.s.rows * a.n_heads;
-    if (p.nrec > 16) hipLaunchKernelGGL((k_rows_combine<4, HD / 4>), dim3((unsigned)rows), dim3(256), 0, st, a, p);
-    else hipLaunchKernelGGL((k_rows_combine<1, HD / 4>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, p);
+    const dim3 four((unsigned)((rows + 3) / 4));
+    if (p.nrec > 16) hipLaunchKernelGGL((k_rows_combine<4, HD / 4, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, p);
+    else if (p.nrec > 256 / HD) hipLaunchKernelGGL((k_rows_combine<1, HD / 4, 4>), four, dim3(256), 0, st, a, p);
+    else hipLaunchKernelGGL((k_rows_combine<1, HD / 4, 1>), four, dim3(256), 0, st, a, p);
 }
 
 size_t launch_attention_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st) {
