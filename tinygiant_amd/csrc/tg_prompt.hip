@@ -791,8 +791,8 @@ __device__ inline void merge_groups(float *lds, int wave, int lane, float &mx, f
  * and skips what a window hides (4,096 tokens, window 128: 43.5, 46.0).
  *
  * Bound for long prompts: the matrix units at the power limit.  8192 tokens of
- * 32 heads of 128: 903 us, 1.22 PFLOP/s counting both products (a large f16
- * product runs at 1.23), the clock at 1.45 GHz.  4,096 tokens of 64 heads of
+ * 32 heads of 128: 898 us, 1.22 PFLOP/s counting both products (a large f16
+ * product runs at 1.23), the clock at 1.45 - 1.6 GHz.  4,096 tokens of 64 heads of
  * 64 with a window of 128: 43.3 us, 142 MB; two rounds of workgroups that load
  * (5 us), compute (8: a block's softmax takes more issue slots than its
  * products) and store (2) with little overlap between those of a CU. */
@@ -1003,8 +1003,8 @@ __global__ __launch_bounds__(64 * MW * KG, HD == 64 && J == 1 ? 4 : 2) void k_ro
  * V lo][32][HD]).
  *
  * Bound: the matrix units and the splitting beside them.  500 rows of 64 heads
- * of 64 behind 30,001 positions: 803 us, 0.93 PFLOP/s counting the three
- * products, 75% of a large f16 product's rate; 2,020 packed rows of 32 heads
+ * of 64 behind 30,001 positions: 788 us, 0.94 PFLOP/s counting the three
+ * products, 77% of a large f16 product's rate; 2,020 packed rows of 32 heads
  * of 128: 59 us, where the longest sequence's last tiles are most of it. */
 constexpr int KF = 32, SPREAD = 12;
 constexpr int ALL_ZERO = 100;   /* exponent of a group of zeros; no other is larger */
