@@ -82,6 +82,37 @@ def test_prefix_matches_plain(tg, layout, prefix, lens, past, window, half):
 
 
 @pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 20, 2 ** 20])
+def test_window_longer_than_any_cache(tg, window, half):
+    for lens, past, prefix in (([3, 40], [500, 9], 0), ([2, 1], [5, 70], 300)):
+        say(f"window={window} half={half} prefix={prefix}")
+        b = Batch(80, 8, 2, 64, lens, past, half, window=window, prefix=prefix)
+        got, was = _run(tg, b)
+        b.check(got, was)
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("nh,nkv,hd", [(1024, 16, 128), (1024, 1024, 8), (64, 1, 128), (1, 1, 128), (1024, 512, 16)])
+def test_ends_of_the_layouts(tg, nh, nkv, hd, half):
+    say(f"layout {nh, nkv, hd} half={half}")
+    for lens, past, prefix in (([2, 1], [70, 0], 0), ([1], [600], 0), ([1, 3], [0, 20], 90)):
+        b = Batch(nh + hd, nh, nkv, hd, lens, past, half, prefix=prefix, sinks=True)
+        got, was = _run(tg, b)
+        b.check(got, was)
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_many_sequences(tg, half):
+    """More sequences than one pass over them takes lanes, of few and no rows."""
+    for n, prefix in ((200, 0), (700, 40)):
+        say(f"{n} sequences half={half}")
+        b = Batch(n, 4, 2, 32, [i % 3 for i in range(n)], [(7 * i) % 40 + (900 if i == 150 else 0) for i in range(n)], half,
+                  prefix=prefix)
+        got, was = _run(tg, b)
+        b.check(got, was)
+
+
+@pytest.mark.parametrize("half", [False, True])
 def test_out_over_q(tg, half):
     for kw in (dict(lens=[70, 3], past=[0, 9]), dict(lens=[2], past=[3000]), dict(lens=[1, 2], past=[5, 0], prefix=400)):
         say(f"out over q {kw} half={half}")

@@ -1578,7 +1578,8 @@ static void attention_rows(const char *who, const float *q_dev, int q_stride, in
     a.kv_k = kv_k_dev, a.kv_v = kv_v_dev;
     a.pre_k = prefix_k_dev, a.pre_v = prefix_v_dev, a.pre_len = prefix_len, a.pre_max = prefix_max;
     a.s = packed_seqs(cu_rows_dev, kv_len_dev, slots_dev, n_seqs, n_rows, n_slots, kv_max);
-    a.window = window, a.sinks = sinks_dev;
+    a.window = window < prefix_len + kv_max ? window : 0;   /* as long as all positions: none */
+    a.sinks = sinks_dev;
     a.n_heads = n_heads, a.n_kv = n_kv_heads, a.head_dim = head_dim;
     a.out = out_dev, a.out_stride = out_stride;
     const hipError_t before = hipPeekAtLastError();
