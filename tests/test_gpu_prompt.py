@@ -104,10 +104,10 @@ def test_ends_of_the_layouts(tg, nh, nkv, hd, half):
 @pytest.mark.parametrize("half", [False, True])
 def test_many_sequences(tg, half):
     """More sequences than one pass over them takes lanes, of few and no rows."""
-    for n, prefix in ((200, 0), (700, 40)):
+    for n, prefix, window in ((200, 0, 0), (700, 40, 0), (700, 0, 16), (5000, 0, 0)):
         say(f"{n} sequences half={half}")
         b = Batch(n, 4, 2, 32, [i % 3 for i in range(n)], [(7 * i) % 40 + (900 if i == 150 else 0) for i in range(n)], half,
-                  prefix=prefix)
+                  prefix=prefix, window=window, lead=3 * (n > 200), tail=1)
         got, was = _run(tg, b)
         b.check(got, was)
 

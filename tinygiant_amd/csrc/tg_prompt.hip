@@ -67,26 +67,46 @@ __device__ inline int seq_of(const PackedSeqs &p, int r) {
     return lo;
 }
 
-/* The sequence of row r, the same r in the whole wave: 64 sequences at a time,
- * all that is read of them in one batch.  False: none. */
+/* A run of at most 64 sequences, among which the last is that starts at or
+ * before `key`; 64 places of those before are asked at a time.  A start is a
+ * row, or with MTILE the place of the sequence's first tile (find_tile). */
+struct Run {
+    int at, count;   /* 0: none */
+};
+template <int MTILE>
+__device__ inline int start_of(int r0, int s, int ratio) {
+    return MTILE ? (int)((unsigned)(r0 * ratio) / (unsigned)(MTILE ? MTILE : 1)) + s : r0;
+}
+template <int MTILE>
+__device__ inline Run wave_narrow(const PackedSeqs &p, int ratio, int key) {
+    const int lane = threadIdx.x & 63;
+    int at = 0, count = p.n;
+    while (count > 64) {
+        const int step = (count + 63) / 64, s = at + min(lane * step, count - 1);
+        const uint64_t m = __ballot(lane * step < count && start_of<MTILE>(min(max(p.cu[s], 0), p.rows), s, ratio) <= key);
+        if (!m) return Run{0, 0};
+        const int k = (63 - __builtin_clzll(m)) * step;
+        at += k, count = min(step, count - k);
+    }
+    return Run{at, count};
+}
+
+/* lane `at`'s sequence, in the whole wave */
+__device__ inline Seq lane_seq(const Seq &q, int at) {
+    return Seq{__builtin_amdgcn_readlane(q.r0, at), __builtin_amdgcn_readlane(q.n, at), __builtin_amdgcn_readlane(q.past, at),
+               __builtin_amdgcn_readlane(q.slot, at)};
+}
+
+/* The sequence of row r, the same r in the whole wave; all that is read of the
+ * last 64 in one batch.  False: none. */
 __device__ inline bool wave_seq_of(const PackedSeqs &p, int r, Seq &q, int &i) {
     const int lane = threadIdx.x & 63;
+    const Run run = wave_narrow<0>(p, 0, r);
     Seq mine = {0, 0, 0, 0};
-    uint64_t m = 0;
-    for (int s0 = 0; s0 < p.n; s0 += 64) {
-        const bool on = s0 + lane < p.n;
-        Seq next = {0, 0, 0, 0};
-        if (on) next = seq_at(p, s0 + lane);
-        const uint64_t from = __ballot(on && next.r0 <= r);
-        if (!from) break;
-        m = from, mine = next;
-    }
+    if (lane < run.count) mine = seq_at(p, run.at + lane);
+    const uint64_t m = __ballot(lane < run.count && mine.r0 <= r);
     if (!m) return false;
-    const int at = 63 - __builtin_clzll(m);   /* the last that starts at or before r */
-    q.r0 = __builtin_amdgcn_readlane(mine.r0, at);
-    q.n = __builtin_amdgcn_readlane(mine.n, at);
-    q.past = __builtin_amdgcn_readlane(mine.past, at);
-    q.slot = __builtin_amdgcn_readlane(mine.slot, at);
+    q = lane_seq(mine, 63 - __builtin_clzll(m));   /* the last that starts at or before r */
     i = r - q.r0;
     return i >= 0 && i < q.n;
 }
@@ -199,6 +219,7 @@ struct RowsPlan {
     int target;             /* spans that the positions of all tiles are cut into, about */
     int unit, pre_unit;     /* a span is a multiple of this; the prefix's */
     int pre_tiles, pre_ns;  /* tiles of the prefix, spans of each */
+    bool search;            /* the sequence of a tile is searched for (find_tile), not counted to (find_span) */
     int nrec;               /* room for a row's records: pre_ns + cap; 0: written directly */
     float *ml, *o;          /* [n_rows * n_heads][nrec][4]: m, l, and in the first own span's the count of those;
                                [..][nrec][head_dim] */
@@ -244,14 +265,49 @@ __device__ inline int wave_scan(int v) {
     return v;
 }
 
-/* Item b of the sequences' spans: tiles of MTILE m-rows, late rows first
- * (they see the most positions), cut into spans of one length for all
- * sequences, so that long and short ones finish together: that length is what
- * cuts the positions of all tiles into about p.target spans (a sequence's
- * tiles count as its longest).  A wave counts 64 sequences at a time; sums of
- * positions are floats, the same in every workgroup. */
+/* the first position that the rows of w's tile see, and the one behind the last */
+__device__ inline int tile_lo(const PromptArgs &a, const Work &w) {
+    return a.window > 0 ? max(0, w.sq.past + w.i0 + 1 - a.window) : 0;
+}
 template <int MTILE>
-__device__ inline bool find_item(const PromptArgs &a, const RowsPlan &p, int ratio, int b, Work &w) {
+__device__ inline int tile_hi(const Work &w, int ratio) {
+    int i1, j1;
+    w.row(MTILE - 1, ratio, i1, j1);
+    return w.sq.past + min(w.sq.n - 1, i1) + 1;
+}
+
+/* Tile b of the sequences' tiles of MTILE m-rows, late rows first (they see
+ * the most positions).  Sequence s has its tiles from place
+ * cu[s] ratio / MTILE + s on, where there is room for them whatever the
+ * sequences before it left over: no sum over those is needed. */
+template <int MTILE>
+__device__ inline bool find_tile(const PromptArgs &a, const RowsPlan &p, int ratio, int b, Work &w) {
+    const PackedSeqs &c = a.s;
+    const int lane = threadIdx.x & 63;
+    const Run run = wave_narrow<MTILE>(c, ratio, b);
+    Seq q = {0, 0, 0, 0};
+    if (lane < run.count) q = seq_at(c, run.at + lane);
+    const uint64_t m = __ballot(lane < run.count && start_of<MTILE>(q.r0, run.at + lane, ratio) <= b);
+    if (!m) return false;
+    const int at = 63 - __builtin_clzll(m);
+    w.sq = lane_seq(q, at);
+    const int place = b - start_of<MTILE>(w.sq.r0, run.at + at, ratio), n = div_up(w.sq.n * ratio, MTILE);
+    if (place >= n) return false;
+    w.m0 = (n - 1 - place) * MTILE;
+    set_rows(w, ratio);
+    w.rec = p.pre_ns, w.count = 1;
+    w.lo = tile_lo(a, w), w.hi = tile_hi<MTILE>(w, ratio);   /* stored last, as in the others: the compiler merges the ends */
+    return true;
+}
+
+/* Item b of the sequences' spans: tiles as above, in order, each cut into
+ * spans of one length for all sequences, so that long and short ones finish
+ * together: that length is what cuts the positions of all tiles into about
+ * p.target spans (a sequence's tiles count as its longest); with p.cap 1, one
+ * span a tile.  A wave counts 64 sequences at a time; sums of positions are
+ * floats, the same in every workgroup. */
+template <int MTILE>
+__device__ inline bool find_span(const PromptArgs &a, const RowsPlan &p, int ratio, int b, Work &w) {
     const PackedSeqs &c = a.s;
     const int lane = threadIdx.x & 63;
     Seq q = {0, 0, 0, 0};
@@ -282,18 +338,12 @@ __device__ inline bool find_item(const PromptArgs &a, const RowsPlan &p, int rat
         const uint64_t past = __ballot(end > b);
         if (past) {
             const int at = __builtin_ctzll(past), n = __builtin_amdgcn_readlane(nt, at);
-            w.sq.r0 = __builtin_amdgcn_readlane(q.r0, at);
-            w.sq.n = __builtin_amdgcn_readlane(q.n, at);
-            w.sq.past = __builtin_amdgcn_readlane(q.past, at);
-            w.sq.slot = __builtin_amdgcn_readlane(q.slot, at);
+            w.sq = lane_seq(q, at);
             if (at) b -= __builtin_amdgcn_readlane(end, at - 1);
             const int split = b / n;
             w.m0 = (n - 1 - (b - split * n)) * MTILE;
             set_rows(w, ratio);
-            int i1, j1;
-            w.row(MTILE - 1, ratio, i1, j1);
-            const int lo = a.window > 0 ? max(0, w.sq.past + w.i0 + 1 - a.window) : 0;
-            const int hi = w.sq.past + min(w.sq.n - 1, i1) + 1;
+            const int lo = tile_lo(a, w), hi = tile_hi<MTILE>(w, ratio);
             int count = div_up(hi - lo, per);
             if (count > p.cap) {
                 per = div_up(div_up(hi - lo, p.cap), p.unit) * p.unit;
@@ -344,7 +394,7 @@ __device__ inline bool find_work(const PromptArgs &a, const RowsPlan &p, int rat
     if (!w.prefix) b -= npre;
     const int item = b / a.n_kv;
     w.kh = b - item * a.n_kv;
-    if (!w.prefix) return find_item<MTILE>(a, p, ratio, item, w);
+    if (!w.prefix) return p.search ? find_tile<MTILE>(a, p, ratio, item, w) : find_span<MTILE>(a, p, ratio, item, w);
     const int split = item / p.pre_tiles;
     const int r0 = min(max(a.s.cu[0], 0), a.s.rows), r1 = min(max(a.s.cu[a.s.n], r0), a.s.rows);
     w.rec = split, w.count = 0;
@@ -1688,7 +1738,12 @@ static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim,
     p.unit = unit(k.own);
     if (n_seqs > 1 && p.cap > 1)   /* room for a sequence much longer than the others */
         p.cap = (int)std::min<long long>({64, (own_sees + p.unit - 1) / p.unit, std::max<long long>(4ll * p.cap, 4ll * p.target / own_tiles)});
-    p.items = (int)std::min(m / SHAPE_ROWS[k.own] + n_seqs, m) + (p.cap > 1 ? p.target : 0);
+    /* 256, 512 and 1,024 rows of as many sequences behind 100 positions, in us:
+     * counted 20.2, 46.1 and 110, searched 22.5, 39.7 and 71 (the places that
+     * sequences leave over are workgroups with nothing to do) */
+    p.search = p.cap == 1 && n_seqs > 256;
+    p.items = p.search ? (int)(m / SHAPE_ROWS[k.own]) + n_seqs
+                       : (int)std::min(m / SHAPE_ROWS[k.own] + n_seqs, m) + (p.cap > 1 ? p.target : 0);
     if (pre_len) {
         k.pre = shape_of(m, 1, n_kv, pre_len, half);
         p.pre_tiles = (int)tiles(k.pre, 1);
