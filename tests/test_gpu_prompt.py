@@ -233,6 +233,39 @@ def test_values_of_many_sizes(tg, hd):
         b.check(got, was)
 
 
+@pytest.mark.parametrize("rows,past", [(9, 40), (60, 300), (300, 700), (1100, 0), (520, 16100)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_values_of_many_sizes_in_long_calls(tg, hd, rows, past):
+    """As above where rows or positions are many: every tenth position is
+    smaller by 2^20, in V or in K; some rows against 64 bits."""
+    say(f"many sizes hd={hd} rows={rows} past={past}")
+    lib, dev, rng = tg.lib(), Dev(tg), np.random.default_rng(rows + hd)
+    nh, nkv, n = 64, 8, rows + past
+    q = (rng.standard_normal((rows, nh, hd)) * 0.5).astype(np.float32)
+    cache = rng.standard_normal((2, 1, nkv, n, hd)).astype(np.float32)
+    for which in (0, 1):
+        k, v = (x.copy() for x in cache)
+        (k, v)[which][:, :, ::10] *= np.float32(2.0 ** -20)
+        out = dev(np.zeros_like(q))
+        scratch = dev.room(lib.tg_hip_attention_prompt_scratch_bytes(rows, 1, nh, nkv, hd, n, 0))
+        lib.tg_hip_clear_error()
+        lib.tg_hip_attention_prompt_dev(dev(q), nh * hd, 0, dev(k), dev(v), 1, n, dev(np.array([0, rows], np.int32)),
+                                        dev(np.array([past], np.int32)), None, 1, rows, 0, None, nh, nkv, hd, out, nh * hd, scratch,
+                                        None)
+        lib.tg_hip_synchronize()
+        assert tg.last_error() == "", tg.last_error()
+        got = dev.read(out, q)
+        for r in {0, 1, rows // 2, rows - 2, rows - 1}:
+            for h in (0, 7, 40, 63):
+                kk, vv = (x[0, h // 8, :past + r + 1].astype(np.float64) for x in (k, v))
+                qq = q[r, h].astype(np.float64)
+                z = kk @ qq * hd ** -0.5
+                p = np.exp(z - z.max())
+                off = (8 * np.sqrt(2 * hd) + 4) * EPS * (np.abs(kk) @ np.abs(qq)).max() * hd ** -0.5 + (8 * np.sqrt(len(z)) + 24) * EPS
+                assert np.all(np.abs(got[r, h] - (p @ vv) / p.sum()) <= 2 * off * np.abs(vv).max()), (which, r, h)
+    dev.free()
+
+
 def test_sequences_that_do_not_fit_are_left_out(tg):
     """A slot out of range, a negative length, rows past kv_max: those
     sequences' rows stay as they were, the others are computed."""

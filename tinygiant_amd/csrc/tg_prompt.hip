@@ -1027,6 +1027,264 @@ __global__ __launch_bounds__(64 * MW * KG, HD == 64 && J == 1 ? 4 : 2) void k_ro
     rows_h<HD, MW, KG, J>(a, p, sh);
 }
 
+/* ---- few rows: positions over the waves ----
+ *
+ * A workgroup of four waves takes 16 m-rows; a wave walks tiles of 16
+ * positions (every fourth) with K and V straight from the cache into the
+ * operands, no LDS and no barrier until the end, where the four waves' sums
+ * meet.  S^T[position][m-row] on 16x16 MFMAs: D lane l holds m-row l % 16,
+ * positions 4 (l / 16) + v, which is B of the second product over positions
+ * 4 (l / 16) + i as it lies.  The second product is f32 (16x16x4) for both
+ * cache types: V converts exactly, the weights are not rounded, and the rate
+ * is above what the cache's bytes allow.  The first is f32 for an f32 cache
+ * and two f16 products (q in two planes) for an f16 one.
+ *
+ * Bound: the cache's bytes.  One row of each of 32 sequences of 2,091 positions
+ * on average, 4 KV heads of 128, f16: 137 MB in 32 us, 4.3 TB/s; at 1,500
+ * positions and less the chain of a workgroup (find its work 1 us, q and the
+ * first tile 3, merge and write 3). */
+typedef float v4f __attribute__((ext_vector_type(4)));
+constexpr int MN = 16;
+
+template <typename T, int HD>
+struct NarrowK {   /* float: K pieces of 4 dims, dims 16 j + 4 kq + e in MFMA (j, e) */
+    static constexpr int J = HD / 16;
+    v4f q[J];
+    u32x4 k[J];
+    __device__ inline float load_q(const PromptArgs &a, const Lane &x, int kq) {
+        const float *src = a.q + (size_t)x.r * a.q_stride + (size_t)x.h * a.head_dim;
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const int d = 16 * j + 4 * kq;
+            q[j] = x.live && d < a.head_dim ? (v4f)*(const f4u *)(src + d) : v4f{0.f, 0.f, 0.f, 0.f};
+        }
+        return LOG2E / sqrtf((float)a.head_dim);
+    }
+    __device__ inline void load_k(Buf kd, uint32_t row, int kq, int hd) {
+#pragma unroll
+        for (int j = 0; j < J; j++) k[j] = ld16(kd, 16 * j + 4 * kq < hd ? row + 64u * j + 16u * (uint32_t)kq : 0x7FFFFF00u);
+    }
+    __device__ inline v4f scores() const {
+        v4f s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;   /* two chains */
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float y = __uint_as_float(k[j][e]);
+                if (e & 1) s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(y, q[j][e], s1, 0, 0, 0);
+                else s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(y, q[j][e], s0, 0, 0, 0);
+            }
+        return s0 + s1;
+    }
+};
+template <int HD>
+struct NarrowK<_Float16, HD> {   /* K pieces of 8 dims, dims 32 j + 8 kq + e in MFMA j */
+    static constexpr int J = HD / 32;
+    h8 qh[J], ql[J];
+    u32x4 k[J];
+    __device__ inline float load_q(const PromptArgs &a, const Lane &x, int kq) {
+        const float *src = a.q + (size_t)x.r * a.q_stride + (size_t)x.h * a.head_dim;
+        f4 u[J], v[J];
+        float big = 0.f;
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const int d = 32 * j + 8 * kq;
+            const bool on = x.live && d < a.head_dim;
+            u[j] = on ? (f4)*(const f4u *)(src + d) : f4{0.f, 0.f, 0.f, 0.f};
+            v[j] = on ? (f4)*(const f4u *)(src + d + 4) : f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 4; e++) big = fmaxf(big, fmaxf(fabsf(u[j][e]), fabsf(v[j][e])));
+        }
+        big = fmaxf(big, __shfl_xor(big, 16, 64));
+        const int ex = scale_exp(fmaxf(big, __shfl_xor(big, 32, 64)));
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float z = __builtin_amdgcn_ldexpf(e < 4 ? u[j][e & 3] : v[j][e & 3], ex);
+                const _Float16 hi = (_Float16)z;
+                qh[j][e] = hi;
+                ql[j][e] = (_Float16)(z - (float)hi);
+            }
+        return __builtin_amdgcn_ldexpf(LOG2E / sqrtf((float)a.head_dim), -ex);
+    }
+    __device__ inline void load_k(Buf kd, uint32_t row, int kq, int hd) {
+#pragma unroll
+        for (int j = 0; j < J; j++) k[j] = ld16(kd, 32 * j + 8 * kq < hd ? row + 64u * j + 16u * (uint32_t)kq : 0x7FFFFF00u);
+    }
+    __device__ inline v4f scores() const {
+        v4f s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const h8 y = __builtin_bit_cast(h8, k[j]);
+            s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, qh[j], s0, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, ql[j], s1, 0, 0, 0);
+        }
+        return s0 + s1;
+    }
+};
+
+/* V of a lane's position: HD / 16 dims; dim(i, t) is the t-th of lane i % 16 */
+template <typename T, int HD>
+struct NarrowV {
+    static constexpr int N = HD / 16;
+    u32x4 v[N / 4];
+    static __device__ inline int dim(int i, int t) { return 64 * (t >> 2) + 4 * i + (t & 3); }
+    __device__ inline void load(Buf vd, uint32_t row, int i, int hd) {
+#pragma unroll
+        for (int n = 0; n < N / 4; n++) v[n] = ld16(vd, 64 * n + 4 * i < hd ? row + 256u * n + 16u * (uint32_t)i : 0x7FFFFF00u);
+    }
+    __device__ inline float at(int t) const { return __uint_as_float(v[t >> 2][t & 3]); }
+};
+template <int HD>
+struct NarrowV<_Float16, HD> {
+    static constexpr int N = HD / 16;
+    typedef _Float16 H __attribute__((ext_vector_type(N)));
+    H v;
+    static __device__ inline int dim(int i, int t) { return N * i + t; }
+    __device__ inline void load(Buf vd, uint32_t row, int i, int hd) {
+        const uint32_t at = N * i < hd ? row + 2u * N * (uint32_t)i : 0x7FFFFF00u;
+        if constexpr (N == 8) v = __builtin_bit_cast(H, ld16(vd, at));
+        else v = __builtin_bit_cast(H, ld8(vd, at));
+    }
+    __device__ inline float at(int t) const { return (float)v[t]; }
+};
+
+template <int HD, int NW>
+struct SharedN {
+    __attribute__((aligned(16))) float mo[NW][MN][HD];
+    float mm[NW][MN], ml[NW][MN];
+    uint32_t bad_rows;
+};
+/* m-rows `from` .. from + 15 of the work's tile, by all NW waves of the workgroup */
+template <typename T, int HD, int NW>
+__device__ inline __attribute__((always_inline)) void rows_n(const PromptArgs &a, const RowsPlan &p, const Work &w, int from,
+                                                             SharedN<HD, NW> &sh) {
+    constexpr int N = HD / 16;
+    auto &mo = sh.mo;
+    auto &mm = sh.mm;
+    auto &ml = sh.ml;
+    auto &bad_rows = sh.bad_rows;
+    const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c16 = lane & 15, kq = lane >> 4;
+    const Lane x = lane_rows(a, w, from, c16, 16, ratio);
+    if (tid == 0) bad_rows = 0;
+
+    const uint32_t rb = (uint32_t)hd * (uint32_t)sizeof(T);
+    const Buf kd = make_buf_uniform(region<T>(a, w, a.kv_k, a.pre_k), (uint32_t)w.hi * rb);
+    const Buf vd = make_buf_uniform(region<T>(a, w, a.kv_v, a.pre_v), (uint32_t)w.hi * rb);
+    NarrowK<T, HD> K;
+    NarrowV<T, HD> V[4];
+    auto load_v = [&](int t0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) V[i].load(vd, (uint32_t)(t0 + 4 * kq + i) * rb, c16, hd);
+    };
+    int t = w.lo + 16 * wave;
+    K.load_k(kd, (uint32_t)(t + c16) * rb, kq, hd);   /* past the span: zeros, no memory access */
+    load_v(t);
+    const float c = K.load_q(a, x, kq);
+    float mx = -INFINITY, l = 0.f;
+    v4f o[N];
+#pragma unroll
+    for (int n = 0; n < N; n++) o[n] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (; t < w.hi; t += 16 * NW) {
+        v4f s = K.scores();
+        K.load_k(kd, (uint32_t)(t + 16 * NW + c16) * rb, kq, hd);
+        const bool masked = t + 15 > x.all_hi || t < x.all_lo;   /* uniform */
+        float top = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            const int pos = t + 4 * kq + v;
+            if (masked) s[v] = pos <= x.last && pos >= x.first ? s[v] : -INFINITY;
+            top = fmaxf(top, s[v]);
+        }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64)) * c;
+        const float mn = fmaxf(mx, top), base = mn == -INFINITY ? 0.f : mn;
+        if (__any(mn > mx)) {
+            const float alpha = __builtin_amdgcn_exp2f(mx - base);
+            l *= alpha;
+#pragma unroll
+            for (int n = 0; n < N; n++) o[n] *= alpha;
+        }
+        mx = mn;
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], c, -base));
+            l += s[v];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int n = 0; n < N; n++) o[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(V[i].at(n), s[i], o[n], 0, 0, 0);
+        load_v(t + 16 * NW);
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+#pragma unroll
+    for (int v = 0; v < 4; v++)
+#pragma unroll
+        for (int n = 0; n < N; n += 4) {
+            const int d = NarrowV<T, HD>::dim(4 * kq + v, n);   /* the next three follow */
+            *(f4 *)&mo[wave][c16][d] = f4{o[n][v], o[n + 1][v], o[n + 2][v], o[n + 3][v]};
+        }
+    if (kq == 0) mm[wave][c16] = mx, ml[wave][c16] = l;
+    __syncthreads();
+    /* the waves' sums as one, in wave order: 16 threads a row, HD / 16 dims each */
+    const bool on = tid < 16 * MN;
+    const int row = (tid >> 4) & (MN - 1), d0 = (tid & 15) * N;
+    const Lane y = lane_rows(a, w, from, row, 16, ratio);
+    float M = mm[0][row];
+#pragma unroll
+    for (int q = 1; q < NW; q++) M = fmaxf(M, mm[q][row]);
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f, r[N];
+#pragma unroll
+    for (int n = 0; n < N; n++) r[n] = 0.f;
+#pragma unroll
+    for (int q = 0; q < NW; q++) {
+        const float e = __builtin_amdgcn_exp2f(mm[q][row] - base);
+        L = fmaf(ml[q][row], e, L);
+#pragma unroll
+        for (int n = 0; n < N; n++) r[n] = fmaf(mo[q][row][d0 + n], e, r[n]);
+    }
+    float nan = L * 0.f;
+#pragma unroll
+    for (int n = 0; n < N; n++) nan = fmaf(r[n], 0.f, nan);
+    if (on && y.live && !(nan == 0.f)) atomicOr(&bad_rows, 1u << row);
+    __syncthreads();
+    const uint32_t bad = bad_rows;
+    if (on && y.live && !((bad >> row) & 1u) && d0 < hd) {
+        float *dst, f = 1.f;
+        if (p.nrec) {
+            const size_t rec = ((size_t)y.r * a.n_heads + y.h) * p.nrec + w.rec;
+            if (d0 == 0) write_ml(p, w, rec, M, L);
+            dst = p.o + rec * hd + d0;
+        } else {
+            if (a.sinks) {
+                const float sk = a.sinks[y.h] * LOG2E, mn = fmaxf(M, sk), b2 = mn == -INFINITY ? 0.f : mn;
+                f = exp2f(M - b2);
+                L = L * f + exp2f(sk - b2);
+            }
+            f /= L;
+            dst = a.out + (size_t)y.r * a.out_stride + (size_t)y.h * hd + d0;
+        }
+        if (!p.nrec || M > -INFINITY) {
+#pragma unroll
+            for (int n = 0; n < N; n += 4) *(f4u *)(dst + n) = f4{r[n] * f, r[n + 1] * f, r[n + 2] * f, r[n + 3] * f};
+        }
+    }
+    for (uint32_t z = bad; z; z &= z - 1) slow_row<T>(a, p, w, from + __builtin_ctz(z), ratio, &mo[0][0][0]);
+}
+
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
+    __shared__ SharedN<HD, 4> sh;
+    Work w;
+    if (find_work<MN>(a, p, a.n_heads / a.n_kv, w)) rows_n<T, HD, 4>(a, p, w, 0, sh);
+}
+
 /* ---- float32 caches on the f16 matrix units ----
  *
  * The same products with K and V split as q and the weights are: x 2^k = hi +
@@ -1045,8 +1303,9 @@ __global__ __launch_bounds__(64 * MW * KG, HD == 64 && J == 1 ? 4 : 2) void k_ro
  * What a position holds must not cost the others their precision, the less so
  * where a row does not see it.  So the positions of a group may differ by
  * 2^SPREAD in their largest magnitudes (zeros aside), and so may the groups
- * of V; where they differ by more, the workgroup's rows are computed value by
- * value, as those are that are not finite.
+ * of V; where they differ by more, the workgroup's rows are computed as few
+ * rows are, with f32 products (rows_n), 16 at a time (1,000 rows of 32 heads
+ * of 128: 292 us instead of 53; value by value 19,400).
  *
  * A tile of 32 positions is loaded into registers two tiles ahead, split and
  * stored to one of two LDS buffers one tile ahead (plane [K hi, K lo, V hi,
@@ -1058,6 +1317,23 @@ __global__ __launch_bounds__(64 * MW * KG, HD == 64 && J == 1 ? 4 : 2) void k_ro
  * of 128: 59 us, where the longest sequence's last tiles are most of it. */
 constexpr int KF = 32, SPREAD = 12;
 constexpr int ALL_ZERO = 100;   /* exponent of a group of zeros; no other is larger */
+
+/* The kernel's arguments read again, for what is hardly ever done: kept from
+ * the start of the kernel, they took scalar registers that the loop needs. */
+struct RowsKernelArgs {
+    PromptArgs a;
+    RowsPlan p;
+};
+__device__ inline RowsKernelArgs kernel_args() {
+    struct Words {
+        uint32_t w[sizeof(RowsKernelArgs) / 4];
+    } k;
+    auto at = (const __attribute__((address_space(4))) uint32_t *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm("" : "+s"(at));
+#pragma unroll
+    for (unsigned i = 0; i < sizeof k / 4; i++) k.w[i] = at[i];
+    return __builtin_bit_cast(RowsKernelArgs, k);
+}
 
 /* HD / 4 lanes hold a position: whether each has a bit in m, or none in any */
 template <int HD>
@@ -1076,7 +1352,8 @@ struct SharedF {
     long long where[KG == 2 ? 32 * MW : 1];
 };
 template <int HD, int MW, int KG>
-__device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a, const RowsPlan &p, SharedF<HD, MW, KG> &sh) {
+__device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a, const RowsPlan &p, SharedF<HD, MW, KG> &sh,
+                                                             SharedN<HD, MW * KG> &shn) {
     constexpr int RB = HD * 2, PLANE = KF * RB;
     constexpr int UNITS = 8 / MW;                    /* groups a wave loads: K 0 .. 3, V 4 .. 7 */
     constexpr int LR = 256 / HD, NL = 8 / LR;        /* rows a load of the wave covers, loads a group */
@@ -1277,7 +1554,7 @@ __device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a
             h8 ph[2], pl[2];
 #pragma unroll
             for (int g = 0; g < 4; g++) {
-                const int d = min(ve[g] - un, SPREAD);   /* more: zeros, or the rows are done again */
+                const int d = min(ve[g] - un, SPREAD);   /* more: zeros, or rows_n does the rows again */
                 const float shg = sh - (float)d;
                 float sum[2] = {0.f, 0.f};
 #pragma unroll
@@ -1307,13 +1584,26 @@ __device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a
         bar_lds();
     }
     if (lane == 0) range[wave][0] = least, range[wave][1] = most;
+    __syncthreads();
+    for (int v = 0; v < MW * KG; v++) least = min(least, range[v][0]), most = max(most, range[v][1]);
+    if (most - least > SPREAD) {
+        const RowsKernelArgs k = kernel_args();
+        Work v;
+        if (!find_work<32 * MW>(k.a, k.p, k.a.n_heads / k.a.n_kv, v)) return;
+        for (int from = 0; from < 32 * MW; from += MN) {
+            int i, j;
+            v.row(from, k.a.n_heads / k.a.n_kv, i, j);
+            if (i >= v.sq.n) return;
+            __syncthreads();
+            rows_n<float, HD, MW * KG>(k.a, k.p, v, from, shn);
+        }
+        return;
+    }
     l = other_half_sum(l);
     if (KG == 2 && w.hi - w.lo > KF) merge_groups<HD, MW>((float *)bufs, wave, lane, mx, l, U, o);
     else __syncthreads();   /* one group, or the second had no tile: all are done with the tiles */
     constexpr int STRIDE = 64 * (HD / 2 + 3) * 4;   /* a wave's share of merge_groups' room */
     if (group == 0) {
-        for (int v = 0; v < MW * KG; v++) least = min(least, range[v][0]), most = max(most, range[v][1]);
-        if (most - least > SPREAD) l = NAN;
         const uint32_t bad = write_rows<HD, true>(a, p, w, x, lane, mx, l, U, o, KG == 2 ? (uint8_t *)bufs + wave * STRIDE : nullptr,
                                                   where + (KG == 2 ? 32 * wave : 0));
         if (lane == 0) bad_rows[wave] = bad;
@@ -1330,265 +1620,11 @@ __device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a
 
 template <int HD, int MW, int KG>
 __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPlan p) {
-    __shared__ SharedF<HD, MW, KG> sh;
-    rows_f<HD, MW, KG>(a, p, sh);
-}
-
-/* ---- few rows: positions over the waves ----
- *
- * A workgroup of four waves takes 16 m-rows; a wave walks tiles of 16
- * positions (every fourth) with K and V straight from the cache into the
- * operands, no LDS and no barrier until the end, where the four waves' sums
- * meet.  S^T[position][m-row] on 16x16 MFMAs: D lane l holds m-row l % 16,
- * positions 4 (l / 16) + v, which is B of the second product over positions
- * 4 (l / 16) + i as it lies.  The second product is f32 (16x16x4) for both
- * cache types: V converts exactly, the weights are not rounded, and the rate
- * is above what the cache's bytes allow.  The first is f32 for an f32 cache
- * and two f16 products (q in two planes) for an f16 one.
- *
- * Bound: the cache's bytes.  One row of each of 32 sequences of 2,091 positions
- * on average, 4 KV heads of 128, f16: 137 MB in 32 us, 4.3 TB/s; at 1,500
- * positions and less the chain of a workgroup (find its work 1 us, q and the
- * first tile 3, merge and write 3). */
-typedef float v4f __attribute__((ext_vector_type(4)));
-constexpr int MN = 16;
-
-template <typename T, int HD>
-struct NarrowK {   /* float: K pieces of 4 dims, dims 16 j + 4 kq + e in MFMA (j, e) */
-    static constexpr int J = HD / 16;
-    v4f q[J];
-    u32x4 k[J];
-    __device__ inline float load_q(const PromptArgs &a, const Lane &x, int kq) {
-        const float *src = a.q + (size_t)x.r * a.q_stride + (size_t)x.h * a.head_dim;
-#pragma unroll
-        for (int j = 0; j < J; j++) {
-            const int d = 16 * j + 4 * kq;
-            q[j] = x.live && d < a.head_dim ? (v4f)*(const f4u *)(src + d) : v4f{0.f, 0.f, 0.f, 0.f};
-        }
-        return LOG2E / sqrtf((float)a.head_dim);
-    }
-    __device__ inline void load_k(Buf kd, uint32_t row, int kq, int hd) {
-#pragma unroll
-        for (int j = 0; j < J; j++) k[j] = ld16(kd, 16 * j + 4 * kq < hd ? row + 64u * j + 16u * (uint32_t)kq : 0x7FFFFF00u);
-    }
-    __device__ inline v4f scores() const {
-        v4f s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;   /* two chains */
-#pragma unroll
-        for (int j = 0; j < J; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float y = __uint_as_float(k[j][e]);
-                if (e & 1) s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(y, q[j][e], s1, 0, 0, 0);
-                else s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(y, q[j][e], s0, 0, 0, 0);
-            }
-        return s0 + s1;
-    }
-};
-template <int HD>
-struct NarrowK<_Float16, HD> {   /* K pieces of 8 dims, dims 32 j + 8 kq + e in MFMA j */
-    static constexpr int J = HD / 32;
-    h8 qh[J], ql[J];
-    u32x4 k[J];
-    __device__ inline float load_q(const PromptArgs &a, const Lane &x, int kq) {
-        const float *src = a.q + (size_t)x.r * a.q_stride + (size_t)x.h * a.head_dim;
-        f4 u[J], v[J];
-        float big = 0.f;
-#pragma unroll
-        for (int j = 0; j < J; j++) {
-            const int d = 32 * j + 8 * kq;
-            const bool on = x.live && d < a.head_dim;
-            u[j] = on ? (f4)*(const f4u *)(src + d) : f4{0.f, 0.f, 0.f, 0.f};
-            v[j] = on ? (f4)*(const f4u *)(src + d + 4) : f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int e = 0; e < 4; e++) big = fmaxf(big, fmaxf(fabsf(u[j][e]), fabsf(v[j][e])));
-        }
-        big = fmaxf(big, __shfl_xor(big, 16, 64));
-        const int ex = scale_exp(fmaxf(big, __shfl_xor(big, 32, 64)));
-#pragma unroll
-        for (int j = 0; j < J; j++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float z = __builtin_amdgcn_ldexpf(e < 4 ? u[j][e & 3] : v[j][e & 3], ex);
-                const _Float16 hi = (_Float16)z;
-                qh[j][e] = hi;
-                ql[j][e] = (_Float16)(z - (float)hi);
-            }
-        return __builtin_amdgcn_ldexpf(LOG2E / sqrtf((float)a.head_dim), -ex);
-    }
-    __device__ inline void load_k(Buf kd, uint32_t row, int kq, int hd) {
-#pragma unroll
-        for (int j = 0; j < J; j++) k[j] = ld16(kd, 32 * j + 8 * kq < hd ? row + 64u * j + 16u * (uint32_t)kq : 0x7FFFFF00u);
-    }
-    __device__ inline v4f scores() const {
-        v4f s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
-#pragma unroll
-        for (int j = 0; j < J; j++) {
-            const h8 y = __builtin_bit_cast(h8, k[j]);
-            s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, qh[j], s0, 0, 0, 0);
-            s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, ql[j], s1, 0, 0, 0);
-        }
-        return s0 + s1;
-    }
-};
-
-/* V of a lane's position: HD / 16 dims; dim(i, t) is the t-th of lane i % 16 */
-template <typename T, int HD>
-struct NarrowV {
-    static constexpr int N = HD / 16;
-    u32x4 v[N / 4];
-    static __device__ inline int dim(int i, int t) { return 64 * (t >> 2) + 4 * i + (t & 3); }
-    __device__ inline void load(Buf vd, uint32_t row, int i, int hd) {
-#pragma unroll
-        for (int n = 0; n < N / 4; n++) v[n] = ld16(vd, 64 * n + 4 * i < hd ? row + 256u * n + 16u * (uint32_t)i : 0x7FFFFF00u);
-    }
-    __device__ inline float at(int t) const { return __uint_as_float(v[t >> 2][t & 3]); }
-};
-template <int HD>
-struct NarrowV<_Float16, HD> {
-    static constexpr int N = HD / 16;
-    typedef _Float16 H __attribute__((ext_vector_type(N)));
-    H v;
-    static __device__ inline int dim(int i, int t) { return N * i + t; }
-    __device__ inline void load(Buf vd, uint32_t row, int i, int hd) {
-        const uint32_t at = N * i < hd ? row + 2u * N * (uint32_t)i : 0x7FFFFF00u;
-        if constexpr (N == 8) v = __builtin_bit_cast(H, ld16(vd, at));
-        else v = __builtin_bit_cast(H, ld8(vd, at));
-    }
-    __device__ inline float at(int t) const { return (float)v[t]; }
-};
-
-template <int HD, int NW>
-struct SharedN {
-    __attribute__((aligned(16))) float mo[NW][MN][HD];
-    float mm[NW][MN], ml[NW][MN];
-    uint32_t bad_rows;
-};
-template <typename T, int HD, int NW>
-__device__ inline __attribute__((always_inline)) void rows_n(const PromptArgs &a, const RowsPlan &p, SharedN<HD, NW> &sh) {
-    constexpr int N = HD / 16;
-    auto &mo = sh.mo;
-    auto &mm = sh.mm;
-    auto &ml = sh.ml;
-    auto &bad_rows = sh.bad_rows;
-    const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
-    Work w;
-    if (!find_work<MN>(a, p, ratio, w)) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int c16 = lane & 15, kq = lane >> 4;
-    const Lane x = lane_rows(a, w, 0, c16, 16, ratio);
-    if (tid == 0) bad_rows = 0;
-
-    const uint32_t rb = (uint32_t)hd * (uint32_t)sizeof(T);
-    const Buf kd = make_buf_uniform(region<T>(a, w, a.kv_k, a.pre_k), (uint32_t)w.hi * rb);
-    const Buf vd = make_buf_uniform(region<T>(a, w, a.kv_v, a.pre_v), (uint32_t)w.hi * rb);
-    NarrowK<T, HD> K;
-    NarrowV<T, HD> V[4];
-    auto load_v = [&](int t0) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) V[i].load(vd, (uint32_t)(t0 + 4 * kq + i) * rb, c16, hd);
-    };
-    int t = w.lo + 16 * wave;
-    K.load_k(kd, (uint32_t)(t + c16) * rb, kq, hd);   /* past the span: zeros, no memory access */
-    load_v(t);
-    const float c = K.load_q(a, x, kq);
-    float mx = -INFINITY, l = 0.f;
-    v4f o[N];
-#pragma unroll
-    for (int n = 0; n < N; n++) o[n] = v4f{0.f, 0.f, 0.f, 0.f};
-    for (; t < w.hi; t += 16 * NW) {
-        v4f s = K.scores();
-        K.load_k(kd, (uint32_t)(t + 16 * NW + c16) * rb, kq, hd);
-        const bool masked = t + 15 > x.all_hi || t < x.all_lo;   /* uniform */
-        float top = -INFINITY;
-#pragma unroll
-        for (int v = 0; v < 4; v++) {
-            const int pos = t + 4 * kq + v;
-            if (masked) s[v] = pos <= x.last && pos >= x.first ? s[v] : -INFINITY;
-            top = fmaxf(top, s[v]);
-        }
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64)) * c;
-        const float mn = fmaxf(mx, top), base = mn == -INFINITY ? 0.f : mn;
-        if (__any(mn > mx)) {
-            const float alpha = __builtin_amdgcn_exp2f(mx - base);
-            l *= alpha;
-#pragma unroll
-            for (int n = 0; n < N; n++) o[n] *= alpha;
-        }
-        mx = mn;
-#pragma unroll
-        for (int v = 0; v < 4; v++) {
-            s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], c, -base));
-            l += s[v];
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int n = 0; n < N; n++) o[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(V[i].at(n), s[i], o[n], 0, 0, 0);
-        load_v(t + 16 * NW);
-    }
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-#pragma unroll
-    for (int v = 0; v < 4; v++)
-#pragma unroll
-        for (int n = 0; n < N; n += 4) {
-            const int d = NarrowV<T, HD>::dim(4 * kq + v, n);   /* the next three follow */
-            *(f4 *)&mo[wave][c16][d] = f4{o[n][v], o[n + 1][v], o[n + 2][v], o[n + 3][v]};
-        }
-    if (kq == 0) mm[wave][c16] = mx, ml[wave][c16] = l;
-    __syncthreads();
-    /* the waves' sums as one, in wave order: 16 threads a row, HD / 16 dims each */
-    const bool on = tid < 16 * MN;
-    const int row = (tid >> 4) & (MN - 1), d0 = (tid & 15) * N;
-    const Lane y = lane_rows(a, w, 0, row, 16, ratio);
-    float M = mm[0][row];
-#pragma unroll
-    for (int q = 1; q < NW; q++) M = fmaxf(M, mm[q][row]);
-    const float base = M == -INFINITY ? 0.f : M;
-    float L = 0.f, r[N];
-#pragma unroll
-    for (int n = 0; n < N; n++) r[n] = 0.f;
-#pragma unroll
-    for (int q = 0; q < NW; q++) {
-        const float e = __builtin_amdgcn_exp2f(mm[q][row] - base);
-        L = fmaf(ml[q][row], e, L);
-#pragma unroll
-        for (int n = 0; n < N; n++) r[n] = fmaf(mo[q][row][d0 + n], e, r[n]);
-    }
-    float nan = L * 0.f;
-#pragma unroll
-    for (int n = 0; n < N; n++) nan = fmaf(r[n], 0.f, nan);
-    if (on && y.live && !(nan == 0.f)) atomicOr(&bad_rows, 1u << row);
-    __syncthreads();
-    const uint32_t bad = bad_rows;
-    if (on && y.live && !((bad >> row) & 1u) && d0 < hd) {
-        float *dst, f = 1.f;
-        if (p.nrec) {
-            const size_t rec = ((size_t)y.r * a.n_heads + y.h) * p.nrec + w.rec;
-            if (d0 == 0) write_ml(p, w, rec, M, L);
-            dst = p.o + rec * hd + d0;
-        } else {
-            if (a.sinks) {
-                const float sk = a.sinks[y.h] * LOG2E, mn = fmaxf(M, sk), b2 = mn == -INFINITY ? 0.f : mn;
-                f = exp2f(M - b2);
-                L = L * f + exp2f(sk - b2);
-            }
-            f /= L;
-            dst = a.out + (size_t)y.r * a.out_stride + (size_t)y.h * hd + d0;
-        }
-        if (!p.nrec || M > -INFINITY) {
-#pragma unroll
-            for (int n = 0; n < N; n += 4) *(f4u *)(dst + n) = f4{r[n] * f, r[n + 1] * f, r[n + 2] * f, r[n + 3] * f};
-        }
-    }
-    for (uint32_t z = bad; z; z &= z - 1) slow_row<T>(a, p, w, __builtin_ctz(z), ratio, &mo[0][0][0]);
-}
-
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
-    __shared__ SharedN<HD, 4> sh;
-    rows_n<T, HD, 4>(a, p, sh);
+    __shared__ union {
+        SharedF<HD, MW, KG> f;
+        SharedN<HD, MW * KG> n;
+    } sh;
+    rows_f<HD, MW, KG>(a, p, sh.f, sh.n);
 }
 
 /* The records of a row and head, and its sink, as one: W waves each, wave g
