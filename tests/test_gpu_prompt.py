@@ -82,6 +82,26 @@ def test_prefix_matches_plain(tg, layout, prefix, lens, past, window, half):
 
 
 @pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("layout", [(64, 8, 64), (32, 4, 128), (40, 1, 16)])
+@pytest.mark.parametrize("prefix,window", [(600, 0), (300, 0), (600, 250)])
+def test_prefix_of_a_batch(tg, layout, prefix, window, half):
+    """One row of each of many sequences behind a prefix, a few of other
+    lengths among them; f32 caches also with positions of very different
+    sizes, in the prefix and in the sequences' own."""
+    nh, nkv, hd = layout
+    lens, past = [1] * 18 + [0, 2, 1], [100 + 7 * i for i in range(20)] + [0]
+    for sizes in ([False] if half else [False, True]):
+        say(f"prefix of a batch {layout} prefix={prefix} window={window} half={half} sizes={sizes}")
+        b = Batch(prefix + nh, nh, nkv, hd, lens, past, half, window=window, sinks=nkv == 4, prefix=prefix, lead=1, tail=1)
+        if sizes:
+            b.pv[:, 3:prefix:40] *= np.float32(2.0 ** -20)
+            b.v[:, :, 5::30] *= np.float32(2.0 ** -20)
+            b.pk[:, 7:prefix:50] *= np.float32(2.0 ** -20)
+        got, was = _run(tg, b)
+        b.check(got, was)
+
+
+@pytest.mark.parametrize("half", [False, True])
 @pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 20, 2 ** 20])
 def test_window_longer_than_any_cache(tg, window, half):
     for lens, past, prefix in (([3, 40], [500, 9], 0), ([2, 1], [5, 70], 300)):

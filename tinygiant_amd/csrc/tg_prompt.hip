@@ -26,6 +26,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "tg_device.hpp"
 #include "tg_prompt.h"
@@ -1627,6 +1628,25 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_rows_f(PromptArgs a, RowsPl
     rows_f<HD, MW, KG>(a, p, sh.f, sh.n);
 }
 
+/* A prefix's tiles of 128 m-rows and the sequences' of 16 in one launch: a CU
+ * takes a workgroup of each, so that the products of the ones, which run at
+ * the power limit, pass while the others wait for their caches. */
+template <typename T, int HD>
+__global__ __launch_bounds__(256, 2) void k_rows_both(PromptArgs a, RowsPlan p) {
+    constexpr bool HALF = sizeof(T) == 2;
+    __shared__ union {
+        std::conditional_t<HALF, SharedH<HD, 4, 1>, SharedF<HD, 4, 1>> wide;
+        SharedN<HD, 4> narrow;
+    } sh;
+    if ((int)blockIdx.x < p.pre_tiles * p.pre_ns * a.n_kv) {
+        if constexpr (HALF) rows_h<HD, 4, 1, 2>(a, p, sh.wide);
+        else rows_f<HD, 4, 1>(a, p, sh.wide, sh.narrow);
+        return;
+    }
+    Work w;
+    if (find_work<MN>(a, p, a.n_heads / a.n_kv, w)) rows_n<T, HD, 4>(a, p, w, 0, sh.narrow);
+}
+
 /* The records of a row and head, and its sink, as one: W waves each, wave g
  * the records g (mod W), G lanes a record (four dims a lane), N records of a
  * lane's loads at a time.  1,536 rows of 25
@@ -1727,6 +1747,7 @@ constexpr int SHAPE_ROWS[] = {16, 128, 128, 128, 256}, SHAPE_THREADS[] = {256, 2
 struct Cut {
     RowsPlan p;
     Shape own, pre;
+    bool both;   /* of different shapes, in one launch */
 };
 /* The shape for m m-rows (a KV head) in `seqs` sequences that see `positions`.
  * 9 rows of 8 heads on narrow and wide: 13.6 and 19.6 us behind 1,000
@@ -1785,6 +1806,13 @@ static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim,
         p.pre_tiles = (int)tiles(k.pre, 1);
         p.pre_unit = unit(k.pre);
         p.pre_ns = spans(k.pre, (long long)p.pre_tiles * n_kv, pre_len, true);
+        /* In us, two launches and one: 48 rows behind 8,000 positions and up to
+         * 500 of their own, 4 KV heads of 128, 44.2 and 33.9 (f16), 55.7 and
+         * 48.4 (f32).  With f32 caches the prefix's part alone is slower in this
+         * form, which shows where it is most of the work: 24 rows behind 20,000
+         * and 30 of their own 56.6 and 68.5. */
+        k.both = k.own == NARROW && k.pre != NARROW && k.pre != TALL &&
+                 (half || 2ll * n_seqs * own_sees >= (long long)p.pre_tiles * pre_len);
     }
     p.nrec = p.cap + p.pre_ns > 1 ? p.cap + p.pre_ns : 0;
     return k;
@@ -1840,7 +1868,11 @@ static void launch_rows(const PromptArgs &a, const Cut &k, bool half, void *scra
     RowsPlan p = k.p;
     p.ml = (float *)scratch;
     p.o = (float *)((uint8_t *)scratch + ml_bytes(p, a.s.rows, a.n_heads));
-    if (p.pre_tiles && k.own != k.pre) {
+    if (k.both) {
+        const dim3 grid((unsigned)((p.items + p.pre_tiles * p.pre_ns) * a.n_kv));
+        if (half) hipLaunchKernelGGL((k_rows_both<_Float16, HD>), grid, dim3(256), 0, st, a, p);
+        else hipLaunchKernelGGL((k_rows_both<float, HD>), grid, dim3(256), 0, st, a, p);
+    } else if (p.pre_tiles && k.own != k.pre) {
         RowsPlan one = p;
         one.items = 0;
         launch_part<HD>(a, one, half, k.pre, st);
