@@ -121,7 +121,7 @@ __device__ inline bool wave_seq_of(const PackedSeqs &p, int r, Seq &q, int &i) {
  * tg_rms_norm's (csrc/libtinygiant.c:680-698), the rotation
  * apply_rope_inplace's (:702-719); an f16 cache gets K and V rounded once, to
  * nearest.  Bound: the bytes.  4,001 rows of 64 + 2 x 8 heads of 64 into an f32
- * cache: 165 MB in 32.9 us, 5.0 TB/s, a large copy's rate; 8 rows 5.6 us, the
+ * cache: 165 MB in 32.9 us, 5.0 TB/s, a large copy's rate; 8 rows 6 us, the
  * launch and two dependent reads. */
 template <bool HALF, int G>
 __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
@@ -1751,7 +1751,8 @@ struct Cut {
 };
 /* The shape for m m-rows (a KV head) in `seqs` sequences that see `positions`.
  * 9 rows of 8 heads on narrow and wide: 13.6 and 19.6 us behind 1,000
- * positions (f32; f16 13.2 and 16.1), 29.0 and 26.6 behind 8,000. */
+ * positions (f32; f16 13.2 and 16.1), 29.0 and 23.7 behind 8,000; 16
+ * sequences of them behind 2,000 92 and 47 (f16 65 and 33). */
 constexpr long long NARROW_WORK = 1 << 18, TALL_WORK = 512 * 4096;
 constexpr int SHORT_BELOW = 512;
 static Shape shape_of(long long m, long long seqs, int n_kv, int positions, bool half) {
