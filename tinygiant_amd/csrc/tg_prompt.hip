@@ -1304,9 +1304,10 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
  * What a position holds must not cost the others their precision, the less so
  * where a row does not see it.  So the positions of a group may differ by
  * 2^SPREAD in their largest magnitudes (zeros aside), and so may the groups
- * of V; where they differ by more, the workgroup's rows are computed as few
- * rows are, with f32 products (rows_n), 16 at a time (1,000 rows of 32 heads
- * of 128: 292 us instead of 53; value by value 19,400).
+ * of V; where they differ by more, or a group that is not all zeros lies below
+ * 2^-85, the workgroup's rows are computed as few rows are, with f32 products
+ * (rows_n), 16 at a time (1,000 rows of 32 heads of 128: 292 us instead of 53;
+ * value by value 19,400).
  *
  * A tile of 32 positions is loaded into registers two tiles ahead, split and
  * stored to one of two LDS buffers one tile ahead (plane [K hi, K lo, V hi,
@@ -1317,7 +1318,11 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
  * products, 77% of a large f16 product's rate; 2,020 packed rows of 32 heads
  * of 128: 59 us, where the longest sequence's last tiles are most of it. */
 constexpr int KF = 32, SPREAD = 12;
-constexpr int ALL_ZERO = 100;   /* exponent of a group of zeros; no other is larger */
+constexpr int ALL_ZERO = 100;   /* exponent of a group of zeros; the others' is less */
+/* scale_exp of a group's largest magnitude, as its word; a word below 42 << 23,
+ * less one step, is below 2^-85 and its exponent would not be */
+__device__ inline int group_exp(uint32_t bits) { return 141 - (int)(bits >> 23); }
+constexpr uint32_t TOO_LOW = ((uint32_t)(142 - ALL_ZERO) << 23) - 1u;
 
 /* The kernel's arguments read again, for what is hardly ever done: kept from
  * the start of the kernel, they took scalar registers that the loop needs. */
@@ -1392,7 +1397,11 @@ __device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a
         }
     };
     const uint64_t padding = __ballot(ldim >= hd);
-    int least = ALL_ZERO, most = -2 * ALL_ZERO;   /* exponents of the wave's groups of V; 1000: a group is too wide */
+    /* Of the wave's groups the least magnitude but zeros, less one step (zeros
+     * become the largest word), and V's largest; 0: a group that no scale serves */
+    uint32_t lowest[UNITS], highest = 0;
+#pragma unroll
+    for (int u = 0; u < UNITS; u++) lowest[u] = ~0u;
     auto split_tile = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < UNITS; u++) {
@@ -1420,7 +1429,7 @@ __device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a
                 }
                 bits = wave_umax(fin);
             }
-            const int ex = min(141 - (int)(bits >> 23), ALL_ZERO);   /* scale_exp's */
+            const int ex = min(group_exp(bits), ALL_ZERO);
             /* every position comes near the largest: mostly in each lane's
              * share of each, else it takes one lane of a position, or zeros */
             const float near = __uint_as_float(bits > ((uint32_t)SPREAD << 23) ? bits - ((uint32_t)SPREAD << 23) : 0u);
@@ -1431,9 +1440,10 @@ __device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a
                 bool narrow = true;
 #pragma unroll
                 for (int j = 0; j < NL; j++) narrow = narrow && every_row<HD>(__ballot(top[j] >= near), __ballot(top[j] > 0.f));
-                if (!narrow) most = 1000;
+                if (!narrow) lowest[u] = 0;
             }
-            if (g >= 4 && ex < ALL_ZERO) least = min(least, ex), most = max(most, ex);
+            lowest[u] = min(lowest[u], bits - 1u);
+            if (u == UNITS - 1) highest = max(highest, bits);
             const float f = __uint_as_float((uint32_t)(ex + 127) << 23);
             if (lane == 0) exps[b][g] = ex;
 #pragma unroll
@@ -1584,6 +1594,13 @@ __device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a
         if (!early && more) next_tile(t, b ^ 1);
         bar_lds();
     }
+    int least = ALL_ZERO, most = -2 * ALL_ZERO;   /* exponents of the wave's groups of V; 1000: rows_n's rows */
+    if (UNITS == 2 || mwave >= 4) {
+        if (highest) least = group_exp(highest), most = group_exp(lowest[UNITS - 1] + 1u);
+    }
+#pragma unroll
+    for (int u = 0; u < UNITS; u++)
+        if (lowest[u] < TOO_LOW) most = 1000;
     if (lane == 0) range[wave][0] = least, range[wave][1] = most;
     __syncthreads();
     for (int v = 0; v < MW * KG; v++) least = min(least, range[v][0]), most = max(most, range[v][1]);
