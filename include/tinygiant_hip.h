@@ -306,7 +306,11 @@ void tg_hip_kv_append_dev(const float *q_dev, const float *k_dev, const float *v
  * 2^-85 (zeros aside), rows are computed again with f32 products: as exact,
  * but five to six times slower.
  * scratch_dev holds tg_hip_attention_prompt_scratch_bytes(...) bytes
- * (prefix_len 0), 16-byte aligned; it may be NULL where that is 0. */
+ * (prefix_len 0), 16-byte aligned; it may be NULL where that is 0.  The size
+ * is enough for every call of at most as many rows, sequences, positions
+ * (kv_max) and prefix positions, of either cache type and any window, with
+ * these heads: one allocation for a program's largest sizes serves all its
+ * calls.  (Of two calls the one of fewer rows may need more.) */
 void tg_hip_attention_prompt_dev(const float *q_dev, int q_stride, int kv_type, const void *kv_k_dev,
                                  const void *kv_v_dev, int n_slots, int kv_max, const int32_t *cu_rows_dev,
                                  const int32_t *kv_len_dev, const int32_t *slots_dev, int n_seqs, int n_rows, int window,

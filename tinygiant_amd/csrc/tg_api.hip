@@ -1572,7 +1572,6 @@ static void attention_rows(const char *who, const float *q_dev, int q_stride, in
         set_err("%s: out over q needs the same stride", who);
         return;
     }
-    ensure_init();
     PromptArgs a = {};
     a.q = q_dev, a.q_stride = q_stride;
     a.kv_k = kv_k_dev, a.kv_v = kv_v_dev;
@@ -1582,12 +1581,14 @@ static void attention_rows(const char *who, const float *q_dev, int q_stride, in
     a.sinks = sinks_dev;
     a.n_heads = n_heads, a.n_kv = n_kv_heads, a.head_dim = head_dim;
     a.out = out_dev, a.out_stride = out_stride;
-    const hipError_t before = hipPeekAtLastError();
-    const size_t need = launch_attention_rows(a, kv_type == TG_KV_F16, scratch_dev, stream ? (hipStream_t)stream : g.st);
-    if (need) {
+    const size_t need = attention_rows_need(a, kv_type == TG_KV_F16);
+    if (need && (!scratch_dev || ((uintptr_t)scratch_dev & 15))) {
         set_err("%s: needs %zu bytes of 16-byte aligned scratch", who, need);
         return;
     }
+    ensure_init();
+    const hipError_t before = hipPeekAtLastError();
+    launch_attention_rows(a, kv_type == TG_KV_F16, scratch_dev, stream ? (hipStream_t)stream : g.st);
     check_launch(who, before);
 }
 

@@ -61,9 +61,10 @@ struct PromptArgs {
     float *out;
     int out_stride;
 };
-/* 0, or the scratch bytes that are needed where `scratch` is null or not
- * 16-byte aligned (nothing is launched then) */
-size_t launch_attention_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st);
+/* scratch: attention_rows_need(a, half) bytes, 16-byte aligned */
+void launch_attention_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st);
+size_t attention_rows_need(const PromptArgs &a, bool half);
+/* enough for every call of at most these sizes, of any cache type and window */
 size_t attention_rows_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len);
 
 }  // namespace tg

@@ -1778,11 +1778,11 @@ static Shape shape_of(long long m, long long seqs, int n_kv, int positions, bool
     if (!half && m / 256 * n_kv * positions >= TALL_WORK) return TALL;
     return m / 128 * n_kv > 512 ? FULL : WIDE;
 }
-static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len, int window,
-                    bool half, const Shape *own) {
+static Cut rows_cut(const PromptArgs &a, bool half) {
     Cut k = {};
     RowsPlan &p = k.p;
-    const int ratio = n_heads / n_kv;
+    const int n_rows = a.s.rows, n_seqs = a.s.n, n_kv = a.n_kv, head_dim = a.head_dim, kv_max = a.s.kv_max;
+    const int pre_len = a.pre_len, window = a.window, ratio = a.n_heads / n_kv;
     const long long m = (long long)n_rows * ratio;
     /* Spans of a tile at `positions`: us(n) = time of a span + what the
      * records of n spans take to write and read (+ the combine's launch,
@@ -1805,7 +1805,7 @@ static Cut rows_cut(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim,
     };
     auto tiles = [&](Shape s, long long seqs) { return std::max((m + SHAPE_ROWS[s] - 1) / SHAPE_ROWS[s], seqs); };
     auto sees = [&](int rows) { return window > 0 ? (int)std::min<long long>(kv_max, (long long)window + rows / ratio + 1) : kv_max; };
-    k.own = own ? *own : shape_of(m, n_seqs, n_kv, sees(128), half);
+    k.own = shape_of(m, n_seqs, n_kv, sees(128), half);
     const int own_sees = sees(SHAPE_ROWS[k.own]);
     const long long own_tiles = tiles(k.own, n_seqs);
     p.cap = spans(k.own, own_tiles * n_kv, own_sees, pre_len > 0);
@@ -1844,21 +1844,22 @@ static size_t scratch_bytes(const RowsPlan &p, int n_rows, int n_heads, int head
     return p.nrec ? ml_bytes(p, n_rows, n_heads) + (size_t)n_rows * n_heads * p.nrec * head_dim * 4 : 0;
 }
 
-/* For either cache type and any window: with one shape, a window only takes
- * spans away (the best count rises with the positions, and so do its bounds);
- * so the most over the shapes that some window leads to. */
+/* For every call of at most these sizes, so that a program's one allocation
+ * serves a prompt and the decode steps behind it: fewer rows are cut into more
+ * spans, and what a call needs does not rise with its rows.  Tiles of a shape
+ * are cut only while their spans, with those of the other tiles, are at most
+ * the workgroups that run at once; of several sequences, four times as many.  So
+ * the m-rows times their spans are at most the m-rows of so many tiles. */
 size_t attention_rows_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max, int pre_len) {
-    const long long m = (long long)n_rows * (n_heads / n_kv), tall = m / 256 * n_kv;
-    /* the largest number of positions for each */
-    const long long ends[] = {kv_max, NARROW_WORK / m, SHORT_BELOW - 1, tall ? (TALL_WORK - 1) / tall : kv_max};
-    size_t most = 0;
-    for (int half = 0; half < 2; half++)
-        for (const long long e : ends) {
-            const Shape s = shape_of(m, n_seqs, n_kv, (int)std::min<long long>(e, kv_max), half);
-            const Cut k = rows_cut(n_rows, n_seqs, n_heads, n_kv, head_dim, kv_max, pre_len, 0, half, &s);
-            most = std::max(most, scratch_bytes(k.p, n_rows, n_heads, head_dim));
-        }
-    return most;
+    const long long m = (long long)n_rows * (n_heads / n_kv), row_heads = (long long)n_rows * n_heads;
+    auto cut = [&](int positions, int times) {   /* records of a part that is cut */
+        const long long spans = std::min(64, (positions + 63) / 64);
+        const bool tall = m / 256 * n_kv * positions >= TALL_WORK;
+        return spans == 1 ? 0 : std::min(row_heads * spans, (m <= 16 ? 16ll * 512 : tall ? 256ll * 256 : 128ll * 256) * times);
+    };
+    long long records = cut(kv_max, n_seqs > 1 ? 4 : 1);
+    if (pre_len) records = std::max(records, row_heads) + std::max(cut(pre_len, 1), row_heads);
+    return records ? (size_t)records * (16 + 4 * (size_t)head_dim) + 256 : 0;
 }
 
 /* the workgroups of one part, or of both */
@@ -1908,14 +1909,14 @@ static void launch_rows(const PromptArgs &a, const Cut &k, bool half, void *scra
     else hipLaunchKernelGGL((k_rows_combine<1, HD / 4, 1>), four, dim3(256), 0, st, a, p);
 }
 
-size_t launch_attention_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st) {
-    const Cut k = rows_cut(a.s.rows, a.s.n, a.n_heads, a.n_kv, a.head_dim, a.s.kv_max, a.pre_len, a.window, half,
-                           nullptr);
-    const size_t need = scratch_bytes(k.p, a.s.rows, a.n_heads, a.head_dim);
-    if (need && (!scratch || ((uintptr_t)scratch & 15))) return need;
+size_t attention_rows_need(const PromptArgs &a, bool half) {
+    return scratch_bytes(rows_cut(a, half).p, a.s.rows, a.n_heads, a.head_dim);
+}
+
+void launch_attention_rows(const PromptArgs &a, bool half, void *scratch, hipStream_t st) {
+    const Cut k = rows_cut(a, half);
     if (a.head_dim > 64) launch_rows<128>(a, k, half, scratch, st);
     else launch_rows<64>(a, k, half, scratch, st);
-    return 0;
 }
 
 }  // namespace tg
