@@ -6,7 +6,7 @@ import sys
 import numpy as np
 import pytest
 
-from tests._packed import EPS, Dev
+from tests._packed import EPS, Batch, Dev
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +101,73 @@ def test_tiny_caches(tg, hd, shape):
         q, k = q * np.float32(2.0 ** power), k * np.float32(2.0 ** -power)
         say(f"tiny caches {shape} hd={hd} K 2^-{power}")
         _check(_attend(tg, q, k, v), q, k, v)
+
+
+def _one_position(q, k, at=20):
+    """Nearly all of the weight on one position, for the rows that see it."""
+    q[:, :, 1], k[:, at, 1] = 4.0, 8.0 * q.shape[-1] ** 0.5
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_channels_of_different_sizes(tg, hd, shape):
+    """One channel far above the others at every position: in K, where q has a
+    zero for it, and in V, where each channel is an output of its own; and one
+    far below the others.  A little: the matrix units' path.  A lot: f32."""
+    for power in (10, 30, 80):
+        q, k, v = _inputs(hd + shape[2], shape, hd)
+        q[:, :, 7] = 0
+        k[:, :, 7] *= np.float32(2.0 ** power)
+        say(f"channels {shape} hd={hd} K 2^{power}")
+        say(f"  worst error / tolerance {_check(_attend(tg, q, k, v), q, k, v, weights=power == 10):.3f}")
+    for power in (10, 30, 80, -10, -20, -60):
+        q, k, v = _inputs(hd + shape[2], shape, hd)
+        _one_position(q, k)
+        v[:, :, 7] *= np.float32(2.0 ** power)
+        say(f"channels {shape} hd={hd} V 2^{power}")
+        say(f"  worst error / tolerance {_check(_attend(tg, q, k, v), q, k, v, weights=abs(power) == 10):.3f}")
+
+
+@pytest.mark.parametrize("hd", [64, 72, 128])
+def test_channels_of_zeros(tg, hd):
+    """Channels that are zeros throughout, and in some groups only, are none
+    of different sizes; beside infinities that no row sees, channels still are."""
+    shape = (8, 2, 130, 300)
+    q, k, v = _inputs(hd, shape, hd)
+    _one_position(q, k)
+    k[:, :, 9], v[:, :, 9] = 0, 0
+    k[:, 40:200, 11], v[:, 64:72, 12:15] = 0, 0
+    say(f"channels of zeros hd={hd}")
+    got = _attend(tg, q, k, v)
+    _check(got, q, k, v)
+    assert np.all(got[:, :, 9] == 0)
+    q, k, v = _inputs(hd, shape, hd)
+    _one_position(q, k)
+    v[:, :, 7] *= np.float32(2.0 ** -20)
+    ref = v.copy()
+    k[:, -1], v[:, -1] = np.inf, np.nan   # the last row's alone
+    say("  beside infinities")
+    got = _attend(tg, q, k, v)
+    assert np.isnan(got[-1]).all()
+    _check(got[:-1], q[:-1], k[:, :-1], ref[:, :-1], weights=False)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_channels_of_few_positions(tg, hd):
+    """A shared prefix of fewer positions than share a scale.  A channel of V
+    that is 2^-30 throughout is the same computation, times that."""
+    for prefix in (1, 5, 7, 13):
+        say(f"channels of a prefix of {prefix} hd={hd}")
+        b = Batch(prefix + hd, 8, 2, hd, [1] * 70, [i % 3 for i in range(70)], False, prefix=prefix)
+        ref, tol = b.attend()
+        for t in (b.v, b.pv):
+            t[..., 7] *= np.float32(2.0 ** -30)
+        dev = Dev(tg)
+        tg.lib().tg_hip_clear_error()
+        out, _ = b.call(dev)
+        tg.lib().tg_hip_synchronize()
+        assert tg.last_error() == "", tg.last_error()
+        got = dev.read(out, b.q).astype(np.float64)
+        dev.free()
+        got.reshape(b.rows, 8, hd)[:, :, 7] *= 2.0 ** 30
+        assert np.all(np.abs(got - ref) <= tol), float((np.abs(got - ref) / tol).max())

@@ -1302,9 +1302,13 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
  * take 2^(U - k), which is part of their exponent and taken back in their sum.
  *
  * What a position holds must not cost the others their precision, the less so
- * where a row does not see it.  So the positions of a group may differ by
- * 2^SPREAD in their largest magnitudes (zeros aside), and so may the groups
- * of V; where they differ by more, or a group that is not all zeros lies below
+ * where a row does not see it, and a channel that is large throughout not
+ * that of the others, which are outputs of their own (V) or all that counts
+ * where q is small in it (K).  So the positions of a group may differ by
+ * 2^SPREAD in their largest magnitudes (zeros aside), its channels too (then a
+ * value is off by 2^-27 of its channel's largest in the group at most; fewer
+ * positions than 8, the last of a span, have small values by chance and are not
+ * asked, unless they are all there is), and so may the groups of V; where they differ by more, or a group that is not all zeros lies below
  * 2^-85, the workgroup's rows are computed as few rows are, with f32 products
  * (rows_n), 16 at a time (1,000 rows of 32 heads of 128: 292 us instead of 53;
  * value by value 19,400).
@@ -1341,12 +1345,24 @@ __device__ inline RowsKernelArgs kernel_args() {
     return __builtin_bit_cast(RowsKernelArgs, k);
 }
 
-/* HD / 4 lanes hold a position: whether each has a bit in m, or none in any */
+/* the largest of the HD / 4 lanes that hold a position, and of the lanes HD / 4
+ * apart, which hold the same dims */
+__device__ inline uint32_t swap_umax(uint32_t v, bool rows) {
+    const auto r = rows ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max((uint32_t)r[0], (uint32_t)r[1]);
+}
 template <int HD>
-__device__ inline bool every_row(uint64_t m, uint64_t any) {
-    if (HD == 128) return ((uint32_t)m || !(uint32_t)any) && ((uint32_t)(m >> 32) || !(uint32_t)(any >> 32));
-    constexpr uint64_t L = 0x7FFF7FFF7FFF7FFFull;   /* 16-bit fields: the top bit of those that are not 0 */
-    return ((((m & L) + L) | m | ~(((any & L) + L) | any)) | L) == ~0ull;
+__device__ inline uint32_t row_umax(uint32_t v) {
+    v = max(v, (uint32_t)dpp_i<0xB1>((int)v));
+    v = max(v, (uint32_t)dpp_i<0x4E>((int)v));
+    v = max(v, (uint32_t)dpp_i<0x141>((int)v));
+    v = max(v, (uint32_t)dpp_i<0x140>((int)v));
+    return HD == 128 ? swap_umax(v, true) : v;
+}
+template <int HD>
+__device__ inline uint32_t dim_umax(uint32_t v) {
+    v = swap_umax(v, false);
+    return HD == 64 ? swap_umax(v, true) : v;
 }
 
 template <int HD, int MW, int KG>
@@ -1402,45 +1418,64 @@ __device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a
     uint32_t lowest[UNITS], highest = 0;
 #pragma unroll
     for (int u = 0; u < UNITS; u++) lowest[u] = ~0u;
+    bool few = false;   /* some group's channels differ, perhaps one of less than 8 positions */
     auto split_tile = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < UNITS; u++) {
             const int g = u * MW + mwave;
-            float top[NL], big = 0.f;
+            float top[NL], col[4] = {0.f, 0.f, 0.f, 0.f}, big = 0.f;   /* of the lane's positions, of its dims */
 #pragma unroll
             for (int j = 0; j < NL; j++) {
                 const f4 y = __builtin_bit_cast(f4, raw[u][j]);
                 top[j] = max_nan(max_nan(max_nan(fabsf(y[0]), fabsf(y[1])), fabsf(y[2])), fabsf(y[3]));
                 big = max_nan(big, top[j]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) col[e] = max_nan(col[e], fabsf(y[e]));
             }
             uint32_t bits = wave_umax(__float_as_uint(big));
-            if (bits >= 0x7F800000u) {   /* uniform: the largest of the finite ones */
-                uint32_t fin = 0;
+            if (__builtin_expect(bits >= 0x7F800000u, 0)) {   /* uniform: the largest of the finite ones */
+                uint32_t fin = 0, of_col[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int j = 0; j < NL; j++) {
                     uint32_t of_row = 0;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const uint32_t y = raw[u][j][e] & 0x7FFFFFFFu;
-                        of_row = max(of_row, y < 0x7F800000u ? y : 0u);
+                        uint32_t y = raw[u][j][e] & 0x7FFFFFFFu;
+                        y = y < 0x7F800000u ? y : 0u;
+                        of_row = max(of_row, y), of_col[e] = max(of_col[e], y);
                     }
                     top[j] = __uint_as_float(of_row);
                     fin = max(fin, of_row);
                 }
+#pragma unroll
+                for (int e = 0; e < 4; e++) col[e] = __uint_as_float(of_col[e]);
                 bits = wave_umax(fin);
             }
             const int ex = min(group_exp(bits), ALL_ZERO);
-            /* every position comes near the largest: mostly in each lane's
-             * share of each, else it takes one lane of a position, or zeros */
+            /* every position and every channel come near the largest: mostly
+             * in each lane's share of each, else it takes one lane of a position
+             * or channel, or zeros */
             const float near = __uint_as_float(bits > ((uint32_t)SPREAD << 23) ? bits - ((uint32_t)SPREAD << 23) : 0u);
             float low = top[0];
 #pragma unroll
-            for (int j = 1; j < NL; j++) low = fminf(low, top[j]);
-            if ((__ballot(low >= near) | padding) != ~0ull) {
-                bool narrow = true;
+            for (int j = 1; j < NL; j++) low = __builtin_elementwise_minimum(low, top[j]);
 #pragma unroll
-                for (int j = 0; j < NL; j++) narrow = narrow && every_row<HD>(__ballot(top[j] >= near), __ballot(top[j] > 0.f));
-                if (!narrow) lowest[u] = 0;
+            for (int e = 0; e < 4; e++) low = __builtin_elementwise_minimum(low, col[e]);
+            if (__builtin_expect((__ballot(low >= near) | padding) != ~0ull, 0)) {
+                bool row = true, dim = true, there = true;
+#pragma unroll
+                for (int j = 0; j < NL; j++) {
+                    const uint32_t x = row_umax<HD>(__float_as_uint(top[j]));
+                    row = row && (x == 0 || __uint_as_float(x) >= near), there = there && x != 0;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t x = dim_umax<HD>(__float_as_uint(col[e]));
+                    dim = dim && (x == 0 || __uint_as_float(x) >= near);
+                }
+                const bool dims = __all(dim);
+                if (!__all(row) || (!dims && __all(there))) lowest[u] = 0;
+                few = few || !dims;
             }
             lowest[u] = min(lowest[u], bits - 1u);
             if (u == UNITS - 1) highest = max(highest, bits);
@@ -1600,7 +1635,7 @@ __device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a
     }
 #pragma unroll
     for (int u = 0; u < UNITS; u++)
-        if (lowest[u] < TOO_LOW) most = 1000;
+        if (lowest[u] < TOO_LOW || (few && w.hi - w.lo < 8)) most = 1000;
     if (lane == 0) range[wave][0] = least, range[wave][1] = most;
     __syncthreads();
     for (int v = 0; v < MW * KG; v++) least = min(least, range[v][0]), most = max(most, range[v][1]);
