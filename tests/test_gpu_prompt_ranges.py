@@ -171,3 +171,18 @@ def test_channels_of_few_positions(tg, hd):
         dev.free()
         got.reshape(b.rows, 8, hd)[:, :, 7] *= 2.0 ** 30
         assert np.all(np.abs(got - ref) <= tol), float((np.abs(got - ref) / tol).max())
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_powers_of_two_between_queries_and_keys(tg, hd, shape):
+    """A power of two taken from q and given to K changes no bit of the scores,
+    nor of the way they are computed: rows of small queries, whose last tile
+    ends inside a group, are not computed value by value."""
+    q, k, v = _inputs(hd + shape[2], shape, hd)
+    say(f"powers of two {shape} hd={hd}")
+    first = _attend(tg, q, k, v)
+    _check(first, q, k, v)
+    for power in (-60, -20, 20, 45, 60, 80):
+        got = _attend(tg, q * np.float32(2.0 ** -power), k * np.float32(2.0 ** power), v)
+        assert got.tobytes() == first.tobytes(), power

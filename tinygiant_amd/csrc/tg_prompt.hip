@@ -1577,7 +1577,9 @@ __device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a
             float cg[4], top = -INFINITY;
 #pragma unroll
             for (int g = 0; g < 4; g++) {
-                cg[g] = __builtin_amdgcn_ldexpf(c, -ke[g]);
+                /* no further down than a normal value, where every score vanishes: 0 * -inf
+                 * would send the rows of a group of zeros and small q to slow_row */
+                cg[g] = fmaxf(__builtin_amdgcn_ldexpf(c, -ke[g]), 0x1p-126f);
                 top = max_nan(top, max_nan(max_nan(max_nan(s[4 * g], s[4 * g + 1]), s[4 * g + 2]), s[4 * g + 3]) * cg[g]);
             }
             top = other_half_max(top);
