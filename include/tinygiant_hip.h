@@ -265,11 +265,14 @@ size_t tg_hip_attention_scratch_bytes(int embed_dim, int n_heads, int n_kv_heads
  *             n_heads / n_kv_heads integral and <= 64, kv_max <= 2^20,
  *             n_rows <= 2^22, n_seqs <= 2^16, n_rows * n_heads <= 2^25,
  *             n_seqs * n_kv_heads <= 2^20
- *   strides   in floats from row to row, of at least a row's heads and at most
- *             2^21
+ *   strides   in floats from row to row, of at least a row's heads; the
+ *             attention calls' at most 2^21
  * cu_rows, kv_len and slots are device arrays that the host does not see: a
  * sequence whose slot is not below n_slots, or whose rows do not fit kv_max,
  * is left out (its rows of the outputs and the caches stay as they were).
+ * A call is cut for sequences of up to kv_max positions, so one over caches
+ * with room for many more than are in them is right but not as fast as over
+ * caches that fit.
  * n_rows = 0 or n_seqs = 0 does nothing.  A launch that HIP refuses is
  * reported by tg_hip_last_error().  All of it can be captured and replayed;
  * calls that overlap in time need scratch of their own.
@@ -298,8 +301,14 @@ void tg_hip_kv_append_dev(const float *q_dev, const float *k_dev, const float *v
  * chunks behind cached positions, verify passes and batches of one row a
  * sequence are all this call.  out may be q with q's stride.  Values of
  * positions that a row does not see never reach it, infinities and NaN
- * included.  The arithmetic is f32 for both cache types (sums in f32; 16-bit
- * operands of the matrix units only in exact or compensated form).
+ * included.  Sums and the softmax's statistics are f32 for both cache types,
+ * sums of weights times values taken before the division.  Operands of the
+ * matrix units that f16 does not hold are two f16 values, 22 bits: of q, or
+ * 2^-39 of its head's largest magnitude where that is more; of the weights, or
+ * 2^-33 of the row's largest; of K and V of f32 caches, or 2^-39 of the largest
+ * of 8 neighbouring positions.  With values of ordinary spread that is f32's
+ * accuracy; a query with one dimension 2^17 above all that counts in the
+ * others loses bits of these.
  * Rows that come out not finite are computed again value by value: as exact,
  * but many times slower.  Where nearby positions of an f32 cache differ by
  * more than 2^12 in magnitude, or the channels of eight neighbouring positions

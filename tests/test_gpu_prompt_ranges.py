@@ -186,3 +186,28 @@ def test_powers_of_two_between_queries_and_keys(tg, hd, shape):
     for power in (-60, -20, 20, 45, 60, 80):
         got = _attend(tg, q * np.float32(2.0 ** -power), k * np.float32(2.0 ** power), v)
         assert got.tobytes() == first.tobytes(), power
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("lens,past", [([40], [300]), ([2], [300]), ([300], [0])])
+def test_queries_of_different_sizes(tg, lens, past, half):
+    """One dimension of q far above the others, where K is 0: q keeps 2^-39 of
+    its head's largest magnitude, so scores are off by that times the sum of
+    |k|, beside what they are off without it."""
+    for power in (10, 18, 24):
+        say(f"queries {lens} half={half} 2^{power}")
+        b = Batch(power, 8, 2, 64, lens, past, half, q_scale=0.5)
+        q = b.q.reshape(b.rows, 8, 64)
+        b.k[..., 7], q[:, :, 7] = 0, 0
+        ref, tol = b.attend()
+        q[:, :, 7] = 2.0 ** power
+        off = 2.0 ** (power - 39) * np.abs(b.k[b.slots[0], :, :b.lens[0] + b.past[0]].astype(np.float64)).sum(-1).max() / 8
+        tol = tol + 2 * off * np.abs(b.v[b.slots[0], :, :b.lens[0] + b.past[0]].astype(np.float64)).max()
+        dev = Dev(tg)
+        tg.lib().tg_hip_clear_error()
+        out, was = b.call(dev)
+        tg.lib().tg_hip_synchronize()
+        assert tg.last_error() == "", tg.last_error()
+        got = dev.read(out, b.q)
+        dev.free()
+        say(f"  worst error / tolerance {b.check(got, was, (ref, tol)):.3f}")
