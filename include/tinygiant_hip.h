@@ -313,7 +313,7 @@ void tg_hip_kv_append_dev(const float *q_dev, const float *k_dev, const float *v
  * but many times slower.  Where nearby positions of an f32 cache differ by
  * more than 2^12 in magnitude, or the channels of eight neighbouring positions
  * do, or all their values lie below 2^-85 (zeros aside), rows are computed
- * again with f32 products: as exact, but five to six times slower.
+ * again with f32 products: as exact, but about five times slower.
  * scratch_dev holds tg_hip_attention_prompt_scratch_bytes(...) bytes
  * (prefix_len 0), 16-byte aligned; it may be NULL where that is 0.  The size
  * is enough for every call of at most as many rows, sequences, positions

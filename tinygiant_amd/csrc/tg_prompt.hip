@@ -519,8 +519,8 @@ __device__ void slow_row(const PromptArgs &a, const RowsPlan &p, const Work &w, 
  * weights are taken times 2^SHIFT.
  *
  * The reference exponent m follows a row's largest score only when that is
- * more than LAG above it, so most tiles rescale nothing (8192 tokens: 917 us,
- * with m the largest score 939).  SHIFT + LAG stays below f16's largest, 2^16.
+ * more than LAG above it, so most tiles rescale nothing (8,192 tokens: 883 us,
+ * with m the largest score 910).  SHIFT + LAG stays below f16's largest, 2^16.
  *
  * K and V tiles of 64 positions go to LDS by direct copies, two buffers; the
  * 16-byte pieces of a row are permuted by its position (swz) so that neither
@@ -838,13 +838,13 @@ __device__ inline void merge_groups(float *lds, int wave, int lane, float &mx, f
 
 /* MW waves of 32 m-rows; with KG = 2, two groups of them take the tiles in
  * turn.  J blocks of 32 positions are computed together: two overlap their
- * latencies (8192 tokens: 918 us, one at a time 928), one is half the code
- * and skips what a window hides (4,096 tokens, window 128: 43.5, 46.0).
+ * latencies (8,192 tokens: 883 us, one at a time 911), one is half the code
+ * and skips what a window hides (4,096 tokens, window 128: 42.9, 45.4).
  *
- * Bound for long prompts: the matrix units at the power limit.  8192 tokens of
- * 32 heads of 128: 898 us, 1.22 PFLOP/s counting both products (a large f16
- * product runs at 1.23), the clock at 1.45 - 1.6 GHz.  4,096 tokens of 64 heads of
- * 64 with a window of 128: 43.3 us, 142 MB; two rounds of workgroups that load
+ * Bound for long prompts: the matrix units at the power limit.  8,192 tokens of
+ * 32 heads of 128: 883 us (923 on another card), 1.25 PFLOP/s counting both
+ * products (a large f16 product runs at 1.23), the clock at 1.45 - 1.6 GHz.  4,096 tokens of 64 heads of
+ * 64 with a window of 128: 42.9 us, 142 MB; two rounds of workgroups that load
  * (5 us), compute (8: a block's softmax takes more issue slots than its
  * products) and store (2) with little overlap between those of a CU. */
 template <int HD, int MW, int KG>
@@ -972,7 +972,7 @@ __device__ inline __attribute__((always_inline)) void rows_h(const PromptArgs &a
                     for (int v = 0; v < 16; v++) o[d][v] *= alpha;
             }
             const float sh = mx == -INFINITY ? 0.f : SHIFT_H - mx;
-            /* the scheduler's order of MFMAs and exponentials: 8192 tokens 934 us without, 919 */
+            /* the scheduler's order of MFMAs and exponentials: 8,192 tokens 896 us without, 883 */
             __builtin_amdgcn_iglp_opt(2);
             h8 ph[2 * J], pl[2 * J];
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -1308,17 +1308,18 @@ __global__ __launch_bounds__(256) void k_rows_n(PromptArgs a, RowsPlan p) {
  * 2^SPREAD in their largest magnitudes (zeros aside), its channels too (then a
  * value is off by 2^-27 of its channel's largest in the group at most; fewer
  * positions than 8, the last of a span, have small values by chance and are not
- * asked, unless they are all there is), and so may the groups of V; where they differ by more, or a group that is not all zeros lies below
- * 2^-85, the workgroup's rows are computed as few rows are, with f32 products
- * (rows_n), 16 at a time (1,000 rows of 32 heads of 128: 292 us instead of 53;
- * value by value 19,400).
+ * asked, unless they are all there is), and so may the groups of V; where
+ * they differ by more, or a group that is not all zeros lies below 2^-85, the
+ * workgroup's rows are computed as few rows are, with f32 products (rows_n), 16
+ * at a time (1,000 rows of 32 heads of 128: 254 us instead of 51; value by
+ * value 19,400).
  *
  * A tile of 32 positions is loaded into registers two tiles ahead, split and
  * stored to one of two LDS buffers one tile ahead (plane [K hi, K lo, V hi,
  * V lo][32][HD]).
  *
  * Bound: the matrix units and the splitting beside them.  500 rows of 64 heads
- * of 64 behind 30,001 positions: 788 us, 0.94 PFLOP/s counting the three
+ * of 64 behind 30,001 positions: 793 us, 0.94 PFLOP/s counting the three
  * products, 77% of a large f16 product's rate; 2,020 packed rows of 32 heads
  * of 128: 59 us, where the longest sequence's last tiles are most of it. */
 constexpr int KF = 32, SPREAD = 12;
@@ -1530,8 +1531,8 @@ __device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a
 
     /* Of the two waves of a SIMD one splits its share of the next tile before
      * it computes and one behind, so that one's VALU work meets the other's
-     * MFMAs (500 rows of 64-value heads behind 30,001: 857 us, both behind, and
-     * 818; 4,096 rows of 128: 419 and 410).  Workgroups of four waves share
+     * MFMAs (500 rows of 64-value heads behind 30,001: 821 us, both behind, and
+     * 793; 4,096 rows of 128: 405 and 398).  Workgroups of four waves share
      * the SIMDs with others, whose barriers are their own. */
     const bool early = KG == 2 ? group == 1 : MW == 8 && wave >= 4;
     auto next_tile = [&](int t, int to) __attribute__((always_inline)) {
@@ -1597,7 +1598,7 @@ __device__ inline __attribute__((always_inline)) void rows_f(const PromptArgs &a
             }
             U = un;
             const float sh = mx == -INFINITY ? 0.f : SHIFT_F - mx;
-            /* the scheduler's order of MFMAs and exponentials: 500 rows behind 30,001 813 us without, 802 */
+            /* the scheduler's order of MFMAs and exponentials: 4,096 rows 402 us without, 398; 500 behind 30,001 789 and 793 */
             __builtin_amdgcn_iglp_opt(3);
             h8 ph[2], pl[2];
 #pragma unroll
@@ -1789,13 +1790,13 @@ __global__ __launch_bounds__(256) void k_rows_combine(PromptArgs a, RowsPlan p) 
  *   narrow  16 m-rows a workgroup, positions over its waves
  *   wide    128 m-rows, two groups of four waves on tiles in turn: two waves
  *           a SIMD where there are few workgroups (1,024 tokens of 32 heads of
- *           128, f16 and f32: 33.1 and 52.2 us, full 36.7 and 70.6)
+ *           128, f16 and f32: 31.9 and 52.4 us, full 36.1 and 71.6)
  *   short   128 m-rows, four waves, for few positions a row (128 tokens, f16:
  *           11.6 us, wide 12.3)
  *   full    the same, two workgroups a CU on long spans (8,192 tokens, f16:
- *           907 us, wide 963; 3,000 146 and 153; 2,048 78 and 74)
+ *           883 us, wide 925; 3,000 144 and 150; 2,048 77 and 72)
  *   tall    256 m-rows, eight waves, long f32 caches: half the splitting of K
- *           and V a row (4,096 tokens: 403 us, full 468; 3,000 250 and 248) */
+ *           and V a row (4,096 tokens: 398 us, full 466; 3,000 248 and 248) */
 enum Shape { NARROW, SHORT, WIDE, FULL, TALL };
 constexpr int SHAPE_ROWS[] = {16, 128, 128, 128, 256}, SHAPE_THREADS[] = {256, 256, 512, 256, 512};
 struct Cut {
