@@ -305,10 +305,13 @@ void tg_hip_kv_append_dev(const float *q_dev, const float *k_dev, const float *v
  * sums of weights times values taken before the division.  Operands of the
  * matrix units that f16 does not hold are two f16 values, 22 bits: of q, or
  * 2^-39 of its head's largest magnitude where that is more; of the weights, or
- * 2^-33 of the row's largest; of K and V of f32 caches, or 2^-39 of the largest
- * of 8 neighbouring positions.  With values of ordinary spread that is f32's
- * accuracy; a query with one dimension 2^17 above all that counts in the
- * others loses bits of these.
+ * 2^-33 of the row's largest (f32 caches: 2^-37, times as much as V of the
+ * position and its neighbours lies below the largest, at most 2^12 times); of
+ * K and V of f32 caches, or 2^-39 of the largest of 8 neighbouring positions.
+ * With values of ordinary spread that is f32's accuracy; a query with one
+ * dimension 2^17 above all that counts in the others loses bits of these, and
+ * a dimension in which only positions of vanishing weight have values loses
+ * bits of the output.
  * Rows that come out not finite are computed again value by value: as exact,
  * but many times slower.  Where nearby positions of an f32 cache differ by
  * more than 2^12 in magnitude, or the channels of eight neighbouring positions
