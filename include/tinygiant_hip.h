@@ -343,6 +343,119 @@ void tg_hip_attention_prefix_dev(const float *q_dev, int q_stride, int kv_type, 
                                  const float *sinks_dev, int n_heads, int n_kv_heads, int head_dim, float *out_dev,
                                  int out_stride, void *scratch_dev, void *stream);
 
+/* ---- rotary positions ----
+ * Pair i of a head's first rot_dim values at position p turns by the angle
+ * p f_i.  The reference has one table for whole heads in half layout
+ * (apply_rope_inplace, csrc/libtinygiant.c:702-719); the calls below and
+ * tg_hip_paged_append_dev also turn part of a head, and interleaved pairs.
+ * rot_dim is a multiple of 8; values from rot_dim on stay as they are.
+ *   interleaved 0: pair i is (i, i + rot_dim / 2), 1: (2 i, 2 i + 1)
+ *
+ * tg_hip_rope_tables_dev fills cos, sin [rope_len][rot_dim / 2] for positions
+ * first .. first + rope_len - 1: mscale cos(p f_i), mscale sin(p f_i), angles in
+ * 64 bits, each rounded once.  f_i from F_i = theta^(-2 i / rot_dim) (theta > 1) by
+ *   scaling 0  F_i
+ *           1  F_i / factor (positions stretched)
+ *           2  theta factor^(rot_dim / (rot_dim - 2)) in theta's place
+ *           3  by parts: pair b(t) = rot_dim ln(orig_len / (2 pi t)) / (2 ln theta)
+ *              turns t times in orig_len positions; F_i before pair b(low),
+ *              F_i / factor behind pair b(high) (held to 0 .. rot_dim - 1), between them
+ *              the mean with weights that change linearly with i; low > high
+ *           4  the same with b(low) rounded down, b(high) up
+ *           5  smooth: F_i where it turns high times or more in orig_len
+ *              positions, F_i / factor where low times or fewer, between them the mean
+ *              with weights that change linearly with the number; low < high
+ * factor is not used by 0, orig_len, low and high only by 3 to 5.  rope_len <=
+ * 2^20, first <= 2^30, rot_dim in 8..256. */
+void tg_hip_rope_tables_dev(float *cos_dev, float *sin_dev, int rope_len, int first, int rot_dim, double theta,
+                            int scaling, float factor, int orig_len, float low, float high, float mscale, void *stream);
+/* Turns rows of n_heads heads, x [n_rows][x_stride], at positions pos [n_rows]
+ * of the tables [rope_len][rot_dim / 2] into out (which may be x with its
+ * stride): queries and keys in front of tg_hip_kv_append_dev without tables,
+ * for instance.  A row whose position is not in the tables is left out (its
+ * row of out stays as it was).  head_dim a multiple of 8 and <= 1024,
+ * n_heads <= 1024; strides in floats. */
+void tg_hip_rope_dev(const float *x_dev, int x_stride, const int32_t *pos_dev, const float *rope_cos_dev,
+                     const float *rope_sin_dev, int rope_len, int rot_dim, int interleaved, int n_rows, int n_heads,
+                     int head_dim, float *out_dev, int out_stride, void *stream);
+
+/* ---- caches of 8 bits in pages ----
+ * No counterpart in the reference.  A page holds page_size positions (a power of
+ * two, 16..1024) of every KV head, one signed byte a value:
+ *   pages_k, pages_v  [n_pages][n_kv_heads][page_size][head_dim], 16-byte aligned
+ *   exps_k, exps_v    [n_pages][n_kv_heads][page_size / 16]: byte b is for 16
+ *                     positions of a head, whose values are n 2^(b - 127), b in 85..169
+ *   table             [n_seqs][table_stride]: the pages of each sequence in
+ *                     order; several may list the same pages (a shared prefix)
+ * rows, cu_rows and kv_len are those of the packed rows above, without slots:
+ * row i of sequence s is at position kv_len[s] + i.  table, cu_rows and kv_len
+ * are device arrays that the host does not see: a sequence whose rows do not
+ * fit its row of the table (nor 2^20 positions, nor max_kv) is left out, its
+ * rows of the outputs and its pages stay as they were; a table's entry outside
+ * 0..n_pages - 1 stands for no page.  head_dim a multiple of 16 and <= 128,
+ * n_heads / n_kv_heads integral and <= 64, n_heads <= 1024, n_pages * n_kv_heads *
+ * page_size / 16 < 2^31; the other limits are those above.
+ * n_rows = 0 or n_seqs = 0 does nothing.  A launch that HIP refuses is
+ * reported by tg_hip_last_error().  All of it can be captured and replayed.
+ *
+ * tg_hip_paged_append_dev norms and turns the rows as tg_hip_kv_append_dev does
+ * (rot_dim and interleaved as above, tables both NULL: no rotation; a row past the
+ * tables is left out), stores K and V and writes the query heads into q_out.
+ * A block's exponent is the least e in -42..42 with |x| <= 127 2^e for all x that
+ * the call stores in it, but not below the one it has if earlier rows of the
+ * sequence are in it; those are then rounded again, n 2^(e_old - e) to
+ * nearest even, and so is x 2^-e, computed in 64 bits from the
+ * f32 inputs: the bytes are the formula's, and a call's are the same as
+ * often as it is repeated.  All roundings of a value together are off by at most one
+ * step of the block's last exponent.  (What precision a value keeps hangs on how
+ * rows are dealt to calls.)  A block that takes in a value beyond 127 2^42, an
+ * infinity or a NaN gets the byte 255 and is NaN until it is begun
+ * anew: by a call whose sequence has no earlier rows in it.  Rows in a
+ * missing page are not stored.  Two sequences of a call must not write the
+ * same block of a page; a shared block is copied before it is written. */
+void tg_hip_paged_append_dev(const float *q_dev, const float *k_dev, const float *v_dev, int q_stride, int kv_stride,
+                             const float *q_norm_w_dev, const float *k_norm_w_dev, float eps, const float *rope_cos_dev,
+                             const float *rope_sin_dev, int rope_len, int rot_dim, int interleaved,
+                             const int32_t *cu_rows_dev, const int32_t *kv_len_dev, int n_seqs, int n_rows,
+                             int8_t *pages_k_dev, int8_t *pages_v_dev, uint8_t *exps_k_dev, uint8_t *exps_v_dev,
+                             int n_pages, int page_size, const int32_t *table_dev, int table_stride, int n_heads,
+                             int n_kv_heads, int head_dim, float *q_out_dev, int q_out_stride, void *stream);
+/* Positions 0 .. len[s] - 1 of each sequence as values, float32 (kv_type 0) or
+ * float16 (1, rounded to nearest), into slot slots[s] (NULL: s) of kv_k, kv_v
+ * [n_slots][n_kv_heads][kv_max][head_dim], 16-byte aligned: the caches of
+ * tg_hip_attention_dev and of the packed rows above.  Positions without a page
+ * and blocks whose byte is outside 85..169 come out NaN.  A sequence whose slot is not below
+ * n_slots, or whose length is past kv_max or its row of the table, is left
+ * out; the slots' other positions stay as they were. */
+void tg_hip_paged_read_dev(const int8_t *pages_k_dev, const int8_t *pages_v_dev, const uint8_t *exps_k_dev,
+                           const uint8_t *exps_v_dev, int n_pages, int page_size, const int32_t *table_dev,
+                           int table_stride, const int32_t *len_dev, int n_seqs, int n_kv_heads, int head_dim, int kv_type,
+                           void *kv_k_dev, void *kv_v_dev, const int32_t *slots_dev, int n_slots, int kv_max,
+                           void *stream);
+/* Causal attention of the rows over their sequences' pages, after
+ * tg_hip_paged_append_dev has stored their K and V: scores, window and sinks
+ * as in tg_hip_attention_prompt_dev.  max_kv, at most table_stride * page_size, is what no
+ * sequence's positions pass (kv_len[s] and its rows): the call is cut for
+ * that, so a program gives the longest that the call may meet and not the
+ * table's room.  Values of positions that a row does not see never reach it.
+ * A row that sees a position without a page, or of a block whose byte is
+ * outside 85..169, is NaN; so is one whose query is not finite.  K and V are
+ * exact; of q 24 bits of its head's largest magnitude are kept (a head below 2^-80
+ * scores 0), of the weights 22, or 2^-33 of the largest weight times value
+ * of the row; sums and the softmax's statistics are f32.  out may be q with q's stride.
+ * scratch_dev holds tg_hip_attention_paged_scratch_bytes(...) bytes, 16-byte
+ * aligned; it may be NULL where that is 0.  The size is enough for every call of
+ * at most as many rows, sequences and positions (max_kv) with these heads.
+ * Calls that overlap in time need scratch of their own. */
+void tg_hip_attention_paged_dev(const float *q_dev, int q_stride, const int8_t *pages_k_dev, const int8_t *pages_v_dev,
+                                const uint8_t *exps_k_dev, const uint8_t *exps_v_dev, int n_pages, int page_size,
+                                const int32_t *table_dev, int table_stride, const int32_t *cu_rows_dev,
+                                const int32_t *kv_len_dev, int n_seqs, int n_rows, int max_kv, int window,
+                                const float *sinks_dev, int n_heads, int n_kv_heads, int head_dim, float *out_dev,
+                                int out_stride, void *scratch_dev, void *stream);
+size_t tg_hip_attention_paged_scratch_bytes(int n_rows, int n_seqs, int n_heads, int n_kv_heads, int head_dim,
+                                            int max_kv);
+
 /* Adjusts k rows of logits [k][nrows] before a token is chosen from them, in
  * this order, each step one f32 operation rounded to nearest:
  *   l = l > 0 ? l / repetition : l * repetition   tokens in the row's history

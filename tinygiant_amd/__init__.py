@@ -18,6 +18,7 @@ FMT_Q4K, FMT_F16, FMT_Q6K, FMT_MXFP4, FMT_Q80 = 0, 1, 2, 3, 4
 FMT_NAMES = {"q4_k": 0, "float16": 1, "q6_k": 2, "mxfp4": 3, "q8_0": 4}   # tinygiant/engine.py:21
 ACT_SILU, ACT_GPTOSS = 0, 1
 KV_F32, KV_F16 = 0, 1   # element type of a KV cache (tg_hip_kv_append_dev, tg_hip_attention_prompt_dev)
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS, ROPE_PARTS_WHOLE, ROPE_SMOOTH = range(6)   # tg_hip_rope_tables_dev
 Q8_DTYPE = np.dtype([("scale", "<f4"), ("sum", "<i4"), ("bsums", "<i4", (8,)), ("qs", "i1", (256,))])
 
 _LIB = None

@@ -13,6 +13,7 @@ VP = ctypes.c_void_p
 CI = ctypes.c_int
 CF = ctypes.c_float
 SZ = ctypes.c_size_t
+CD = ctypes.c_double
 U64 = ctypes.c_uint64
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -110,6 +111,14 @@ def register_extensions(lib):
                                            VP, VP])
     _reg(lib.tg_hip_attention_prefix_dev, [VP, CI, CI, VP, VP, CI, CI, VP, VP, CI, CI, VP, VP, VP, CI, CI, CI, VP, CI,
                                            CI, CI, VP, CI, VP, VP])
+    _reg(lib.tg_hip_rope_tables_dev, [VP, VP, CI, CI, CI, CD, CI, CF, CI, CF, CF, CF, VP])
+    _reg(lib.tg_hip_rope_dev, [VP, CI, VP, VP, VP, CI, CI, CI, CI, CI, CI, VP, CI, VP])
+    _reg(lib.tg_hip_paged_append_dev, [VP, VP, VP, CI, CI, VP, VP, CF, VP, VP, CI, CI, CI, VP, VP, CI, CI, VP, VP, VP, VP,
+                                       CI, CI, VP, CI, CI, CI, CI, VP, CI, VP])
+    _reg(lib.tg_hip_paged_read_dev, [VP, VP, VP, VP, CI, CI, VP, CI, VP, CI, CI, CI, CI, VP, VP, VP, CI, CI, VP])
+    _reg(lib.tg_hip_attention_paged_scratch_bytes, [CI, CI, CI, CI, CI, CI], SZ)
+    _reg(lib.tg_hip_attention_paged_dev, [VP, CI, VP, VP, VP, VP, CI, CI, VP, CI, VP, VP, CI, CI, CI, CI, VP, CI, CI, CI, VP,
+                                          CI, VP, VP])
     _reg(lib.tg_hip_logits_scratch_bytes, [CI, CI], SZ)
     _reg(lib.tg_hip_logits_adjust_dev, [VP, VP, CI, CI, VP, CI, VP, VP, VP, VP, VP, CI, VP, VP, CI, VP, VP, VP, VP])
     _reg(lib.tg_hip_upload_file, [ctypes.c_char_p, ctypes.c_uint64, ctypes.c_uint64, VP, ctypes.c_uint64],

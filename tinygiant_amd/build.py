@@ -28,7 +28,7 @@ HIP_FLAGS = [
 # VGPRs (no accumulator-register reads before the scale arithmetic)
 HIP_EXTRA = {"tg_grouped_k.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 HIP_SOURCES = ["tg_kernels.hip", "tg_grouped.hip", "tg_grouped_k.hip", "tg_decode.hip", "tg_decode_mx.hip", "tg_decode_rows.hip", "tg_head.hip", "tg_route.hip", "tg_attn.hip",
-               "tg_prompt.hip", "tg_logits.hip", "tg_api.hip"]
+               "tg_prompt.hip", "tg_paged.hip", "tg_rope.hip", "tg_logits.hip", "tg_api.hip"]
 CXX_SOURCES = ["tg_host_ops.cpp"]
 
 

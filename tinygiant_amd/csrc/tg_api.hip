@@ -38,6 +38,7 @@
 #include "tg_route.h"
 #include "tg_kernels.h"
 #include "tg_logits.h"
+#include "tg_paged.h"
 #include "tg_prompt.h"
 #include "tg_synth.h"
 
@@ -1612,6 +1613,273 @@ TG_API void tg_hip_attention_prefix_dev(const float *q_dev, int q_stride, int kv
     attention_rows("tg_hip_attention_prefix_dev", q_dev, q_stride, kv_type, kv_k_dev, kv_v_dev, n_slots, kv_max,
                    prefix_k_dev, prefix_v_dev, prefix_len, prefix_max, cu_rows_dev, kv_len_dev, slots_dev, n_seqs, n_rows,
                    window, sinks_dev, n_heads, n_kv_heads, head_dim, out_dev, out_stride, scratch_dev, stream);
+}
+
+/* ---- rotary positions ---- */
+static bool turn_validate(const char *who, const float *cos, const float *sin, int rope_len, int rot_dim, int head_dim) {
+    if (!cos != !sin || (cos && (rope_len <= 0 || rot_dim <= 0 || rot_dim % 8 || rot_dim > head_dim)) ||
+        (((uintptr_t)cos | (uintptr_t)sin) & 3)) {
+        set_err("%s: need both RoPE tables, 4-byte aligned, with rope_len >= 1 and rot_dim a multiple of 8 in 8..head_dim, or "
+                "neither", who);
+        return false;
+    }
+    return true;
+}
+
+TG_API void tg_hip_rope_tables_dev(float *cos_dev, float *sin_dev, int rope_len, int first, int rot_dim, double theta,
+                                   int scaling, float factor, int orig_len, float low, float high, float mscale,
+                                   void *stream) {
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    static const char who[] = "tg_hip_rope_tables_dev";
+    enum { PLAIN, LINEAR, BASE, PARTS, PARTS_WHOLE, SMOOTH };
+    if (rope_len < 0 || rope_len > PROMPT_MAX_KV || first < 0 || first > (1 << 30) || rot_dim < 8 || rot_dim % 8 ||
+        rot_dim > 2 * ROPE_MAX_PAIRS || !(theta > 1.0) || !(theta < 1e30) || scaling < PLAIN || scaling > SMOOTH ||
+        !(fabsf(mscale) < INFINITY)) {
+        set_err("%s: need 0 <= rope_len <= %d, first in 0..2^30, rot_dim a multiple of 8 in 8..%d, theta in 1..1e30, a known "
+                "scaling and a finite mscale", who, PROMPT_MAX_KV, 2 * ROPE_MAX_PAIRS);
+        return;
+    }
+    if (scaling != PLAIN && !(factor > 0.f && factor < INFINITY)) {
+        set_err("%s: a scaled table needs a positive finite factor", who);
+        return;
+    }
+    if (scaling >= PARTS && (orig_len <= 0 || !(low > 0.f && low < INFINITY) || !(high > 0.f && high < INFINITY) ||
+                             (scaling == SMOOTH ? !(low < high) : !(low > high)))) {
+        set_err("%s: needs orig_len >= 1 and positive low and high, low > high for frequencies scaled by parts, low < high "
+                "for the smooth form", who);
+        return;
+    }
+    if (!rope_len) return;
+    if (!cos_dev || !sin_dev || (((uintptr_t)cos_dev | (uintptr_t)sin_dev) & 3)) {
+        set_err("%s: null or not 4-byte aligned table", who);
+        return;
+    }
+    ensure_init();
+    RopeTablesArgs a = {};
+    a.cos = cos_dev, a.sin = sin_dev, a.len = rope_len, a.first = first, a.pairs = rot_dim / 2, a.mscale = mscale;
+    const double two_pi = 6.283185307179586476925;
+    double lo = 0, hi = 0;
+    if (scaling == PARTS || scaling == PARTS_WHOLE) {
+        auto pair_of = [&](double turns) { return rot_dim * log(orig_len / (turns * two_pi)) / (2 * log(theta)); };
+        lo = pair_of(low), hi = pair_of(high);
+        if (scaling == PARTS_WHOLE) lo = floor(lo), hi = ceil(hi);
+        lo = std::max(lo, 0.0), hi = std::min(hi, rot_dim - 1.0);
+    }
+    const double base = scaling == BASE ? theta * pow((double)factor, rot_dim / (rot_dim - 2.0)) : theta;
+    for (int i = 0; i < a.pairs; i++) {
+        double f = pow(base, -2.0 * i / rot_dim), share = 1.0;   /* of the unscaled frequency */
+        if (scaling == LINEAR) share = 0.0;
+        else if (scaling == PARTS || scaling == PARTS_WHOLE) share = 1.0 - std::min(1.0, std::max(0.0, (i - lo) / std::max(hi - lo, 1e-3)));
+        else if (scaling == SMOOTH) share = std::min(1.0, std::max(0.0, (orig_len * f / two_pi - low) / ((double)high - low)));
+        if (share < 1.0) f = f * share + f / factor * (1.0 - share);
+        a.turns[i] = f / two_pi;
+    }
+    const hipError_t before = hipPeekAtLastError();
+    launch_rope_tables(a, stream ? (hipStream_t)stream : g.st);
+    check_launch(who, before);
+}
+
+TG_API void tg_hip_rope_dev(const float *x_dev, int x_stride, const int32_t *pos_dev, const float *rope_cos_dev,
+                            const float *rope_sin_dev, int rope_len, int rot_dim, int interleaved, int n_rows, int n_heads,
+                            int head_dim, float *out_dev, int out_stride, void *stream) {
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    static const char who[] = "tg_hip_rope_dev";
+    if (n_rows < 0 || n_rows > PROMPT_MAX_ROWS || n_heads <= 0 || n_heads > 1024 || head_dim <= 0 || head_dim % 8 ||
+        head_dim > 1024 || (long long)n_rows * ((n_heads * (head_dim / 8) + 255) / 256) >= (1 << 24)) {
+        set_err("%s: unsupported shape (0 <= n_rows <= %d, n_heads in 1..1024, head_dim %% 8 == 0 and <= 1024, n_rows times "
+                "n_heads * head_dim in units of 2048 below 2^24)", who, PROMPT_MAX_ROWS);
+        return;
+    }
+    if (x_stride < n_heads * head_dim || out_stride < n_heads * head_dim || (x_dev && x_dev == out_dev && x_stride != out_stride)) {
+        set_err("%s: need strides of at least n_heads * head_dim, and the same for out over x", who);
+        return;
+    }
+    if (!n_rows) return;
+    if (!x_dev || !out_dev || !pos_dev || !rope_cos_dev || (((uintptr_t)x_dev | (uintptr_t)out_dev | (uintptr_t)pos_dev) & 3)) {
+        set_err("%s: null or not 4-byte aligned rows, positions or tables", who);
+        return;
+    }
+    if (!turn_validate(who, rope_cos_dev, rope_sin_dev, rope_len, rot_dim, head_dim)) return;
+    ensure_init();
+    RopeArgs a = {};
+    a.x = x_dev, a.x_stride = x_stride, a.pos = pos_dev;
+    a.turn = Turn{rope_cos_dev, rope_sin_dev, rope_len, rot_dim, interleaved != 0};
+    a.rows = n_rows, a.heads = n_heads, a.head_dim = head_dim;
+    a.out = out_dev, a.out_stride = out_stride;
+    const hipError_t before = hipPeekAtLastError();
+    launch_rope(a, stream ? (hipStream_t)stream : g.st);
+    check_launch(who, before);
+}
+
+/* ---- 8-bit caches in pages ---- */
+static bool pages_validate(const char *who, const void *k, const void *v, const void *ek, const void *ev, int n_pages,
+                           int page_size, const int32_t *table, int stride, int n_seqs, int n_kv, int head_dim,
+                           bool work, Pages &p) {
+    if (page_size < PAGE_BLOCK || page_size > PAGE_MAX || (page_size & (page_size - 1)) || n_pages <= 0 || stride <= 0 ||
+        (long long)stride * page_size > (1ll << 30) || n_seqs < 0 || n_seqs > PROMPT_MAX_SEQS || n_kv <= 0 || n_kv > 1024 ||
+        head_dim <= 0 || head_dim % 16 || head_dim > PROMPT_MAX_HEAD_DIM) {
+        set_err("%s: need page_size a power of two in %d..%d, n_pages >= 1, table_stride >= 1 with at most 2^30 positions, "
+                "0 <= n_seqs <= %d, n_kv_heads in 1..1024, head_dim %% 16 == 0 and <= %d", who, PAGE_BLOCK, PAGE_MAX,
+                PROMPT_MAX_SEQS, PROMPT_MAX_HEAD_DIM);
+        return false;
+    }
+    if ((long long)n_pages * n_kv * (page_size / PAGE_BLOCK) >= (1ll << 31) || (long long)n_seqs * n_kv > PROMPT_MAX_SEQ_HEADS) {
+        set_err("%s: too many pages or sequences (n_pages * n_kv_heads * page_size / %d < 2^31, n_seqs * n_kv_heads <= %d)",
+                who, PAGE_BLOCK, PROMPT_MAX_SEQ_HEADS);
+        return false;
+    }
+    if (work && (!k || !v || !ek || !ev || !table || (((uintptr_t)k | (uintptr_t)v) & 15) || ((uintptr_t)table & 3))) {
+        set_err("%s: null pages, exponents or table, or pages not 16-byte aligned", who);
+        return false;
+    }
+    p = Pages{(int8_t *)k, (int8_t *)v, (uint8_t *)ek, (uint8_t *)ev, table, n_pages, stride, __builtin_ctz(page_size / PAGE_BLOCK)};
+    return true;
+}
+
+static bool paged_rows_validate(const char *who, const int32_t *cu_rows, int n_seqs, int n_rows, int n_heads, int n_kv) {
+    if (n_rows < 0 || n_rows > PROMPT_MAX_ROWS || n_heads <= 0 || n_heads > 1024 || n_heads % n_kv ||
+        n_heads / n_kv > PROMPT_MAX_GQA || (long long)n_rows * n_heads > PROMPT_MAX_ROW_HEADS) {
+        set_err("%s: need 0 <= n_rows <= %d, n_heads <= 1024, n_heads / n_kv_heads integral and <= %d, n_rows * n_heads <= %d",
+                who, PROMPT_MAX_ROWS, PROMPT_MAX_GQA, PROMPT_MAX_ROW_HEADS);
+        return false;
+    }
+    if (n_seqs && n_rows && !cu_rows) {
+        set_err("%s: null cu_rows", who);
+        return false;
+    }
+    return true;
+}
+
+TG_API void tg_hip_paged_append_dev(const float *q_dev, const float *k_dev, const float *v_dev, int q_stride, int kv_stride,
+                                    const float *q_norm_w_dev, const float *k_norm_w_dev, float eps,
+                                    const float *rope_cos_dev, const float *rope_sin_dev, int rope_len, int rot_dim,
+                                    int interleaved, const int32_t *cu_rows_dev, const int32_t *kv_len_dev, int n_seqs,
+                                    int n_rows, int8_t *pages_k_dev, int8_t *pages_v_dev, uint8_t *exps_k_dev,
+                                    uint8_t *exps_v_dev, int n_pages, int page_size, const int32_t *table_dev,
+                                    int table_stride, int n_heads, int n_kv_heads, int head_dim, float *q_out_dev,
+                                    int q_out_stride, void *stream) {
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    static const char who[] = "tg_hip_paged_append_dev";
+    PagedAppendArgs a = {};
+    if (!pages_validate(who, pages_k_dev, pages_v_dev, exps_k_dev, exps_v_dev, n_pages, page_size, table_dev, table_stride,
+                        n_seqs, n_kv_heads, head_dim, n_seqs && n_rows, a.pages) ||
+        !paged_rows_validate(who, cu_rows_dev, n_seqs, n_rows, n_heads, n_kv_heads) ||
+        !turn_validate(who, rope_cos_dev, rope_sin_dev, rope_len, rot_dim, head_dim))
+        return;
+    if (q_out_dev && (!q_dev || q_stride < n_heads * head_dim || q_out_stride < n_heads * head_dim ||
+                      (q_out_dev == q_dev && q_out_stride != q_stride))) {
+        set_err("%s: q_out without q, a stride below n_heads * head_dim, or q_out over q with another stride", who);
+        return;
+    }
+    if (kv_stride < n_kv_heads * head_dim) {
+        set_err("%s: need kv_stride >= n_kv_heads * head_dim", who);
+        return;
+    }
+    if (!n_seqs || !n_rows) return;
+    if (!k_dev || !v_dev || (((uintptr_t)q_dev | (uintptr_t)k_dev | (uintptr_t)v_dev | (uintptr_t)q_out_dev) & 3)) {
+        set_err("%s: null k or v, or rows that are not 4-byte aligned", who);
+        return;
+    }
+    ensure_init();
+    a.q = q_dev, a.k = k_dev, a.v = v_dev;
+    a.q_stride = q_stride, a.kv_stride = kv_stride;
+    a.q_norm = q_norm_w_dev, a.k_norm = k_norm_w_dev, a.eps = eps;
+    a.turn = Turn{rope_cos_dev, rope_sin_dev, rope_len, rot_dim, interleaved != 0};
+    a.s = packed_seqs(cu_rows_dev, kv_len_dev, nullptr, n_seqs, n_rows, n_seqs,
+                      std::min(table_stride * page_size, PROMPT_MAX_KV));
+    a.n_heads = n_heads, a.n_kv = n_kv_heads, a.head_dim = head_dim;
+    a.q_out = q_out_dev, a.q_out_stride = q_out_stride;
+    const hipError_t before = hipPeekAtLastError();
+    launch_paged_append(a, stream ? (hipStream_t)stream : g.st);
+    check_launch(who, before);
+}
+
+TG_API void tg_hip_paged_read_dev(const int8_t *pages_k_dev, const int8_t *pages_v_dev, const uint8_t *exps_k_dev,
+                                  const uint8_t *exps_v_dev, int n_pages, int page_size, const int32_t *table_dev,
+                                  int table_stride, const int32_t *len_dev, int n_seqs, int n_kv_heads, int head_dim,
+                                  int kv_type, void *kv_k_dev, void *kv_v_dev, const int32_t *slots_dev, int n_slots,
+                                  int kv_max, void *stream) {
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    static const char who[] = "tg_hip_paged_read_dev";
+    PagedReadArgs a = {};
+    if (!pages_validate(who, pages_k_dev, pages_v_dev, exps_k_dev, exps_v_dev, n_pages, page_size, table_dev, table_stride,
+                        n_seqs, n_kv_heads, head_dim, n_seqs > 0, a.pages))
+        return;
+    if ((kv_type != TG_KV_F32 && kv_type != TG_KV_F16) || n_slots <= 0 || kv_max <= 0 || kv_max > PROMPT_MAX_KV) {
+        set_err("%s: need kv_type 0 (float32) or 1 (float16), n_slots >= 1, 1 <= kv_max <= %d", who, PROMPT_MAX_KV);
+        return;
+    }
+    if (!n_seqs) return;
+    if (!len_dev || !kv_k_dev || !kv_v_dev || (((uintptr_t)kv_k_dev | (uintptr_t)kv_v_dev) & 15)) {
+        set_err("%s: null lengths, or slots that are null or not 16-byte aligned", who);
+        return;
+    }
+    ensure_init();
+    a.len = len_dev, a.slot = slots_dev, a.n = n_seqs, a.n_kv = n_kv_heads, a.head_dim = head_dim;
+    a.k = kv_k_dev, a.v = kv_v_dev, a.n_slots = n_slots, a.kv_max = kv_max;
+    a.most = std::min(kv_max, table_stride * page_size);
+    const hipError_t before = hipPeekAtLastError();
+    launch_paged_read(a, kv_type == TG_KV_F16, stream ? (hipStream_t)stream : g.st);
+    check_launch(who, before);
+}
+
+TG_API size_t tg_hip_attention_paged_scratch_bytes(int n_rows, int n_seqs, int n_heads, int n_kv_heads, int head_dim,
+                                                   int max_kv) {
+    if (n_rows <= 0 || n_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || head_dim <= 0 ||
+        head_dim > PROMPT_MAX_HEAD_DIM || max_kv <= 0 || n_rows > PROMPT_MAX_ROWS || n_seqs > PROMPT_MAX_SEQS ||
+        n_heads > 1024 || max_kv > PROMPT_MAX_KV)
+        return 0;
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    return attention_paged_scratch(n_rows, n_seqs, n_heads, n_kv_heads, head_dim, max_kv);
+}
+
+TG_API void tg_hip_attention_paged_dev(const float *q_dev, int q_stride, const int8_t *pages_k_dev,
+                                       const int8_t *pages_v_dev, const uint8_t *exps_k_dev, const uint8_t *exps_v_dev,
+                                       int n_pages, int page_size, const int32_t *table_dev, int table_stride,
+                                       const int32_t *cu_rows_dev, const int32_t *kv_len_dev, int n_seqs, int n_rows,
+                                       int max_kv, int window, const float *sinks_dev, int n_heads, int n_kv_heads,
+                                       int head_dim, float *out_dev, int out_stride, void *scratch_dev, void *stream) {
+    std::lock_guard<std::recursive_mutex> lk(g_mu);
+    static const char who[] = "tg_hip_attention_paged_dev";
+    Pages pages;
+    if (!pages_validate(who, pages_k_dev, pages_v_dev, exps_k_dev, exps_v_dev, n_pages, page_size, table_dev, table_stride,
+                        n_seqs, n_kv_heads, head_dim, n_seqs && n_rows, pages) ||
+        !paged_rows_validate(who, cu_rows_dev, n_seqs, n_rows, n_heads, n_kv_heads))
+        return;
+    if (max_kv <= 0 || max_kv > PROMPT_MAX_KV || max_kv > table_stride * page_size) {
+        set_err("%s: need 1 <= max_kv <= %d and <= table_stride * page_size", who, PROMPT_MAX_KV);
+        return;
+    }
+    if (window < 0 || q_stride < n_heads * head_dim || out_stride < n_heads * head_dim || q_stride > PROMPT_MAX_STRIDE ||
+        out_stride > PROMPT_MAX_STRIDE) {
+        set_err("%s: need window >= 0 and strides of at least n_heads * head_dim and at most %d", who, PROMPT_MAX_STRIDE);
+        return;
+    }
+    if (!n_seqs || !n_rows) return;
+    if (!q_dev || !out_dev || (((uintptr_t)q_dev | (uintptr_t)out_dev) & 3)) {
+        set_err("%s: null or not 4-byte aligned q or out", who);
+        return;
+    }
+    if (q_dev == out_dev && q_stride != out_stride) {
+        set_err("%s: out over q needs the same stride", who);
+        return;
+    }
+    PromptArgs a = {};
+    a.q = q_dev, a.q_stride = q_stride;
+    a.s = packed_seqs(cu_rows_dev, kv_len_dev, nullptr, n_seqs, n_rows, n_seqs, max_kv);
+    a.window = window < max_kv ? window : 0;   /* as long as all positions: none */
+    a.sinks = sinks_dev;
+    a.n_heads = n_heads, a.n_kv = n_kv_heads, a.head_dim = head_dim;
+    a.out = out_dev, a.out_stride = out_stride;
+    const size_t need = attention_paged_need(a);
+    if (need && (!scratch_dev || ((uintptr_t)scratch_dev & 15))) {
+        set_err("%s: needs %zu bytes of 16-byte aligned scratch", who, need);
+        return;
+    }
+    ensure_init();
+    const hipError_t before = hipPeekAtLastError();
+    launch_attention_paged(a, pages, scratch_dev, stream ? (hipStream_t)stream : g.st);
+    check_launch(who, before);
 }
 
 /* ---- logits: penalties, biases, a grammar's mask ---- */

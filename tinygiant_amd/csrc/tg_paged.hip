@@ -1,0 +1,679 @@
+/*
+ * tg_paged.hip -- caches of signed bytes in pages: rows of several sequences
+ * into them, back out, and attention over them.
+ *
+ * A value is n 2^e: n a byte, e one exponent for a block of 16 positions of a
+ * KV head, for K and V each.  A block's exponent rises when a later row needs
+ * more, which re-rounds the rows that it holds; a power of two doubles at
+ * least, so that all of a value's roundings together are off by at most one
+ * step of the last unit (an arbitrary scale that creeps up could add half a
+ * step each time), and applying it is exact.
+ *
+ *   append     K and V of each row, normed and turned, into its page
+ *              (k_paged_append)
+ *   read       positions as f32 or f16, into slots of a dense cache
+ *              (k_paged_read)
+ *   attention  the formulas of tg_prompt.hip; kernels by sizes (paged_cut):
+ *              k_paged_n   16 query rows of a KV head a workgroup
+ *              k_paged_w   128
+ */
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "tg_paged.h"
+#include "tg_rows.hpp"
+#include "tg_turn.hpp"
+
+namespace tg {
+
+namespace {
+
+/* Place of block j of sequence s and KV head kh among all blocks of the
+ * pages (< 2^31); -1: no page */
+__device__ inline int block_at(const Pages &p, int n_kv, int s, int kh, int j) {
+    const int page = p.table[(size_t)s * p.stride + (j >> p.shift)];
+    return (unsigned)page < (unsigned)p.n_pages ? ((page * n_kv + kh) << p.shift) + (j & ((1 << p.shift) - 1)) : -1;
+}
+__device__ inline bool good_exp(int byte) { return (unsigned)(byte - (127 + PAGE_EXP_MIN)) <= (unsigned)(PAGE_EXP_MAX - PAGE_EXP_MIN); }
+/* 2^(byte - 127) and 2^(127 - byte) */
+__device__ inline float exp_up(int byte) { return __int_as_float(byte << 23); }
+__device__ inline float exp_down(int byte) { return __int_as_float((254 - byte) << 23); }
+
+__device__ inline int wave_imax(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
+/* The least e with |x| <= 127 2^e: x = m 2^k, m in [1/2, 1), and 127 / 128 is
+ * the border.  Values beyond the exponents' range, infinities and NaN
+ * (which no comparison holds for) give more than PAGE_EXP_MAX. */
+__device__ inline int block_exp(double big) {
+    if (!(big <= 127.0 * (double)(1ll << PAGE_EXP_MAX))) return PAGE_EXP_MAX + 1;
+    if (big == 0.0) return PAGE_EXP_MIN;
+    const int e = __builtin_amdgcn_frexp_exp(big) - 7 + (__builtin_amdgcn_frexp_mant(big) > 127.0 / 128.0);
+    return max(e, PAGE_EXP_MIN);
+}
+
+/* Where sequence s's blocks are among a call's, at most two more than n / 16
+ * of its n rows touch */
+__device__ inline int block_start(int r0, int s) { return (r0 >> 4) + 2 * s; }
+/* the last sequence whose place is at or before b, by the whole wave */
+__device__ inline bool seq_of_block(const PackedSeqs &p, int b, Seq &q, int &s, int &place) {
+    const int lane = threadIdx.x & 63;
+    int at = 0, count = p.n;
+    while (count > 64) {
+        const int step = (count + 63) / 64, t = at + min(lane * step, count - 1);
+        const uint64_t m = __ballot(lane * step < count && block_start(min(max(p.cu[t], 0), p.rows), t) <= b);
+        if (!m) return false;
+        const int k = (63 - __builtin_clzll(m)) * step;
+        at += k, count = min(step, count - k);
+    }
+    Seq mine = {0, 0, 0, 0};
+    if (lane < count) mine = seq_at(p, at + lane);
+    const uint64_t m = __ballot(lane < count && block_start(mine.r0, at + lane) <= b);
+    if (!m) return false;
+    const int k = 63 - __builtin_clzll(m);
+    q = lane_seq(mine, k);
+    s = at + k;
+    place = b - block_start(q.r0, s);
+    return q.n > 0;
+}
+
+/* K (v: V) rows of one block and head by one wave: G lanes a row, 64 / G rows
+ * at a time, everything in registers.  From the norm to the byte all is in 64
+ * bits, so that what is stored is the formula's nearest byte; the rate of
+ * 64-bit operations is half that of 32 here and the kernel waits for memory. */
+template <int G>
+__device__ inline void append_block(const PagedAppendArgs &a, const Seq &q, int s, int j, int kh, bool v) {
+    constexpr int PER = 64 / G, N = PAGE_BLOCK / PER;
+    const int lane = threadIdx.x & 63, row = lane / G, l = lane % G, hd = a.head_dim;
+    const int B = block_at(a.pages, a.n_kv, s, kh, j);
+    if (B < 0) return;
+    const bool on = 8 * l < hd;
+    uint8_t *eb = (v ? a.pages.ev : a.pages.ek) + B;
+    int8_t *page = (v ? a.pages.v : a.pages.k) + (size_t)B * PAGE_BLOCK * hd;
+    const int old_rows = max(0, min(PAGE_BLOCK, q.past - PAGE_BLOCK * j));   /* rows that it holds */
+    const int old = old_rows ? *eb : 127 + PAGE_EXP_MIN;
+    Turn turn = a.turn;
+    if (v) turn.cos = nullptr;
+    const Pieces p = turn_pieces(turn, l);
+    const float *nw = v ? nullptr : a.k_norm;
+    d4 x[N], y[N];
+    bool live[N];
+    double big = 0.0;
+    bool odd = false;   /* a value that is not finite */
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        const int pos = PAGE_BLOCK * j + PER * n + row, i = pos - q.past;
+        live[n] = i >= 0 && i < q.n && (!a.turn.cos || pos < a.turn.len);
+        f4 u = {0.f, 0.f, 0.f, 0.f}, w = u;
+        if (live[n] && on) {
+            const float *src = (v ? a.v : a.k) + (size_t)(q.r0 + i) * a.kv_stride + (size_t)kh * hd;
+            u = *(const f4u *)(src + p.a), w = *(const f4u *)(src + p.b);
+        }
+        x[n] = __builtin_convertvector(u, d4), y[n] = __builtin_convertvector(w, d4);
+        if (nw) {
+            double ss = 0.0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) ss += x[n][e] * x[n][e] + y[n][e] * y[n][e];
+#pragma unroll
+            for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+            if (on) {
+                const double f = 1.0 / sqrt(ss / (double)hd + (double)a.eps);
+                x[n] = x[n] * f * __builtin_convertvector((f4)*(const f4u *)(nw + p.a), d4);
+                y[n] = y[n] * f * __builtin_convertvector((f4)*(const f4u *)(nw + p.b), d4);
+            }
+        }
+        if (p.turned && live[n] && on) {
+            const size_t at = (size_t)pos * (turn.dim / 2) + 4 * l;
+            turn_pair(turn.inter, __builtin_convertvector((f4)*(const f4u *)(turn.cos + at), d4),
+                      __builtin_convertvector((f4)*(const f4u *)(turn.sin + at), d4), x[n], y[n]);
+        }
+        if (live[n] && on) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const double f = fabs(x[n][e]), g = fabs(y[n][e]);
+                odd |= !(f < INFINITY) || !(g < INFINITY);
+                big = fmax(big, fmax(f, g));
+            }
+        }
+    }
+    const uint64_t any = __ballot(live[0] || live[1] || (N > 2 && (live[2 % N] || live[3 % N])));
+    if (!any) return;
+    int e = wave_imax(odd ? PAGE_EXP_MAX + 1 : block_exp(big));
+    if (old_rows) e = max(e, good_exp(old) ? old - 127 : PAGE_EXP_MAX + 1);
+    const bool bad = e > PAGE_EXP_MAX;
+    const double f = __builtin_amdgcn_ldexp(1.0, -e);
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        if (!live[n] || !on) continue;
+        uint32_t lo = 0, hi = 0;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            lo |= ((uint32_t)(int)__builtin_rint(x[n][c] * f) & 255u) << (8 * c);
+            hi |= ((uint32_t)(int)__builtin_rint(y[n][c] * f) & 255u) << (8 * c);
+        }
+        int8_t *dst = page + (PER * n + row) * hd;
+        *(uint32_t *)(dst + p.a) = bad ? 0u : lo;
+        *(uint32_t *)(dst + p.b) = bad ? 0u : hi;
+    }
+    if (!bad && old_rows && e > old - 127) {   /* the rows before these in the new unit */
+        const float g = exp_up(254 - (e - (old - 127)) - 127);
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            if (PER * n + row >= old_rows || !on) continue;
+            uint32_t *at = (uint32_t *)(page + (PER * n + row) * hd + 8 * l);
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const uint32_t w = at[c];
+                uint32_t z = 0;
+#pragma unroll
+                for (int b = 0; b < 4; b++)
+                    z |= ((uint32_t)(int)__builtin_rintf((float)(int8_t)(w >> (8 * b)) * g) & 255u) << (8 * b);
+                at[c] = z;
+            }
+        }
+    }
+    if (lane == 0) *eb = bad ? PAGE_EXP_NAN : (uint8_t)(e + 127);
+}
+
+}  // namespace
+
+/* ---- append ----
+ * Workgroups of two kinds: those of the first `rows` (0 without q_out) turn a
+ * row's query heads, as k_kv_append does; the others have a wave for each
+ * block, KV head and one of K and V.  Two blocks more a sequence than its rows
+ * fill have room (block_start), so that no lengths are summed. */
+template <int G>
+__global__ __launch_bounds__(256) void k_paged_append(PagedAppendArgs a, int rows) {
+    const int tid = threadIdx.x, hd = a.head_dim;
+    if ((int)blockIdx.x >= rows) {
+        const long long unit = (long long)((int)blockIdx.x - rows) * 4 + __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int item = (int)(unit / (2 * a.n_kv)), rest = (int)(unit - (long long)item * (2 * a.n_kv));
+        Seq q;
+        int s, place;
+        if (!seq_of_block(a.s, item, q, s, place)) return;
+        const int j = (q.past >> 4) + place;
+        if (place < 0 || PAGE_BLOCK * j >= q.past + q.n) return;
+        append_block<G>(a, q, s, j, rest >> 1, rest & 1);
+        return;
+    }
+    const int r = (int)blockIdx.x;
+    Seq q;
+    int i;
+    if (!wave_seq_of(a.s, r, q, i)) return;
+    const int pos = q.past + i;
+    if (a.turn.cos && pos >= a.turn.len) return;
+    const int seg = tid / G, l = tid % G;
+    const bool on = 8 * l < hd;
+    const Pieces p = turn_pieces(a.turn, l);
+    f4 c = {1.f, 1.f, 1.f, 1.f}, sn = {0.f, 0.f, 0.f, 0.f};
+    if (p.turned && on) {
+        c = *(const f4u *)(a.turn.cos + (size_t)pos * (a.turn.dim / 2) + 4 * l);
+        sn = *(const f4u *)(a.turn.sin + (size_t)pos * (a.turn.dim / 2) + 4 * l);
+    }
+    for (int h0 = 0; h0 < a.n_heads; h0 += 256 / G) {
+        const int h = h0 + seg;
+        const bool live = h < a.n_heads && on;
+        const float *src = a.q + (size_t)r * a.q_stride + (size_t)h * hd;
+        f4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+        if (live) x = *(const f4u *)(src + p.a), y = *(const f4u *)(src + p.b);
+        if (a.q_norm) {
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) ss += x[e] * x[e] + y[e] * y[e];
+#pragma unroll
+            for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+            if (on) {
+                const float f = 1.f / sqrtf(ss / (float)hd + a.eps);
+                x = x * f * (f4)*(const f4u *)(a.q_norm + p.a);
+                y = y * f * (f4)*(const f4u *)(a.q_norm + p.b);
+            }
+        }
+        if (!live) continue;
+        if (p.turned) turn_pair(a.turn.inter, c, sn, x, y);
+        float *dst = a.q_out + (size_t)r * a.q_out_stride + (size_t)h * hd;
+        *(f4u *)(dst + p.a) = x;
+        *(f4u *)(dst + p.b) = y;
+    }
+}
+
+void launch_paged_append(const PagedAppendArgs &a, hipStream_t st) {
+    const int rows = a.q_out ? a.s.rows : 0;
+    const long long items = (long long)(a.s.rows >> 4) + 2ll * a.s.n;
+    const dim3 grid((unsigned)(rows + (items * 2 * a.n_kv + 3) / 4)), block(256);
+    if (a.head_dim <= 64) hipLaunchKernelGGL((k_paged_append<8>), grid, block, 0, st, a, rows);
+    else hipLaunchKernelGGL((k_paged_append<16>), grid, block, 0, st, a, rows);
+}
+
+/* ---- read ----
+ * A block's bytes and its rows in a slot both lie in one piece, so a wave
+ * turns 4 bytes a lane into 16 (8 of f16) in order.  Bound: the stores. */
+template <typename T>
+__global__ __launch_bounds__(256) void k_paged_read(PagedReadArgs a, int per) {
+    typedef T V __attribute__((ext_vector_type(4)));
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hd = a.head_dim;
+    int at = blockIdx.x / per;
+    const int v = at & 1, kh = (at >> 1) % a.n_kv, s = (at >> 1) / a.n_kv;
+    at = blockIdx.x - at * per;
+    const int len = a.len[s], slot = a.slot ? a.slot[s] : s;
+    if (slot < 0 || slot >= a.n_slots || len < 0 || len > a.most) return;
+    T *const to = (T *)(v ? a.v : a.k) + ((size_t)slot * a.n_kv + kh) * a.kv_max * hd;
+    for (int j = 4 * at + wave; PAGE_BLOCK * j < len; j += 4 * per) {
+        const int n = min(PAGE_BLOCK, len - PAGE_BLOCK * j) * hd / 4, B = block_at(a.pages, a.n_kv, s, kh, j);
+        float f = __int_as_float(0x7FC00000);
+        uint32_t w[8] = {};
+        if (B >= 0) {
+            const uint32_t *src = (const uint32_t *)((v ? a.pages.v : a.pages.k) + (size_t)B * PAGE_BLOCK * hd);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (64 * i + lane < n) w[i] = src[64 * i + lane];
+            const int e = (v ? a.pages.ev : a.pages.ek)[B];
+            if (good_exp(e)) f = exp_up(e);
+        }
+        T *dst = to + (size_t)(PAGE_BLOCK * j) * hd;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (64 * i + lane < n) {
+                V y;
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = (T)((float)(int8_t)(w[i] >> (8 * e)) * f);
+                *(V *)(dst + 4 * (64 * i + lane)) = y;
+            }
+    }
+}
+
+void launch_paged_read(const PagedReadArgs &a, bool half, hipStream_t st) {
+    /* one group of four blocks a workgroup, more where the slots have room for so many that the grid would not */
+    const long long heads = 2ll * a.n_kv * a.n, groups = (a.most + 4 * PAGE_BLOCK - 1) / (4 * PAGE_BLOCK);
+    const int per = (int)std::max(1ll, std::min(groups, (1ll << 20) / heads));
+    const dim3 grid((unsigned)(heads * per)), block(256);
+    if (half) hipLaunchKernelGGL((k_paged_read<_Float16>), grid, block, 0, st, a, per);
+    else hipLaunchKernelGGL((k_paged_read<float>), grid, block, 0, st, a, per);
+}
+
+/* ---- attention ----
+ *
+ * Weights go to the matrix units with V's power of two in them: the product
+ * takes 2^(z_j + e_j - m) n_j, z_j a score in base 2, e_j the exponent of V's
+ * block, and the reference m follows the largest z_j + e_j of blocks seen.
+ * So whatever counts most in the output is near 1 there, however the blocks'
+ * magnitudes differ, and nothing but small integers is V.  The sum l of
+ * 2^(z_j - m) takes each block's sum times 2^-e_j; with exponents within
+ * +-42 f32 holds both.  m is a whole number: every rescaling is exact.
+ *
+ * Bytes are finite, so what a row does not see meets a weight of 0 and no
+ * value; rows that see a position of a block without a page, or one that
+ * holds a value that was not finite, are NaN, and so are those whose query is
+ * not finite (poison: l is NaN). */
+namespace {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+constexpr int QMAX = 8300000;    /* three signed digits of base 256 */
+constexpr float TINY = 1e-37f;   /* factors stay above 0: -inf * 0 would be NaN */
+
+/* A wave's next 64 blocks, one a lane: where they are, and their exponents'
+ * bytes (K, V << 8) with bit 16 for one that makes rows NaN */
+struct Blocks {
+    int at, exps;
+};
+__device__ inline Blocks load_blocks(const PromptArgs &a, const Pages &p, const Work &w, int j, bool there) {
+    Blocks b = {0, 127 | 127 << 8};
+    if (!there) return b;
+    const int B = block_at(p, a.n_kv, w.sq.slot, w.kh, j);
+    if (B < 0) {
+        b.exps |= 1 << 16;
+        return b;
+    }
+    const int ek = p.ek[B], ev = p.ev[B];
+    b.at = B;
+    if (good_exp(ek) && good_exp(ev)) b.exps = ek | ev << 8;
+    else b.exps |= 1 << 16;
+    return b;
+}
+
+/* whole blocks: a span starts at one and, but for the tile's last, ends at one */
+template <int MTILE>
+__device__ inline bool find_blocks(const PromptArgs &a, const RowsPlan &p, int ratio, Work &w) {
+    if (!find_work<MTILE>(a, p, ratio, w)) return false;
+    if (w.hi < tile_hi<MTILE>(w, ratio)) w.hi &= ~(PAGE_BLOCK - 1);
+    w.lo &= ~(PAGE_BLOCK - 1);
+    return true;
+}
+
+__device__ inline float max16(float v) {   /* with the lanes 16 apart */
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return max_nan(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+/* four bytes, two pairs of f16 */
+__device__ inline void to_half(uint32_t w, h2 &a, h2 &b) {
+    const h2 bias = {(_Float16)1152.f, (_Float16)1152.f};
+    w ^= 0x80808080u;   /* + 128; under the top byte of 1024 that is 1024 + 128 + n */
+    a = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - bias;
+    b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - bias;
+}
+
+/* ---- few rows: positions over the waves ----
+ *
+ * A workgroup of four waves takes MT tiles of 16 m-rows; a wave walks blocks
+ * in pairs (every fourth pair), bytes straight from the pages into registers,
+ * no LDS and no barrier until the four waves' sums meet.
+ *
+ * S^T[position][m-row] is integer: K as it is, q as three signed digits of
+ * base 256 of q 2^s, its head's largest value to 2^22 .. 2^23 (24 bits of it),
+ * on v_mfma_i32_16x16x64_i8.  A digit's sum is exact and below 2^21; joined
+ * they are rounded once.  D lane l holds m-row l % 16, positions 4 (l / 16) + v.
+ * O^T[dim][m-row] is f16 (16x16x32) over both blocks' 32 positions in the
+ * order in which the lanes hold their weights, split in two f16; the lanes
+ * load V rows 4 (l / 16) .. + 3 of each block, dims HD / 16 (l % 16) .., and one byte
+ * permutation a pair both transposes and widens them. */
+constexpr int MN = 16;
+template <int HD>
+struct SharedPN {
+    __attribute__((aligned(16))) float mo[4][MN][HD];
+    float mm[4][MN], ml[4][MN];
+};
+template <int HD, int MT>
+__global__ __launch_bounds__(256, 2) void k_paged_n(PromptArgs a, Pages pg, RowsPlan p) {
+    constexpr int N = HD / 16, J = HD / 64, WORDS = N / 4;
+    __shared__ SharedPN<HD> sh;
+    const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
+    Work w;
+    if (!find_blocks<MN * MT>(a, p, ratio, w)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c16 = lane & 15, kq = lane >> 4;
+
+    /* step n of the wave: blocks j0 + 8 n + 2 wave, + 1; a chunk is 32 steps */
+    const int j0 = (w.lo >> 4) + 2 * wave, steps = max(0, (w.hi - w.lo - 32 * wave + 127) >> 7);
+    auto chunk = [&](int n) {
+        const int j = j0 + 8 * (n + (lane >> 1)) + (lane & 1);
+        return load_blocks(a, pg, w, j, PAGE_BLOCK * j < w.hi);
+    };
+    Blocks bl = chunk(0);
+    const size_t bytes = (size_t)PAGE_BLOCK * hd;
+    uint32_t koff[J], voff[4];
+#pragma unroll
+    for (int j = 0; j < J; j++) koff[j] = 64 * j + 16 * kq < hd ? c16 * hd + 64 * j + 16 * kq : 0;   /* q is 0 there */
+#pragma unroll
+    for (int e = 0; e < 4; e++) voff[e] = N * c16 < hd ? (4 * kq + e) * hd + N * c16 : 0;            /* not written */
+    struct Raw {
+        u32x4 k[2][J];
+        uint32_t v[8][WORDS];
+    };
+    auto load = [&](int i, Raw &r) __attribute__((always_inline)) {   /* blocks i, i + 1 of the chunk */
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const size_t at = (size_t)__builtin_amdgcn_readlane(bl.at, i + t) * bytes;
+            const int8_t *kb = pg.k + at, *vb = pg.v + at;
+#pragma unroll
+            for (int j = 0; j < J; j++) r.k[t][j] = *(const u32x4 *)(kb + koff[j]);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int n = 0; n < WORDS; n++) r.v[4 * t + e][n] = *(const uint32_t *)(vb + voff[e] + 4 * n);
+        }
+    };
+    Raw cur;
+    load(0, cur);   /* without steps: block 0 of the pages, which is there */
+
+    Lane x[MT];
+    v4i q[MT][3][J];
+    float c[MT], mx[MT], l[MT];
+    v4f o[MT][N];
+    const float base2 = LOG2E / sqrtf((float)hd);
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+        x[m] = lane_rows(a, w, MN * m, c16, MN, ratio);
+        const float *src = a.q + (size_t)x[m].r * a.q_stride + (size_t)x[m].h * hd;
+        f4 u[J][4];
+        float big = 0.f;
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                const int d = 64 * j + 16 * kq + 4 * n;
+                u[j][n] = x[m].live && d < hd ? (f4)*(const f4u *)(src + d) : f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 4; e++) big = max_nan(big, fabsf(u[j][n][e]));
+            }
+        big = other_half_max(max16(big));
+        /* 2^s that takes the largest to QMAX at most; a query below 2^-80 scores 0 */
+        const bool fine = big < INFINITY, some = fine && big > 0x1p-80f;
+        const int ex = some ? (__builtin_amdgcn_frexp_mantf(big) > (float)QMAX / 0x1p23f ? 22 : 23) - __builtin_amdgcn_frexp_expf(big) : 0;
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                uint32_t y[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    y[e] = some ? (uint32_t)((int)__builtin_rintf(__builtin_amdgcn_ldexpf(u[j][n][e], ex)) + 0x808080) : 0x808080u;
+#pragma unroll
+                for (int b = 0; b < 3; b++) {
+                    const uint32_t sel = (uint32_t)(b | (4 + b) << 8);
+                    const uint32_t lo = __builtin_amdgcn_perm(y[1], y[0], sel), hi = __builtin_amdgcn_perm(y[3], y[2], sel);
+                    q[m][b][j][n] = (int)(__builtin_amdgcn_perm(hi, lo, 0x05040100u) ^ 0x80808080u);
+                }
+            }
+        c[m] = __builtin_amdgcn_ldexpf(base2, -ex);
+        mx[m] = -INFINITY, l[m] = fine ? 0.f : __int_as_float(0x7FC00000);
+#pragma unroll
+        for (int n = 0; n < N; n++) o[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const float one = opaque_one();
+    for (int n = 0; n < steps; n++) {
+        const int i = 2 * (n & 31), t = w.lo + 32 * wave + 128 * n;
+        int ex[2];
+#pragma unroll
+        for (int b = 0; b < 2; b++) ex[b] = __builtin_amdgcn_readlane(bl.exps, i + b);
+        const Raw r = cur;
+        if (n + 1 < steps) {
+            if (((n + 1) & 31) == 0) bl = chunk(n + 1);
+            load(2 * ((n + 1) & 31), cur);
+        }
+        h8 ph[MT], pl[MT];
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            float s[2][4], ck[2], top = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                v4i d[3];
+#pragma unroll
+                for (int g = 0; g < 3; g++) {
+                    d[g] = v4i{0, 0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < J; j++)
+                        d[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, r.k[b][j]), q[m][g][j], d[g], 0, 0, 0);
+                }
+                ck[b] = fmaxf(c[m] * exp_up(ex[b] & 255), TINY);
+#pragma unroll
+                for (int v = 0; v < 4; v++) s[b][v] = fmaf((float)(d[2][v] * 256 + d[1][v]), 256.f, (float)d[0][v]);
+            }
+            if (t + 31 > x[m].all_hi || t < x[m].all_lo) {   /* uniform */
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        const int pos = t + 16 * b + 4 * kq + v;
+                        s[b][v] = pos <= x[m].last && pos >= x[m].first ? s[b][v] : -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const float u = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3]));
+                top = fmaxf(top, fmaf(u, ck[b], (float)((ex[b] >> 8 & 255) - 127)));
+            }
+            top = other_half_max(max16(top));
+            if (__any(top > mx[m] + LAG_H)) {
+                const float mn = fmaxf(mx[m], ceilf(top));
+                const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[m] - mn);
+                mx[m] = mn;
+                l[m] *= alpha;
+#pragma unroll
+                for (int k = 0; k < N; k++) o[m][k] *= alpha;
+            }
+            const float ref = mx[m] == -INFINITY ? 0.f : SHIFT_H - mx[m];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const int ev = ex[b] >> 8 & 255;
+                const float add = ref + (float)(ev - 127);
+                float e[4];
+#pragma unroll
+                for (int v = 0; v < 4; v++) e[v] = __builtin_amdgcn_exp2f(fmaf(s[b][v], ck[b], add));
+                l[m] = fmaf((e[0] + e[1]) + (e[2] + e[3]), exp_down(ev), l[m]);
+#pragma unroll
+                for (int v = 0; v < 4; v += 2) {
+                    h2 hi, lo;
+                    split2(e[v], e[v + 1], e[v], e[v + 1], one, hi, lo);
+                    ph[m][4 * b + v] = hi[0], ph[m][4 * b + v + 1] = hi[1];
+                    pl[m][4 * b + v] = lo[0], pl[m][4 * b + v + 1] = lo[1];
+                }
+            }
+            if ((ex[0] | ex[1]) >> 16) {   /* uniform, hardly ever */
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+                    if (ex[b] >> 16 && x[m].first <= t + 16 * b + 15 && x[m].last >= t + 16 * b) l[m] = __int_as_float(0x7FC00000);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            h8 v;
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const h2 bias = {(_Float16)1152.f, (_Float16)1152.f};
+                const uint32_t sel = 0x0C000C00u | (uint32_t)(4 + (k & 3)) << 16 | (uint32_t)(k & 3);
+                const h2 y = __builtin_bit_cast(h2, __builtin_amdgcn_perm(r.v[e + 1][k >> 2], r.v[e][k >> 2], sel) ^ 0x64806480u) - bias;
+                v[e] = y[0], v[e + 1] = y[1];
+            }
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                o[m][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[m], o[m][k], 0, 0, 0);
+                o[m][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[m], o[m][k], 0, 0, 0);
+            }
+        }
+    }
+
+    /* the waves' sums as one, in wave order: 16 threads a row, HD / 16 dims each */
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+        l[m] += __shfl_xor(l[m], 16, 64);
+        l[m] += __shfl_xor(l[m], 32, 64);
+        if (m) __syncthreads();
+#pragma unroll
+        for (int v = 0; v < 4; v++)
+#pragma unroll
+            for (int n = 0; n < N; n += 4)
+                *(f4 *)&sh.mo[wave][c16][N * (4 * kq + v) + n] = f4{o[m][n][v], o[m][n + 1][v], o[m][n + 2][v], o[m][n + 3][v]};
+        if (kq == 0) sh.mm[wave][c16] = mx[m], sh.ml[wave][c16] = l[m];
+        __syncthreads();
+        const int row = tid >> 4, d0 = (tid & 15) * N;
+        const Lane y = lane_rows(a, w, MN * m, row, MN, ratio);
+        float M = sh.mm[0][row];
+#pragma unroll
+        for (int g = 1; g < 4; g++) M = fmaxf(M, sh.mm[g][row]);
+        const float base = M == -INFINITY ? 0.f : M;
+        float L = 0.f, r[N];
+#pragma unroll
+        for (int n = 0; n < N; n++) r[n] = 0.f;
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const float e = __builtin_amdgcn_exp2f(sh.mm[g][row] - base);
+            L = fmaf(sh.ml[g][row], e, L);
+#pragma unroll
+            for (int n = 0; n < N; n++) r[n] = fmaf(sh.mo[g][row][d0 + n], e, r[n]);
+        }
+        if (!y.live || d0 >= hd) continue;
+        float *dst, f;
+        if (p.nrec) {
+            const size_t rec = ((size_t)y.r * a.n_heads + y.h) * p.nrec + w.rec;
+            f = 0x1p-8f;   /* 2^-SHIFT_H */
+            if (d0 == 0) write_ml(p, w, rec, M, L * f);
+            if (M == -INFINITY) continue;   /* a record of no position has no sums */
+            dst = p.o + rec * hd + d0;
+        } else {
+            f = 1.f;
+            if (a.sinks) {
+                const float ref = M - SHIFT_H, sk = a.sinks[y.h] * LOG2E, mn = fmaxf(ref, sk), b2 = mn == -INFINITY ? 0.f : mn;
+                f = exp2f(ref - b2);
+                L = L * f + exp2f(sk - b2);
+            }
+            f /= L;
+            dst = a.out + (size_t)y.r * a.out_stride + (size_t)y.h * hd + d0;
+        }
+#pragma unroll
+        for (int n = 0; n < N; n += 4) *(f4u *)(dst + n) = f4{r[n] * f, r[n + 1] * f, r[n + 2] * f, r[n + 3] * f};
+    }
+}
+
+}  // namespace
+
+static_assert(SHIFT_H == 8.f, "k_paged_n's 2^-8");
+
+/* How a call is cut, from the host's arguments alone (the lengths are on the
+ * device), as rows_cut does for dense caches. */
+static RowsPlan paged_cut(const PromptArgs &a) {
+    RowsPlan p = {};
+    const int n_seqs = a.s.n, n_kv = a.n_kv, ratio = a.n_heads / n_kv;
+    const long long m = (long long)a.s.rows * ratio, tile = MN;
+    const int sees = a.window > 0 ? (int)std::min<long long>(a.s.kv_max, (long long)a.window + tile / ratio + 1) : a.s.kv_max;
+    const long long tiles = std::max((m + tile - 1) / tile, (long long)n_seqs), wgs = tiles * n_kv;
+    p.target = std::max(1, 512 / n_kv);
+    p.unit = 128;
+    const double t = sees * (1.0 / 128) * (a.head_dim > 64 ? 1 : 0.5), r = (double)m * n_kv * a.head_dim * 8 / 4.5e6;
+    const int most = (int)std::min<long long>({64, (sees + p.unit - 1) / p.unit, std::max(1ll, 512 / wgs)});
+    auto us = [&](int n) { return t / n + r * n + (n == 1 ? -r : 4); };
+    const int n = std::max(1, std::min(most, (int)std::sqrt(t / r)));
+    const int best = n < most && us(n + 1) < us(n) ? n + 1 : n;
+    p.cap = us(best) < us(1) ? best : 1;
+    if (n_seqs > 1 && p.cap > 1)
+        p.cap = (int)std::min<long long>({64, (sees + p.unit - 1) / p.unit, std::max<long long>(4ll * p.cap, 4ll * p.target / tiles)});
+    p.search = p.cap == 1 && n_seqs > 256;
+    p.items = p.search ? (int)(m / tile) + n_seqs : (int)std::min(m / tile + n_seqs, m) + (p.cap > 1 ? p.target : 0);
+    p.nrec = p.cap > 1 ? p.cap : 0;
+    return p;
+}
+
+static size_t ml_bytes(const RowsPlan &p, const PromptArgs &a) {
+    return ((size_t)a.s.rows * a.n_heads * p.nrec * 16 + 255) & ~(size_t)255;
+}
+
+size_t attention_paged_need(const PromptArgs &a) {
+    const RowsPlan p = paged_cut(a);
+    return p.nrec ? ml_bytes(p, a) + (size_t)a.s.rows * a.n_heads * p.nrec * a.head_dim * 4 : 0;
+}
+
+/* For every call of at most these sizes: tiles are cut only while their spans
+ * are at most the workgroups that run at once, with several sequences four
+ * times as many, so the m-rows times their spans are at most the m-rows of
+ * so many tiles. */
+size_t attention_paged_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max) {
+    const long long row_heads = (long long)n_rows * n_heads, spans = std::min(64, (kv_max + 127) / 128);
+    if (spans == 1) return 0;
+    const long long records = std::min(row_heads * spans, 16ll * 512 * (n_seqs > 1 ? 4 : 1));
+    return (size_t)records * (16 + 4 * (size_t)head_dim) + 256;
+}
+
+template <int HD>
+static void launch_paged(const PromptArgs &a, const Pages &pg, const RowsPlan &p, hipStream_t st) {
+    const dim3 grid((unsigned)(p.items * a.n_kv));
+    hipLaunchKernelGGL((k_paged_n<HD, 1>), grid, dim3(256), 0, st, a, pg, p);
+}
+
+void launch_attention_paged(const PromptArgs &a, const Pages &pg, void *scratch, hipStream_t st) {
+    RowsPlan p = paged_cut(a);
+    p.ml = (float *)scratch;
+    p.o = (float *)((uint8_t *)scratch + ml_bytes(p, a));
+    if (a.head_dim > 64) launch_paged<128>(a, pg, p, st);
+    else launch_paged<64>(a, pg, p, st);
+    if (p.nrec) launch_rows_combine(a, p, st);
+}
+
+}  // namespace tg

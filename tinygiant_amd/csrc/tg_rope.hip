@@ -1,0 +1,102 @@
+/*
+ * tg_rope.hip -- rotary positions: tables of cosines and sines, rows turned.
+ *
+ * The reference's engine makes one table on the host and turns whole heads in
+ * half layout (apply_rope_inplace, csrc/libtinygiant.c:702-719).
+ */
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "tg_paged.h"
+#include "tg_turn.hpp"
+
+namespace tg {
+
+/* ---- tables ----
+ * cos and sin of 2 pi t, t = position * (frequency / 2 pi) turns.  t is a
+ * product in 64 bits, off by 2^-53 of itself: 2^-33 turns at position 2^20 of
+ * the fastest pair.  Its nearest quarter is taken off, which is exact, and the rest,
+ * at most an eighth of a turn, goes through the Taylor sums of both functions
+ * in 64 bits to below 2^-50, so that what is stored is the f32 nearest to the
+ * formula's value (a 32-bit product is off by 0.06 turns there).  A lane has
+ * four pairs of a position, 16 bytes of each table.
+ * Bound: the stores, beside about 30 64-bit operations a pair. */
+__device__ inline void turn_of(double t, double &c, double &s) {
+    t -= __builtin_rint(t);
+    const double k = __builtin_rint(4.0 * t);
+    const double x = (t - 0.25 * k) * 6.283185307179586476925, y = x * x;
+    double p = -7.6471637318198165e-13;                 /* -1 / 15! */
+    p = fma(p, y, 1.6059043836821614e-10);
+    p = fma(p, y, -2.5052108385441719e-08);
+    p = fma(p, y, 2.7557319223985893e-06);
+    p = fma(p, y, -1.9841269841269841e-04);
+    p = fma(p, y, 8.3333333333333333e-03);
+    p = fma(p, y, -1.6666666666666666e-01);
+    const double sn = fma(x * y, p, x);
+    double q = 4.7794773323873853e-14;                  /* 1 / 16! */
+    q = fma(q, y, -1.1470745597729725e-11);
+    q = fma(q, y, 2.0876756987868099e-09);
+    q = fma(q, y, -2.7557319223985891e-07);
+    q = fma(q, y, 2.4801587301587302e-05);
+    q = fma(q, y, -1.3888888888888889e-03);
+    q = fma(q, y, 4.1666666666666664e-02);
+    q = fma(q, y, -0.5);
+    const double cs = fma(q, y, 1.0);
+    const int n = (int)k;   /* -2 .. 2 quarters */
+    const double a = n & 1 ? sn : cs, b = n & 1 ? cs : sn;
+    c = n == 1 || n == 2 || n == -2 ? -a : a;
+    s = n == -1 || n == 2 || n == -2 ? -b : b;
+}
+
+__global__ __launch_bounds__(256) void k_rope_tables(RopeTablesArgs a) {
+    const int per = a.pairs / 4;
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= (long long)a.len * per) return;
+    const int row = (int)(at / per), i = 4 * (int)(at - (long long)row * per);
+    const double pos = (double)((long long)a.first + row), m = (double)a.mscale;
+    f4 c, s;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        double x, y;
+        turn_of(pos * a.turns[i + e], x, y);
+        c[e] = (float)(x * m), s[e] = (float)(y * m);
+    }
+    *(f4u *)(a.cos + 4 * at) = c;
+    *(f4u *)(a.sin + 4 * at) = s;
+}
+
+void launch_rope_tables(const RopeTablesArgs &a, hipStream_t st) {
+    const long long n = (long long)a.len * (a.pairs / 4);
+    hipLaunchKernelGGL(k_rope_tables, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+}
+
+/* ---- rows ----
+ * A lane takes eight values of a head in two pieces of four that hold whole
+ * pairs (turn_pieces), so that nothing is exchanged and out may be x.  A
+ * workgroup has 256 such units of a row's.  Bound: the rows' bytes. */
+__global__ __launch_bounds__(256) void k_rope(RopeArgs a) {
+    const int per = a.head_dim / 8;   /* units of a head */
+    const int u = (int)blockIdx.y * 256 + (int)threadIdx.x, r = (int)blockIdx.x;
+    if (u >= a.heads * per) return;
+    const int pos = a.pos[r];
+    if (pos < 0 || pos >= a.turn.len) return;
+    const int h = u / per, l = u - h * per;
+    const Pieces p = turn_pieces(a.turn, l);
+    const float *src = a.x + (size_t)r * a.x_stride + (size_t)h * a.head_dim;
+    float *dst = a.out + (size_t)r * a.out_stride + (size_t)h * a.head_dim;
+    f4 x = *(const f4u *)(src + p.a), y = *(const f4u *)(src + p.b);
+    if (p.turned) {
+        const f4 c = *(const f4u *)(a.turn.cos + (size_t)pos * (a.turn.dim / 2) + 4 * l);
+        const f4 s = *(const f4u *)(a.turn.sin + (size_t)pos * (a.turn.dim / 2) + 4 * l);
+        turn_pair(a.turn.inter, c, s, x, y);
+    }
+    *(f4u *)(dst + p.a) = x;
+    *(f4u *)(dst + p.b) = y;
+}
+
+void launch_rope(const RopeArgs &a, hipStream_t st) {
+    const int units = a.heads * (a.head_dim / 8);
+    hipLaunchKernelGGL(k_rope, dim3((unsigned)a.rows, (unsigned)((units + 255) / 256)), dim3(256), 0, st, a);
+}
+
+}  // namespace tg
