@@ -316,6 +316,7 @@ namespace {
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef int v4i __attribute__((ext_vector_type(4)));
 constexpr int QMAX = 8300000;    /* three signed digits of base 256 */
+constexpr float UNSHIFT = 1.f / (float)(1 << (int)SHIFT_H);
 constexpr float TINY = 1e-37f;   /* factors stay above 0: -inf * 0 would be NaN */
 
 /* A wave's next 64 blocks, one a lane: where they are, and their exponents'
@@ -594,7 +595,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_n(PromptArgs a, Pages pg, Rows
         float *dst, f;
         if (p.nrec) {
             const size_t rec = ((size_t)y.r * a.n_heads + y.h) * p.nrec + w.rec;
-            f = 0x1p-8f;   /* 2^-SHIFT_H */
+            f = UNSHIFT;
             if (d0 == 0) write_ml(p, w, rec, M, L * f);
             if (M == -INFINITY) continue;   /* a record of no position has no sums */
             dst = p.o + rec * hd + d0;
@@ -613,66 +614,370 @@ __global__ __launch_bounds__(256, 2) void k_paged_n(PromptArgs a, Pages pg, Rows
     }
 }
 
+/* ---- many rows ----
+ *
+ * The products of k_rows_h (tg_prompt.hip), 32 m-rows a wave on 32x32x16 f16:
+ * S^T = K Q^T with q as two f16, O^T += V^T P^T with the weights as two.  Bytes
+ * are loaded two tiles of 64 positions ahead and widened to f16, which holds
+ * them, as they are stored to one of two LDS buffers one tile ahead.  With
+ * KG = 2, two groups of MW waves take the tiles in turn; J blocks of 32
+ * positions are computed together. */
+template <int HD, int MW, int KG>
+struct SharedPW {
+    __attribute__((aligned(1024))) uint8_t bufs[KG][2][2][KT * HD * 2];
+    long long where[KG == 2 ? 32 * MW : 1];
+};
+
+/* The wave's rows finished, as write_rows does for dense caches; a NaN is the
+ * row's own here. */
+template <int HD>
+__device__ inline void write_paged(const PromptArgs &a, const RowsPlan &p, const Work &w, const Lane &x, int lane, float mx, float l,
+                                   const f16v (&o)[HD / 32], uint8_t *stage, long long *where) {
+    const int half = lane >> 5, row = lane & 31, hd = a.head_dim;
+    bool write = x.live;
+    long long at;
+    float f;
+    if (p.nrec) {
+        const size_t rec = ((size_t)x.r * a.n_heads + x.h) * p.nrec + w.rec;
+        f = UNSHIFT;
+        if (write && half == 0) write_ml(p, w, rec, mx, l * f);
+        write = write && mx > -INFINITY;      /* a record of no position has no sums */
+        at = (long long)(rec * hd);
+    } else {
+        f = 1.f;
+        if (a.sinks && write) {
+            const float ref = mx - SHIFT_H, sk = a.sinks[x.h] * LOG2E, M = fmaxf(ref, sk), base = M == -INFINITY ? 0.f : M;
+            f = exp2f(ref - base);
+            l = l * f + exp2f(sk - base);
+        }
+        f /= l;
+        at = (long long)x.r * a.out_stride + (long long)x.h * hd;
+    }
+    if (stage && half == 0) where[row] = write ? at : -1;
+    float *dst = (p.nrec ? p.o : a.out) + at;
+#pragma unroll
+    for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            const int dim = 32 * d + 8 * v + 4 * half;
+            f4 y;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = o[d][4 * v + e] * f;
+            if (stage) *(f4 *)(stage + row * (HD * 4) + row_piece<HD>(row, 8 * d + 2 * v + half)) = y;
+            else if (write && dim < hd) *(f4u *)(dst + dim) = y;
+        }
+}
+
+template <int HD, int MW, int KG, int J>
+__global__ __launch_bounds__(64 * MW * KG, 2) void k_paged_w(PromptArgs a, Pages pg, RowsPlan p) {
+    constexpr int RB = HD * 2, TILE = KT * RB;          /* bytes of a row in LDS, of a tile of K or V */
+    constexpr int DB = HD / 32, STEPS = HD / 16;
+    constexpr int LR = 1024 / HD, NL = KT / LR / MW;    /* rows a load of the wave covers, loads a tile and matrix */
+    static_assert(NL >= 1 && 16 % LR == 0, "a load is of one block");
+    __shared__ SharedPW<HD, MW, KG> sh;
+    auto &bufs = sh.bufs;
+    const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
+    Work w;
+    if (!find_blocks<32 * MW>(a, p, ratio, w)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int half = lane >> 5, group = wave / MW, mwave = wave % MW;
+    static_assert(KG == 1 || sizeof bufs >= MW * 256 * (HD / 2 + 3), "merge_groups");
+    uint8_t(*buf)[2][TILE] = bufs[group];
+
+    /* tile n: blocks j0 + 4 n ..; a chunk of blocks is 16 tiles */
+    const int j0 = w.lo >> 4, tiles = (w.hi - w.lo + KT - 1) / KT;
+    auto chunk = [&](int n) {
+        const int j = j0 + 4 * (n & ~15) + lane;
+        return load_blocks(a, pg, w, j, PAGE_BLOCK * j < w.hi);
+    };
+    Blocks bl = chunk(0);
+    int have = 0;   /* the chunk that bl is of */
+    const size_t bytes = (size_t)PAGE_BLOCK * hd;
+    const int lrow = lane / (HD / 16), piece = lane % (HD / 16);
+    const bool on = 16 * piece < hd;
+    u32x4 raw[2][NL];
+    int next[4];   /* exponents of the tile in raw */
+    auto load = [&](int n) __attribute__((always_inline)) {
+        if (n >> 4 != have) bl = chunk(n), have = n >> 4;
+#pragma unroll
+        for (int b = 0; b < 4; b++) next[b] = __builtin_amdgcn_readlane(bl.exps, (4 * n & 63) + b);
+#pragma unroll
+        for (int k = 0; k < NL; k++) {
+            const int row = LR * (mwave + MW * k);
+            const size_t at = (size_t)__builtin_amdgcn_readlane(bl.at, (4 * n & 63) + (row >> 4)) * bytes;
+            const uint32_t off = (uint32_t)(((row & 15) + lrow) * hd + 16 * piece);
+            raw[0][k] = raw[1][k] = u32x4{0, 0, 0, 0};
+            if (on) raw[0][k] = *(const u32x4 *)(pg.k + at + off), raw[1][k] = *(const u32x4 *)(pg.v + at + off);
+        }
+    };
+    auto store = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int k = 0; k < NL; k++) {
+                const int key = LR * (mwave + MW * k) + lrow;
+                h2 y[8];
+#pragma unroll
+                for (int e = 0; e < 4; e++) to_half(raw[m][k][e], y[2 * e], y[2 * e + 1]);
+                uint8_t *at = &buf[b][m][key * RB];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const h8 z = {y[4 * e][0], y[4 * e][1], y[4 * e + 1][0], y[4 * e + 1][1],
+                                  y[4 * e + 2][0], y[4 * e + 2][1], y[4 * e + 3][0], y[4 * e + 3][1]};
+                    *(h8 *)(at + (((2 * piece + e) ^ swz<HD>(key)) << 4)) = z;
+                }
+            }
+    };
+    load(group);
+    static_assert(KG == 1 || 32 * MW * HD * 4 == sizeof bufs / 2, "q fits");
+    if constexpr (KG == 2) copy_q<HD, 32 * MW>(a, w, ratio, wave, MW * KG, bufs[0][1][0], bufs[1][1][0]);
+    const Lane x = lane_rows(a, w, 32 * mwave, lane & 31, 32, ratio);
+    h8 qh[STEPS], ql[STEPS];
+    float c;
+    if constexpr (KG == 2) {
+        wait_copies();
+        bar_lds();
+        const uint8_t *mine = bufs[mwave / (MW / 2)][1][0] + (mwave % (MW / 2) * 32 + (lane & 31)) * (HD * 4);
+        c = load_q<HD>(hd, half, [&](int i) { return *(const f4 *)(mine + row_piece<HD>(lane & 31, i)); }, qh, ql);
+    } else {
+        c = load_q<HD>(hd, half, memory_q(a, x), qh, ql);
+    }
+    /* a query that is not finite makes its row NaN, and its f16 nothing else's: the m-row is the lane */
+    float l = 0.f;
+#pragma unroll
+    for (int s = 0; s < STEPS; s++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) l = fmaf((float)qh[s][e], 0.f, l);
+    f16v o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) o[d][v] = 0.f;
+    float mx = -INFINITY;
+    const uint32_t kaddr = k_operand<HD>(lane);
+    uint32_t vaddr[DB][2];
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) vaddr[d][e] = TILE + v_operand<HD>(lane, d, e);
+    const float one = opaque_one();
+
+    int stored[4], ex[4];
+    store(0);
+#pragma unroll
+    for (int e = 0; e < 4; e++) stored[e] = next[e];
+    if (group + KG < tiles) load(group + KG);
+    int b = 0;
+    for (int n0 = 0; n0 < tiles; n0 += KG, b ^= 1) {
+        const int n = n0 + group, t = w.lo + KT * n;
+        bar_lds();   /* every wave has stored this tile, and is done with the other buffer */
+#pragma unroll
+        for (int e = 0; e < 4; e++) ex[e] = stored[e];
+        if (n + KG < tiles) {
+            store(b ^ 1);
+#pragma unroll
+            for (int e = 0; e < 4; e++) stored[e] = next[e];
+            if (n + 2 * KG < tiles) load(n + 2 * KG);
+        }
+        if (t > x.any_hi || t + KT <= x.any_lo || n >= tiles) continue;   /* uniform in the wave */
+#pragma unroll 1
+        for (int i = 0; i < KT; i += 32 * J) {
+            const int at = t + i;
+            if (J == 1 && (at > x.any_hi || at + 32 <= x.any_lo)) continue;
+            const Lds tile = (Lds)buf[b][0] + i * RB;
+            int eg[2 * J];   /* of each 16 positions */
+#pragma unroll
+            for (int g = 0; g < 2 * J; g++) eg[g] = J == 1 && i ? ex[2 + g] : ex[g];
+            f16v s[J];
+            h8 k0[J], k1[J];
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+#pragma unroll
+                for (int v = 0; v < 16; v++) s[j][v] = 0.f;
+                k0[j] = lds_row(tile + kaddr + j * 32 * RB);
+            }
+#pragma unroll
+            for (int st = 0; st < STEPS; st++) {   /* the next step's operands are read a step ahead */
+                const Lds ahead = tile + (kaddr ^ (uint32_t)((st + 1) << 5));
+#pragma unroll
+                for (int j = 0; j < J; j++) k1[j] = st + 1 < STEPS ? lds_row(ahead + j * 32 * RB) : k0[j];
+#pragma unroll
+                for (int j = 0; j < J; j++) s[j] = MFMA_H(k0[j], ql[st], s[j]);
+#pragma unroll
+                for (int j = 0; j < J; j++) s[j] = MFMA_H(k0[j], qh[st], s[j]);
+#pragma unroll
+                for (int j = 0; j < J; j++) k0[j] = k1[j];
+            }
+            auto column = [&](int u) __attribute__((always_inline)) {
+                const int q = u / DB, d = u % DB;
+                return h8_of(lds_column(tile + vaddr[d][0] + q * 16 * RB), lds_column(tile + vaddr[d][1] + q * 16 * RB));
+            };
+            h8 v0 = column(0), v1 = column(1);
+            float top = -INFINITY, ck[2 * J];
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                mask_scores(s[j], at + 32 * j + 4 * half, x);
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    float u = s[j][8 * g];
+#pragma unroll
+                    for (int v = 1; v < 8; v++) u = max_nan(u, s[j][8 * g + v]);
+                    ck[2 * j + g] = fmaxf(c * exp_up(eg[2 * j + g] & 255), TINY);
+                    top = max_nan(top, fmaf(u, ck[2 * j + g], (float)((eg[2 * j + g] >> 8 & 255) - 127)));
+                }
+            }
+            top = other_half_max(top);
+            if (__any(top > mx + LAG_H)) {
+                const float mn = max_nan(mx, ceilf(top));
+                const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
+                mx = mn;
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < DB; d++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) o[d][v] *= alpha;
+            }
+            const float ref = mx == -INFINITY ? 0.f : SHIFT_H - mx;
+            __builtin_amdgcn_iglp_opt(2);
+            h8 ph[2 * J], pl[2 * J];
+#pragma unroll
+            for (int g = 0; g < 2 * J; g++) {
+                const float add = ref + (float)((eg[g] >> 8 & 255) - 127);
+                float sum[2] = {0.f, 0.f};
+#pragma unroll
+                for (int v = 0; v < 8; v += 2) {
+                    const float e0 = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + v], ck[g], add));
+                    const float e1 = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + v + 1], ck[g], add));
+                    sum[0] += e0, sum[1] += e1;
+                    h2 hi, lo;
+                    split2(e0, e1, e0, e1, one, hi, lo);
+                    ph[g][v] = hi[0], ph[g][v + 1] = hi[1], pl[g][v] = lo[0], pl[g][v + 1] = lo[1];
+                }
+                l = fmaf(sum[0] + sum[1], exp_down(eg[g] >> 8 & 255), l);
+            }
+#pragma unroll
+            for (int u = 0; u < 2 * J * DB; u += 2) {
+                const bool more = u + 2 < 2 * J * DB;
+                const h8 n0 = more ? column(u + 2) : v0, n1 = more ? column(u + 3) : v1;
+                const int q = u / DB, d = u % DB;
+                o[d] = MFMA_H(v0, pl[q], o[d]);
+                o[d + 1] = MFMA_H(v1, pl[q], o[d + 1]);
+                o[d] = MFMA_H(v0, ph[q], o[d]);
+                o[d + 1] = MFMA_H(v1, ph[q], o[d + 1]);
+                v0 = n0, v1 = n1;
+            }
+            int odd = 0;
+#pragma unroll
+            for (int g = 0; g < 2 * J; g++) odd |= eg[g];
+            if (odd >> 16) {   /* uniform, hardly ever */
+#pragma unroll
+                for (int g = 0; g < 2 * J; g++)
+                    if (eg[g] >> 16 && x.first <= at + 16 * g + 15 && x.last >= at + 16 * g) l = __int_as_float(0x7FC00000);
+            }
+        }
+    }
+    l = other_half_sum(l);
+    int oexp = 0;
+    if (KG == 2 && tiles > 1) merge_groups<HD, MW>((float *)bufs, wave, lane, mx, l, oexp, o);
+    else __syncthreads();   /* one group, or the second had no tile: all are done with the tiles */
+    constexpr int STRIDE = 64 * (HD / 2 + 3) * 4;   /* a wave's share of merge_groups' room */
+    if (group == 0)
+        write_paged<HD>(a, p, w, x, lane, mx, l, o, KG == 2 ? (uint8_t *)bufs + wave * STRIDE : nullptr,
+                        sh.where + (KG == 2 ? 32 * wave : 0));
+    if constexpr (KG == 2) {
+        __syncthreads();
+        store_rows<HD, 32 * MW>(hd, (const uint8_t *)bufs, STRIDE, sh.where, p.nrec ? p.o : a.out, wave, MW * KG);
+    }
+}
+
 }  // namespace
 
-static_assert(SHIFT_H == 8.f, "k_paged_n's 2^-8");
-
 /* How a call is cut, from the host's arguments alone (the lengths are on the
- * device), as rows_cut does for dense caches. */
-static RowsPlan paged_cut(const PromptArgs &a) {
-    RowsPlan p = {};
+ * device), as rows_cut does for dense caches:
+ *   narrow  16 m-rows a workgroup, positions over its waves
+ *   wide    128 m-rows, two groups of four waves on tiles in turn
+ *   short   128 m-rows, four waves, for few positions a row
+ *   full    the same, two workgroups a CU on long spans */
+namespace {
+
+enum Shape { NARROW, SHORT, WIDE, FULL };
+constexpr int SHAPE_ROWS[] = {16, 128, 128, 128};
+constexpr long long NARROW_WORK = 1 << 18;
+constexpr int SHORT_BELOW = 512;
+struct Cut {
+    RowsPlan p;
+    Shape shape;
+};
+Shape shape_of(long long m, long long seqs, int n_kv, int positions) {
+    if (m <= 16 * seqs || (m <= 128 * seqs && m * positions <= NARROW_WORK)) return NARROW;
+    if (positions < SHORT_BELOW) return SHORT;
+    return m / 128 * n_kv > 512 ? FULL : WIDE;
+}
+
+Cut paged_cut(const PromptArgs &a) {
+    Cut k = {};
+    RowsPlan &p = k.p;
     const int n_seqs = a.s.n, n_kv = a.n_kv, ratio = a.n_heads / n_kv;
-    const long long m = (long long)a.s.rows * ratio, tile = MN;
-    const int sees = a.window > 0 ? (int)std::min<long long>(a.s.kv_max, (long long)a.window + tile / ratio + 1) : a.s.kv_max;
+    const long long m = (long long)a.s.rows * ratio;
+    auto sees = [&](int rows) { return a.window > 0 ? (int)std::min<long long>(a.s.kv_max, (long long)a.window + rows / ratio + 1) : a.s.kv_max; };
+    k.shape = shape_of(m, n_seqs, n_kv, sees(128));
+    const int tile = SHAPE_ROWS[k.shape], positions = sees(tile), slots = k.shape == NARROW ? 512 : 256;
     const long long tiles = std::max((m + tile - 1) / tile, (long long)n_seqs), wgs = tiles * n_kv;
-    p.target = std::max(1, 512 / n_kv);
+    p.target = std::max(1, slots / n_kv);
     p.unit = 128;
-    const double t = sees * (1.0 / 128) * (a.head_dim > 64 ? 1 : 0.5), r = (double)m * n_kv * a.head_dim * 8 / 4.5e6;
-    const int most = (int)std::min<long long>({64, (sees + p.unit - 1) / p.unit, std::max(1ll, 512 / wgs)});
+    /* us(n): a span's positions, and what n records a row take to write and read, at 4.5 TB/s, with the combine's launch */
+    const double t = positions * (k.shape == NARROW ? 1.0 : 3.4) / 128 * (a.head_dim > 64 ? 1 : 0.5);
+    const double r = (double)m * n_kv * a.head_dim * 8 / 4.5e6;
+    const int most = (int)std::min<long long>({64, (positions + p.unit - 1) / p.unit, std::max(1ll, slots / wgs)});
     auto us = [&](int n) { return t / n + r * n + (n == 1 ? -r : 4); };
-    const int n = std::max(1, std::min(most, (int)std::sqrt(t / r)));
+    const int n = std::max(1, std::min(most, (int)std::sqrt(t / r)));   /* the best, or the next */
     const int best = n < most && us(n + 1) < us(n) ? n + 1 : n;
     p.cap = us(best) < us(1) ? best : 1;
-    if (n_seqs > 1 && p.cap > 1)
-        p.cap = (int)std::min<long long>({64, (sees + p.unit - 1) / p.unit, std::max<long long>(4ll * p.cap, 4ll * p.target / tiles)});
+    if (n_seqs > 1 && p.cap > 1)   /* room for a sequence much longer than the others */
+        p.cap = (int)std::min<long long>({64, (positions + p.unit - 1) / p.unit, std::max<long long>(4ll * p.cap, 4ll * p.target / tiles)});
     p.search = p.cap == 1 && n_seqs > 256;
     p.items = p.search ? (int)(m / tile) + n_seqs : (int)std::min(m / tile + n_seqs, m) + (p.cap > 1 ? p.target : 0);
     p.nrec = p.cap > 1 ? p.cap : 0;
-    return p;
+    return k;
 }
 
-static size_t ml_bytes(const RowsPlan &p, const PromptArgs &a) {
-    return ((size_t)a.s.rows * a.n_heads * p.nrec * 16 + 255) & ~(size_t)255;
+size_t ml_bytes(const RowsPlan &p, const PromptArgs &a) { return ((size_t)a.s.rows * a.n_heads * p.nrec * 16 + 255) & ~(size_t)255; }
+
+template <int HD>
+void launch_paged(const PromptArgs &a, const Pages &pg, const Cut &k, const RowsPlan &p, hipStream_t st) {
+    const dim3 grid((unsigned)(p.items * a.n_kv));
+    if (k.shape == NARROW) hipLaunchKernelGGL((k_paged_n<HD, 1>), grid, dim3(256), 0, st, a, pg, p);
+    else if (k.shape == SHORT) hipLaunchKernelGGL((k_paged_w<HD, 4, 1, 1>), grid, dim3(256), 0, st, a, pg, p);
+    else if (k.shape == WIDE) hipLaunchKernelGGL((k_paged_w<HD, 4, 2, 2>), grid, dim3(512), 0, st, a, pg, p);
+    else hipLaunchKernelGGL((k_paged_w<HD, 4, 1, 2>), grid, dim3(256), 0, st, a, pg, p);
 }
+
+}  // namespace
 
 size_t attention_paged_need(const PromptArgs &a) {
-    const RowsPlan p = paged_cut(a);
+    const RowsPlan p = paged_cut(a).p;
     return p.nrec ? ml_bytes(p, a) + (size_t)a.s.rows * a.n_heads * p.nrec * a.head_dim * 4 : 0;
 }
 
-/* For every call of at most these sizes: tiles are cut only while their spans
- * are at most the workgroups that run at once, with several sequences four
- * times as many, so the m-rows times their spans are at most the m-rows of
- * so many tiles. */
+/* For every call of at most these sizes: tiles of a shape are cut only while
+ * their spans are at most the workgroups that run at once, with several
+ * sequences four times as many, so the m-rows times their spans are at most the
+ * m-rows of so many tiles. */
 size_t attention_paged_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max) {
+    const long long m = (long long)n_rows * (n_heads / n_kv);
     const long long row_heads = (long long)n_rows * n_heads, spans = std::min(64, (kv_max + 127) / 128);
     if (spans == 1) return 0;
-    const long long records = std::min(row_heads * spans, 16ll * 512 * (n_seqs > 1 ? 4 : 1));
+    const long long records = std::min(row_heads * spans, (m <= 16 ? 16ll * 512 : 128ll * 256) * (n_seqs > 1 ? 4 : 1));
     return (size_t)records * (16 + 4 * (size_t)head_dim) + 256;
 }
 
-template <int HD>
-static void launch_paged(const PromptArgs &a, const Pages &pg, const RowsPlan &p, hipStream_t st) {
-    const dim3 grid((unsigned)(p.items * a.n_kv));
-    hipLaunchKernelGGL((k_paged_n<HD, 1>), grid, dim3(256), 0, st, a, pg, p);
-}
-
 void launch_attention_paged(const PromptArgs &a, const Pages &pg, void *scratch, hipStream_t st) {
-    RowsPlan p = paged_cut(a);
+    const Cut k = paged_cut(a);
+    RowsPlan p = k.p;
     p.ml = (float *)scratch;
     p.o = (float *)((uint8_t *)scratch + ml_bytes(p, a));
-    if (a.head_dim > 64) launch_paged<128>(a, pg, p, st);
-    else launch_paged<64>(a, pg, p, st);
+    if (a.head_dim > 64) launch_paged<128>(a, pg, k, p, st);
+    else launch_paged<64>(a, pg, k, p, st);
     if (p.nrec) launch_rows_combine(a, p, st);
 }
 
