@@ -465,6 +465,25 @@ def test_attention_long(tg, nh, nkv, hd, lens, past, size):
     say(f"  worst error / tolerance {_attend(tg, Attend(sum(lens), nh, nkv, hd, lens, past, size, sinks=hd == 64, spread=4)):.3f}")
 
 
+@pytest.mark.parametrize("nh,nkv,hd", [(32, 4, 128), (16, 2, 64), (15, 3, 80), (8, 8, 96), (64, 1, 32)])
+@pytest.mark.parametrize("lens,past,window", [
+    ([1, 200, 9, 0, 1, 40], [900, 0, 2200, 5, 40, 600], 0), ([300, 1], [30, 3500], 0), ([1, 150, 1, 180], [4000, 2500, 0, 0], 0),
+    ([17, 16, 130, 1], [1500, 700, 20, 3000], 600), ([1] * 20 + [260], [61 * i for i in range(20)] + [500], 0), ([400, 0, 129], [0, 0, 1400], 0)])
+def test_attention_mixed(tg, nh, nkv, hd, lens, past, window):
+    """Prompts, chunks, verify passes and single tokens in one call."""
+    say(f"attention mixed {nh, nkv, hd} lens={lens} past={past} window={window}")
+    a = Attend(sum(lens) + hd, nh, nkv, hd, lens, past, 32, window=window, sinks=nkv != 2, lead=2, tail=1, spread=3)
+    say(f"  worst error / tolerance {_attend(tg, a):.3f}")
+
+
+def test_attention_mixed_many(tg):
+    """More sequences than a wave looks at, and more tiles than are cut."""
+    say("attention mixed, many sequences")
+    _attend(tg, Attend(31, 8, 2, 32, [40 if i % 3 else 1 for i in range(150)], [(13 * i) % 600 for i in range(150)]))
+    say("attention mixed, many tiles")
+    _attend(tg, Attend(32, 64, 8, 16, [300] * 7 + [1, 0, 3], [(90 * i) % 500 for i in range(10)], room=200))
+
+
 @pytest.mark.parametrize("nh,nkv,hd", [(1024, 16, 128), (1024, 1024, 16), (64, 1, 128), (1, 1, 128), (1024, 512, 16)])
 def test_ends_of_the_layouts(tg, nh, nkv, hd):
     say(f"attention {nh, nkv, hd}")

@@ -1673,6 +1673,7 @@ TG_API void tg_hip_rope_tables_dev(float *cos_dev, float *sin_dev, int rope_len,
         else if (scaling == SMOOTH) share = std::min(1.0, std::max(0.0, (orig_len * f / two_pi - low) / ((double)high - low)));
         if (share < 1.0) f = f * share + f / factor * (1.0 - share);
         a.turns[i] = f / two_pi;
+        a.step_cos[i] = cos(f), a.step_sin[i] = sin(f);
     }
     const hipError_t before = hipPeekAtLastError();
     launch_rope_tables(a, stream ? (hipStream_t)stream : g.st);

@@ -18,6 +18,7 @@
  *              k_paged_w   128
  */
 #include <hip/hip_runtime.h>
+#include <limits.h>
 #include <math.h>
 #include <stdint.h>
 
@@ -339,13 +340,107 @@ __device__ inline Blocks load_blocks(const PromptArgs &a, const Pages &p, const 
     return b;
 }
 
-/* whole blocks: a span starts at one and, but for the tile's last, ends at one */
+/* One part of a call: the sequences of at least `least` and at most `most`
+ * m-rows.  Where a part's tiles are cut, spans of a dense part write records
+ * as those of dense caches do, [row and head][nrec]; those of a part of a
+ * mixed call [item][KV head][m-row of the tile], as only some tiles are cut
+ * and it is not known which: a tile of one span writes its rows at once, and
+ * where the records of the others are stands at the tile's place in `tiles`. */
+struct Part {
+    RowsPlan p;
+    int least, most;
+    struct Tile {
+        int item, count, step, last;   /* of the first span; spans; from one to the next, but the last one's */
+    } *tiles;                          /* null: dense */
+};
+struct Class {
+    int least, most, ratio;
+    __device__ inline void operator()(Seq &q) const {
+        const int m = q.n * ratio;
+        if (m < least || m > most) q.n = 0;
+    }
+};
+
+/* tiles of 16 are of sequences with at most 8 */
+constexpr int FEW = 128;
 template <int MTILE>
-__device__ inline bool find_blocks(const PromptArgs &a, const RowsPlan &p, int ratio, Work &w) {
-    if (!find_work<MTILE>(a, p, ratio, w)) return false;
+__device__ inline int tile_place(const Work &w, int ratio) {
+    return (MTILE == 16 ? w.sq.slot * (FEW / 16) : start_of<MTILE>(w.sq.r0, w.sq.slot, ratio)) + w.m0 / MTILE;
+}
+/* Item b of a call of at most 64 sequences: as find_span, but the whole spans of
+ * all tiles come first and what is left of each behind them, so that short
+ * spans fill the end.  last: the item of the tile's last span. */
+template <int MTILE>
+__device__ inline bool find_cut(const PromptArgs &a, const RowsPlan &p, int ratio, int b, Work &w, const Class &keep, int &last) {
+    const int lane = threadIdx.x & 63;
+    Seq q = {0, 0, 0, 0};
+    if (lane < a.s.n) q = seq_at(a.s, lane);
+    keep(q);
+    const int nt = div_up(q.n * ratio, MTILE), end = q.past + q.n;
+    const int sees = a.window > 0 ? min(end, a.window + (MTILE - 1) / ratio + 1) : end;   /* at most */
+    const float sum = wave_sum((float)nt * (float)sees);
+    int per = div_up(max(1, (int)fminf(ceilf(sum / (float)p.target), 1e9f)), p.unit) * p.unit;
+    if (div_up(sees, per) > p.cap) per = div_up(div_up(sees, p.cap), p.unit) * p.unit;
+    const int whole_end = wave_scan(nt * (int)((unsigned)sees / (unsigned)per)), rest_end = wave_scan(nt);
+    const int wholes = __builtin_amdgcn_readlane(whole_end, 63);
+    const bool rest = b >= wholes;
+    const int place = rest ? b - wholes : b;
+    const uint64_t past = __ballot((rest ? rest_end : whole_end) > place);
+    if (!past) return false;
+    const int at = __builtin_ctzll(past), n = __builtin_amdgcn_readlane(nt, at);
+    const int whole0 = at ? __builtin_amdgcn_readlane(whole_end, at - 1) : 0, rest0 = at ? __builtin_amdgcn_readlane(rest_end, at - 1) : 0;
+    per = __builtin_amdgcn_readlane(per, at);
+    w.sq = lane_seq(q, at);
+    const int in = place - (rest ? rest0 : whole0);
+    int split = rest ? 0 : in / n;
+    const int tile = in - split * n;
+    w.m0 = (n - 1 - tile) * MTILE;
+    set_rows(w, ratio);
+    const int lo = tile_lo(a, w), hi = tile_hi<MTILE>(w, ratio), whole = (int)((unsigned)(hi - lo) / (unsigned)per);
+    const bool left = hi - lo > whole * per;
+    if (rest ? !left : split >= whole) return false;
+    if (rest) split = whole;
+    w.rec = p.pre_ns + split;
+    w.count = split ? 0 : whole + left;
+    last = left ? wholes + rest0 + tile : whole0 + (whole - 1) * n + tile;
+    w.lo = lo + split * per;
+    w.hi = min(hi, w.lo + per);
+    return true;
+}
+
+/* The work of item b / n_kv.  Whole blocks: a span starts at one and, but for
+ * the tile's last, ends at one. */
+template <int MTILE>
+__device__ inline bool find_blocks(const PromptArgs &a, const Part &pt, int ratio, int b, Work &w) {
+    const RowsPlan &p = pt.p;
+    const int item = b / a.n_kv;
+    w.prefix = false;
+    w.kh = b - item * a.n_kv;
+    const Class keep = {pt.least, pt.most, ratio};
+    int last = -1;
+    if (p.search) {
+        if (!find_tile<MTILE>(a, p, ratio, item, w, keep)) return false;
+    } else if (p.cap > 1 && a.s.n <= 64) {
+        if (!find_cut<MTILE>(a, p, ratio, item, w, keep, last)) return false;
+    } else if (!find_span<MTILE>(a, p, ratio, item, w, keep)) {
+        return false;
+    }
     if (w.hi < tile_hi<MTILE>(w, ratio)) w.hi &= ~(PAGE_BLOCK - 1);
     w.lo &= ~(PAGE_BLOCK - 1);
+    if (pt.tiles) {
+        if (w.count && w.kh == 0 && threadIdx.x == 0) {
+            const int n = div_up(w.sq.n * ratio, MTILE);
+            pt.tiles[tile_place<MTILE>(w, ratio)] = Part::Tile{item, w.count, n, last < 0 ? item + (w.count - 1) * n : last};
+        }
+        w.rec = item;
+    }
     return true;
+}
+/* where m-row `at` of the tile goes: -1 straight to the output, else its record */
+template <int MTILE>
+__device__ inline long long record_of(const PromptArgs &a, const Part &pt, const Work &w, const Lane &x, int at) {
+    if (pt.tiles) return w.count == 1 ? -1 : ((long long)w.rec * a.n_kv + w.kh) * MTILE + at;
+    return pt.p.nrec ? ((long long)x.r * a.n_heads + x.h) * pt.p.nrec + w.rec : -1;
 }
 
 __device__ inline float max16(float v) {   /* with the lanes 16 apart */
@@ -382,12 +477,13 @@ struct SharedPN {
     float mm[4][MN], ml[4][MN];
 };
 template <int HD, int MT>
-__global__ __launch_bounds__(256, 2) void k_paged_n(PromptArgs a, Pages pg, RowsPlan p) {
+__device__ inline __attribute__((always_inline)) void paged_n(const PromptArgs &a, const Pages &pg, const Part &pt, int item,
+                                                              SharedPN<HD> &sh) {
     constexpr int N = HD / 16, J = HD / 64, WORDS = N / 4;
-    __shared__ SharedPN<HD> sh;
     const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
+    const RowsPlan &p = pt.p;
     Work w;
-    if (!find_blocks<MN * MT>(a, p, ratio, w)) return;
+    if (!find_blocks<MN * MT>(a, pt, ratio, item, w)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c16 = lane & 15, kq = lane >> 4;
 
@@ -593,8 +689,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_n(PromptArgs a, Pages pg, Rows
         }
         if (!y.live || d0 >= hd) continue;
         float *dst, f;
-        if (p.nrec) {
-            const size_t rec = ((size_t)y.r * a.n_heads + y.h) * p.nrec + w.rec;
+        const long long rec = record_of<MN * MT>(a, pt, w, y, MN * m + row);
+        if (rec >= 0) {
             f = UNSHIFT;
             if (d0 == 0) write_ml(p, w, rec, M, L * f);
             if (M == -INFINITY) continue;   /* a record of no position has no sums */
@@ -614,6 +710,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_n(PromptArgs a, Pages pg, Rows
     }
 }
 
+template <int HD, int MT>
+__global__ __launch_bounds__(256, 2) void k_paged_n(PromptArgs a, Pages pg, Part pt) {
+    __shared__ SharedPN<HD> sh;
+    paged_n<HD, MT>(a, pg, pt, blockIdx.x, sh);
+}
+
 /* ---- many rows ----
  *
  * The products of k_rows_h (tg_prompt.hip), 32 m-rows a wave on 32x32x16 f16:
@@ -630,19 +732,19 @@ struct SharedPW {
 
 /* The wave's rows finished, as write_rows does for dense caches; a NaN is the
  * row's own here. */
-template <int HD>
-__device__ inline void write_paged(const PromptArgs &a, const RowsPlan &p, const Work &w, const Lane &x, int lane, float mx, float l,
-                                   const f16v (&o)[HD / 32], uint8_t *stage, long long *where) {
+template <int HD, int MTILE>
+__device__ inline void write_paged(const PromptArgs &a, const Part &pt, const Work &w, const Lane &x, int from, int lane, float mx,
+                                   float l, const f16v (&o)[HD / 32], uint8_t *stage, long long *where) {
     const int half = lane >> 5, row = lane & 31, hd = a.head_dim;
     bool write = x.live;
     long long at;
     float f;
-    if (p.nrec) {
-        const size_t rec = ((size_t)x.r * a.n_heads + x.h) * p.nrec + w.rec;
+    const long long rec = record_of<MTILE>(a, pt, w, x, from + row);   /* uniform whether there is one */
+    if (rec >= 0) {
         f = UNSHIFT;
-        if (write && half == 0) write_ml(p, w, rec, mx, l * f);
+        if (write && half == 0) write_ml(pt.p, w, rec, mx, l * f);
         write = write && mx > -INFINITY;      /* a record of no position has no sums */
-        at = (long long)(rec * hd);
+        at = rec * hd;
     } else {
         f = 1.f;
         if (a.sinks && write) {
@@ -654,7 +756,7 @@ __device__ inline void write_paged(const PromptArgs &a, const RowsPlan &p, const
         at = (long long)x.r * a.out_stride + (long long)x.h * hd;
     }
     if (stage && half == 0) where[row] = write ? at : -1;
-    float *dst = (p.nrec ? p.o : a.out) + at;
+    float *dst = (rec >= 0 ? pt.p.o : a.out) + at;
 #pragma unroll
     for (int d = 0; d < HD / 32; d++)
 #pragma unroll
@@ -669,16 +771,16 @@ __device__ inline void write_paged(const PromptArgs &a, const RowsPlan &p, const
 }
 
 template <int HD, int MW, int KG, int J>
-__global__ __launch_bounds__(64 * MW * KG, 2) void k_paged_w(PromptArgs a, Pages pg, RowsPlan p) {
+__device__ inline __attribute__((always_inline)) void paged_w(const PromptArgs &a, const Pages &pg, const Part &pt, int item,
+                                                              SharedPW<HD, MW, KG> &sh) {
     constexpr int RB = HD * 2, TILE = KT * RB;          /* bytes of a row in LDS, of a tile of K or V */
     constexpr int DB = HD / 32, STEPS = HD / 16;
     constexpr int LR = 1024 / HD, NL = KT / LR / MW;    /* rows a load of the wave covers, loads a tile and matrix */
     static_assert(NL >= 1 && 16 % LR == 0, "a load is of one block");
-    __shared__ SharedPW<HD, MW, KG> sh;
     auto &bufs = sh.bufs;
     const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
     Work w;
-    if (!find_blocks<32 * MW>(a, p, ratio, w)) return;
+    if (!find_blocks<32 * MW>(a, pt, ratio, item, w)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int half = lane >> 5, group = wave / MW, mwave = wave % MW;
     static_assert(KG == 1 || sizeof bufs >= MW * 256 * (HD / 2 + 3), "merge_groups");
@@ -882,12 +984,106 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_paged_w(PromptArgs a, Pages
     else __syncthreads();   /* one group, or the second had no tile: all are done with the tiles */
     constexpr int STRIDE = 64 * (HD / 2 + 3) * 4;   /* a wave's share of merge_groups' room */
     if (group == 0)
-        write_paged<HD>(a, p, w, x, lane, mx, l, o, KG == 2 ? (uint8_t *)bufs + wave * STRIDE : nullptr,
-                        sh.where + (KG == 2 ? 32 * wave : 0));
+        write_paged<HD, 32 * MW>(a, pt, w, x, 32 * mwave, lane, mx, l, o, KG == 2 ? (uint8_t *)bufs + wave * STRIDE : nullptr,
+                                 sh.where + (KG == 2 ? 32 * wave : 0));
     if constexpr (KG == 2) {
         __syncthreads();
-        store_rows<HD, 32 * MW>(hd, (const uint8_t *)bufs, STRIDE, sh.where, p.nrec ? p.o : a.out, wave, MW * KG);
+        const bool records = pt.tiles ? w.count != 1 : pt.p.nrec > 0;
+        store_rows<HD, 32 * MW>(hd, (const uint8_t *)bufs, STRIDE, sh.where, records ? pt.p.o : a.out, wave, MW * KG);
     }
+}
+
+template <int HD, int MW, int KG, int J>
+__global__ __launch_bounds__(64 * MW * KG, 2) void k_paged_w(PromptArgs a, Pages pg, Part pt) {
+    __shared__ SharedPW<HD, MW, KG> sh;
+    paged_w<HD, MW, KG, J>(a, pg, pt, blockIdx.x, sh);
+}
+
+/* A mixed call in one launch: sequences of many rows in tiles of 128, those of
+ * few in tiles of 16, each kind cut into spans by its own positions. */
+template <int HD>
+__global__ __launch_bounds__(256, 2) void k_paged_both(PromptArgs a, Pages pg, Part many, Part few) {
+    __shared__ union {
+        SharedPW<HD, 4, 1> w;
+        SharedPN<HD> n;
+    } sh;
+    const int first = many.p.items * a.n_kv;
+    if ((int)blockIdx.x < first) paged_w<HD, 4, 1, 2>(a, pg, many, blockIdx.x, sh.w);
+    else paged_n<HD, 1>(a, pg, few, (int)blockIdx.x - first, sh.n);
+}
+
+/* The records of a cut tile's rows as one: a workgroup of 16 waves has a KV
+ * head and a tile of 16 rows, or half of one of 128; a wave a row at a time,
+ * HD / 4 lanes a record. */
+template <int HD, int MTILE>
+__device__ inline __attribute__((always_inline)) void join_tile(const PromptArgs &a, const Part &pt, int b) {
+    constexpr int G = HD / 4, PER = 64 / G, N = 4, ROWS = MTILE == 16 ? 16 : 64;
+    const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int place = b / a.n_kv, from = 0;
+    Work w;
+    w.prefix = false, w.kh = b - place * a.n_kv;
+    const Class keep = {pt.least, pt.most, ratio};
+    if constexpr (MTILE == 16) {
+        const int s = place / (FEW / 16);
+        w.sq = seq_at(a.s, s);
+        keep(w.sq);
+        w.m0 = 16 * (place - s * (FEW / 16));
+        if (w.m0 >= w.sq.n * ratio) return;
+        set_rows(w, ratio);
+    } else {
+        from = 64 * (place & 1);
+        if (!find_tile<MTILE>(a, pt.p, ratio, place >> 1, w, keep)) return;
+        place = tile_place<MTILE>(w, ratio);
+    }
+    const Part::Tile tile = pt.tiles[place];
+    if (tile.count <= 1) return;
+    const int rows = min(from + ROWS, min(MTILE, w.sq.n * ratio - w.m0)), g = lane / G, d = 4 * (lane % G);
+    for (int m = from + wave; m < rows; m += 16) {
+        int i, j;
+        w.row(m, ratio, i, j);
+        const int r = w.sq.r0 + i, h = w.kh * ratio + j;
+        const float sink = a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
+        auto rec = [&](int c) {
+            return ((size_t)(c == tile.count - 1 ? tile.last : tile.item + c * tile.step) * a.n_kv + w.kh) * MTILE + m;
+        };
+        f4 stat = {-INFINITY, 0.f, 0.f, 0.f}, y[N];   /* at most 64 records */
+        if (lane < tile.count) stat = *(const f4 *)(pt.p.ml + 4 * rec(lane));
+        auto load = [&](int c0) {
+#pragma unroll
+            for (int q = 0; q < N; q++) {
+                const int c = c0 + q * PER + g;
+                y[q] = f4{0.f, 0.f, 0.f, 0.f};
+                if (c < tile.count && d < hd) y[q] = *(const f4 *)(pt.p.o + rec(c) * hd + d);
+            }
+        };
+        load(0);
+        const float M = fmaxf(wave_max(stat[0]), sink), base = M == -INFINITY ? 0.f : M;
+        /* -1: a record of no position, whose sums are not written */
+        const float e = stat[0] != -INFINITY ? exp2f(stat[0] - base) : -1.f;
+        float l = wave_sum(e < 0.f ? 0.f : stat[1] * e);
+        f4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int c0 = 0; c0 < tile.count; c0 += N * PER) {
+            if (c0) load(c0);
+#pragma unroll
+            for (int q = 0; q < N; q++) {
+                const int c = c0 + q * PER + g;
+                const float f = __shfl(e, c & 63, 64);
+                if (c < tile.count && !(f < 0.f)) o += y[q] * f;
+            }
+        }
+#pragma unroll
+        for (int q = 32; q >= G; q >>= 1)
+#pragma unroll
+            for (int k = 0; k < 4; k++) o[k] += __shfl_xor(o[k], q, 64);
+        if (a.sinks) l += exp2f(sink - base);
+        if (lane < G && d < hd) *(f4u *)(a.out + (size_t)r * a.out_stride + (size_t)h * hd + d) = o * (1.f / l);
+    }
+}
+template <int HD>
+__global__ __launch_bounds__(1024) void k_paged_join(PromptArgs a, Part many, Part few, int first) {
+    if ((int)blockIdx.x < first) join_tile<HD, 16>(a, few, blockIdx.x);
+    else join_tile<HD, 128>(a, many, (int)blockIdx.x - first);
 }
 
 }  // namespace
@@ -897,88 +1093,155 @@ __global__ __launch_bounds__(64 * MW * KG, 2) void k_paged_w(PromptArgs a, Pages
  *   narrow  16 m-rows a workgroup, positions over its waves
  *   wide    128 m-rows, two groups of four waves on tiles in turn
  *   short   128 m-rows, four waves, for few positions a row
- *   full    the same, two workgroups a CU on long spans */
+ *   full    the same, two workgroups a CU on long spans
+ *   mixed   several sequences, of many rows together: full for those of more
+ *           than FEW m-rows, narrow for the others */
 namespace {
 
-enum Shape { NARROW, SHORT, WIDE, FULL };
-constexpr int SHAPE_ROWS[] = {16, 128, 128, 128};
+enum Shape { NARROW, SHORT, WIDE, FULL, MIXED };
 constexpr long long NARROW_WORK = 1 << 18;
-constexpr int SHORT_BELOW = 512;
+constexpr int SHORT_BELOW = 512, MOST_SPANS = 64;
 struct Cut {
-    RowsPlan p;
     Shape shape;
+    Part part, few;   /* few: of a mixed call */
 };
 Shape shape_of(long long m, long long seqs, int n_kv, int positions) {
     if (m <= 16 * seqs || (m <= 128 * seqs && m * positions <= NARROW_WORK)) return NARROW;
     if (positions < SHORT_BELOW) return SHORT;
+    if (seqs > 1) return MIXED;
     return m / 128 * n_kv > 512 ? FULL : WIDE;
+}
+
+/* a mixed call's part in tiles of `tile` m-rows; beyond `often` workgroups there
+ * are enough of them to keep the chip busy without cuts */
+constexpr int OFTEN = 1024;
+Part mixed_part(const PromptArgs &a, long long m, int tile, int slots, int least, int most) {
+    Part k = {};
+    k.least = least, k.most = most;
+    long long tiles = std::min(m / tile + a.s.n, m);
+    if (most < INT_MAX) tiles = std::min(tiles, (long long)a.s.n * ((most + tile - 1) / tile));
+    k.p.target = std::max(1, slots / a.n_kv);
+    k.p.unit = 128;
+    k.p.cap = tiles * a.n_kv > OFTEN && least > 1 ? 1 : 64;
+    k.p.items = (int)tiles + (k.p.cap > 1 ? k.p.target : 0);
+    return k;
 }
 
 Cut paged_cut(const PromptArgs &a) {
     Cut k = {};
-    RowsPlan &p = k.p;
     const int n_seqs = a.s.n, n_kv = a.n_kv, ratio = a.n_heads / n_kv;
     const long long m = (long long)a.s.rows * ratio;
     auto sees = [&](int rows) { return a.window > 0 ? (int)std::min<long long>(a.s.kv_max, (long long)a.window + rows / ratio + 1) : a.s.kv_max; };
     k.shape = shape_of(m, n_seqs, n_kv, sees(128));
-    const int tile = SHAPE_ROWS[k.shape], positions = sees(tile), slots = k.shape == NARROW ? 512 : 256;
+    if (k.shape == MIXED) {
+        k.part = mixed_part(a, m, 128, (m / 128 + n_seqs) * n_kv > 256 ? 256 : 512, FEW + 1, INT_MAX);
+        k.few = mixed_part(a, m, 16, 512, 1, FEW);
+        return k;
+    }
+    k.part.least = 1, k.part.most = INT_MAX;
+    RowsPlan &p = k.part.p;
+    const int tile = k.shape == NARROW ? 16 : 128, positions = sees(tile);
+    const int slots = k.shape == NARROW ? 512 : 256;
     const long long tiles = std::max((m + tile - 1) / tile, (long long)n_seqs), wgs = tiles * n_kv;
-    p.target = std::max(1, slots / n_kv);
+    /* of several sequences fewer than run at once: what their cuts leave over fills the rest (64 rows behind 61 .. 8,314
+     * positions, 4 KV heads of 128: 65.9 us; as many as run 74.3, half 74.0) */
+    p.target = std::max(1, (k.shape == NARROW && n_seqs > 1 && a.head_dim > 64 ? 384 : slots) / n_kv);
     p.unit = 128;
     /* us(n): a span's positions, and what n records a row take to write and read, at 4.5 TB/s, with the combine's launch */
     const double t = positions * (k.shape == NARROW ? 1.0 : 3.4) / 128 * (a.head_dim > 64 ? 1 : 0.5);
     const double r = (double)m * n_kv * a.head_dim * 8 / 4.5e6;
-    const int most = (int)std::min<long long>({64, (positions + p.unit - 1) / p.unit, std::max(1ll, slots / wgs)});
+    const int most = (int)std::min<long long>({MOST_SPANS, (positions + p.unit - 1) / p.unit, std::max(1ll, slots / wgs)});
     auto us = [&](int n) { return t / n + r * n + (n == 1 ? -r : 4); };
     const int n = std::max(1, std::min(most, (int)std::sqrt(t / r)));   /* the best, or the next */
     const int best = n < most && us(n + 1) < us(n) ? n + 1 : n;
     p.cap = us(best) < us(1) ? best : 1;
     if (n_seqs > 1 && p.cap > 1)   /* room for a sequence much longer than the others */
-        p.cap = (int)std::min<long long>({64, (positions + p.unit - 1) / p.unit, std::max<long long>(4ll * p.cap, 4ll * p.target / tiles)});
+        p.cap = (int)std::min<long long>({MOST_SPANS, (positions + p.unit - 1) / p.unit, std::max<long long>(4ll * p.cap, 4ll * p.target / tiles)});
     p.search = p.cap == 1 && n_seqs > 256;
     p.items = p.search ? (int)(m / tile) + n_seqs : (int)std::min(m / tile + n_seqs, m) + (p.cap > 1 ? p.target : 0);
     p.nrec = p.cap > 1 ? p.cap : 0;
     return k;
 }
 
-size_t ml_bytes(const RowsPlan &p, const PromptArgs &a) { return ((size_t)a.s.rows * a.n_heads * p.nrec * 16 + 255) & ~(size_t)255; }
+/* A call's scratch, in order: statistics and sums of the records, of a mixed
+ * call those of both parts and where each tile's are */
+struct Room {
+    size_t records, places;   /* of a part */
+    size_t ml() const { return (records * 16 + 255) & ~(size_t)255; }
+    size_t o(int hd) const { return records * 4 * (size_t)hd; }
+    size_t at() const { return (places * sizeof(Part::Tile) + 255) & ~(size_t)255; }
+    size_t all(int hd) const { return ml() + o(hd) + at(); }
+};
+Room room_of(const PromptArgs &a, const Part &k, int tile, bool mixed) {
+    if (k.p.cap <= 1) return Room{0, 0};
+    if (!mixed) return Room{(size_t)a.s.rows * a.n_heads * k.p.nrec, 0};
+    const long long m = (long long)a.s.rows * (a.n_heads / a.n_kv);
+    return Room{(size_t)k.p.items * a.n_kv * tile, (size_t)(tile == 16 ? a.s.n * (FEW / 16) : m / tile + a.s.n)};
+}
+int tile_of(Shape s) { return s == NARROW ? 16 : 128; }
 
 template <int HD>
-void launch_paged(const PromptArgs &a, const Pages &pg, const Cut &k, const RowsPlan &p, hipStream_t st) {
-    const dim3 grid((unsigned)(p.items * a.n_kv));
-    if (k.shape == NARROW) hipLaunchKernelGGL((k_paged_n<HD, 1>), grid, dim3(256), 0, st, a, pg, p);
-    else if (k.shape == SHORT) hipLaunchKernelGGL((k_paged_w<HD, 4, 1, 1>), grid, dim3(256), 0, st, a, pg, p);
-    else if (k.shape == WIDE) hipLaunchKernelGGL((k_paged_w<HD, 4, 2, 2>), grid, dim3(512), 0, st, a, pg, p);
-    else hipLaunchKernelGGL((k_paged_w<HD, 4, 1, 2>), grid, dim3(256), 0, st, a, pg, p);
+void launch_paged(const PromptArgs &a, const Pages &pg, const Cut &k, hipStream_t st) {
+    const dim3 grid((unsigned)((k.part.p.items + k.few.p.items) * a.n_kv));
+#define PAGED(threads, ...) hipLaunchKernelGGL((__VA_ARGS__), grid, dim3(threads), 0, st, a, pg, k.part)
+    if (k.shape == NARROW) PAGED(256, k_paged_n<HD, 1>);
+    else if (k.shape == SHORT) PAGED(256, k_paged_w<HD, 4, 1, 1>);
+    else if (k.shape == WIDE) PAGED(512, k_paged_w<HD, 4, 2, 2>);
+    else if (k.shape == FULL) PAGED(256, k_paged_w<HD, 4, 1, 2>);
+#undef PAGED
+    else {
+        hipLaunchKernelGGL((k_paged_both<HD>), grid, dim3(256), 0, st, a, pg, k.part, k.few);
+        const long long m = (long long)a.s.rows * (a.n_heads / a.n_kv);
+        const int first = a.s.n * (FEW / 16) * a.n_kv, more = k.part.p.cap > 1 ? (int)(m / 128 + a.s.n) * 2 * a.n_kv : 0;
+        hipLaunchKernelGGL((k_paged_join<HD>), dim3((unsigned)(first + more)), dim3(1024), 0, st, a, k.part, k.few, first);
+    }
 }
 
 }  // namespace
 
 size_t attention_paged_need(const PromptArgs &a) {
-    const RowsPlan p = paged_cut(a).p;
-    return p.nrec ? ml_bytes(p, a) + (size_t)a.s.rows * a.n_heads * p.nrec * a.head_dim * 4 : 0;
+    const Cut k = paged_cut(a);
+    const bool mixed = k.shape == MIXED;
+    return room_of(a, k.part, tile_of(k.shape), mixed).all(a.head_dim) + (mixed ? room_of(a, k.few, 16, true).all(a.head_dim) : 0);
 }
 
-/* For every call of at most these sizes: tiles of a shape are cut only while
- * their spans are at most the workgroups that run at once, with several
+/* For every call of at most these sizes.  Tiles of a dense cut are cut only
+ * while their spans are at most the workgroups that run at once, with several
  * sequences four times as many, so the m-rows times their spans are at most the
- * m-rows of so many tiles. */
+ * m-rows of so many tiles.  A mixed call has a record's room for every m-row
+ * of its items: those of many rows at most OFTEN and what the target adds, or none. */
 size_t attention_paged_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max) {
     const long long m = (long long)n_rows * (n_heads / n_kv);
-    const long long row_heads = (long long)n_rows * n_heads, spans = std::min(64, (kv_max + 127) / 128);
+    const long long row_heads = (long long)n_rows * n_heads, spans = std::min(MOST_SPANS, (kv_max + 127) / 128);
     if (spans == 1) return 0;
-    const long long records = std::min(row_heads * spans, (m <= 16 ? 16ll * 512 : 128ll * 256) * (n_seqs > 1 ? 4 : 1));
-    return (size_t)records * (16 + 4 * (size_t)head_dim) + 256;
+    auto bytes = [&](long long records) { return (size_t)records * (16 + 4 * (size_t)head_dim) + 256; };
+    size_t most = bytes(std::min(row_heads * spans, (m <= 16 ? 16ll * 512 : 128ll * 256) * (n_seqs > 1 ? 4 : 1)));
+    if (n_seqs > 1 && kv_max >= SHORT_BELOW && m > 16) {
+        const long long target = std::max(1, 512 / n_kv);
+        const long long many = std::min(std::min(m / 128 + n_seqs, m), (long long)OFTEN / n_kv) + target;
+        const long long few = std::min(std::min(m / 16 + n_seqs, m), 8ll * n_seqs) + target;
+        const size_t places = (size_t)(m / 128 + n_seqs + (FEW / 16) * (long long)n_seqs) * sizeof(Part::Tile) + 512;
+        most = std::max(most, bytes(many * n_kv * 128) + bytes(few * n_kv * 16) + places);
+    }
+    return most;
 }
 
 void launch_attention_paged(const PromptArgs &a, const Pages &pg, void *scratch, hipStream_t st) {
-    const Cut k = paged_cut(a);
-    RowsPlan p = k.p;
-    p.ml = (float *)scratch;
-    p.o = (float *)((uint8_t *)scratch + ml_bytes(p, a));
-    if (a.head_dim > 64) launch_paged<128>(a, pg, k, p, st);
-    else launch_paged<64>(a, pg, k, p, st);
-    if (p.nrec) launch_rows_combine(a, p, st);
+    Cut k = paged_cut(a);
+    const bool mixed = k.shape == MIXED;
+    uint8_t *at = (uint8_t *)scratch;
+    auto place = [&](Part &x, int tile) {
+        const Room room = room_of(a, x, tile, mixed);
+        x.p.ml = (float *)at;
+        x.p.o = (float *)(at + room.ml());
+        x.tiles = room.places ? (Part::Tile *)(at + room.ml() + room.o(a.head_dim)) : nullptr;
+        at += room.all(a.head_dim);
+    };
+    place(k.part, tile_of(k.shape));
+    if (mixed) place(k.few, 16);
+    if (a.head_dim > 64) launch_paged<128>(a, pg, k, st);
+    else launch_paged<64>(a, pg, k, st);
+    if (k.part.p.nrec) launch_rows_combine(a, k.part.p, st);
 }
 
 }  // namespace tg

@@ -10,6 +10,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "tg_device.hpp"
 #include "tg_prompt.h"
 #include "tg_xchg.hpp"
@@ -173,17 +175,22 @@ __device__ inline int tile_hi(const Work &w, int ratio) {
     return w.sq.past + min(w.sq.n - 1, i1) + 1;
 }
 
+/* which sequences a part of a call takes: all.  Another type gives a sequence
+ * that its part leaves to others no rows. */
+struct Everyone {};
+
 /* Tile b of the sequences' tiles of MTILE m-rows, late rows first (they see
  * the most positions).  Sequence s has its tiles from place
  * cu[s] ratio / MTILE + s on, where there is room for them whatever the
  * sequences before it left over: no sum over those is needed. */
-template <int MTILE>
-__device__ inline bool find_tile(const PromptArgs &a, const RowsPlan &p, int ratio, int b, Work &w) {
+template <int MTILE, class Keep = Everyone>
+__device__ inline bool find_tile(const PromptArgs &a, const RowsPlan &p, int ratio, int b, Work &w, Keep keep = {}) {
     const PackedSeqs &c = a.s;
     const int lane = threadIdx.x & 63;
     const Run run = wave_narrow<MTILE>(c, ratio, b);
     Seq q = {0, 0, 0, 0};
     if (lane < run.count) q = seq_at(c, run.at + lane);
+    if constexpr (!std::is_same_v<Keep, Everyone>) keep(q);
     const uint64_t m = __ballot(lane < run.count && start_of<MTILE>(q.r0, run.at + lane, ratio) <= b);
     if (!m) return false;
     const int at = 63 - __builtin_clzll(m);
@@ -203,14 +210,15 @@ __device__ inline bool find_tile(const PromptArgs &a, const RowsPlan &p, int rat
  * p.target spans (a sequence's tiles count as its longest); with p.cap 1, one
  * span a tile.  A wave counts 64 sequences at a time; sums of positions are
  * floats, the same in every workgroup. */
-template <int MTILE>
-__device__ inline bool find_span(const PromptArgs &a, const RowsPlan &p, int ratio, int b, Work &w) {
+template <int MTILE, class Keep = Everyone>
+__device__ inline bool find_span(const PromptArgs &a, const RowsPlan &p, int ratio, int b, Work &w, Keep keep = {}) {
     const PackedSeqs &c = a.s;
     const int lane = threadIdx.x & 63;
     Seq q = {0, 0, 0, 0};
     auto load = [&](int s0) {
         q.n = 0;
         if (s0 + lane < c.n) q = seq_at(c, s0 + lane);
+        if constexpr (!std::is_same_v<Keep, Everyone>) keep(q);
     };
     auto tiles = [&]() { return div_up(q.n * ratio, MTILE); };
     auto sees = [&]() {   /* positions of the sequence's tiles, at most */
