@@ -1666,14 +1666,16 @@ TG_API void tg_hip_rope_tables_dev(float *cos_dev, float *sin_dev, int rope_len,
         lo = std::max(lo, 0.0), hi = std::min(hi, rot_dim - 1.0);
     }
     const double base = scaling == BASE ? theta * pow((double)factor, rot_dim / (rot_dim - 2.0)) : theta;
-    for (int i = 0; i < a.pairs; i++) {
-        double f = pow(base, -2.0 * i / rot_dim), share = 1.0;   /* of the unscaled frequency */
+    /* base^(-2 i / rot_dim), one factor a pair: 64 bits of mantissa leave less than 2^-56 of error in 128 of them */
+    const long double ratio = powl((long double)base, -2.0L / rot_dim);
+    long double power = 1.0L;
+    for (int i = 0; i < a.pairs; i++, power *= ratio) {
+        double f = (double)power, share = 1.0;   /* of the unscaled frequency */
         if (scaling == LINEAR) share = 0.0;
         else if (scaling == PARTS || scaling == PARTS_WHOLE) share = 1.0 - std::min(1.0, std::max(0.0, (i - lo) / std::max(hi - lo, 1e-3)));
         else if (scaling == SMOOTH) share = std::min(1.0, std::max(0.0, (orig_len * f / two_pi - low) / ((double)high - low)));
         if (share < 1.0) f = f * share + f / factor * (1.0 - share);
         a.turns[i] = f / two_pi;
-        a.step_cos[i] = cos(f), a.step_sin[i] = sin(f);
     }
     const hipError_t before = hipPeekAtLastError();
     launch_rope_tables(a, stream ? (hipStream_t)stream : g.st);

@@ -67,7 +67,6 @@ struct RopeTablesArgs {
     int len, first, pairs;
     float mscale;
     double turns[ROPE_MAX_PAIRS];   /* frequency / (2 pi): turns a position */
-    double step_cos[ROPE_MAX_PAIRS], step_sin[ROPE_MAX_PAIRS];   /* of one position */
 };
 void launch_rope_tables(const RopeTablesArgs &a, hipStream_t st);
 

@@ -361,11 +361,11 @@ struct Class {
     }
 };
 
-/* tiles of 16 are of sequences with at most 8 */
+/* a part of at most FEW m-rows a sequence has that many places for each */
 constexpr int FEW = 128;
 template <int MTILE>
-__device__ inline int tile_place(const Work &w, int ratio) {
-    return (MTILE == 16 ? w.sq.slot * (FEW / 16) : start_of<MTILE>(w.sq.r0, w.sq.slot, ratio)) + w.m0 / MTILE;
+__device__ inline int tile_place(const Part &pt, const Work &w, int ratio) {
+    return (pt.most == FEW ? w.sq.slot * (FEW / MTILE) : start_of<MTILE>(w.sq.r0, w.sq.slot, ratio)) + w.m0 / MTILE;
 }
 /* Item b of a call of at most 64 sequences: as find_span, but the whole spans of
  * all tiles come first and what is left of each behind them, so that short
@@ -430,7 +430,7 @@ __device__ inline bool find_blocks(const PromptArgs &a, const Part &pt, int rati
     if (pt.tiles) {
         if (w.count && w.kh == 0 && threadIdx.x == 0) {
             const int n = div_up(w.sq.n * ratio, MTILE);
-            pt.tiles[tile_place<MTILE>(w, ratio)] = Part::Tile{item, w.count, n, last < 0 ? item + (w.count - 1) * n : last};
+            pt.tiles[tile_place<MTILE>(pt, w, ratio)] = Part::Tile{item, w.count, n, last < 0 ? item + (w.count - 1) * n : last};
         }
         w.rec = item;
     }
@@ -1024,17 +1024,17 @@ __device__ inline __attribute__((always_inline)) void join_tile(const PromptArgs
     Work w;
     w.prefix = false, w.kh = b - place * a.n_kv;
     const Class keep = {pt.least, pt.most, ratio};
-    if constexpr (MTILE == 16) {
-        const int s = place / (FEW / 16);
+    if (pt.most == FEW) {
+        const int s = place / (FEW / MTILE);
         w.sq = seq_at(a.s, s);
         keep(w.sq);
-        w.m0 = 16 * (place - s * (FEW / 16));
+        w.m0 = MTILE * (place - s * (FEW / MTILE));
         if (w.m0 >= w.sq.n * ratio) return;
         set_rows(w, ratio);
     } else {
-        from = 64 * (place & 1);
-        if (!find_tile<MTILE>(a, pt.p, ratio, place >> 1, w, keep)) return;
-        place = tile_place<MTILE>(w, ratio);
+        from = ROWS * (place % (MTILE / ROWS));
+        if (!find_tile<MTILE>(a, pt.p, ratio, place / (MTILE / ROWS), w, keep)) return;
+        place = tile_place<MTILE>(pt, w, ratio);
     }
     const Part::Tile tile = pt.tiles[place];
     if (tile.count <= 1) return;
@@ -1103,6 +1103,7 @@ constexpr long long NARROW_WORK = 1 << 18;
 constexpr int SHORT_BELOW = 512, MOST_SPANS = 64;
 struct Cut {
     Shape shape;
+    bool items;       /* records by item */
     Part part, few;   /* few: of a mixed call */
 };
 Shape shape_of(long long m, long long seqs, int n_kv, int positions) {
@@ -1112,17 +1113,19 @@ Shape shape_of(long long m, long long seqs, int n_kv, int positions) {
     return m / 128 * n_kv > 512 ? FULL : WIDE;
 }
 
-/* a mixed call's part in tiles of `tile` m-rows; beyond `often` workgroups there
- * are enough of them to keep the chip busy without cuts */
+/* A part in tiles of `tile` m-rows whose records are by item.  Beyond OFTEN
+ * workgroups (of 128 m-rows; twice as many of 16) there are enough of them
+ * to keep the chip busy without cuts. */
 constexpr int OFTEN = 1024;
-Part mixed_part(const PromptArgs &a, long long m, int tile, int slots, int least, int most) {
+int often(int tile) { return tile == 16 ? 2 * OFTEN : OFTEN; }
+Part item_part(const PromptArgs &a, long long m, int tile, int slots, int least, int most) {
     Part k = {};
     k.least = least, k.most = most;
     long long tiles = std::min(m / tile + a.s.n, m);
-    if (most < INT_MAX) tiles = std::min(tiles, (long long)a.s.n * ((most + tile - 1) / tile));
+    if (most == FEW) tiles = std::min(tiles, (long long)a.s.n * (FEW / tile));
     k.p.target = std::max(1, slots / a.n_kv);
     k.p.unit = 128;
-    k.p.cap = tiles * a.n_kv > OFTEN && least > 1 ? 1 : 64;
+    k.p.cap = tiles * a.n_kv > often(tile) ? 1 : MOST_SPANS;
     k.p.items = (int)tiles + (k.p.cap > 1 ? k.p.target : 0);
     return k;
 }
@@ -1134,8 +1137,11 @@ Cut paged_cut(const PromptArgs &a) {
     auto sees = [&](int rows) { return a.window > 0 ? (int)std::min<long long>(a.s.kv_max, (long long)a.window + rows / ratio + 1) : a.s.kv_max; };
     k.shape = shape_of(m, n_seqs, n_kv, sees(128));
     if (k.shape == MIXED) {
-        k.part = mixed_part(a, m, 128, (m / 128 + n_seqs) * n_kv > 256 ? 256 : 512, FEW + 1, INT_MAX);
-        k.few = mixed_part(a, m, 16, 512, 1, FEW);
+        /* us of 1 .. 1,000 rows in seven sequences, then 60 rows and a chunk of 500, then 300 rows behind 3,500 and one (8 heads
+         * of 64): targets of 256 55.8, 90.6, 76.8, of 512 58.3, 109, 65.2 */
+        k.items = true;
+        k.part = item_part(a, m, 128, (m / 128 + n_seqs) * n_kv > 256 ? 256 : 512, FEW + 1, INT_MAX);
+        k.few = item_part(a, m, 16, 512, 1, FEW);
         return k;
     }
     k.part.least = 1, k.part.most = INT_MAX;
@@ -1145,16 +1151,27 @@ Cut paged_cut(const PromptArgs &a) {
     const long long tiles = std::max((m + tile - 1) / tile, (long long)n_seqs), wgs = tiles * n_kv;
     /* of several sequences fewer than run at once: what their cuts leave over fills the rest (64 rows behind 61 .. 8,314
      * positions, 4 KV heads of 128: 65.9 us; as many as run 74.3, half 74.0) */
-    p.target = std::max(1, (k.shape == NARROW && n_seqs > 1 && a.head_dim > 64 ? 384 : slots) / n_kv);
+    const int at_once = k.shape == NARROW && n_seqs > 1 && a.head_dim > 64 ? 384 : slots;
+    p.target = std::max(1, at_once / n_kv);
     p.unit = 128;
     /* us(n): a span's positions, and what n records a row take to write and read, at 4.5 TB/s, with the combine's launch */
     const double t = positions * (k.shape == NARROW ? 1.0 : 3.4) / 128 * (a.head_dim > 64 ? 1 : 0.5);
     const double r = (double)m * n_kv * a.head_dim * 8 / 4.5e6;
-    const int most = (int)std::min<long long>({MOST_SPANS, (positions + p.unit - 1) / p.unit, std::max(1ll, slots / wgs)});
+    const bool several = k.shape == NARROW && n_seqs > 1;   /* the longest may be much longer than the others: two at least */
+    const int most = (int)std::min<long long>({MOST_SPANS, (positions + p.unit - 1) / p.unit, std::max(several ? 2ll : 1ll, slots / wgs)});
     auto us = [&](int n) { return t / n + r * n + (n == 1 ? -r : 4); };
     const int n = std::max(1, std::min(most, (int)std::sqrt(t / r)));   /* the best, or the next */
     const int best = n < most && us(n + 1) < us(n) ? n + 1 : n;
     p.cap = us(best) < us(1) ? best : 1;
+    if (several && p.cap > 1) {
+        const Part by_item = item_part(a, m, tile, at_once, 1, INT_MAX);
+        if (by_item.p.cap > 1) {
+            k.items = true;
+            k.part = by_item;
+            return k;
+        }
+        p.cap = 1;
+    }
     if (n_seqs > 1 && p.cap > 1)   /* room for a sequence much longer than the others */
         p.cap = (int)std::min<long long>({MOST_SPANS, (positions + p.unit - 1) / p.unit, std::max<long long>(4ll * p.cap, 4ll * p.target / tiles)});
     p.search = p.cap == 1 && n_seqs > 256;
@@ -1163,8 +1180,8 @@ Cut paged_cut(const PromptArgs &a) {
     return k;
 }
 
-/* A call's scratch, in order: statistics and sums of the records, of a mixed
- * call those of both parts and where each tile's are */
+/* A part's scratch, in order: statistics and sums of the records, and where
+ * each tile's are, if by item */
 struct Room {
     size_t records, places;   /* of a part */
     size_t ml() const { return (records * 16 + 255) & ~(size_t)255; }
@@ -1172,11 +1189,11 @@ struct Room {
     size_t at() const { return (places * sizeof(Part::Tile) + 255) & ~(size_t)255; }
     size_t all(int hd) const { return ml() + o(hd) + at(); }
 };
-Room room_of(const PromptArgs &a, const Part &k, int tile, bool mixed) {
+Room room_of(const PromptArgs &a, const Part &k, int tile, bool items) {
     if (k.p.cap <= 1) return Room{0, 0};
-    if (!mixed) return Room{(size_t)a.s.rows * a.n_heads * k.p.nrec, 0};
+    if (!items) return Room{(size_t)a.s.rows * a.n_heads * k.p.nrec, 0};
     const long long m = (long long)a.s.rows * (a.n_heads / a.n_kv);
-    return Room{(size_t)k.p.items * a.n_kv * tile, (size_t)(tile == 16 ? a.s.n * (FEW / 16) : m / tile + a.s.n)};
+    return Room{(size_t)k.p.items * a.n_kv * tile, (size_t)(k.most == FEW ? a.s.n * (FEW / tile) : m / tile + a.s.n)};
 }
 int tile_of(Shape s) { return s == NARROW ? 16 : 128; }
 
@@ -1189,59 +1206,63 @@ void launch_paged(const PromptArgs &a, const Pages &pg, const Cut &k, hipStream_
     else if (k.shape == WIDE) PAGED(512, k_paged_w<HD, 4, 2, 2>);
     else if (k.shape == FULL) PAGED(256, k_paged_w<HD, 4, 1, 2>);
 #undef PAGED
-    else {
-        hipLaunchKernelGGL((k_paged_both<HD>), grid, dim3(256), 0, st, a, pg, k.part, k.few);
-        const long long m = (long long)a.s.rows * (a.n_heads / a.n_kv);
-        const int first = a.s.n * (FEW / 16) * a.n_kv, more = k.part.p.cap > 1 ? (int)(m / 128 + a.s.n) * 2 * a.n_kv : 0;
-        hipLaunchKernelGGL((k_paged_join<HD>), dim3((unsigned)(first + more)), dim3(1024), 0, st, a, k.part, k.few, first);
+    else hipLaunchKernelGGL((k_paged_both<HD>), grid, dim3(256), 0, st, a, pg, k.part, k.few);
+    if (!k.items) {
+        if (k.part.p.nrec) launch_rows_combine(a, k.part.p, st);
+        return;
     }
+    /* tiles of 16, then halves of those of 128 */
+    const Part &small = k.shape == MIXED ? k.few : k.part, &large = k.part;
+    const long long m = (long long)a.s.rows * (a.n_heads / a.n_kv);
+    const int first = (small.p.cap <= 1 ? 0 : small.most == FEW ? a.s.n * (FEW / 16) : (int)(m / 16) + a.s.n) * a.n_kv;
+    const int more = (k.shape != MIXED || large.p.cap <= 1 ? 0 : 2 * ((int)(m / 128) + a.s.n)) * a.n_kv;
+    if (first + more) hipLaunchKernelGGL((k_paged_join<HD>), dim3((unsigned)(first + more)), dim3(1024), 0, st, a, large, small, first);
 }
 
 }  // namespace
 
 size_t attention_paged_need(const PromptArgs &a) {
     const Cut k = paged_cut(a);
-    const bool mixed = k.shape == MIXED;
-    return room_of(a, k.part, tile_of(k.shape), mixed).all(a.head_dim) + (mixed ? room_of(a, k.few, 16, true).all(a.head_dim) : 0);
+    return room_of(a, k.part, tile_of(k.shape), k.items).all(a.head_dim) +
+           (k.shape == MIXED ? room_of(a, k.few, 16, true).all(a.head_dim) : 0);
 }
 
 /* For every call of at most these sizes.  Tiles of a dense cut are cut only
  * while their spans are at most the workgroups that run at once, with several
  * sequences four times as many, so the m-rows times their spans are at most the
- * m-rows of so many tiles.  A mixed call has a record's room for every m-row
- * of its items: those of many rows at most OFTEN and what the target adds, or none. */
+ * m-rows of so many tiles.  Records by item have room for every m-row of the
+ * items: tiles up to often() workgroups, or none, and what the target adds. */
 size_t attention_paged_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, int head_dim, int kv_max) {
     const long long m = (long long)n_rows * (n_heads / n_kv);
     const long long row_heads = (long long)n_rows * n_heads, spans = std::min(MOST_SPANS, (kv_max + 127) / 128);
     if (spans == 1) return 0;
-    auto bytes = [&](long long records) { return (size_t)records * (16 + 4 * (size_t)head_dim) + 256; };
+    auto bytes = [&](long long records) { return (size_t)records * (16 + 4 * (size_t)head_dim) + 512; };
     size_t most = bytes(std::min(row_heads * spans, (m <= 16 ? 16ll * 512 : 128ll * 256) * (n_seqs > 1 ? 4 : 1)));
-    if (n_seqs > 1 && kv_max >= SHORT_BELOW && m > 16) {
-        const long long target = std::max(1, 512 / n_kv);
-        const long long many = std::min(std::min(m / 128 + n_seqs, m), (long long)OFTEN / n_kv) + target;
-        const long long few = std::min(std::min(m / 16 + n_seqs, m), 8ll * n_seqs) + target;
-        const size_t places = (size_t)(m / 128 + n_seqs + (FEW / 16) * (long long)n_seqs) * sizeof(Part::Tile) + 512;
-        most = std::max(most, bytes(many * n_kv * 128) + bytes(few * n_kv * 16) + places);
+    if (n_seqs > 1) {
+        auto part = [&](int tile) {
+            const long long tiles = std::min(std::min(m / tile + n_seqs, m), std::max(1ll, (long long)often(tile) / n_kv));
+            return bytes((tiles + std::max(1, 512 / n_kv)) * n_kv * tile);
+        };
+        const size_t places = (size_t)(m / 128 + m / 16 + (FEW / 16 + 1) * (long long)n_seqs) * sizeof(Part::Tile) + 512;
+        most = std::max(most, part(128) + part(16) + places);
     }
     return most;
 }
 
 void launch_attention_paged(const PromptArgs &a, const Pages &pg, void *scratch, hipStream_t st) {
     Cut k = paged_cut(a);
-    const bool mixed = k.shape == MIXED;
     uint8_t *at = (uint8_t *)scratch;
     auto place = [&](Part &x, int tile) {
-        const Room room = room_of(a, x, tile, mixed);
+        const Room room = room_of(a, x, tile, k.items);
         x.p.ml = (float *)at;
         x.p.o = (float *)(at + room.ml());
         x.tiles = room.places ? (Part::Tile *)(at + room.ml() + room.o(a.head_dim)) : nullptr;
         at += room.all(a.head_dim);
     };
     place(k.part, tile_of(k.shape));
-    if (mixed) place(k.few, 16);
+    if (k.shape == MIXED) place(k.few, 16);
     if (a.head_dim > 64) launch_paged<128>(a, pg, k, st);
     else launch_paged<64>(a, pg, k, st);
-    if (k.part.p.nrec) launch_rows_combine(a, k.part.p, st);
 }
 
 }  // namespace tg

@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256) void k_rope_tables(RopeTablesArgs a) {
     for (int e = 0; e < 4; e++) {
         turn_of(pos * a.turns[i + e], x[e], y[e]);
         x[e] *= m, y[e] *= m;
-        c1[e] = a.step_cos[i + e], s1[e] = a.step_sin[i + e];
+        if (ROWS > 1) turn_of(a.turns[i + e], c1[e], s1[e]);
     }
 #pragma unroll
     for (int n = 0; n < ROWS; n++) {
@@ -75,7 +75,7 @@ __global__ __launch_bounds__(256) void k_rope_tables(RopeTablesArgs a) {
         *(f4u *)(a.cos + to) = c;
         *(f4u *)(a.sin + to) = s;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
+        for (int e = 0; ROWS > 1 && e < 4; e++) {
             const double u = x[e] * c1[e] - y[e] * s1[e];
             y[e] = y[e] * c1[e] + x[e] * s1[e];
             x[e] = u;
