@@ -516,6 +516,9 @@ def test_attention_score_ranges(tg, q_scale):
     say(f"attention q_scale={q_scale}")
     for hd in (64, 128):
         _attend(tg, Attend(11, 8, 2, hd, [50, 1, 140], [20, 700, 0], q_scale=q_scale, sinks=True))
+        a = Attend(12, 8, 2, hd, [50, 1, 140], [20, 700, 0], q_scale=q_scale)   # the smallest factor that a score can have
+        a.pages.ek[:] = 127 + LEAST
+        _attend(tg, a)
 
 
 @pytest.mark.parametrize("which", ["k", "v"])

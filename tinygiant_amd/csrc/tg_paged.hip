@@ -318,7 +318,9 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 typedef int v4i __attribute__((ext_vector_type(4)));
 constexpr int QMAX = 8300000;    /* three signed digits of base 256 */
 constexpr float UNSHIFT = 1.f / (float)(1 << (int)SHIFT_H);
-constexpr float TINY = 1e-37f;   /* factors stay above 0: -inf * 0 would be NaN */
+/* A score's factor c 2^e stays above 0 (-inf * 0 would be NaN): q's own power of two is at most 2^103, its f16 planes' 2^100,
+ * log2 e / sqrt(head_dim) above 2^-3, and f32's least is 2^-149. */
+static_assert(103 + 3 - PAGE_EXP_MIN < 149, "a score's factor");
 
 /* A wave's next 64 blocks, one a lane: where they are, and their exponents'
  * bytes (K, V << 8) with bit 16 for one that makes rows NaN */
@@ -590,7 +592,7 @@ __device__ inline __attribute__((always_inline)) void paged_n(const PromptArgs &
                     for (int j = 0; j < J; j++)
                         d[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, r.k[b][j]), q[m][g][j], d[g], 0, 0, 0);
                 }
-                ck[b] = fmaxf(c[m] * exp_up(ex[b] & 255), TINY);
+                ck[b] = c[m] * exp_up(ex[b] & 255);
 #pragma unroll
                 for (int v = 0; v < 4; v++) s[b][v] = fmaf((float)(d[2][v] * 256 + d[1][v]), 256.f, (float)d[0][v]);
             }
@@ -775,7 +777,8 @@ __device__ inline __attribute__((always_inline)) void paged_w(const PromptArgs &
                                                               SharedPW<HD, MW, KG> &sh) {
     constexpr int RB = HD * 2, TILE = KT * RB;          /* bytes of a row in LDS, of a tile of K or V */
     constexpr int DB = HD / 32, STEPS = HD / 16;
-    constexpr int LR = 1024 / HD, NL = KT / LR / MW;    /* rows a load of the wave covers, loads a tile and matrix */
+    constexpr int LR = 1024 / HD, LOADS = KT / LR;      /* rows a load of a wave covers, loads of a tile of K or V */
+    constexpr int NL = 2 * LOADS / MW;                  /* a wave's: mwave + MW k of K's, then V's */
     static_assert(NL >= 1 && 16 % LR == 0, "a load is of one block");
     auto &bufs = sh.bufs;
     const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
@@ -797,38 +800,36 @@ __device__ inline __attribute__((always_inline)) void paged_w(const PromptArgs &
     const size_t bytes = (size_t)PAGE_BLOCK * hd;
     const int lrow = lane / (HD / 16), piece = lane % (HD / 16);
     const bool on = 16 * piece < hd;
-    u32x4 raw[2][NL];
-    int next[4];   /* exponents of the tile in raw */
+    u32x4 raw[NL];
     auto load = [&](int n) __attribute__((always_inline)) {
         if (n >> 4 != have) bl = chunk(n), have = n >> 4;
 #pragma unroll
-        for (int b = 0; b < 4; b++) next[b] = __builtin_amdgcn_readlane(bl.exps, (4 * n & 63) + b);
-#pragma unroll
         for (int k = 0; k < NL; k++) {
-            const int row = LR * (mwave + MW * k);
+            const int u = mwave + MW * k, row = LR * (u % LOADS);
             const size_t at = (size_t)__builtin_amdgcn_readlane(bl.at, (4 * n & 63) + (row >> 4)) * bytes;
             const uint32_t off = (uint32_t)(((row & 15) + lrow) * hd + 16 * piece);
-            raw[0][k] = raw[1][k] = u32x4{0, 0, 0, 0};
-            if (on) raw[0][k] = *(const u32x4 *)(pg.k + at + off), raw[1][k] = *(const u32x4 *)(pg.v + at + off);
+            raw[k] = u32x4{0, 0, 0, 0};
+            if (on) raw[k] = *(const u32x4 *)((u < LOADS ? pg.k : pg.v) + at + off);
         }
     };
-    auto store = [&](int b) __attribute__((always_inline)) {
+    int stored[4];   /* the stored tile's exponents */
+    auto store = [&](int n, int b) __attribute__((always_inline)) {
 #pragma unroll
-        for (int m = 0; m < 2; m++)
+        for (int e = 0; e < 4; e++) stored[e] = __builtin_amdgcn_readlane(bl.exps, (4 * n & 63) + e);
 #pragma unroll
-            for (int k = 0; k < NL; k++) {
-                const int key = LR * (mwave + MW * k) + lrow;
-                h2 y[8];
+        for (int k = 0; k < NL; k++) {
+            const int u = mwave + MW * k, key = LR * (u % LOADS) + lrow;
+            h2 y[8];
 #pragma unroll
-                for (int e = 0; e < 4; e++) to_half(raw[m][k][e], y[2 * e], y[2 * e + 1]);
-                uint8_t *at = &buf[b][m][key * RB];
+            for (int e = 0; e < 4; e++) to_half(raw[k][e], y[2 * e], y[2 * e + 1]);
+            uint8_t *at = &buf[b][u < LOADS ? 0 : 1][key * RB];
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const h8 z = {y[4 * e][0], y[4 * e][1], y[4 * e + 1][0], y[4 * e + 1][1],
-                                  y[4 * e + 2][0], y[4 * e + 2][1], y[4 * e + 3][0], y[4 * e + 3][1]};
-                    *(h8 *)(at + (((2 * piece + e) ^ swz<HD>(key)) << 4)) = z;
-                }
+            for (int e = 0; e < 2; e++) {
+                const h8 z = {y[4 * e][0], y[4 * e][1], y[4 * e + 1][0], y[4 * e + 1][1],
+                              y[4 * e + 2][0], y[4 * e + 2][1], y[4 * e + 3][0], y[4 * e + 3][1]};
+                *(h8 *)(at + (((2 * piece + e) ^ swz<HD>(key)) << 4)) = z;
             }
+        }
     };
     load(group);
     static_assert(KG == 1 || 32 * MW * HD * 4 == sizeof bufs / 2, "q fits");
@@ -864,10 +865,8 @@ __device__ inline __attribute__((always_inline)) void paged_w(const PromptArgs &
         for (int e = 0; e < 2; e++) vaddr[d][e] = TILE + v_operand<HD>(lane, d, e);
     const float one = opaque_one();
 
-    int stored[4], ex[4];
-    store(0);
-#pragma unroll
-    for (int e = 0; e < 4; e++) stored[e] = next[e];
+    int ex[4];
+    store(group, 0);
     if (group + KG < tiles) load(group + KG);
     int b = 0;
     for (int n0 = 0; n0 < tiles; n0 += KG, b ^= 1) {
@@ -876,9 +875,7 @@ __device__ inline __attribute__((always_inline)) void paged_w(const PromptArgs &
 #pragma unroll
         for (int e = 0; e < 4; e++) ex[e] = stored[e];
         if (n + KG < tiles) {
-            store(b ^ 1);
-#pragma unroll
-            for (int e = 0; e < 4; e++) stored[e] = next[e];
+            store(n + KG, b ^ 1);
             if (n + 2 * KG < tiles) load(n + 2 * KG);
         }
         if (t > x.any_hi || t + KT <= x.any_lo || n >= tiles) continue;   /* uniform in the wave */
@@ -924,7 +921,7 @@ __device__ inline __attribute__((always_inline)) void paged_w(const PromptArgs &
                     float u = s[j][8 * g];
 #pragma unroll
                     for (int v = 1; v < 8; v++) u = max_nan(u, s[j][8 * g + v]);
-                    ck[2 * j + g] = fmaxf(c * exp_up(eg[2 * j + g] & 255), TINY);
+                    ck[2 * j + g] = c * exp_up(eg[2 * j + g] & 255);
                     top = max_nan(top, fmaf(u, ck[2 * j + g], (float)((eg[2 * j + g] >> 8 & 255) - 127)));
                 }
             }
@@ -1094,11 +1091,15 @@ __global__ __launch_bounds__(1024) void k_paged_join(PromptArgs a, Part many, Pa
  *   wide    128 m-rows, two groups of four waves on tiles in turn
  *   short   128 m-rows, four waves, for few positions a row
  *   full    the same, two workgroups a CU on long spans
+ *   tall    256 m-rows, eight waves: half the widening a row, where there are
+ *           enough of them (32 heads of 128: 4,096 rows 250 us, full 279; 8,192 930 and 966; 2,999
+ *           161 and 154; heads of 64, bound by the softmax's issue, 299 and 296)
  *   mixed   several sequences, of many rows together: full for those of more
  *           than FEW m-rows, narrow for the others */
 namespace {
 
-enum Shape { NARROW, SHORT, WIDE, FULL, MIXED };
+enum Shape { NARROW, SHORT, WIDE, FULL, TALL, MIXED };
+int tile_of(Shape s) { return s == NARROW ? 16 : s == TALL ? 256 : 128; }
 constexpr long long NARROW_WORK = 1 << 18;
 constexpr int SHORT_BELOW = 512, MOST_SPANS = 64;
 struct Cut {
@@ -1106,10 +1107,11 @@ struct Cut {
     bool items;       /* records by item */
     Part part, few;   /* few: of a mixed call */
 };
-Shape shape_of(long long m, long long seqs, int n_kv, int positions) {
+Shape shape_of(long long m, long long seqs, int n_kv, int head_dim, int positions) {
     if (m <= 16 * seqs || (m <= 128 * seqs && m * positions <= NARROW_WORK)) return NARROW;
     if (positions < SHORT_BELOW) return SHORT;
     if (seqs > 1) return MIXED;
+    if (head_dim > 64 && m / 256 * n_kv >= 512) return TALL;
     return m / 128 * n_kv > 512 ? FULL : WIDE;
 }
 
@@ -1135,7 +1137,7 @@ Cut paged_cut(const PromptArgs &a) {
     const int n_seqs = a.s.n, n_kv = a.n_kv, ratio = a.n_heads / n_kv;
     const long long m = (long long)a.s.rows * ratio;
     auto sees = [&](int rows) { return a.window > 0 ? (int)std::min<long long>(a.s.kv_max, (long long)a.window + rows / ratio + 1) : a.s.kv_max; };
-    k.shape = shape_of(m, n_seqs, n_kv, sees(128));
+    k.shape = shape_of(m, n_seqs, n_kv, a.head_dim, sees(128));
     if (k.shape == MIXED) {
         /* us of 1 .. 1,000 rows in seven sequences, then 60 rows and a chunk of 500, then 300 rows behind 3,500 and one (8 heads
          * of 64): targets of 256 55.8, 90.6, 76.8, of 512 58.3, 109, 65.2 */
@@ -1146,7 +1148,7 @@ Cut paged_cut(const PromptArgs &a) {
     }
     k.part.least = 1, k.part.most = INT_MAX;
     RowsPlan &p = k.part.p;
-    const int tile = k.shape == NARROW ? 16 : 128, positions = sees(tile);
+    const int tile = tile_of(k.shape), positions = sees(tile);
     const int slots = k.shape == NARROW ? 512 : 256;
     const long long tiles = std::max((m + tile - 1) / tile, (long long)n_seqs), wgs = tiles * n_kv;
     /* of several sequences fewer than run at once: what their cuts leave over fills the rest (64 rows behind 61 .. 8,314
@@ -1195,7 +1197,6 @@ Room room_of(const PromptArgs &a, const Part &k, int tile, bool items) {
     const long long m = (long long)a.s.rows * (a.n_heads / a.n_kv);
     return Room{(size_t)k.p.items * a.n_kv * tile, (size_t)(k.most == FEW ? a.s.n * (FEW / tile) : m / tile + a.s.n)};
 }
-int tile_of(Shape s) { return s == NARROW ? 16 : 128; }
 
 template <int HD>
 void launch_paged(const PromptArgs &a, const Pages &pg, const Cut &k, hipStream_t st) {
@@ -1205,6 +1206,7 @@ void launch_paged(const PromptArgs &a, const Pages &pg, const Cut &k, hipStream_
     else if (k.shape == SHORT) PAGED(256, k_paged_w<HD, 4, 1, 1>);
     else if (k.shape == WIDE) PAGED(512, k_paged_w<HD, 4, 2, 2>);
     else if (k.shape == FULL) PAGED(256, k_paged_w<HD, 4, 1, 2>);
+    else if (k.shape == TALL) PAGED(512, k_paged_w<HD, 8, 1, 2>);
 #undef PAGED
     else hipLaunchKernelGGL((k_paged_both<HD>), grid, dim3(256), 0, st, a, pg, k.part, k.few);
     if (!k.items) {
