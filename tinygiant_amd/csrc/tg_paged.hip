@@ -1156,24 +1156,28 @@ Cut paged_cut(const PromptArgs &a) {
     const int at_once = k.shape == NARROW && n_seqs > 1 && a.head_dim > 64 ? 384 : slots;
     p.target = std::max(1, at_once / n_kv);
     p.unit = 128;
-    /* us(n): a span's positions, and what n records a row take to write and read, at 4.5 TB/s, with the combine's launch */
-    const double t = positions * (k.shape == NARROW ? 1.0 : 3.4) / 128 * (a.head_dim > 64 ? 1 : 0.5);
+    /* us(n): a span's positions (measured on workgroups alone: one row of 64 + 8 heads of 64 behind 1,000 and 4,000 positions 11.0
+     * and 26.9 us uncut, of 32 + 4 of 128 13.7 and 33.7), and what n records a row take to write and read, at 4.5 TB/s, with the
+     * combine's launch */
+    const double t = positions * (k.shape == NARROW ? (a.head_dim > 64 ? 0.9 : 0.75) : (a.head_dim > 64 ? 3.4 : 1.7)) / 128;
     const double r = (double)m * n_kv * a.head_dim * 8 / 4.5e6;
-    const bool several = k.shape == NARROW && n_seqs > 1;   /* the longest may be much longer than the others: two at least */
-    const int most = (int)std::min<long long>({MOST_SPANS, (positions + p.unit - 1) / p.unit, std::max(several ? 2ll : 1ll, slots / wgs)});
+    if (k.shape == NARROW && n_seqs > 1) {
+        /* Cut, all finish together; uncut, the longest takes t while the others, half as long on average, fill the rest: what
+         * that leaves idle against the second kernel's time.  64 rows of 64 + 8 heads behind up to 2,000 positions 20 us uncut and
+         * 25 cut, 48 behind up to 6,000 52 and 38.  A quarter of t always counts: one may be far longer than the others. */
+        const double idle = t * (1 - std::min(0.75, wgs / (2.0 * slots)));
+        const Part cut = item_part(a, m, tile, at_once, 1, INT_MAX);
+        k.items = positions > 2 * p.unit && idle > 6 && cut.p.cap > 1;
+        if (k.items) {
+            k.part = cut;
+            return k;
+        }
+    }
+    const int most = (int)std::min<long long>({MOST_SPANS, (positions + p.unit - 1) / p.unit, std::max(1ll, slots / wgs)});
     auto us = [&](int n) { return t / n + r * n + (n == 1 ? -r : 4); };
     const int n = std::max(1, std::min(most, (int)std::sqrt(t / r)));   /* the best, or the next */
     const int best = n < most && us(n + 1) < us(n) ? n + 1 : n;
-    p.cap = us(best) < us(1) ? best : 1;
-    if (several && p.cap > 1) {
-        const Part by_item = item_part(a, m, tile, at_once, 1, INT_MAX);
-        if (by_item.p.cap > 1) {
-            k.items = true;
-            k.part = by_item;
-            return k;
-        }
-        p.cap = 1;
-    }
+    p.cap = us(best) < us(1) && !(k.shape == NARROW && n_seqs > 1) ? best : 1;
     if (n_seqs > 1 && p.cap > 1)   /* room for a sequence much longer than the others */
         p.cap = (int)std::min<long long>({MOST_SPANS, (positions + p.unit - 1) / p.unit, std::max<long long>(4ll * p.cap, 4ll * p.target / tiles)});
     p.search = p.cap == 1 && n_seqs > 256;
