@@ -44,10 +44,25 @@ __device__ inline bool good_exp(int byte) { return (unsigned)(byte - (127 + PAGE
 __device__ inline float exp_up(int byte) { return __int_as_float(byte << 23); }
 __device__ inline float exp_down(int byte) { return __int_as_float((254 - byte) << 23); }
 
-__device__ inline int wave_imax(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
-    return v;
+/* sum over groups of G lanes (8 or 16), in each of them */
+template <int CTRL>
+__device__ inline double dpp_d(double v) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    return __longlong_as_double((long long)((uint64_t)(uint32_t)dpp_i<CTRL>((int)(u >> 32)) << 32 | (uint32_t)dpp_i<CTRL>((int)(uint32_t)u)));
+}
+template <int G>
+__device__ inline double group_sum(double v) {
+    v += dpp_d<0xB1>(v);    /* lanes 1 and 2 apart, then mirrors of 8 and of 16 */
+    v += dpp_d<0x4E>(v);
+    v += dpp_d<0x141>(v);
+    return G == 16 ? v + dpp_d<0x140>(v) : v;
+}
+/* 1 / sqrt(x): the instruction's 2^-26 or better, doubled twice by Newton's step */
+__device__ inline double rsqrt_d(double x) {
+    double r = __builtin_amdgcn_rsq(x);
+    const double h = 0.5 * x;
+    r = fma(r, fma(-h * r, r, 0.5), r);
+    return fma(r, fma(-h * r, r, 0.5), r);
 }
 
 /* The least e with |x| <= 127 2^e: x = m 2^k, m in [1/2, 1), and 127 / 128 is
@@ -85,123 +100,135 @@ __device__ inline bool seq_of_block(const PackedSeqs &p, int b, Seq &q, int &s, 
     return q.n > 0;
 }
 
-/* K (v: V) rows of one block and head by one wave: G lanes a row, 64 / G rows
- * at a time, everything in registers.  From the norm to the byte all is in 64
- * bits, so that what is stored is the formula's nearest byte; the rate of
- * 64-bit operations is half that of 32 here and the kernel waits for memory. */
+/* What a wave has of a block of K or V of a head: 64 / G rows, G lanes each.
+ * From the norm to the byte all is in 64 bits, so that what is stored is the
+ * formula's nearest byte; the rate of 64-bit operations is half that of 32 here and
+ * the kernel waits for memory. */
+struct BlockRows {
+    d4 x, y;
+    Pieces p;
+    int8_t *page;      /* the lane's row */
+    uint8_t *exp;
+    int old, old_rows;
+    int e;             /* the exponent that the wave's rows need, NO_ROWS: it has none */
+    bool live, on;
+};
+constexpr int NO_ROWS = -1000;
 template <int G>
-__device__ inline void append_block(const PagedAppendArgs &a, const Seq &q, int s, int j, int kh, bool v) {
-    constexpr int PER = 64 / G, N = PAGE_BLOCK / PER;
-    const int lane = threadIdx.x & 63, row = lane / G, l = lane % G, hd = a.head_dim;
+__device__ inline BlockRows block_rows(const PagedAppendArgs &a, const Seq &q, int s, int j, int kh, bool v, int sub) {
+    const int lane = threadIdx.x & 63, row = sub * (64 / G) + lane / G, l = lane % G, hd = a.head_dim;
+    BlockRows b = {};
+    b.e = NO_ROWS;
     const int B = block_at(a.pages, a.n_kv, s, kh, j);
-    if (B < 0) return;
-    const bool on = 8 * l < hd;
-    uint8_t *eb = (v ? a.pages.ev : a.pages.ek) + B;
-    int8_t *page = (v ? a.pages.v : a.pages.k) + (size_t)B * PAGE_BLOCK * hd;
-    const int old_rows = max(0, min(PAGE_BLOCK, q.past - PAGE_BLOCK * j));   /* rows that it holds */
-    const int old = old_rows ? *eb : 127 + PAGE_EXP_MIN;
+    if (B < 0) return b;
+    b.on = 8 * l < hd;
+    b.exp = (v ? a.pages.ev : a.pages.ek) + B;
+    b.page = (v ? a.pages.v : a.pages.k) + ((size_t)B * PAGE_BLOCK + row) * hd;
+    b.old_rows = max(0, min(PAGE_BLOCK, q.past - PAGE_BLOCK * j));   /* rows that the block holds */
+    b.old = b.old_rows ? *b.exp : 127 + PAGE_EXP_MIN;
     Turn turn = a.turn;
     if (v) turn.cos = nullptr;
-    const Pieces p = turn_pieces(turn, l);
+    b.p = turn_pieces(turn, l);
     const float *nw = v ? nullptr : a.k_norm;
-    d4 x[N], y[N];
-    bool live[N];
-    double big = 0.0;
-    bool odd = false;   /* a value that is not finite */
-#pragma unroll
-    for (int n = 0; n < N; n++) {
-        const int pos = PAGE_BLOCK * j + PER * n + row, i = pos - q.past;
-        live[n] = i >= 0 && i < q.n && (!a.turn.cos || pos < a.turn.len);
-        f4 u = {0.f, 0.f, 0.f, 0.f}, w = u;
-        if (live[n] && on) {
-            const float *src = (v ? a.v : a.k) + (size_t)(q.r0 + i) * a.kv_stride + (size_t)kh * hd;
-            u = *(const f4u *)(src + p.a), w = *(const f4u *)(src + p.b);
-        }
-        x[n] = __builtin_convertvector(u, d4), y[n] = __builtin_convertvector(w, d4);
-        if (nw) {
-            double ss = 0.0;
-#pragma unroll
-            for (int e = 0; e < 4; e++) ss += x[n][e] * x[n][e] + y[n][e] * y[n][e];
-#pragma unroll
-            for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-            if (on) {
-                const double f = 1.0 / sqrt(ss / (double)hd + (double)a.eps);
-                x[n] = x[n] * f * __builtin_convertvector((f4)*(const f4u *)(nw + p.a), d4);
-                y[n] = y[n] * f * __builtin_convertvector((f4)*(const f4u *)(nw + p.b), d4);
-            }
-        }
-        if (p.turned && live[n] && on) {
+    const int pos = PAGE_BLOCK * j + row, i = pos - q.past;
+    b.live = i >= 0 && i < q.n && (!a.turn.cos || pos < a.turn.len);
+    if (!__ballot(b.live)) return b;
+    f4 u = {0.f, 0.f, 0.f, 0.f}, w = u, c = u, sn = u;
+    if (b.live && b.on) {
+        const float *src = (v ? a.v : a.k) + (size_t)(q.r0 + i) * a.kv_stride + (size_t)kh * hd;
+        u = *(const f4u *)(src + b.p.a), w = *(const f4u *)(src + b.p.b);
+        if (b.p.turned) {
             const size_t at = (size_t)pos * (turn.dim / 2) + 4 * l;
-            turn_pair(turn.inter, __builtin_convertvector((f4)*(const f4u *)(turn.cos + at), d4),
-                      __builtin_convertvector((f4)*(const f4u *)(turn.sin + at), d4), x[n], y[n]);
-        }
-        if (live[n] && on) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const double f = fabs(x[n][e]), g = fabs(y[n][e]);
-                odd |= !(f < INFINITY) || !(g < INFINITY);
-                big = fmax(big, fmax(f, g));
-            }
+            c = *(const f4u *)(turn.cos + at), sn = *(const f4u *)(turn.sin + at);
         }
     }
-    const uint64_t any = __ballot(live[0] || live[1] || (N > 2 && (live[2 % N] || live[3 % N])));
-    if (!any) return;
-    int e = wave_imax(odd ? PAGE_EXP_MAX + 1 : block_exp(big));
-    if (old_rows) e = max(e, good_exp(old) ? old - 127 : PAGE_EXP_MAX + 1);
-    const bool bad = e > PAGE_EXP_MAX;
-    const double f = __builtin_amdgcn_ldexp(1.0, -e);
+    b.x = __builtin_convertvector(u, d4), b.y = __builtin_convertvector(w, d4);
+    if (nw) {
+        double ss = 0.0;
 #pragma unroll
-    for (int n = 0; n < N; n++) {
-        if (!live[n] || !on) continue;
+        for (int e = 0; e < 4; e++) ss += b.x[e] * b.x[e] + b.y[e] * b.y[e];
+        ss = group_sum<G>(ss);
+        if (b.on) {
+            const double f = rsqrt_d(ss / (double)hd + (double)a.eps);
+            b.x = b.x * f * __builtin_convertvector((f4)*(const f4u *)(nw + b.p.a), d4);
+            b.y = b.y * f * __builtin_convertvector((f4)*(const f4u *)(nw + b.p.b), d4);
+        }
+    }
+    if (b.p.turned) turn_pair(turn.inter, __builtin_convertvector(c, d4), __builtin_convertvector(sn, d4), b.x, b.y);
+    double big = 0.0;
+    bool odd = false;   /* a value that is not finite */
+    if (b.live && b.on) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const double f = fabs(b.x[e]), g = fabs(b.y[e]);
+            odd |= !(f < INFINITY) || !(g < INFINITY);
+            big = fmax(big, fmax(f, g));
+        }
+    }
+    const int mine = odd ? PAGE_EXP_MAX + 1 : block_exp(big);
+    b.e = (int)wave_umax((uint32_t)(mine - NO_ROWS)) + NO_ROWS;
+    return b;
+}
+/* ... stored with the exponent that the rows of all waves need */
+__device__ inline void store_block(const BlockRows &b, int e, int row, int l, bool first) {
+    if (b.old_rows) e = max(e, good_exp(b.old) ? b.old - 127 : PAGE_EXP_MAX + 1);
+    const bool bad = e > PAGE_EXP_MAX;
+    if (b.on && b.live) {
+        const double f = __builtin_amdgcn_ldexp(1.0, -e);
         uint32_t lo = 0, hi = 0;
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-            lo |= ((uint32_t)(int)__builtin_rint(x[n][c] * f) & 255u) << (8 * c);
-            hi |= ((uint32_t)(int)__builtin_rint(y[n][c] * f) & 255u) << (8 * c);
+            lo |= ((uint32_t)(int)__builtin_rint(b.x[c] * f) & 255u) << (8 * c);
+            hi |= ((uint32_t)(int)__builtin_rint(b.y[c] * f) & 255u) << (8 * c);
         }
-        int8_t *dst = page + (PER * n + row) * hd;
-        *(uint32_t *)(dst + p.a) = bad ? 0u : lo;
-        *(uint32_t *)(dst + p.b) = bad ? 0u : hi;
-    }
-    if (!bad && old_rows && e > old - 127) {   /* the rows before these in the new unit */
-        const float g = exp_up(254 - (e - (old - 127)) - 127);
+        *(uint32_t *)(b.page + b.p.a) = bad ? 0u : lo;
+        *(uint32_t *)(b.page + b.p.b) = bad ? 0u : hi;
+    } else if (b.on && !bad && row < b.old_rows && e > b.old - 127) {   /* rows from before in the new unit */
+        const float g = exp_up(127 - (e - (b.old - 127)));
+        uint32_t *at = (uint32_t *)(b.page + 8 * l);
 #pragma unroll
-        for (int n = 0; n < N; n++) {
-            if (PER * n + row >= old_rows || !on) continue;
-            uint32_t *at = (uint32_t *)(page + (PER * n + row) * hd + 8 * l);
+        for (int c = 0; c < 2; c++) {
+            const uint32_t w = at[c];
+            uint32_t z = 0;
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const uint32_t w = at[c];
-                uint32_t z = 0;
-#pragma unroll
-                for (int b = 0; b < 4; b++)
-                    z |= ((uint32_t)(int)__builtin_rintf((float)(int8_t)(w >> (8 * b)) * g) & 255u) << (8 * b);
-                at[c] = z;
-            }
+            for (int k = 0; k < 4; k++) z |= ((uint32_t)(int)__builtin_rintf((float)(int8_t)(w >> (8 * k)) * g) & 255u) << (8 * k);
+            at[c] = z;
         }
     }
-    if (lane == 0) *eb = bad ? PAGE_EXP_NAN : (uint8_t)(e + 127);
+    if (first) *b.exp = bad ? PAGE_EXP_NAN : (uint8_t)(e + 127);
 }
 
 }  // namespace
 
 /* ---- append ----
  * Workgroups of two kinds: those of the first `rows` (0 without q_out) turn a
- * row's query heads, as k_kv_append does; the others have a wave for each
- * block, KV head and one of K and V.  Two blocks more a sequence than its rows
+ * row's query heads, as k_kv_append does; the others have four waves (heads of
+ * up to 64 values: two) for each block, KV head and one of K and V (all 16 rows
+ * by one wave: 1,000 rows of 4 KV heads of 128 15.1 us).  Two blocks more a sequence than its rows
  * fill have room (block_start), so that no lengths are summed. */
 template <int G>
 __global__ __launch_bounds__(256) void k_paged_append(PagedAppendArgs a, int rows) {
     const int tid = threadIdx.x, hd = a.head_dim;
     if ((int)blockIdx.x >= rows) {
-        const long long unit = (long long)((int)blockIdx.x - rows) * 4 + __builtin_amdgcn_readfirstlane(tid >> 6);
+        constexpr int WAVES = PAGE_BLOCK * G / 64;   /* of a block */
+        __shared__ int need[4];
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), sub = wave % WAVES, lane = tid & 63;
+        const long long unit = (long long)((int)blockIdx.x - rows) * (4 / WAVES) + wave / WAVES;
         const int item = (int)(unit / (2 * a.n_kv)), rest = (int)(unit - (long long)item * (2 * a.n_kv));
+        BlockRows b = {};
+        b.e = NO_ROWS;
         Seq q;
         int s, place;
-        if (!seq_of_block(a.s, item, q, s, place)) return;
-        const int j = (q.past >> 4) + place;
-        if (place < 0 || PAGE_BLOCK * j >= q.past + q.n) return;
-        append_block<G>(a, q, s, j, rest >> 1, rest & 1);
+        if (seq_of_block(a.s, item, q, s, place)) {
+            const int j = (q.past >> 4) + place;
+            if (place >= 0 && PAGE_BLOCK * j < q.past + q.n) b = block_rows<G>(a, q, s, j, rest >> 1, rest & 1, sub);
+        }
+        if (lane == 0) need[wave] = b.e;
+        __syncthreads();
+        int e = NO_ROWS;
+#pragma unroll
+        for (int k = 0; k < WAVES; k++) e = max(e, need[wave - sub + k]);
+        if (e > NO_ROWS) store_block(b, e, sub * (64 / G) + lane / G, lane % G, sub == 0 && lane == 0);
         return;
     }
     const int r = (int)blockIdx.x;
@@ -247,7 +274,8 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppendArgs a, int row
 void launch_paged_append(const PagedAppendArgs &a, hipStream_t st) {
     const int rows = a.q_out ? a.s.rows : 0;
     const long long items = (long long)(a.s.rows >> 4) + 2ll * a.s.n;
-    const dim3 grid((unsigned)(rows + (items * 2 * a.n_kv + 3) / 4)), block(256);
+    const int units = a.head_dim <= 64 ? 2 : 1;   /* of a workgroup */
+    const dim3 grid((unsigned)(rows + (items * 2 * a.n_kv + units - 1) / units)), block(256);
     if (a.head_dim <= 64) hipLaunchKernelGGL((k_paged_append<8>), grid, block, 0, st, a, rows);
     else hipLaunchKernelGGL((k_paged_append<16>), grid, block, 0, st, a, rows);
 }
