@@ -827,7 +827,8 @@ __device__ inline __attribute__((always_inline)) void paged_w(const PromptArgs &
     int have = 0;   /* the chunk that bl is of */
     const size_t bytes = (size_t)PAGE_BLOCK * hd;
     const int lrow = lane / (HD / 16), piece = lane % (HD / 16);
-    const bool on = 16 * piece < hd;
+    /* pieces past head_dim get its first: finite, q is 0 there, and of V such dims are not written */
+    const uint32_t lane_off = (uint32_t)(lrow * hd + (16 * piece < hd ? 16 * piece : 0));
     u32x4 raw[NL];
     auto load = [&](int n) __attribute__((always_inline)) {
         if (n >> 4 != have) bl = chunk(n), have = n >> 4;
@@ -835,9 +836,7 @@ __device__ inline __attribute__((always_inline)) void paged_w(const PromptArgs &
         for (int k = 0; k < NL; k++) {
             const int u = mwave + MW * k, row = LR * (u % LOADS);
             const size_t at = (size_t)__builtin_amdgcn_readlane(bl.at, (4 * n & 63) + (row >> 4)) * bytes;
-            const uint32_t off = (uint32_t)(((row & 15) + lrow) * hd + 16 * piece);
-            raw[k] = u32x4{0, 0, 0, 0};
-            if (on) raw[k] = *(const u32x4 *)((u < LOADS ? pg.k : pg.v) + at + off);
+            raw[k] = *(const u32x4 *)((u < LOADS ? pg.k : pg.v) + at + (uint32_t)((row & 15) * hd) + lane_off);
         }
     };
     int stored[4];   /* the stored tile's exponents */
