@@ -411,8 +411,10 @@ void tg_hip_rope_dev(const float *x_dev, int x_stride, const int32_t *pos_dev, c
  * rows are dealt to calls.)  A block that takes in a value beyond 127 2^42, an
  * infinity or a NaN gets the byte 255 and is NaN until it is begun
  * anew: by a call whose sequence has no earlier rows in it.  Rows in a
- * missing page are not stored.  Two sequences of a call must not write the
- * same block of a page; a shared block is copied before it is written. */
+ * missing page are not stored.  A call must not write a block of a page for
+ * two sequences, or for two places of one; a shared block is copied before it is
+ * written.  Rows may be taken back (a smaller kv_len in the next call); their
+ * blocks keep the exponents. */
 void tg_hip_paged_append_dev(const float *q_dev, const float *k_dev, const float *v_dev, int q_stride, int kv_stride,
                              const float *q_norm_w_dev, const float *k_norm_w_dev, float eps, const float *rope_cos_dev,
                              const float *rope_sin_dev, int rope_len, int rot_dim, int interleaved,

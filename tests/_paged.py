@@ -97,8 +97,9 @@ class Pages:
                 exps[page, h, b] = e + 127
 
 
-def attend(q, pages, cu, lens, past, nh, window=0, sinks=None):
-    """(out, tolerance) of every packed row, NaN where no sequence is; q [rows][nh * hd].
+def attend(q, pages, cu, lens, past, nh, window=0, sinks=None, only=None):
+    """(out, tolerance) of every packed row (`only`: of these rows, a dict of row: heads), NaN where no sequence is;
+    q [rows][nh * hd].
 
     Tolerance, in natural units of a score, all relative to the largest |v|.
     q is held to half a step of 2^-22 of its head's largest value Q, times the
@@ -115,10 +116,10 @@ def attend(q, pages, cu, lens, past, nh, window=0, sinks=None):
     group, scale = nh // nkv, hd ** -0.5
     for s, (n, p) in enumerate(zip(lens, past)):
         keys, vals = pages.values("k", s, p + n), pages.values("v", s, p + n)
-        for i in range(n):
+        for i in range(n) if only is None else [r - cu[s] for r in only if 0 <= r - cu[s] < n]:
             last = p + i
             lo = max(0, last + 1 - window) if window else 0
-            for h in range(nh):
+            for h in range(nh) if only is None else only[cu[s] + i]:
                 k, v = keys[h // group, lo:last + 1], vals[h // group, lo:last + 1]
                 x = q[cu[s] + i, h * hd:(h + 1) * hd].astype(np.float64)
                 with np.errstate(invalid="ignore", over="ignore"):

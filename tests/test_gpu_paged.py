@@ -426,7 +426,7 @@ class Attend:
         fine = ~np.isnan(ref)
         err = np.abs(got - ref)[fine]
         assert np.all(err <= tol[fine]), float((err / tol[fine]).max())
-        return float((err / tol[fine]).max()) if err.size else 0.0
+        return float((err / np.maximum(tol[fine], 1e-300)).max()) if err.size else 0.0
 
 
 def _attend(tg, a, **kw):
@@ -474,6 +474,62 @@ def test_attention_mixed(tg, nh, nkv, hd, lens, past, window):
     say(f"attention mixed {nh, nkv, hd} lens={lens} past={past} window={window}")
     a = Attend(sum(lens) + hd, nh, nkv, hd, lens, past, 32, window=window, sinks=nkv != 2, lead=2, tail=1, spread=3)
     say(f"  worst error / tolerance {_attend(tg, a):.3f}")
+
+
+@pytest.mark.parametrize("nh,nkv,hd,lens,past,window,size", [
+    (32, 4, 128, [4100], [20], 0, 64), (28, 2, 112, [4700], [0], 0, 16), (32, 4, 128, [4300], [700], 900, 128), (64, 8, 64, [2200], [33], 0, 32),
+    (64, 8, 32, [2100], [0], 300, 1024), (32, 4, 128, [2100, 3, 2500], [100, 4000, 0], 0, 64), (16, 16, 80, [5000], [0], 0, 64)])
+def test_attention_of_long_prompts(tg, nh, nkv, hd, lens, past, window, size):
+    """Rows all over a call of many, two heads each; all rows are finite and some see a block that is NaN."""
+    say(f"attention of long prompts {nh, nkv, hd} lens={lens} past={past} window={window}")
+    a, dev = Attend(sum(lens), nh, nkv, hd, lens, past, size, window=window, sinks=hd < 80, lead=1, tail=1, spread=3), Dev(tg)
+    at = past[0] + lens[0] // 2
+    a.pages.ev[a.pages.table[0, at // size], nkv - 1, at % size // 16] = 255
+    rng = np.random.default_rng(1)
+    rows = {1, 2, a.rows - 2, 1 + lens[0] // 2, 1 + lens[0] // 2 + 5} | {int(r) for r in rng.integers(1, a.rows - 1, 25)}
+    only = {r: [int(h) for h in rng.choice(nh, 2, replace=False)] + [nh - 1] for r in rows}
+    ref, tol = attend(a.q, a.pages, a.cu, lens, past, nh, window, a.sinks, only)
+    a.call(dev)
+    done(tg)
+    got = dev.read(a.out, a.q)
+    seen = 0
+    for r, heads in only.items():
+        s = next(i for i in range(a.n) if a.cu[i] <= r < a.cu[i + 1])
+        last = past[s] + r - a.cu[s]
+        lo = max(0, last + 1 - window) if window else 0
+        for h in heads:
+            x = slice(h * hd, h * hd + hd)
+            nan = s == 0 and h // (nh // nkv) == nkv - 1 and last >= at // 16 * 16 and lo <= at // 16 * 16 + 15
+            seen += nan
+            if nan:
+                assert np.isnan(got[r, x]).all(), (r, h)
+            else:
+                assert np.all(np.abs(got[r, x] - ref[r, x]) <= tol[r, x]), (r, h)
+    assert seen
+    assert np.array_equal(got[0], a.was[0]) and np.array_equal(got[-1], a.was[-1])
+    heads = got[1:-1].reshape(-1, nh, hd)[:, :(nkv - 1) * (nh // nkv)]
+    assert np.isfinite(heads).all()
+    dev.free()
+
+
+def test_mixed_graph(tg):
+    """A mixed call captured once, replayed with other lengths: other tiles are cut then."""
+    say("mixed graph")
+    lib, dev = tg.lib(), Dev(tg)
+    a = Attend(33, 16, 2, 64, [200, 1, 9, 1], [100, 2500, 900, 30], size=32, room=1200)
+    for s in range(4):
+        a.pages.fill(a.rng, s, a.max_kv)
+    a.call(dev)
+    done(tg)
+    g = Graph(lambda stream: a.queue(lib, stream))
+    for past in ([100, 2500, 900, 30], [3000, 5, 0, 3500], [0, 0, 3000, 0], [1500, 1500, 1500, 1500]):
+        now = np.array(past, np.int32)
+        lib.tg_hip_memcpy_h2d(a.len_ptr, now.ctypes.data, now.nbytes)
+        lib.tg_hip_memcpy_h2d(a.out, a.was.ctypes.data, a.was.nbytes)
+        g.replay()
+        a.check(tg, dev, attend(a.q, a.pages, a.cu, a.lens, past, 16))
+    g.free()
+    dev.free()
 
 
 def test_attention_mixed_many(tg):
