@@ -438,6 +438,50 @@ __device__ inline bool find_cut(const PromptArgs &a, const RowsPlan &p, int rati
     return true;
 }
 
+/* Item b of a call of at most 64 sequences in tiles of 128: the shortest span
+ * that makes no more of them than run at once, or than half as many beyond the
+ * tiles that there are anyway; a tile's spans are of one length.  Too many or
+ * too uneven spans cost more than they fill: each writes 128 records.  Cut as
+ * tiles of 16 are (find_cut), two sequences of 256 rows behind 15,000
+ * positions took 463 us (64 + 8 heads of 64; so 276), eight single tokens and two chunks of
+ * 512 behind 1,000 and 6,000 174 (32 + 4 of 128; 148), seven sequences of 1 to 1,000
+ * rows as long (56). */
+template <int MTILE>
+__device__ inline bool find_even(const PromptArgs &a, const RowsPlan &p, int ratio, int b, Work &w, const Class &keep) {
+    const int lane = threadIdx.x & 63;
+    Seq q = {0, 0, 0, 0};
+    if (lane < a.s.n) q = seq_at(a.s, lane);
+    keep(q);
+    const int nt = div_up(q.n * ratio, MTILE), end = q.past + q.n;
+    const int sees = nt ? a.window > 0 ? min(end, a.window + (MTILE - 1) / ratio + 1) : end : 0;   /* at most */
+    const int tiles = __builtin_amdgcn_readlane(wave_scan(nt), 63), limit = max(p.target, tiles + p.target / 2);
+    int lo = 0, hi = div_up((int)wave_umax((uint32_t)sees), KT);   /* per is in (lo, hi], in tiles of positions */
+    while (hi - lo > 1) {
+        const int per = (lo + hi) >> 1;
+        const bool fits = __builtin_amdgcn_readlane(wave_scan(nt * min(div_up(sees, per * KT), p.cap)), 63) <= limit;
+        hi = fits ? per : hi, lo = fits ? lo : per;
+    }
+    if (!hi) return false;
+    const int n = max(1, min(div_up(sees, hi * KT), p.cap));
+    int per = div_up(div_up(sees, n), KT) * KT;
+    const int ends = wave_scan(nt * n);
+    const uint64_t past = __ballot(ends > b);
+    if (!past) return false;
+    const int at = __builtin_ctzll(past), steps = __builtin_amdgcn_readlane(nt, at);
+    const int in = b - (at ? __builtin_amdgcn_readlane(ends, at - 1) : 0), split = in / steps;
+    per = __builtin_amdgcn_readlane(per, at);
+    w.sq = lane_seq(q, at);
+    w.m0 = (steps - 1 - (in - split * steps)) * MTILE;
+    set_rows(w, ratio);
+    const int first = tile_lo(a, w), last = tile_hi<MTILE>(w, ratio), count = div_up(last - first, per);
+    if (split >= count) return false;
+    w.rec = p.pre_ns + split;
+    w.count = split ? 0 : count;
+    w.lo = first + split * per;
+    w.hi = min(last, w.lo + per);
+    return true;
+}
+
 /* The work of item b / n_kv.  Whole blocks: a span starts at one and, but for
  * the tile's last, ends at one. */
 template <int MTILE>
@@ -450,6 +494,8 @@ __device__ inline bool find_blocks(const PromptArgs &a, const Part &pt, int rati
     int last = -1;
     if (p.search) {
         if (!find_tile<MTILE>(a, p, ratio, item, w, keep)) return false;
+    } else if (pt.tiles && MTILE == 128 && a.s.n <= 64) {
+        if (!find_even<MTILE>(a, p, ratio, item, w, keep)) return false;
     } else if (p.cap > 1 && a.s.n <= 64) {
         if (!find_cut<MTILE>(a, p, ratio, item, w, keep, last)) return false;
     } else if (!find_span<MTILE>(a, p, ratio, item, w, keep)) {
@@ -1166,10 +1212,8 @@ Cut paged_cut(const PromptArgs &a) {
     auto sees = [&](int rows) { return a.window > 0 ? (int)std::min<long long>(a.s.kv_max, (long long)a.window + rows / ratio + 1) : a.s.kv_max; };
     k.shape = shape_of(m, n_seqs, n_kv, a.head_dim, sees(128));
     if (k.shape == MIXED) {
-        /* us of 1 .. 1,000 rows in seven sequences, then 60 rows and a chunk of 500, then 300 rows behind 3,500 and one (8 heads
-         * of 64): targets of 256 55.8, 90.6, 76.8, of 512 58.3, 109, 65.2 */
         k.items = true;
-        k.part = item_part(a, m, 128, (m / 128 + n_seqs) * n_kv > 256 ? 256 : 512, FEW + 1, INT_MAX);
+        k.part = item_part(a, m, 128, 512, FEW + 1, INT_MAX);
         k.few = item_part(a, m, 16, 512, 1, FEW);
         return k;
     }
