@@ -548,7 +548,7 @@ __device__ inline void to_half(uint32_t w, h2 &a, h2 &b) {
 
 /* ---- few rows: positions over the waves ----
  *
- * A workgroup of four waves takes MT tiles of 16 m-rows; a wave walks blocks
+ * A workgroup of four waves takes 16 m-rows; a wave walks blocks
  * in pairs (every fourth pair), bytes straight from the pages into registers,
  * no LDS and no barrier until the four waves' sums meet.
  *
@@ -559,21 +559,28 @@ __device__ inline void to_half(uint32_t w, h2 &a, h2 &b) {
  * O^T[dim][m-row] is f16 (16x16x32) over both blocks' 32 positions in the
  * order in which the lanes hold their weights, split in two f16; the lanes
  * load V rows 4 (l / 16) .. + 3 of each block, dims HD / 16 (l % 16) .., and one byte
- * permutation a pair both transposes and widens them. */
+ * permutation a pair both transposes and widens them.
+ *
+ * Bound: the pages' bytes where they are many.  64 rows of 32 + 4 heads of 128
+ * behind 61 .. 8,314 positions, 277 MB: 50 us, 5.5 TB/s (256 behind 4,000 each 185 us
+ * with the second kernel, 5.7 TB/s); one of 64 + 8 heads of 64 behind 30,001 12 us, where
+ * the chain of a workgroup is most: its lengths, its table, its first blocks, then
+ * four steps.  (Two steps loaded ahead take 20 registers more and no time less; 32 m-rows a
+ * workgroup 15.4 us instead of 12.2 at nine rows behind 1,000 positions.) */
 constexpr int MN = 16;
 template <int HD>
 struct SharedPN {
     __attribute__((aligned(16))) float mo[4][MN][HD];
     float mm[4][MN], ml[4][MN];
 };
-template <int HD, int MT>
+template <int HD>
 __device__ inline __attribute__((always_inline)) void paged_n(const PromptArgs &a, const Pages &pg, const Part &pt, int item,
                                                               SharedPN<HD> &sh) {
     constexpr int N = HD / 16, J = HD / 64, WORDS = N / 4;
     const int ratio = a.n_heads / a.n_kv, hd = a.head_dim;
     const RowsPlan &p = pt.p;
     Work w;
-    if (!find_blocks<MN * MT>(a, pt, ratio, item, w)) return;
+    if (!find_blocks<MN>(a, pt, ratio, item, w)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c16 = lane & 15, kq = lane >> 4;
 
@@ -610,50 +617,45 @@ __device__ inline __attribute__((always_inline)) void paged_n(const PromptArgs &
     Raw cur;
     load(0, cur);   /* without steps: block 0 of the pages, which is there */
 
-    Lane x[MT];
-    v4i q[MT][3][J];
-    float c[MT], mx[MT], l[MT];
-    v4f o[MT][N];
+    v4i q[3][J];
+    v4f o[N];
     const float base2 = LOG2E / sqrtf((float)hd);
+    const Lane x = lane_rows(a, w, 0, c16, MN, ratio);
+    const float *src = a.q + (size_t)x.r * a.q_stride + (size_t)x.h * hd;
+    f4 u[J][4];
+    float big = 0.f;
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
-        x[m] = lane_rows(a, w, MN * m, c16, MN, ratio);
-        const float *src = a.q + (size_t)x[m].r * a.q_stride + (size_t)x[m].h * hd;
-        f4 u[J][4];
-        float big = 0.f;
+    for (int j = 0; j < J; j++)
 #pragma unroll
-        for (int j = 0; j < J; j++)
+        for (int n = 0; n < 4; n++) {
+            const int d = 64 * j + 16 * kq + 4 * n;
+            u[j][n] = x.live && d < hd ? (f4)*(const f4u *)(src + d) : f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int n = 0; n < 4; n++) {
-                const int d = 64 * j + 16 * kq + 4 * n;
-                u[j][n] = x[m].live && d < hd ? (f4)*(const f4u *)(src + d) : f4{0.f, 0.f, 0.f, 0.f};
+            for (int e = 0; e < 4; e++) big = max_nan(big, fabsf(u[j][n][e]));
+        }
+    big = other_half_max(max16(big));
+    /* 2^s that takes the largest to QMAX at most; a query below 2^-80 scores 0 */
+    const bool fine = big < INFINITY, some = fine && big > 0x1p-80f;
+    const int ex = some ? (__builtin_amdgcn_frexp_mantf(big) > (float)QMAX / 0x1p23f ? 22 : 23) - __builtin_amdgcn_frexp_expf(big) : 0;
 #pragma unroll
-                for (int e = 0; e < 4; e++) big = max_nan(big, fabsf(u[j][n][e]));
+    for (int j = 0; j < J; j++)
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+            uint32_t y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                y[e] = some ? (uint32_t)((int)__builtin_rintf(__builtin_amdgcn_ldexpf(u[j][n][e], ex)) + 0x808080) : 0x808080u;
+#pragma unroll
+            for (int b = 0; b < 3; b++) {
+                const uint32_t sel = (uint32_t)(b | (4 + b) << 8);
+                const uint32_t lo = __builtin_amdgcn_perm(y[1], y[0], sel), hi = __builtin_amdgcn_perm(y[3], y[2], sel);
+                q[b][j][n] = (int)(__builtin_amdgcn_perm(hi, lo, 0x05040100u) ^ 0x80808080u);
             }
-        big = other_half_max(max16(big));
-        /* 2^s that takes the largest to QMAX at most; a query below 2^-80 scores 0 */
-        const bool fine = big < INFINITY, some = fine && big > 0x1p-80f;
-        const int ex = some ? (__builtin_amdgcn_frexp_mantf(big) > (float)QMAX / 0x1p23f ? 22 : 23) - __builtin_amdgcn_frexp_expf(big) : 0;
+        }
+    const float c = __builtin_amdgcn_ldexpf(base2, -ex);
+    float mx = -INFINITY, l = fine ? 0.f : __int_as_float(0x7FC00000);
 #pragma unroll
-        for (int j = 0; j < J; j++)
-#pragma unroll
-            for (int n = 0; n < 4; n++) {
-                uint32_t y[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    y[e] = some ? (uint32_t)((int)__builtin_rintf(__builtin_amdgcn_ldexpf(u[j][n][e], ex)) + 0x808080) : 0x808080u;
-#pragma unroll
-                for (int b = 0; b < 3; b++) {
-                    const uint32_t sel = (uint32_t)(b | (4 + b) << 8);
-                    const uint32_t lo = __builtin_amdgcn_perm(y[1], y[0], sel), hi = __builtin_amdgcn_perm(y[3], y[2], sel);
-                    q[m][b][j][n] = (int)(__builtin_amdgcn_perm(hi, lo, 0x05040100u) ^ 0x80808080u);
-                }
-            }
-        c[m] = __builtin_amdgcn_ldexpf(base2, -ex);
-        mx[m] = -INFINITY, l[m] = fine ? 0.f : __int_as_float(0x7FC00000);
-#pragma unroll
-        for (int n = 0; n < N; n++) o[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int n = 0; n < N; n++) o[n] = v4f{0.f, 0.f, 0.f, 0.f};
 
     const float one = opaque_one();
     for (int n = 0; n < steps; n++) {
@@ -666,69 +668,66 @@ __device__ inline __attribute__((always_inline)) void paged_n(const PromptArgs &
             if (((n + 1) & 31) == 0) bl = chunk(n + 1);
             load(2 * ((n + 1) & 31), cur);
         }
-        h8 ph[MT], pl[MT];
+        h8 ph, pl;
+        float s[2][4], ck[2], top = -INFINITY;
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            float s[2][4], ck[2], top = -INFINITY;
+        for (int b = 0; b < 2; b++) {
+            v4i d[3];
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
-                v4i d[3];
+            for (int g = 0; g < 3; g++) {
+                d[g] = v4i{0, 0, 0, 0};
 #pragma unroll
-                for (int g = 0; g < 3; g++) {
-                    d[g] = v4i{0, 0, 0, 0};
+                for (int j = 0; j < J; j++)
+                    d[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, r.k[b][j]), q[g][j], d[g], 0, 0, 0);
+            }
+            ck[b] = c * exp_up(ex[b] & 255);
 #pragma unroll
-                    for (int j = 0; j < J; j++)
-                        d[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, r.k[b][j]), q[m][g][j], d[g], 0, 0, 0);
+            for (int v = 0; v < 4; v++) s[b][v] = fmaf((float)(d[2][v] * 256 + d[1][v]), 256.f, (float)d[0][v]);
+        }
+        if (t + 31 > x.all_hi || t < x.all_lo) {   /* uniform */
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    const int pos = t + 16 * b + 4 * kq + v;
+                    s[b][v] = pos <= x.last && pos >= x.first ? s[b][v] : -INFINITY;
                 }
-                ck[b] = c[m] * exp_up(ex[b] & 255);
+        }
 #pragma unroll
-                for (int v = 0; v < 4; v++) s[b][v] = fmaf((float)(d[2][v] * 256 + d[1][v]), 256.f, (float)d[0][v]);
+        for (int b = 0; b < 2; b++) {
+            const float u = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3]));
+            top = fmaxf(top, fmaf(u, ck[b], (float)((ex[b] >> 8 & 255) - 127)));
+        }
+        top = other_half_max(max16(top));
+        if (__any(top > mx + LAG_H)) {
+            const float mn = fmaxf(mx, ceilf(top));
+            const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
+            mx = mn;
+            l *= alpha;
+#pragma unroll
+            for (int k = 0; k < N; k++) o[k] *= alpha;
+        }
+        const float ref = mx == -INFINITY ? 0.f : SHIFT_H - mx;
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int ev = ex[b] >> 8 & 255;
+            const float add = ref + (float)(ev - 127);
+            float e[4];
+#pragma unroll
+            for (int v = 0; v < 4; v++) e[v] = __builtin_amdgcn_exp2f(fmaf(s[b][v], ck[b], add));
+            l = fmaf((e[0] + e[1]) + (e[2] + e[3]), exp_down(ev), l);
+#pragma unroll
+            for (int v = 0; v < 4; v += 2) {
+                h2 hi, lo;
+                split2(e[v], e[v + 1], e[v], e[v + 1], one, hi, lo);
+                ph[4 * b + v] = hi[0], ph[4 * b + v + 1] = hi[1];
+                pl[4 * b + v] = lo[0], pl[4 * b + v + 1] = lo[1];
             }
-            if (t + 31 > x[m].all_hi || t < x[m].all_lo) {   /* uniform */
+        }
+        if ((ex[0] | ex[1]) >> 16) {   /* uniform, hardly ever */
 #pragma unroll
-                for (int b = 0; b < 2; b++)
-#pragma unroll
-                    for (int v = 0; v < 4; v++) {
-                        const int pos = t + 16 * b + 4 * kq + v;
-                        s[b][v] = pos <= x[m].last && pos >= x[m].first ? s[b][v] : -INFINITY;
-                    }
-            }
-#pragma unroll
-            for (int b = 0; b < 2; b++) {
-                const float u = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3]));
-                top = fmaxf(top, fmaf(u, ck[b], (float)((ex[b] >> 8 & 255) - 127)));
-            }
-            top = other_half_max(max16(top));
-            if (__any(top > mx[m] + LAG_H)) {
-                const float mn = fmaxf(mx[m], ceilf(top));
-                const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[m] - mn);
-                mx[m] = mn;
-                l[m] *= alpha;
-#pragma unroll
-                for (int k = 0; k < N; k++) o[m][k] *= alpha;
-            }
-            const float ref = mx[m] == -INFINITY ? 0.f : SHIFT_H - mx[m];
-#pragma unroll
-            for (int b = 0; b < 2; b++) {
-                const int ev = ex[b] >> 8 & 255;
-                const float add = ref + (float)(ev - 127);
-                float e[4];
-#pragma unroll
-                for (int v = 0; v < 4; v++) e[v] = __builtin_amdgcn_exp2f(fmaf(s[b][v], ck[b], add));
-                l[m] = fmaf((e[0] + e[1]) + (e[2] + e[3]), exp_down(ev), l[m]);
-#pragma unroll
-                for (int v = 0; v < 4; v += 2) {
-                    h2 hi, lo;
-                    split2(e[v], e[v + 1], e[v], e[v + 1], one, hi, lo);
-                    ph[m][4 * b + v] = hi[0], ph[m][4 * b + v + 1] = hi[1];
-                    pl[m][4 * b + v] = lo[0], pl[m][4 * b + v + 1] = lo[1];
-                }
-            }
-            if ((ex[0] | ex[1]) >> 16) {   /* uniform, hardly ever */
-#pragma unroll
-                for (int b = 0; b < 2; b++)
-                    if (ex[b] >> 16 && x[m].first <= t + 16 * b + 15 && x[m].last >= t + 16 * b) l[m] = __int_as_float(0x7FC00000);
-            }
+            for (int b = 0; b < 2; b++)
+                if (ex[b] >> 16 && x.first <= t + 16 * b + 15 && x.last >= t + 16 * b) l = __int_as_float(0x7FC00000);
         }
 #pragma unroll
         for (int k = 0; k < N; k++) {
@@ -740,70 +739,63 @@ __device__ inline __attribute__((always_inline)) void paged_n(const PromptArgs &
                 const h2 y = __builtin_bit_cast(h2, __builtin_amdgcn_perm(r.v[e + 1][k >> 2], r.v[e][k >> 2], sel) ^ 0x64806480u) - bias;
                 v[e] = y[0], v[e + 1] = y[1];
             }
-#pragma unroll
-            for (int m = 0; m < MT; m++) {
-                o[m][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[m], o[m][k], 0, 0, 0);
-                o[m][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[m], o[m][k], 0, 0, 0);
-            }
+            o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[k], 0, 0, 0);
+            o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, o[k], 0, 0, 0);
         }
     }
 
     /* the waves' sums as one, in wave order: 16 threads a row, HD / 16 dims each */
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
-        l[m] += __shfl_xor(l[m], 16, 64);
-        l[m] += __shfl_xor(l[m], 32, 64);
-        if (m) __syncthreads();
+    for (int v = 0; v < 4; v++)
 #pragma unroll
-        for (int v = 0; v < 4; v++)
+        for (int n = 0; n < N; n += 4)
+            *(f4 *)&sh.mo[wave][c16][N * (4 * kq + v) + n] = f4{o[n][v], o[n + 1][v], o[n + 2][v], o[n + 3][v]};
+    if (kq == 0) sh.mm[wave][c16] = mx, sh.ml[wave][c16] = l;
+    __syncthreads();
+    const int row = tid >> 4, d0 = (tid & 15) * N;
+    const Lane y = lane_rows(a, w, 0, row, MN, ratio);
+    float M = sh.mm[0][row];
 #pragma unroll
-            for (int n = 0; n < N; n += 4)
-                *(f4 *)&sh.mo[wave][c16][N * (4 * kq + v) + n] = f4{o[m][n][v], o[m][n + 1][v], o[m][n + 2][v], o[m][n + 3][v]};
-        if (kq == 0) sh.mm[wave][c16] = mx[m], sh.ml[wave][c16] = l[m];
-        __syncthreads();
-        const int row = tid >> 4, d0 = (tid & 15) * N;
-        const Lane y = lane_rows(a, w, MN * m, row, MN, ratio);
-        float M = sh.mm[0][row];
+    for (int g = 1; g < 4; g++) M = fmaxf(M, sh.mm[g][row]);
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f, r[N];
 #pragma unroll
-        for (int g = 1; g < 4; g++) M = fmaxf(M, sh.mm[g][row]);
-        const float base = M == -INFINITY ? 0.f : M;
-        float L = 0.f, r[N];
+    for (int n = 0; n < N; n++) r[n] = 0.f;
 #pragma unroll
-        for (int n = 0; n < N; n++) r[n] = 0.f;
+    for (int g = 0; g < 4; g++) {
+        const float e = __builtin_amdgcn_exp2f(sh.mm[g][row] - base);
+        L = fmaf(sh.ml[g][row], e, L);
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const float e = __builtin_amdgcn_exp2f(sh.mm[g][row] - base);
-            L = fmaf(sh.ml[g][row], e, L);
-#pragma unroll
-            for (int n = 0; n < N; n++) r[n] = fmaf(sh.mo[g][row][d0 + n], e, r[n]);
-        }
-        if (!y.live || d0 >= hd) continue;
-        float *dst, f;
-        const long long rec = record_of<MN * MT>(a, pt, w, y, MN * m + row);
-        if (rec >= 0) {
-            f = UNSHIFT;
-            if (d0 == 0) write_ml(p, w, rec, M, L * f);
-            if (M == -INFINITY) continue;   /* a record of no position has no sums */
-            dst = p.o + rec * hd + d0;
-        } else {
-            f = 1.f;
-            if (a.sinks) {
-                const float ref = M - SHIFT_H, sk = a.sinks[y.h] * LOG2E, mn = fmaxf(ref, sk), b2 = mn == -INFINITY ? 0.f : mn;
-                f = exp2f(ref - b2);
-                L = L * f + exp2f(sk - b2);
-            }
-            f /= L;
-            dst = a.out + (size_t)y.r * a.out_stride + (size_t)y.h * hd + d0;
-        }
-#pragma unroll
-        for (int n = 0; n < N; n += 4) *(f4u *)(dst + n) = f4{r[n] * f, r[n + 1] * f, r[n + 2] * f, r[n + 3] * f};
+        for (int n = 0; n < N; n++) r[n] = fmaf(sh.mo[g][row][d0 + n], e, r[n]);
     }
+    if (!y.live || d0 >= hd) return;
+    float *dst, f;
+    const long long rec = record_of<MN>(a, pt, w, y, row);
+    if (rec >= 0) {
+        f = UNSHIFT;
+        if (d0 == 0) write_ml(p, w, rec, M, L * f);
+        if (M == -INFINITY) return;   /* a record of no position has no sums */
+        dst = p.o + rec * hd + d0;
+    } else {
+        f = 1.f;
+        if (a.sinks) {
+            const float ref = M - SHIFT_H, sk = a.sinks[y.h] * LOG2E, mn = fmaxf(ref, sk), b2 = mn == -INFINITY ? 0.f : mn;
+            f = exp2f(ref - b2);
+            L = L * f + exp2f(sk - b2);
+        }
+        f /= L;
+        dst = a.out + (size_t)y.r * a.out_stride + (size_t)y.h * hd + d0;
+    }
+#pragma unroll
+    for (int n = 0; n < N; n += 4) *(f4u *)(dst + n) = f4{r[n] * f, r[n + 1] * f, r[n + 2] * f, r[n + 3] * f};
 }
 
-template <int HD, int MT>
+template <int HD>
 __global__ __launch_bounds__(256, 2) void k_paged_n(PromptArgs a, Pages pg, Part pt) {
     __shared__ SharedPN<HD> sh;
-    paged_n<HD, MT>(a, pg, pt, blockIdx.x, sh);
+    paged_n<HD>(a, pg, pt, blockIdx.x, sh);
 }
 
 /* ---- many rows ----
@@ -813,7 +805,16 @@ __global__ __launch_bounds__(256, 2) void k_paged_n(PromptArgs a, Pages pg, Part
  * are loaded two tiles of 64 positions ahead and widened to f16, which holds
  * them, as they are stored to one of two LDS buffers one tile ahead.  With
  * KG = 2, two groups of MW waves take the tiles in turn; J blocks of 32
- * positions are computed together. */
+ * positions are computed together.
+ *
+ * Bound for long prompts: the matrix units at the power limit and the issue of
+ * the softmax beside them.  8,192 rows of 32 heads of 128: 909 us, 1.21 PFLOP/s
+ * counting both products (a large f16 product runs at 1.15 - 1.2); of 64 heads of 64
+ * 1,048, where a product is half as long and the softmax is not: three waves a
+ * SIMD, 168 registers (two 1,098).  Widening costs a quarter more VALU
+ * instructions than f16 caches take.  (Integer products for the scores, as few rows have, would be a
+ * quarter less of the first product and twice that in joining its digits; the widening before the
+ * products in half of the waves and behind them in the others changed nothing.) */
 template <int HD, int MW, int KG>
 struct SharedPW {
     __attribute__((aligned(1024))) uint8_t bufs[KG][2][2][KT * HD * 2];
@@ -1078,22 +1079,24 @@ __device__ inline __attribute__((always_inline)) void paged_w(const PromptArgs &
 }
 
 template <int HD, int MW, int KG, int J>
-__global__ __launch_bounds__(64 * MW * KG, 2) void k_paged_w(PromptArgs a, Pages pg, Part pt) {
+__global__ __launch_bounds__(64 * MW * KG, HD == 64 && MW * KG == 4 ? 3 : 2) void k_paged_w(PromptArgs a, Pages pg, Part pt) {
     __shared__ SharedPW<HD, MW, KG> sh;
     paged_w<HD, MW, KG, J>(a, pg, pt, blockIdx.x, sh);
 }
 
 /* A mixed call in one launch: sequences of many rows in tiles of 128, those of
- * few in tiles of 16, each kind cut into spans by its own positions. */
+ * few in tiles of 16, each kind cut into spans by its own positions.  In two
+ * launches 60 single tokens and a chunk of 500 rows took 119 us (32 + 4 heads of 128; so 108 - 112), seven
+ * sequences of 1 to 1,000 rows 73 (55 - 62). */
 template <int HD>
-__global__ __launch_bounds__(256, 2) void k_paged_both(PromptArgs a, Pages pg, Part many, Part few) {
+__global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_both(PromptArgs a, Pages pg, Part many, Part few) {
     __shared__ union {
         SharedPW<HD, 4, 1> w;
         SharedPN<HD> n;
     } sh;
     const int first = many.p.items * a.n_kv;
     if ((int)blockIdx.x < first) paged_w<HD, 4, 1, 2>(a, pg, many, blockIdx.x, sh.w);
-    else paged_n<HD, 1>(a, pg, few, (int)blockIdx.x - first, sh.n);
+    else paged_n<HD>(a, pg, few, (int)blockIdx.x - first, sh.n);
 }
 
 /* The records of a cut tile's rows as one: a workgroup of 16 waves has a KV
@@ -1187,15 +1190,28 @@ namespace {
 
 enum Shape { NARROW, SHORT, WIDE, FULL, TALL, MIXED };
 int tile_of(Shape s) { return s == NARROW ? 16 : s == TALL ? 256 : 128; }
-constexpr long long NARROW_WORK = 1 << 18;
 constexpr int SHORT_BELOW = 512, MOST_SPANS = 64;
 struct Cut {
     Shape shape;
     bool items;       /* records by item */
     Part part, few;   /* few: of a mixed call */
 };
-Shape shape_of(long long m, long long seqs, int n_kv, int head_dim, int positions) {
-    if (m <= 16 * seqs || (m <= 128 * seqs && m * positions <= NARROW_WORK)) return NARROW;
+/* Whether tiles of 16 take less time, in us, from fits to one call of many shapes (1 to 1,500 rows behind 0 to 16,000 positions,
+ * 32 + 4 heads of 128 and 64 + 8 of 64; off by a tenth mostly): what starts, each workgroup, and each 2^20 pairs of an
+ * m-row and a position.  Tiles of 128 do the pairs faster and start later.  128 rows 8.8 us in tiles of 16 and 13.5 in tiles
+ * of 128, 300 behind 1,000 positions 30.7 and 34.9, 1,024 44.2 and 39.5, nine behind 4,000 14.3 and 19.7, 100 behind 8,000 58.3
+ * and 45.6 (heads of 128). */
+bool narrow_is_faster(long long m, long long rows, long long seqs, int n_kv, int head_dim, int positions, bool window) {
+    const bool big = head_dim > 64;
+    /* how many positions a row sees on average: of a chunk known, of several sequences half the longest's */
+    const double seen = seqs > 1 ? positions / 2.0 : window ? positions : positions - (double)std::min<long long>(rows, positions) / 2;
+    const double pairs = m * seen * n_kv / (1 << 20), wgs = (double)std::max(m / 16, seqs) * n_kv;
+    const double narrow = (wgs < 512 && positions > 640 ? 10 : 5) + wgs * (big ? 0.0115 : 0.005) + pairs * (big ? 1.5 : 1.05);
+    if (positions < SHORT_BELOW) return narrow < 8 + positions * (big ? 0.035 : 0.022) * std::max(1.0, wgs / 8 / 512);
+    return narrow < (seqs > 1 ? 8 : 0) + (big ? 19 : 14) + wgs * (big ? 0.004 : 0.002) + pairs * (big ? 1.05 : 0.64);
+}
+Shape shape_of(long long m, long long rows, long long seqs, int n_kv, int head_dim, int positions, bool window) {
+    if (m <= 16 * seqs || narrow_is_faster(m, rows, seqs, n_kv, head_dim, positions, window)) return NARROW;
     if (positions < SHORT_BELOW) return SHORT;
     if (seqs > 1) return MIXED;
     if (head_dim > 64 && m / 256 * n_kv >= 512) return TALL;
@@ -1224,7 +1240,7 @@ Cut paged_cut(const PromptArgs &a) {
     const int n_seqs = a.s.n, n_kv = a.n_kv, ratio = a.n_heads / n_kv;
     const long long m = (long long)a.s.rows * ratio;
     auto sees = [&](int rows) { return a.window > 0 ? (int)std::min<long long>(a.s.kv_max, (long long)a.window + rows / ratio + 1) : a.s.kv_max; };
-    k.shape = shape_of(m, n_seqs, n_kv, a.head_dim, sees(128));
+    k.shape = shape_of(m, a.s.rows, n_seqs, n_kv, a.head_dim, sees(128), a.window > 0);
     if (k.shape == MIXED) {
         k.items = true;
         k.part = item_part(a, m, 128, 512, FEW + 1, INT_MAX);
@@ -1291,13 +1307,16 @@ template <int HD>
 void launch_paged(const PromptArgs &a, const Pages &pg, const Cut &k, hipStream_t st) {
     const dim3 grid((unsigned)((k.part.p.items + k.few.p.items) * a.n_kv));
 #define PAGED(threads, ...) hipLaunchKernelGGL((__VA_ARGS__), grid, dim3(threads), 0, st, a, pg, k.part)
-    if (k.shape == NARROW) PAGED(256, k_paged_n<HD, 1>);
+    if (k.shape == NARROW) PAGED(256, k_paged_n<HD>);
     else if (k.shape == SHORT) PAGED(256, k_paged_w<HD, 4, 1, 1>);
     else if (k.shape == WIDE) PAGED(512, k_paged_w<HD, 4, 2, 2>);
     else if (k.shape == FULL) PAGED(256, k_paged_w<HD, 4, 1, 2>);
-    else if (k.shape == TALL) PAGED(512, k_paged_w<HD, 8, 1, 2>);
+    else if (k.shape == TALL) {
+        if constexpr (HD > 64) PAGED(512, k_paged_w<HD, 8, 1, 2>);   /* no smaller head is TALL (shape_of) */
+    } else {
+        hipLaunchKernelGGL((k_paged_both<HD>), grid, dim3(256), 0, st, a, pg, k.part, k.few);
+    }
 #undef PAGED
-    else hipLaunchKernelGGL((k_paged_both<HD>), grid, dim3(256), 0, st, a, pg, k.part, k.few);
     if (!k.items) {
         if (k.part.p.nrec) launch_rows_combine(a, k.part.p, st);
         return;
