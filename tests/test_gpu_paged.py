@@ -673,6 +673,51 @@ def test_shared_pages(tg):
     _attend(tg, a)
 
 
+def test_null_lengths(tg):
+    """Without kv_len every sequence begins at position 0."""
+    say("null kv_len")
+    lib, dev = tg.lib(), Dev(tg)
+    x = Append(34, 8, 2, 64, [20, 3, 40], [0, 0, 0], 32, rot=16)
+    x.call(dev)
+    args = list(x.args)
+    args[14] = None
+    for ptr, t in zip(x.ptr, x.pages.arrays()):
+        lib.tg_hip_memcpy_h2d(ptr, t.ctypes.data, t.nbytes)
+    lib.tg_hip_paged_append_dev(*args, None)
+    x.check(tg, dev)
+    a = Attend(35, 8, 2, 64, [20, 3, 40], [0, 0, 0], 32)
+    a.call(dev)
+    args = list(a.args)
+    args[11] = None
+    lib.tg_hip_memcpy_h2d(a.out, a.was.ctypes.data, a.was.nbytes)
+    lib.tg_hip_attention_paged_dev(*args, None)
+    a.check(tg, dev)
+    dev.free()
+
+
+@pytest.mark.parametrize("n,nh,nkv,hd", [(128, 32, 4, 128), (100, 64, 8, 64), (300, 8, 1, 96)])
+def test_single_tokens_of_many(tg, n, nh, nkv, hd):
+    """Single tokens whose lengths lie far apart: the long ones are cut, more sequences than a wave looks at at once."""
+    say(f"single tokens of {n} sequences {nh, nkv, hd}")
+    past = [(37 * i * i) % 90 for i in range(n)]
+    past[n // 2], past[3], past[-1] = 9000, 5000, 7001
+    lens = [1] * n
+    lens[5] = 0
+    a, dev = Attend(n, nh, nkv, hd, lens, past, 64, sinks=hd == 64), Dev(tg)
+    rows = [0, 1, 3, 4, 5, n // 2 - 1, n // 2, n - 2] + [int(r) for r in a.rng.integers(0, n - 1, 10)]
+    only = {r: [0, nh // 2, nh - 1] for r in rows}
+    ref, tol = attend(a.q, a.pages, a.cu, lens, past, nh, 0, a.sinks, only)
+    a.call(dev)
+    done(tg)
+    got = dev.read(a.out, a.q)
+    for r, heads in only.items():
+        for h in heads:
+            x = slice(h * hd, h * hd + hd)
+            assert np.all(np.abs(got[r, x] - ref[r, x]) <= tol[r, x]), (r, h)
+    assert np.isfinite(got).all()
+    dev.free()
+
+
 # ------------------------------------------------------------------ graphs, streams, together
 
 def test_graph(tg):
