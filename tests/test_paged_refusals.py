@@ -147,6 +147,29 @@ def test_sizes_rise_with_every_argument(tg):
         assert size(a, b, nh, nkv, hd, c) <= size(rows, n, nh, nkv, hd, kv), (rows, n, nh, nkv, hd, kv, a, b, c)
 
 
+def test_scratch_serves_mixed_calls(tg):
+    """Calls that always need scratch, so that they are refused and no device is asked: some many rows and some few behind long
+    contexts."""
+    lib, rng, seen = tg.lib(), np.random.default_rng(5), 0
+    for _ in range(3000):
+        nkv = int(rng.choice([1, 2, 4, 8]))
+        nh = nkv * int(rng.choice([1, 2, 4, 8, 16]))
+        hd, n, kv = int(rng.choice([16, 64, 80, 128])), int(rng.integers(2, 12)), int(rng.integers(8192, 100000))
+        rows = int(rng.integers(600, 4000))
+        size = lib.tg_hip_attention_paged_scratch_bytes(rows, n, nh, nkv, hd, kv)
+        for a, b, c in ((rows, n, kv), (rows, smaller(rng, n), kv), (max(600, smaller(rng, rows)), n, max(8192, smaller(rng, kv)))):
+            if (a * nh // nkv // 128 + b) * nkv > 1000 or a * nh // nkv < 600 or b < 2:
+                continue
+            lib.tg_hip_clear_error()
+            lib.tg_hip_attention_paged_dev(*_attend(rows=a, n=b, max_kv=c, nh=nh, nkv=nkv, hd=hd, q_stride=nh * hd, out_stride=nh * hd,
+                                                    stride=1 << 14, scratch=P + 4))
+            said = tg.last_error()
+            assert "needs" in said and int(said.split("needs ")[1].split()[0]) <= size, (rows, n, nh, nkv, hd, kv, a, b, c, said, size)
+            seen += 1
+    lib.tg_hip_clear_error()
+    assert seen > 3000
+
+
 @pytest.mark.gpu
 def test_scratch_serves_smaller_calls(tg):
     """Given scratch at an odd place a call says how much it needs; its rows are none, so one that needs nothing runs."""
