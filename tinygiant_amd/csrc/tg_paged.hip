@@ -465,10 +465,16 @@ __device__ inline bool find_even(const PromptArgs &a, const RowsPlan &p, int rat
     const int lane = threadIdx.x & 63;
     Seq q = {0, 0, 0, 0};
     if (lane < a.s.n) q = seq_at(a.s, lane);
+    const int end = q.past + q.n, seen = a.window > 0 ? min(end, a.window + (MTILE - 1) / ratio + 1) : end;   /* at most */
+    const float all = (float)div_up(q.n * ratio, 16) * (float)seen;
     keep(q);
-    const int nt = div_up(q.n * ratio, MTILE), end = q.past + q.n;
-    const int sees = nt ? a.window > 0 ? min(end, a.window + (MTILE - 1) / ratio + 1) : end : 0;   /* at most */
-    const int tiles = __builtin_amdgcn_readlane(wave_scan(nt), 63), limit = max(p.target, tiles + p.target / 2);
+    const int nt = div_up(q.n * ratio, MTILE), sees = nt ? seen : 0;
+    /* Where the other part's blocks take longer to read than these tiles to compute, it gets half of the places: 60 single
+     * tokens behind 2,960 positions and a chunk of 500 behind 1,500 113 us with all, 94 with half (64 + 8 heads of 64
+     * 111 and 84); 31 tokens and a chunk of 512 behind 4,000 114 either way. */
+    const float few = wave_sum(nt ? 0.f : all), many = wave_sum((float)nt * (float)(a.window > 0 ? sees : (q.past + end) / 2));
+    const int places = few > 2.f * many ? p.target / 2 : p.target;
+    const int tiles = __builtin_amdgcn_readlane(wave_scan(nt), 63), limit = max(places, tiles + places / 2);
     int lo = 0, hi = div_up((int)wave_umax((uint32_t)sees), KT);   /* per is in (lo, hi], in tiles of positions */
     while (hi - lo > 1) {
         const int per = (lo + hi) >> 1;
@@ -1086,8 +1092,8 @@ __global__ __launch_bounds__(64 * MW * KG, HD == 64 && MW * KG == 4 ? 3 : 2) voi
 
 /* A mixed call in one launch: sequences of many rows in tiles of 128, those of
  * few in tiles of 16, each kind cut into spans by its own positions.  In two
- * launches 60 single tokens and a chunk of 500 rows took 119 us (32 + 4 heads of 128; so 108 - 112), seven
- * sequences of 1 to 1,000 rows 73 (55 - 62). */
+ * launches 60 single tokens and a chunk of 500 rows took 119 us (32 + 4 heads of 128; in one, cut the same way, 108),
+ * seven sequences of 1 to 1,000 rows 73 (68). */
 template <int HD>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_both(PromptArgs a, Pages pg, Part many, Part few) {
     __shared__ union {
