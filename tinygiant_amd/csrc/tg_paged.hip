@@ -539,6 +539,13 @@ __device__ inline long long record_of(const PromptArgs &a, const Part &pt, const
     return pt.p.nrec ? ((long long)x.r * a.n_heads + x.h) * pt.p.nrec + w.rec : -1;
 }
 
+/* A record's statistics.  m of -inf says that its row sees no position there, and
+ * its sum is left out where records meet; a sum that is NaN has to reach the row
+ * (queries that are not finite may leave m as it began), so m is NaN with it. */
+__device__ inline void write_stat(const RowsPlan &p, const Work &w, size_t rec, float m, float l) {
+    write_ml(p, w, rec, l == l ? m : l, l);
+}
+
 __device__ inline float max16(float v) {   /* with the lanes 16 apart */
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return max_nan(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -781,7 +788,7 @@ __device__ inline __attribute__((always_inline)) void paged_n(const PromptArgs &
     const long long rec = record_of<MN>(a, pt, w, y, row);
     if (rec >= 0) {
         f = UNSHIFT;
-        if (d0 == 0) write_ml(p, w, rec, M, L * f);
+        if (d0 == 0) write_stat(p, w, rec, M, L * f);
         if (M == -INFINITY) return;   /* a record of no position has no sums */
         dst = p.o + rec * hd + d0;
     } else {
@@ -839,7 +846,7 @@ __device__ inline void write_paged(const PromptArgs &a, const Part &pt, const Wo
     const long long rec = record_of<MTILE>(a, pt, w, x, from + row);   /* uniform whether there is one */
     if (rec >= 0) {
         f = UNSHIFT;
-        if (write && half == 0) write_ml(pt.p, w, rec, mx, l * f);
+        if (write && half == 0) write_stat(pt.p, w, rec, mx, l * f);
         write = write && mx > -INFINITY;      /* a record of no position has no sums */
         at = rec * hd;
     } else {
