@@ -444,7 +444,9 @@ void tg_hip_paged_read_dev(const int8_t *pages_k_dev, const int8_t *pages_v_dev,
  * outside 85..169, is NaN; so is one whose query is not finite.  K and V are
  * exact; q keeps 22 bits of each value, or of its head's largest magnitude 24 (a head
  * below 2^-80 scores 0), by how many rows there are; the weights 22, or 2^-33 of the
- * row's largest weight times value; sums and the softmax's statistics are f32.  out may be q with q's stride.
+ * row's largest weight times value; sums and the softmax's statistics are f32.  A row with a score beyond 9.3e7
+ * (2^27 in base 2, where f32 has steps of 16) is NaN, and scores below the negative of that have no weight.  out may be
+ * q with q's stride.
  * scratch_dev holds tg_hip_attention_paged_scratch_bytes(...) bytes, 16-byte
  * aligned; it may be NULL where that is 0.  The size is enough for every call of
  * at most as many rows, sequences and positions (max_kv) with these heads.

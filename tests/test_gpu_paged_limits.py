@@ -1,9 +1,10 @@
-"""GPU checks of paged attention where queries are not finite beside sinks."""
+"""GPU checks of paged attention where queries are not finite beside sinks, and
+where scores are larger than f32 has room for a weight's exponent beside them."""
 
 import numpy as np
 import pytest
 
-from tests._packed import Dev
+from tests._packed import EPS, Dev
 from tests._paged import attend
 from tests.test_gpu_paged import Attend, done, say
 
@@ -47,3 +48,93 @@ def test_queries_not_finite_beside_sinks(tg, nh, nkv, hd, lens, past, bad):
                 want, tol = attend(a.q, a.pages, a.cu, lens, past, nh, sinks=a.sinks, only=some_rows(a, rest))
                 assert np.all(np.abs(got[rest] - want[rest]) <= tol[rest])
             dev.free()
+
+
+def large_scores(seed, nh, nkv, hd, lens, past, powers):
+    """Scores of 2^24 and more in base 2 (1.2e7) that f32 holds: q is 2^p in one dimension and 2^(p - 17) in the next, K a number
+    of 64 .. 127 and one that rises in steps along the positions.  Their sums have 24 bits in every kernel's units, so that no product or
+    sum of a score is rounded, only the factor log2 e / sqrt(head_dim), alike for all of a row's positions."""
+    a = Attend(seed, nh, nkv, hd, lens, past, 32)
+    rng, p = a.rng, a.pages
+    p.k[:] = 0
+    p.ek[:] = 127
+    for s in range(a.n):
+        n = lens[s] + past[s]
+        for h in range(nkv):
+            first = rng.integers(64, 128)
+            rise = -120 + np.cumsum(np.where(rng.random(n) < 0.1, rng.integers(1, 13, n), 0))
+            rise = np.where(rise > 127, rng.integers(100, 128, n), rise)   # the whole way up, then mixed
+            for t in range(n):
+                page, i = p.table[s, t // 32], t % 32
+                p.k[page, h, i, 0], p.k[page, h, i, 1] = first, rise[t]
+    a.q[:] = 0
+    for r in range(a.rows):
+        for h in range(nh):
+            at = 2.0 ** powers[(r + h) % len(powers)]
+            a.q[r, h * hd], a.q[r, h * hd + 1] = at, at * 2.0 ** -17
+    return a
+
+
+def chosen(a):
+    rows = {0, a.rows - 1, *(int(c) for c in a.cu[:-1]), *(int(c) - 1 for c in a.cu[1:]), *range(a.rows // 2, a.rows // 2 + 3)}
+    return some_rows(a, [r for r in rows if 0 <= r < a.rows])
+
+
+@pytest.mark.parametrize("powers", [(19, 20), (20, 21, 22)])
+@pytest.mark.parametrize("nh,nkv,hd,lens,past", CALLS + [(64, 1, 64, [1100], [0]), (64, 2, 128, [2100], [0])])
+def test_large_scores(tg, nh, nkv, hd, lens, past, powers):
+    """Differences of scores, of which those up to 40 count (2^-40 of a weight is nothing), are off by the factor's three
+    roundings and one of their own, 40 (3 + 1) EPS, for numerator and denominator each and log 2 to the base e; the rest as for
+    other scores."""
+    say(f"attention of large scores {nh, nkv, hd, lens, past} {powers}")
+    a = large_scores(42, nh, nkv, hd, lens, past, powers)
+    dev = Dev(tg)
+    a.call(dev)
+    done(tg)
+    got, only = dev.read(a.out, a.q), chosen(a)
+    want, _ = attend(a.q, a.pages, a.cu, lens, past, nh, only=only)
+    rows = sorted(only)
+    n = a.longest
+    big = max(np.abs(a.pages.values("v", s, lens[s] + past[s])).max() for s in range(a.n))
+    tol = (2 * 40 * 4 * EPS + (8 * np.sqrt(n) + 24) * EPS + n * 2.0 ** -31) * big
+    assert np.all(np.isfinite(got[rows])), [(r, int((~np.isfinite(got[r])).sum())) for r in rows]
+    err = np.abs(got[rows] - want[rows])
+    assert np.all(err <= tol), (float(err.max()), tol)
+    dev.free()
+
+
+@pytest.mark.parametrize("sinks", [False, True])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("power", [18, 20, 24, 27, 31, 60, 115])
+@pytest.mark.parametrize("nh,nkv,hd,lens,past", CALLS)
+def test_scores_far_apart(tg, nh, nkv, hd, lens, past, power, sign, sinks):
+    """Scores up to 2^120 whose least difference is 2^-7 of them: up to 2^27 in base 2 the largest takes all of the softmax, several
+    that are equal share it, and what is off is the rounding of the weights and of sums of n of them. Past 2^27 a row is
+    NaN, and where all are below -2^27 the sink's weight is all that is left, or nothing."""
+    say(f"attention of scores far apart {nh, nkv, hd, lens, past} 2^{power} {sign} sinks={sinks}")
+    a = Attend(43, nh, nkv, hd, lens, past, 32, sinks=sinks)
+    a.pages.k[:] = 0
+    a.pages.ek[:] = 127
+    a.pages.k[..., 0] = a.rng.integers(1, 128, a.pages.k.shape[:-1])
+    a.q[:] = 0
+    a.q[:, :nh * hd:hd] = sign * 2.0 ** power
+    dev = Dev(tg)
+    a.call(dev)
+    done(tg)
+    got, only = dev.read(a.out, a.q), chosen(a)
+    want, _ = attend(a.q, a.pages, a.cu, lens, past, nh, sinks=a.sinks, only=only)
+    for s in range(a.n):
+        keys = a.pages.values("k", s, lens[s] + past[s])[:, :, 0]
+        for r in only:
+            if a.cu[s] <= r < a.cu[s + 1]:
+                z = sign * 2.0 ** power * keys[:, :past[s] + r - a.cu[s] + 1].astype(np.float64) * hd ** -0.5 / np.log(2)
+                top = np.repeat(z.max(1), nh // nkv)
+                assert np.all(np.abs(np.abs(top) - 2.0 ** 27) > 2.0 ** 20)
+                want[r].reshape(nh, hd)[(top > 2.0 ** 27) | ((top < -2.0 ** 27) & (not sinks))] = np.nan
+    rows = sorted(only)
+    big = max(np.abs(a.pages.values("v", s, lens[s] + past[s])).max() for s in range(a.n))
+    tol = ((8 * np.sqrt(a.longest) + 24) * EPS + a.longest * 2.0 ** -31) * big
+    assert np.array_equal(np.isnan(got[rows]), np.isnan(want[rows])), (int(np.isnan(got[rows]).sum()), int(np.isnan(want[rows]).sum()))
+    err = np.nan_to_num(np.abs(got[rows] - want[rows]))
+    assert np.all(err <= tol), (float(err.max()), tol)
+    dev.free()
