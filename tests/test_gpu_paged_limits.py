@@ -138,3 +138,28 @@ def test_scores_far_apart(tg, nh, nkv, hd, lens, past, power, sign, sinks):
     err = np.nan_to_num(np.abs(got[rows] - want[rows]))
     assert np.all(err <= tol), (float(err.max()), tol)
     dev.free()
+
+
+@pytest.mark.parametrize("nh,nkv,hd,rows,n,past,fill", [
+    (32, 4, 128, 600, 9, 9000, 0x7F), (32, 4, 128, 600, 9, 9000, 0x00), (64, 8, 64, 500, 20, 900, 0xFF), (32, 4, 128, 40, 30, 4000, 0x11),
+    (64, 8, 64, 3, 41, 6000, 0x01), (32, 4, 128, 700, 90, 2000, 0x01)])
+def test_offsets_that_overlap(tg, nh, nkv, hd, rows, n, past, fill):
+    """Offsets 0, R, 0, R, ... are no packed rows, and what comes out is nothing; but every other sequence has all rows, many
+    more spans than a call of so many rows has room for, and nothing may be read or written outside the arrays, whatever
+    the scratch held."""
+    say(f"attention of overlapping sequences {nh, nkv, hd, rows, n, past} scratch {fill:#x}")
+    lens = [rows // n] * n
+    lens[0] += rows - sum(lens)
+    a = Attend(44, nh, nkv, hd, lens, [past] * n, 64, room=rows)
+    a.cu = (rows * (np.arange(n + 1) % 2)).astype(np.int32)
+    dev, lib = Dev(tg), tg.lib()
+    size = lib.tg_hip_attention_paged_scratch_bytes(a.rows, n, nh, nkv, hd, a.max_kv)
+    assert size
+    a.call(dev)   # in scratch that holds anything
+    was = np.full(size + 64, fill, np.uint8)
+    scratch = dev(was)
+    a.args = (*a.args[:-1], scratch)
+    a.queue(lib)
+    done(tg)
+    assert np.array_equal(dev.read(a.after, a.guard), a.guard) and np.array_equal(dev.read(scratch, was)[size:], was[size:])
+    dev.free()

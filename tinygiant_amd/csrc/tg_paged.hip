@@ -1177,7 +1177,12 @@ __device__ inline __attribute__((always_inline)) void join_tile(const PromptArgs
         place = tile_place<MTILE>(pt, w, ratio);
     }
     const Part::Tile tile = pt.tiles[place];
-    if (tile.count <= 1) return;
+    /* Offsets that decrease overlap, and make more spans than there are items: some are computed by none, and their tile's entry
+     * is whatever the scratch held.  No record outside the part's is read for it. */
+    const unsigned items = (unsigned)pt.p.items;
+    if (tile.count <= 1 || tile.count > pt.p.cap || (unsigned)tile.item >= items || (unsigned)tile.last >= items ||
+        (unsigned)tile.step >= items || (unsigned)tile.item + (unsigned)(tile.count - 2) * (unsigned)tile.step >= items)
+        return;
     const int rows = min(from + ROWS, min(MTILE, w.sq.n * ratio - w.m0)), g = lane / G, d = 4 * (lane % G);
     for (int m = from + wave; m < rows; m += 16) {
         int i, j;
