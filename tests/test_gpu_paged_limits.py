@@ -163,3 +163,28 @@ def test_offsets_that_overlap(tg, nh, nkv, hd, rows, n, past, fill):
     done(tg)
     assert np.array_equal(dev.read(a.after, a.guard), a.guard) and np.array_equal(dev.read(scratch, was)[size:], was[size:])
     dev.free()
+
+
+@pytest.mark.parametrize("nh,nkv,hd,n", [(64, 8, 64, 128), (32, 4, 128, 200), (8, 2, 80, 300)])
+def test_a_deep_chunk_among_single_tokens(tg, nh, nkv, hd, n):
+    """With and without cuts of the chunk, by how many sequences and KV heads there are."""
+    say(f"attention of a chunk among {n} sequences {nh, nkv, hd}")
+    rng = np.random.default_rng(45)
+    lens, past = [1] * n, [int(x) for x in rng.integers(0, 700, n)]
+    lens[n // 3], past[n // 3] = 500 if nh > 8 else 2000, 4000
+    lens[n // 2] = 0
+    a = Attend(45, nh, nkv, hd, lens, past, 64, sinks=True, lead=1, tail=2)
+    at = int(a.cu[n // 3])
+    only = some_rows(a, [1, at - 1, at, at + 1, at + 250, at + lens[n // 3] - 1, at + lens[n // 3], a.rows - 3])
+    want, tol = attend(a.q, a.pages, a.cu, lens, past, nh, sinks=a.sinks, only=only)
+    dev = Dev(tg)
+    a.call(dev)
+    for again in range(3):   # in scratch that holds a call's records
+        done(tg)
+        got, rows = dev.read(a.out, a.q), sorted(only)
+        assert np.all(np.abs(got[rows] - want[rows]) <= tol[rows])
+        assert np.all(np.isfinite(got[1:-2])) and np.all(got[[0, -2, -1]] == 7.0)
+        assert np.array_equal(dev.read(a.after, a.guard), a.guard)
+        a.queue(tg.lib())
+    done(tg)
+    dev.free()

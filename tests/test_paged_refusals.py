@@ -170,6 +170,20 @@ def test_scratch_serves_mixed_calls(tg):
     assert seen > 3000
 
 
+def test_scratch_of_a_chunk_among_single_tokens(tg):
+    """Single tokens have no tiles of 128 m-rows. Of 599 rows of 32 + 4 heads, 4,792 m-rows, at most 37 sequences have more than
+    128, in at most 37 + 37 tiles; 128 spans a KV head may be added by cuts. Tiles of 16: 299 + 100, and 128. A record is
+    16 bytes and a head; a tile's entry 16 bytes, at 37 + 100 places and 8 of each sequence; six roundings to 256."""
+    lib = tg.lib()
+    lib.tg_hip_clear_error()
+    lib.tg_hip_attention_paged_dev(*_attend(rows=599, n=100, max_kv=9000, nh=32, nkv=4, hd=128, q_stride=4096, out_stride=4096, stride=1024,
+                                            scratch=None))
+    said = tg.last_error()
+    lib.tg_hip_clear_error()
+    most = 4 * (128 * (37 + 37 + 128) + 16 * (299 + 100 + 128)) * (16 + 4 * 128) + (37 + 100 + 800) * 16 + 6 * 256
+    assert "needs" in said and int(said.split("needs ")[1].split()[0]) <= most, (said, most)
+
+
 @pytest.mark.gpu
 def test_scratch_serves_smaller_calls(tg):
     """Given scratch at an odd place a call says how much it needs; its rows are none, so one that needs nothing runs."""

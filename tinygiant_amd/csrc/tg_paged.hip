@@ -1277,18 +1277,23 @@ Shape shape_of(long long m, long long rows, long long seqs, int n_kv, int head_d
 }
 
 /* A part in tiles of `tile` m-rows whose records are by item.  Beyond OFTEN
- * workgroups (of 128 m-rows; twice as many of 16) there are enough of them
- * to keep the chip busy without cuts. */
+ * places for tiles (of 128 m-rows; twice as many of 16), each sequence with one
+ * of its own, it is not cut.  Of many single tokens and a chunk that is before
+ * the chunk's own tiles are so many: those places cost the join more than cuts
+ * gain at ordinary depths (128 sequences of 64 + 8 heads, one of them 500 rows, behind
+ * 1,000 positions 53 us uncut and 79 cut; behind 8,000 202 and 191, 30,000 668 and 567). */
 constexpr int OFTEN = 1024;
 int often(int tile) { return tile == 16 ? 2 * OFTEN : OFTEN; }
+/* tiles that there can be at most, of sequences of at least `least` m-rows */
+long long most_tiles(long long m, int n, int tile, int least) { return std::min(m / tile + std::min<long long>(n, m / least), m); }
 Part item_part(const PromptArgs &a, long long m, int tile, int slots, int least, int most) {
     Part k = {};
     k.least = least, k.most = most;
-    long long tiles = std::min(m / tile + a.s.n, m);
-    if (most == FEW) tiles = std::min(tiles, (long long)a.s.n * (FEW / tile));
+    long long tiles = most_tiles(m, a.s.n, tile, least), places = most_tiles(m, a.s.n, tile, 1);
+    if (most == FEW) tiles = places = std::min(tiles, (long long)a.s.n * (FEW / tile));
     k.p.target = std::max(1, slots / a.n_kv);
     k.p.unit = 128;
-    k.p.cap = tiles * a.n_kv > often(tile) ? 1 : MOST_SPANS;
+    k.p.cap = places * a.n_kv > often(tile) ? 1 : MOST_SPANS;
     k.p.items = (int)tiles + (k.p.cap > 1 ? k.p.target : 0);
     return k;
 }
@@ -1407,12 +1412,12 @@ size_t attention_paged_scratch(int n_rows, int n_seqs, int n_heads, int n_kv, in
     auto bytes = [&](long long records) { return (size_t)records * (16 + 4 * (size_t)head_dim) + 512; };
     size_t most = bytes(std::min(row_heads * spans, (m <= 16 ? 16ll * 512 : 128ll * 256) * (n_seqs > 1 ? 4 : 1)));
     if (n_seqs > 1) {
-        auto part = [&](int tile) {
-            const long long tiles = std::min(std::min(m / tile + n_seqs, m), std::max(1ll, (long long)often(tile) / n_kv));
+        auto part = [&](int tile, int least) {
+            const long long tiles = std::min(most_tiles(m, n_seqs, tile, least), std::max(1ll, (long long)often(tile) / n_kv));
             return bytes((tiles + std::max(1, 512 / n_kv)) * n_kv * tile);
         };
         const size_t places = (size_t)(m / 128 + m / 16 + (FEW / 16 + 1) * (long long)n_seqs) * sizeof(Part::Tile) + 512;
-        most = std::max(most, part(128) + part(16) + places);
+        most = std::max(most, part(128, FEW + 1) + part(16, 1) + places);
     }
     return most;
 }
