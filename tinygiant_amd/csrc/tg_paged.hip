@@ -541,16 +541,16 @@ __device__ inline long long record_of(const PromptArgs &a, const Part &pt, const
 
 /* Beyond 2^24 in base 2 f32 does not hold what is added to a score or taken from it: mx + LAG_H, SHIFT_H - mx and its sum with
  * V's exponent would be rounded, by enough for weights that f16 does not hold.  Once a wave has a reference beyond FAR (all of
- * that is exact before it) every larger score moves the reference, and a weight's exponent is the exact difference from it (far_exp);
- * the largest score's own rounding adds 4 at most up to BEYOND.  Past that a row is NaN, and scores below -BEYOND have no
- * weight. */
+ * that is exact before it) each step goes where references move, and a score is replaced by its exact difference from the
+ * reference, with a factor of 1 and nothing else to add but V's exponent; the largest score's own rounding adds 4 at most up to
+ * BEYOND.  Past that a row is NaN, and scores below -BEYOND have no weight. */
 constexpr float FAR = 0x1p23f, BEYOND = 0x1p27f;
 __device__ inline bool far_ref(float &m) {
     if (!__any(fabsf(m) > FAR && m > -INFINITY)) return false;
     m = m < BEYOND ? m > -INFINITY ? fmaxf(m, -BEYOND) : m : __int_as_float(0x7FC00000);
     return true;
 }
-__device__ inline float far_exp(float s, float ck, float ev, float m) { return fmaf(s, ck, -m) + (ev + SHIFT_H); }
+__device__ inline float far_score(float s, float ck, float m) { return fmaf(s, ck, m == -INFINITY ? 0.f : -m) + SHIFT_H; }
 
 /* A record's statistics.  m of -inf says that its row sees no position there, and
  * its sum is left out where records meet; a sum that is NaN has to reach the row
@@ -725,34 +725,33 @@ __device__ inline __attribute__((always_inline)) void paged_n(const PromptArgs &
             top = fmaxf(top, fmaf(u, ck[b], (float)((ex[b] >> 8 & 255) - 127)));
         }
         top = other_half_max(max16(top));
-        if (__any(top - mx > lag)) {
+        float ref = mx;
+        if (__any(top > mx + lag)) {
             float mn = fmaxf(mx, ceilf(top));
-            if (far_ref(mn)) lag = 0.f;
+            ref = mn;
+            if (__builtin_expect(far_ref(mn), false)) {   /* hardly ever */
+                lag = ref = -INFINITY;
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+#pragma unroll
+                    for (int v = 0; v < 4; v++) s[b][v] = far_score(s[b][v], ck[b], mn);
+                    ck[b] = 1.f;
+                }
+            }
             const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
             mx = mn;
             l *= alpha;
 #pragma unroll
             for (int k = 0; k < N; k++) o[k] *= alpha;
         }
-        const float ref = mx == -INFINITY ? 0.f : SHIFT_H - mx;
-        float add[2];
-#pragma unroll
-        for (int b = 0; b < 2; b++) add[b] = ref + (float)((ex[b] >> 8 & 255) - 127);
-        if (lag == 0.f) {   /* uniform, hardly ever */
-            const float m = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-            for (int b = 0; b < 2; b++) {
-#pragma unroll
-                for (int v = 0; v < 4; v++) s[b][v] = far_exp(s[b][v], ck[b], (float)((ex[b] >> 8 & 255) - 127), m);
-                ck[b] = 1.f, add[b] = 0.f;
-            }
-        }
+        ref = ref == -INFINITY ? 0.f : SHIFT_H - ref;
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             const int ev = ex[b] >> 8 & 255;
+            const float add = ref + (float)(ev - 127);
             float e[4];
 #pragma unroll
-            for (int v = 0; v < 4; v++) e[v] = __builtin_amdgcn_exp2f(fmaf(s[b][v], ck[b], add[b]));
+            for (int v = 0; v < 4; v++) e[v] = __builtin_amdgcn_exp2f(fmaf(s[b][v], ck[b], add));
             l = fmaf((e[0] + e[1]) + (e[2] + e[3]), exp_down(ev), l);
 #pragma unroll
             for (int v = 0; v < 4; v += 2) {
@@ -1052,9 +1051,19 @@ __device__ inline __attribute__((always_inline)) void paged_w(const PromptArgs &
                 }
             }
             top = other_half_max(top);
-            if (__any(top - mx > lag)) {
+            float ref = mx;
+            if (__any(top > mx + lag)) {
                 float mn = max_nan(mx, ceilf(top));
-                if (far_ref(mn)) lag = 0.f;
+                ref = mn;
+                if (__builtin_expect(far_ref(mn), false)) {   /* hardly ever */
+                    lag = ref = -INFINITY;
+#pragma unroll
+                    for (int g = 0; g < 2 * J; g++) {
+#pragma unroll
+                        for (int v = 8 * (g & 1); v < 8 * (g & 1) + 8; v++) s[g >> 1][v] = far_score(s[g >> 1][v], ck[g], mn);
+                        ck[g] = 1.f;
+                    }
+                }
                 const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
                 mx = mn;
                 l *= alpha;
@@ -1063,31 +1072,17 @@ __device__ inline __attribute__((always_inline)) void paged_w(const PromptArgs &
 #pragma unroll
                     for (int v = 0; v < 16; v++) o[d][v] *= alpha;
             }
-            const float ref = mx == -INFINITY ? 0.f : SHIFT_H - mx;
-            float add[2 * J];
-#pragma unroll
-            for (int g = 0; g < 2 * J; g++) add[g] = ref + (float)((eg[g] >> 8 & 255) - 127);
-            if (lag == 0.f) {   /* uniform, hardly ever */
-                const float m = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-                for (int g = 0; g < 2 * J; g++) {
-#pragma unroll
-                    for (int v = 0; v < 8; v++) {
-                        const int k = 8 * (g & 1) + v;
-                        s[g >> 1][k] = far_exp(s[g >> 1][k], ck[g], (float)((eg[g] >> 8 & 255) - 127), m);
-                    }
-                    ck[g] = 1.f, add[g] = 0.f;
-                }
-            }
+            ref = ref == -INFINITY ? 0.f : SHIFT_H - ref;
             __builtin_amdgcn_iglp_opt(2);
             h8 ph[2 * J], pl[2 * J];
 #pragma unroll
             for (int g = 0; g < 2 * J; g++) {
+                const float add = ref + (float)((eg[g] >> 8 & 255) - 127);
                 float sum[2] = {0.f, 0.f};
 #pragma unroll
                 for (int v = 0; v < 8; v += 2) {
-                    const float e0 = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + v], ck[g], add[g]));
-                    const float e1 = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + v + 1], ck[g], add[g]));
+                    const float e0 = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + v], ck[g], add));
+                    const float e1 = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + v + 1], ck[g], add));
                     sum[0] += e0, sum[1] += e1;
                     h2 hi, lo;
                     split2(e0, e1, e0, e1, one, hi, lo);
