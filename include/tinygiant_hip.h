@@ -353,7 +353,7 @@ void tg_hip_attention_prefix_dev(const float *q_dev, int q_stride, int kv_type, 
  *
  * tg_hip_rope_tables_dev fills cos, sin [rope_len][rot_dim / 2] for positions
  * first .. first + rope_len - 1: mscale cos(p f_i), mscale sin(p f_i), angles in
- * 64 bits, each rounded once.  f_i from F_i = theta^(-2 i / rot_dim) (theta > 1) by
+ * 64 bits (off by a few 2^-53 of themselves), each rounded once.  f_i from F_i = theta^(-2 i / rot_dim) (theta > 1) by
  *   scaling 0  F_i
  *           1  F_i / factor (positions stretched)
  *           2  theta factor^(rot_dim / (rot_dim - 2)) in theta's place
@@ -428,7 +428,8 @@ void tg_hip_paged_append_dev(const float *q_dev, const float *k_dev, const float
  * tg_hip_attention_dev and of the packed rows above.  Positions without a page
  * and blocks whose byte is outside 85..169 come out NaN.  A sequence whose slot is not below
  * n_slots, or whose length is past kv_max or its row of the table, is left
- * out; the slots' other positions stay as they were. */
+ * out; the slots' other positions stay as they were.  Two sequences of a call
+ * must not have the same slot. */
 void tg_hip_paged_read_dev(const int8_t *pages_k_dev, const int8_t *pages_v_dev, const uint8_t *exps_k_dev,
                            const uint8_t *exps_v_dev, int n_pages, int page_size, const int32_t *table_dev,
                            int table_stride, const int32_t *len_dev, int n_seqs, int n_kv_heads, int head_dim, int kv_type,
@@ -443,10 +444,12 @@ void tg_hip_paged_read_dev(const int8_t *pages_k_dev, const int8_t *pages_v_dev,
  * A row that sees a position without a page, or of a block whose byte is
  * outside 85..169, is NaN; so is one whose query is not finite.  K and V are
  * exact; q keeps 22 bits of each value, or of its head's largest magnitude 24 (a head
- * below 2^-80 scores 0), by how many rows there are; the weights 22, or 2^-33 of the
- * row's largest weight times value; sums and the softmax's statistics are f32.  A row with a score beyond 9.3e7
- * (2^27 in base 2, where f32 has steps of 16) is NaN, and scores below the negative of that have no weight.  out may be
- * q with q's stride.
+ * below 2^-80 scores 0), by how many rows there are; the weights 22, or 2^-32 of the
+ * row's largest product of a weight and its block's power of two (a block whose visible
+ * bytes are small beside it, as one keeps from rows taken back, costs the others bits);
+ * sums and the softmax's statistics are f32.  A row with a score beyond 9.3e7
+ * (2^27 in base 2, where f32 has steps of 16) is NaN, and scores below the negative
+ * of that have no weight.  out may be q with q's stride.
  * scratch_dev holds tg_hip_attention_paged_scratch_bytes(...) bytes, 16-byte
  * aligned; it may be NULL where that is 0.  The size is enough for every call of
  * at most as many rows, sequences and positions (max_kv) with these heads.

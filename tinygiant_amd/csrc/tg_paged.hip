@@ -581,18 +581,20 @@ __device__ inline void to_half(uint32_t w, h2 &a, h2 &b) {
  * S^T[position][m-row] is integer: K as it is, q as three signed digits of
  * base 256 of q 2^s, its head's largest value to 2^22 .. 2^23 (24 bits of it),
  * on v_mfma_i32_16x16x64_i8.  A digit's sum is exact and below 2^21; joined
- * they are rounded once.  D lane l holds m-row l % 16, positions 4 (l / 16) + v.
+ * they are rounded twice, the upper two (below 2^29) as they become f32 and the
+ * whole.  D lane l holds m-row l % 16, positions 4 (l / 16) + v.
  * O^T[dim][m-row] is f16 (16x16x32) over both blocks' 32 positions in the
  * order in which the lanes hold their weights, split in two f16; the lanes
  * load V rows 4 (l / 16) .. + 3 of each block, dims HD / 16 (l % 16) .., and one byte
  * permutation a pair both transposes and widens them.
  *
  * Bound: the pages' bytes where they are many.  64 rows of 32 + 4 heads of 128
- * behind 61 .. 8,314 positions, 277 MB: 50 us, 5.5 TB/s (256 behind 4,000 each 185 us
- * with the second kernel, 5.7 TB/s); one of 64 + 8 heads of 64 behind 30,001 12 us, where
- * the chain of a workgroup is most: its lengths, its table, its first blocks, then
- * four steps.  (Two steps loaded ahead take 20 registers more and no time less; 32 m-rows a
- * workgroup 15.4 us instead of 12.2 at nine rows behind 1,000 positions.) */
+ * behind 61 .. 8,314 positions, 277 MB, over three states in turn: 58.5 - 61 us, 4.6 -
+ * 4.75 TB/s (256 behind 4,000 each, 1,049 MB, 184 - 193 us, 5.4 - 5.7); one of 64 + 8
+ * heads of 64 behind 30,001 11 - 13 us, where the chain of a workgroup is most: its
+ * lengths, its table, its first blocks, then four steps.  (Two steps loaded ahead take 20 registers more and no time less; 32 m-rows a
+ * workgroup 15.4 us instead of 12.2 at nine rows behind 1,000 positions.)  Three
+ * waves a SIMD: 168 registers of heads of 128, 108 of 64, none spilled. */
 constexpr int MN = 16;
 template <int HD>
 struct SharedPN {
@@ -845,10 +847,11 @@ __global__ __launch_bounds__(256, 3) void k_paged_n(PromptArgs a, Pages pg, Part
  * positions are computed together.
  *
  * Bound for long prompts: the matrix units at the power limit and the issue of
- * the softmax beside them.  8,192 rows of 32 heads of 128: 909 us, 1.21 PFLOP/s
+ * the softmax beside them.  8,192 rows of 32 heads of 128: 915 us, 1.20 PFLOP/s
  * counting both products (a large f16 product runs at 1.15 - 1.2); of 64 heads of 64
- * 1,048, where a product is half as long and the softmax is not: three waves a
- * SIMD, 168 registers (two 1,098).  Widening costs a quarter more VALU
+ * 1,060, where a product is half as long and the softmax is not: three waves a
+ * SIMD, 168 registers and 2 spilled (two waves 5% more).  Heads of 128 have 256 registers, of
+ * which 2 (256 rows) to 10 (128 rows in one or two groups) are spilled.  Widening costs a quarter more VALU
  * instructions than f16 caches take.  (Integer products for the scores, as few rows have, would be a
  * quarter less of the first product and twice that in joining its digits; the widening before the
  * products in half of the waves and behind them in the others changed nothing.) */
@@ -1135,7 +1138,8 @@ __global__ __launch_bounds__(64 * MW * KG, HD == 64 && MW * KG == 4 ? 3 : 2) voi
 /* A mixed call in one launch: sequences of many rows in tiles of 128, those of
  * few in tiles of 16, each kind cut into spans by its own positions.  In two
  * launches 60 single tokens and a chunk of 500 rows took 119 us (32 + 4 heads of 128; in one, cut the same way, 108),
- * seven sequences of 1 to 1,000 rows 73 (68). */
+ * seven sequences of 1 to 1,000 rows 73 (68).  Both kinds have the larger one's registers and LDS: at heads of 128 256 (11
+ * spilled) and 65 KB, so that tiles of 16 run at two waves a SIMD here and not at three. */
 template <int HD>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_both(PromptArgs a, Pages pg, Part many, Part few) {
     __shared__ union {

@@ -14,12 +14,14 @@ namespace tg {
 
 /* ---- tables ----
  * cos and sin of 2 pi t, t = position * (frequency / 2 pi) turns.  t is a
- * product in 64 bits, off by 2^-53 of itself: 2^-33 turns at position 2^20 of
- * the fastest pair.  Its nearest quarter is taken off, which is exact, and the rest,
+ * product in 64 bits, off by 2^-53 of itself and by as much again from the
+ * rounded frequency.  Its nearest quarter is taken off, which is exact, and the rest,
  * at most an eighth of a turn, goes through the Taylor sums of both functions
- * in 64 bits to below 2^-50, so that what is stored is the f32 nearest to the
- * formula's value (a 32-bit product is off by 0.06 turns there).  A lane has
- * four pairs of a position, 16 bytes of each table.
+ * in 64 bits to below 2^-50.  So what is stored is off by half an f32 step of
+ * the value and by a few 2^-53 of the angle: of the fastest pair 2e-10 at
+ * position 2^20 (one entry in some 2,000 is not the nearest f32; a sine near 0 has
+ * steps smaller than that) and 2e-7 at 2^30; a 32-bit product is off by 0.06 turns
+ * at 2^20.  A lane has four pairs of a position, 16 bytes of each table.
  * Bound: the stores, beside about 30 64-bit operations a pair. */
 __device__ inline void turn_of(double t, double &c, double &s) {
     t -= __builtin_rint(t);
@@ -50,8 +52,9 @@ __device__ inline void turn_of(double t, double &c, double &s) {
 
 /* A lane has ROWS positions in a row.  Those behind the first are turned on by
  * one position's angle, four products each instead of both sums, off by 2^-53 a
- * step: 131,072 positions of 32 pairs 8.4 us with four, 9.9 with one; 4,096
- * of 64, where there are too few lanes then, 6.8 and 5.4. */
+ * step: 131,072 positions of 32 pairs 8.8 us in the kernel with four, 11.4 with one
+ * (calls 8.0 and 9.9); 4,096 of 64, where there are too few lanes then, 3.5 and 3.0
+ * (calls 5.2). */
 template <int ROWS>
 __global__ __launch_bounds__(256) void k_rope_tables(RopeTablesArgs a) {
     const unsigned per = (unsigned)a.pairs / 4, at = blockIdx.x * 256 + threadIdx.x, group = at / per;
