@@ -311,7 +311,8 @@ void tg_hip_kv_append_dev(const float *q_dev, const float *k_dev, const float *v
  * With values of ordinary spread that is f32's accuracy; a query with one
  * dimension 2^17 above all that counts in the others loses bits of these, and
  * a dimension in which only positions of vanishing weight have values loses
- * bits of the output.
+ * bits of the output.  Among scores of 5.8e6 and more (2^23 in base 2, where f32
+ * has steps of 1) weights can be wrong.
  * Rows that come out not finite are computed again value by value: as exact,
  * but many times slower.  Where nearby positions of an f32 cache differ by
  * more than 2^12 in magnitude, or the channels of eight neighbouring positions
@@ -449,7 +450,8 @@ void tg_hip_paged_read_dev(const int8_t *pages_k_dev, const int8_t *pages_v_dev,
  * bytes are small beside it, as one keeps from rows taken back, costs the others bits);
  * sums and the softmax's statistics are f32.  A row with a score beyond 9.3e7
  * (2^27 in base 2, where f32 has steps of 16) is NaN, and scores below the negative
- * of that have no weight.  out may be q with q's stride.
+ * of that have no weight (a row that has no others is NaN without a sink, 0 with
+ * one).  out may be q with q's stride.
  * scratch_dev holds tg_hip_attention_paged_scratch_bytes(...) bytes, 16-byte
  * aligned; it may be NULL where that is 0.  The size is enough for every call of
  * at most as many rows, sequences and positions (max_kv) with these heads.
